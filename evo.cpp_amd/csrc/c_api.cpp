@@ -29,6 +29,7 @@
 #include "evo/hip_ops.h"
 #include "model.hpp"
 #include "ops.hpp"
+#include "paged.hpp"
 
 namespace {
 
@@ -908,6 +909,146 @@ evo_status evo_hip_attention_ws(const float *projected, size_t rows, size_t widt
                                               capacity * width, capacity, rows, prefix, heads,
                                               heads == 0 ? 0 : width / heads, out, nullptr,
                                               nullptr, s, workspace, workspace_bytes));
+  });
+}
+
+namespace {
+// The structs of a paged call, checked, as the kernels take them.
+evo::Status paged_cache(const evo_hip_paged_cache *cache, evo::hip::PagedCache *out) {
+  const auto invalid = [](const char *why) {
+    return evo::Status{evo::ErrorCode::kInvalidArgument, std::string("invalid_argument: ") + why};
+  };
+  if (cache == nullptr || cache->struct_size < sizeof(evo_hip_paged_cache))
+    return invalid("evo_hip_paged_cache is null or too small");
+  if (cache->dtype != EVO_HIP_BF16 && cache->dtype != EVO_HIP_F16)
+    return invalid("a paged cache is BF16 or F16");
+  if (cache->key_pages == nullptr || cache->value_pages == nullptr ||
+      (reinterpret_cast<uintptr_t>(cache->key_pages) |
+       reinterpret_cast<uintptr_t>(cache->value_pages)) % 16 != 0)
+    return invalid("the pages are null or not 16-byte aligned");
+  if (cache->head_dim != 32 && cache->head_dim != 64 && cache->head_dim != 128)
+    return invalid("head_dim of a paged cache must be 32, 64 or 128");
+  const size_t size = cache->page_size;
+  if (size < 16 || size > 32768 || (size & (size - 1)) != 0)
+    return invalid("page_size must be a power of two from 16 to 32768");
+  if (cache->pages == 0 || cache->pages > std::numeric_limits<int32_t>::max() ||
+      cache->kv_heads == 0 || cache->kv_heads > 65536)
+    return invalid("pages or kv_heads out of range");
+  size_t page = cache->page_stride, head = cache->head_stride, token = cache->token_stride;
+  if (page == 0 && head == 0 && token == 0) {
+    token = cache->head_dim;
+    head = size * token;
+    page = cache->kv_heads * head;
+  }
+  if (page % 8 != 0 || head % 8 != 0 || token % 8 != 0 || token < cache->head_dim)
+    return invalid("page, head and token strides must be multiples of 8, a token's of its head "
+                   "at least");
+  // (A stride of pages * page_stride that overflows is no address.)
+  if (page > std::numeric_limits<size_t>::max() / 4 / cache->pages ||
+      head > std::numeric_limits<size_t>::max() / 4 / cache->kv_heads ||
+      token > std::numeric_limits<size_t>::max() / 4 / size)
+    return invalid("strides out of range");
+  *out = {static_cast<int>(cache->dtype), static_cast<uint16_t *>(cache->key_pages),
+          static_cast<uint16_t *>(cache->value_pages), static_cast<int>(cache->pages),
+          __builtin_ctzll(size), static_cast<int>(cache->kv_heads),
+          static_cast<int>(cache->head_dim), page, head, token};
+  return evo::Status::Ok();
+}
+
+evo::Status paged_batch(const evo_hip_paged_batch *batch, const evo::hip::PagedCache &cache,
+                        evo::hip::PagedBatch *out) {
+  const auto invalid = [](const char *why) {
+    return evo::Status{evo::ErrorCode::kInvalidArgument, std::string("invalid_argument: ") + why};
+  };
+  if (batch == nullptr || batch->struct_size < sizeof(evo_hip_paged_batch))
+    return invalid("evo_hip_paged_batch is null or too small");
+  if (batch->token_start == nullptr || batch->lengths == nullptr || batch->page_table == nullptr)
+    return invalid("token_start, lengths or page_table is null");
+  // Rows times heads and positions stay inside 32 bits.
+  constexpr size_t kMost = size_t{1} << 30;
+  if (batch->sequences == 0 || batch->sequences > (size_t{1} << 20) || batch->tokens == 0 ||
+      batch->tokens > (size_t{1} << 24) || batch->max_tokens == 0 ||
+      batch->max_tokens > batch->tokens || batch->max_length == 0 || batch->max_length > kMost)
+    return invalid("sequences, tokens, max_tokens or max_length out of range");
+  const size_t page = size_t{1} << cache.page_shift;
+  if (batch->table_stride > kMost || (batch->max_length + page - 1) / page > batch->table_stride)
+    return invalid("table_stride holds fewer positions than max_length");
+  if (batch->shared_length % page != 0 || batch->shared_length > batch->max_length ||
+      (batch->shared_length != 0 && batch->shared_table == nullptr))
+    return invalid("shared_length is no multiple of page_size, beyond max_length, or without "
+                   "its table");
+  *out = {static_cast<int>(batch->sequences), static_cast<int>(batch->tokens),
+          static_cast<int>(batch->max_tokens), static_cast<int>(batch->max_length),
+          batch->token_start, batch->lengths, batch->page_table, batch->table_stride,
+          static_cast<int>(batch->shared_length), batch->shared_table, batch->error};
+  return evo::Status::Ok();
+}
+
+evo::Status paged_call(const evo_hip_paged_cache *cache, const evo_hip_paged_batch *batch,
+                       evo::hip::PagedCache *cache_out, evo::hip::PagedBatch *batch_out) {
+  EVO_TRY(paged_cache(cache, cache_out));
+  return paged_batch(batch, *cache_out, batch_out);
+}
+}  // namespace
+
+evo_status evo_hip_paged_append(const evo_hip_paged_cache *cache, const evo_hip_paged_batch *batch,
+                                evo_hip_dtype dtype, const void *projected, size_t row_stride,
+                                size_t heads, int column_split, const float *inv_freq,
+                                size_t rotary_dim, int interleaved, float rope_scale, void *query,
+                                size_t query_stride, void *stream) {
+  return protect([&]() -> evo_status {
+    evo::hip::PagedCache pages;
+    evo::hip::PagedBatch rows;
+    const auto checked = paged_call(cache, batch, &pages, &rows);
+    if (!checked.ok())
+      return publish(checked);
+    const evo::hip::PagedRope rope{inv_freq, rotary_dim, interleaved != 0, rope_scale};
+    return publish(evo::hip::paged_append(pages, rows, static_cast<int>(dtype), projected,
+                                          row_stride, heads, column_split != 0, rope, query,
+                                          query_stride, static_cast<hipStream_t>(stream)));
+  });
+}
+
+size_t evo_hip_paged_attention_workspace_bytes(const evo_hip_paged_cache *cache,
+                                               const evo_hip_paged_batch *batch, size_t heads) {
+  evo::hip::PagedCache pages;
+  evo::hip::PagedBatch rows;
+  if (!paged_call(cache, batch, &pages, &rows).ok())
+    return 0;
+  return evo::hip::paged_attention_workspace_bytes(pages, rows, heads);
+}
+
+evo_status evo_hip_paged_attention(const evo_hip_paged_cache *cache,
+                                   const evo_hip_paged_batch *batch, const void *query,
+                                   size_t query_stride, size_t heads, float scale, void *out,
+                                   size_t out_stride, void *workspace, size_t workspace_bytes,
+                                   void *stream) {
+  return protect([&]() -> evo_status {
+    evo::hip::PagedCache pages;
+    evo::hip::PagedBatch rows;
+    const auto checked = paged_call(cache, batch, &pages, &rows);
+    if (!checked.ok())
+      return publish(checked);
+    return publish(evo::hip::paged_attention(pages, rows, query, query_stride, heads, scale, out,
+                                             out_stride, workspace, workspace_bytes,
+                                             static_cast<hipStream_t>(stream)));
+  });
+}
+
+size_t evo_hip_sample_workspace_bytes(size_t rows, size_t vocab) {
+  return evo::hip::sample_workspace_bytes(rows, vocab);
+}
+
+evo_status evo_hip_sample(evo_hip_dtype dtype, const void *logits, size_t rows, size_t vocab,
+                          size_t row_stride, const float *temperature, const int32_t *top_k,
+                          const float *top_p, const float *min_p, const float *uniform,
+                          uint32_t *tokens, void *workspace, size_t workspace_bytes,
+                          void *stream) {
+  return protect([&]() -> evo_status {
+    return publish(evo::hip::sample_tokens(static_cast<int>(dtype), logits, rows, vocab,
+                                           row_stride, temperature, top_k, top_p, min_p, uniform,
+                                           tokens, workspace, workspace_bytes,
+                                           static_cast<hipStream_t>(stream)));
   });
 }
 

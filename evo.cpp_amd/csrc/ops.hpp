@@ -229,4 +229,34 @@ Status causal_attention(const uint16_t *q, size_t q_plane, const uint16_t *k_cac
                         hipStream_t stream, float *workspace = nullptr,
                         size_t workspace_bytes = 0, bool out_f16 = false);
 
+// ---- Paged cache of several sequences (paged.hpp; paged_append.hip).
+struct PagedCache;
+struct PagedBatch;
+// Type of a projection, logits or cache: the evo_hip_dtype values.
+enum ElementType : int { kElementF32 = 0, kElementBF16 = 1, kElementF16 = 4 };
+struct PagedRope {
+  const float *inv_freq;
+  size_t rotary_dim;
+  bool interleaved;
+  float scale;
+};
+Status paged_append(const PagedCache &cache, const PagedBatch &batch, int dtype,
+                    const void *projected, size_t row_stride, size_t heads, bool column_split,
+                    const PagedRope &rope, void *query, size_t query_stride, hipStream_t stream);
+
+// Attention over the paged cache (paged_attention.hip).
+size_t paged_attention_workspace_bytes(const PagedCache &cache, const PagedBatch &batch,
+                                       size_t heads);
+Status paged_attention(const PagedCache &cache, const PagedBatch &batch, const void *query,
+                       size_t query_stride, size_t heads, float scale, void *out,
+                       size_t out_stride, void *workspace, size_t workspace_bytes,
+                       hipStream_t stream);
+
+// ---- Sampling (sampling.hip).
+size_t sample_workspace_bytes(size_t rows, size_t vocab);
+Status sample_tokens(int dtype, const void *logits, size_t rows, size_t vocab, size_t row_stride,
+                     const float *temperature, const int32_t *top_k, const float *top_p,
+                     const float *min_p, const float *uniform, uint32_t *tokens, void *workspace,
+                     size_t workspace_bytes, hipStream_t stream);
+
 }  // namespace evo::hip

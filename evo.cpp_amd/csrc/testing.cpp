@@ -9,6 +9,7 @@
 #include "gemm_tile.hpp"
 #include "launch_rules.hpp"
 #include "ops.hpp"
+#include "paged.hpp"
 
 #define EVO_TEST_API extern "C" __attribute__((visibility("default")))
 
@@ -102,4 +103,28 @@ EVO_TEST_API int evo_test_fp8_on_tile(int tile, const uint8_t *x, const uint8_t 
   return evo::hip::fp8_linear_on_tile(tile, x, w, out, m, n, k, scale,
                                       static_cast<evo::hip::Fp8Mode>(mode),
                                       static_cast<hipStream_t>(stream)).ok() ? 0 : 1;
+}
+
+// The index rules of the paged cache on host arrays. Fields of `sizes`:
+// sequences, tokens, max_tokens, max_length, shared_length.
+static evo::hip::PagedBatch host_batch(const int *sizes, const int32_t *token_start,
+                                       const int32_t *lengths) {
+  return {sizes[0], sizes[1], sizes[2], sizes[3], token_start, lengths, nullptr, 0, sizes[4],
+          nullptr, nullptr};
+}
+// first, count and length of a sequence; 1 where it is valid.
+EVO_TEST_API int evo_test_paged_rows(const int *sizes, const int32_t *token_start,
+                                     const int32_t *lengths, int sequence, int *rows) {
+  const auto r = evo::hip::sequence_rows(host_batch(sizes, token_start, lengths), sequence);
+  rows[0] = r.first;
+  rows[1] = r.count;
+  rows[2] = r.length;
+  return r.valid ? 1 : 0;
+}
+EVO_TEST_API int evo_test_paged_sequence(const int *sizes, const int32_t *token_start,
+                                         const int32_t *lengths, int token) {
+  return evo::hip::sequence_of(host_batch(sizes, token_start, lengths), token);
+}
+EVO_TEST_API int evo_test_paged_page(const int32_t *table, int index, int pages) {
+  return evo::hip::checked_page(table, index, pages);
 }

@@ -21,6 +21,32 @@ DTYPE_PLANAR = 0x100  # OR-ed into the Hyena dtype: planar projection columns
 DTYPE_BF16_TAPS = 0x200  # OR-ed into the Hyena dtype: inner taps are BF16 values
 FP8_MFMA_K32, FP8_MFMA_K128, FP8_EXACT = 0, 1, 2
 
+PAGED_BAD_SEQUENCE, PAGED_BAD_PAGE = 1, 2  # bits of PagedBatch.error
+
+
+class _Sized(ctypes.Structure):
+    """A parameter struct that knows its struct_size; fields not given are 0 or NULL."""
+
+    def __init__(self, **fields):
+        super().__init__(struct_size=ctypes.sizeof(self), **fields)
+
+
+class PagedCache(_Sized):
+    _fields_ = [("struct_size", c_size), ("dtype", c_int), ("key_pages", c_void),
+                ("value_pages", c_void), ("pages", c_size), ("page_size", c_size),
+                ("kv_heads", c_size), ("head_dim", c_size), ("page_stride", c_size),
+                ("head_stride", c_size), ("token_stride", c_size)]
+
+
+class PagedBatch(_Sized):
+    _fields_ = [("struct_size", c_size), ("sequences", c_size), ("tokens", c_size),
+                ("max_tokens", c_size), ("max_length", c_size), ("token_start", c_void),
+                ("lengths", c_void), ("page_table", c_void), ("table_stride", c_size),
+                ("shared_length", c_size), ("shared_table", c_void), ("error", c_void)]
+
+
+_paged = [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedBatch)]
+
 # name -> (restype, argtypes) for include/evo/hip_ops.h
 _OPS = {
     "evo_hip_hyena_workspace_bytes": (c_size, [c_int, c_size, c_size, c_size]),
@@ -62,6 +88,14 @@ _OPS = {
     "evo_hip_attention_ws": (c_int, [c_void, c_size, c_size, c_size, c_int, c_void, c_float,
                                      c_size, c_void, c_void, c_void, c_size, c_void, c_void,
                                      c_size, c_void]),
+    "evo_hip_paged_append": (c_int, _paged + [c_int, c_void, c_size, c_size, c_int, c_void,
+                                              c_size, c_int, c_float, c_void, c_size, c_void]),
+    "evo_hip_paged_attention_workspace_bytes": (c_size, _paged + [c_size]),
+    "evo_hip_paged_attention": (c_int, _paged + [c_void, c_size, c_size, c_float, c_void, c_size,
+                                                 c_void, c_size, c_void]),
+    "evo_hip_sample_workspace_bytes": (c_size, [c_size, c_size]),
+    "evo_hip_sample": (c_int, [c_int, c_void, c_size, c_size, c_size, c_void, c_void, c_void,
+                               c_void, c_void, c_void, c_void, c_size, c_void]),
 }
 
 

@@ -270,6 +270,151 @@ EVO_API evo_status evo_hip_attention_ws(const float *projected, size_t rows,
                                         float *out, float *workspace,
                                         size_t workspace_bytes, void *stream);
 
+/* ---- Several sequences at a time: a paged key/value cache, the attention
+ * that reads it, and sampling. No counterpart in the reference, whose batch
+ * size is one.
+ *
+ * A paged cache holds the keys and values of any number of sequences in pages
+ * of page_size positions that the caller hands out. Position p of a sequence
+ * lies in page page_table[sequence][p / page_size], slot p % page_size; the
+ * element d of key/value head h there is at
+ *   pages + page * page_stride + h * head_stride + slot * token_stride + d.
+ * dtype: EVO_HIP_BF16 or EVO_HIP_F16. page_size: a power of two from 16 to
+ * 32768. head_dim: 32, 64 or 128. The strides count elements and are
+ * multiples of 8; all three 0 means dense [pages][kv_heads][page_size]
+ * [head_dim]. Both bases are 16-byte aligned. Slots that no sequence has
+ * written may hold anything. */
+typedef struct evo_hip_paged_cache {
+  size_t struct_size;
+  evo_hip_dtype dtype;
+  void *key_pages;
+  void *value_pages;
+  size_t pages;
+  size_t page_size;
+  size_t kv_heads;
+  size_t head_dim;
+  size_t page_stride;
+  size_t head_stride;
+  size_t token_stride;
+} evo_hip_paged_cache;
+
+/* The rows of one call: `tokens` rows of a projection, query or output, of
+ * which sequence s has the rows token_start[s] .. token_start[s + 1] - 1, its
+ * newest tokens. lengths[s] counts its positions, these tokens included, so
+ * its last row is at position lengths[s] - 1. Where it has more rows than
+ * positions, the first ones are padding. Rows behind the last sequence's
+ * (token_start[sequences] < tokens) belong to none and are left as they are.
+ *   max_tokens, max_length: host bounds on a sequence's rows and positions
+ *     (max_length <= table_stride * page_size).
+ *   token_start, lengths, page_table: int32 device arrays, read by each call
+ *     when it runs, so a captured graph follows their changes within the
+ *     bounds; page_table [sequences][table_stride].
+ *   shared_length: positions at the beginning that all sequences share, a
+ *     multiple of page_size (0: none), in the pages of the device array
+ *     shared_table (shared_length / page_size entries). Entries of page_table
+ *     for these positions are not read. Every sequence with rows has
+ *     lengths[s] == 0 or its rows behind the shared positions.
+ *   error: optional device word; the kernels OR the bits below into it and
+ *     never clear it.
+ * The device arrays cannot be checked on the host. A sequence whose entries
+ * break these rules (bounds, order, shared positions) is left out, its rows
+ * left as they are: EVO_HIP_PAGED_BAD_SEQUENCE. A page index outside
+ * [0, pages) that a call needs is never followed: nothing is written there,
+ * and its positions count as masked: EVO_HIP_PAGED_BAD_PAGE. */
+typedef struct evo_hip_paged_batch {
+  size_t struct_size;
+  size_t sequences;
+  size_t tokens;
+  size_t max_tokens;
+  size_t max_length;
+  const int32_t *token_start;
+  const int32_t *lengths;
+  const int32_t *page_table;
+  size_t table_stride;
+  size_t shared_length;
+  const int32_t *shared_table;
+  int32_t *error;
+} evo_hip_paged_batch;
+#define EVO_HIP_PAGED_BAD_SEQUENCE 1
+#define EVO_HIP_PAGED_BAD_PAGE 2
+
+/* Splits the QKV projection of a batch's rows, rotates queries and keys by
+ * their positions, and appends keys and values to the cache in the same pass.
+ *   projected  [tokens][row_stride] F32, BF16 or F16 (dtype); columns
+ *              [query heads | key heads | value heads][head_dim], or with
+ *              column_split [head][query, key, value][head_dim] (heads ==
+ *              kv_heads). heads is a multiple of kv_heads.
+ *   rotation   of the first rotary_dim elements (even, 0: none) of each query
+ *              and key head, by the angle (position / rope_scale) *
+ *              inv_freq[i] (F32 [rotary_dim / 2]), formed in 64 bits so that far
+ *              positions keep their angle. Pair i is (i, rotary_dim / 2 + i),
+ *              or (2i, 2i + 1) when interleaved.
+ *   query      [tokens][query_stride] in the cache's dtype, the rotated
+ *              queries (rows of 16-byte aligned heads, query_stride a multiple
+ *              of 8); padding rows are zeroed and append nothing.
+ * Rounded once, to nearest even; a value beyond FP16 becomes infinity.
+ * Two sequences must not append to the same slot. */
+EVO_API evo_status evo_hip_paged_append(const evo_hip_paged_cache *cache,
+                                        const evo_hip_paged_batch *batch,
+                                        evo_hip_dtype dtype, const void *projected,
+                                        size_t row_stride, size_t heads, int column_split,
+                                        const float *inv_freq, size_t rotary_dim,
+                                        int interleaved, float rope_scale, void *query,
+                                        size_t query_stride, void *stream);
+
+/* Attention of a batch's rows over the cache: for each row and query head h
+ *   out = sum_k softmax_k(scale * query . key[k]) * value[k]
+ * over the positions k up to the row's own, of key/value head
+ * h / (heads / kv_heads); a row that sees none (padding, length 0) is zero.
+ * The rows' own keys are in the cache already (evo_hip_paged_append).
+ *   query  [tokens][query_stride] and out [tokens][out_stride], the cache's
+ *          dtype, heads side by side, 16-byte aligned, strides multiples of 8;
+ *          out may be query.
+ *   scale  positive (1 / sqrt(head_dim) as a rule).
+ * With shared_length the prefix's keys are read once for the rows of all
+ * sequences, not once for each.
+ * Positions beyond a sequence's rows may hold anything; within them, values have
+ * to be finite for the rows before them to be.
+ * The workspace (16-byte aligned, no initial contents) takes the partial
+ * results of keys that are split over blocks; its size depends on the host
+ * fields of the structs and heads alone. Calls that overlap need one each. */
+EVO_API size_t evo_hip_paged_attention_workspace_bytes(const evo_hip_paged_cache *cache,
+                                                       const evo_hip_paged_batch *batch,
+                                                       size_t heads);
+EVO_API evo_status evo_hip_paged_attention(const evo_hip_paged_cache *cache,
+                                           const evo_hip_paged_batch *batch,
+                                           const void *query, size_t query_stride,
+                                           size_t heads, float scale, void *out,
+                                           size_t out_stride, void *workspace,
+                                           size_t workspace_bytes, void *stream);
+
+/* tokens[r] = one token of row r of logits [rows][row_stride] (F32, BF16 or
+ * F16, vocab <= 2^20), in the order and with the cuts of evo_sampler_sample:
+ * tokens by descending logit, equal ones by ascending index; of these the first
+ * top_k (0, or vocab and more: all); weights exp(logit / temperature) in 64 bits;
+ * of these the shortest beginning whose weight reaches top_p of what top-k left
+ * (1: all); of these the ones of at least min_p times the largest weight (0: all);
+ * then the first whose cumulative weight exceeds uniform times the weight left.
+ * temperature 0, or top_k 1: the first token.
+ *   temperature, top_p, min_p (F32), top_k (int32): device [rows], or NULL for
+ *     1, 1, 0 and 0.
+ *   uniform: device F32 [rows], in [0, 1) (beyond: its nearer end).
+ * The device arrays are read when the call runs. A row gets UINT32_MAX where its
+ * logits hold NaN or +infinity or nothing above -infinity, or its parameters are
+ * out of range (temperature negative or not finite, top_k negative, top_p outside
+ * (0, 1], min_p outside [0, 1], any NaN). The token does not depend on the
+ * order in which the GPU works.
+ * The workspace (16-byte aligned, no initial contents) lets few rows of a large
+ * vocabulary be split over blocks; NULL: a block takes a whole row. Calls that
+ * overlap need one each. */
+EVO_API size_t evo_hip_sample_workspace_bytes(size_t rows, size_t vocab);
+EVO_API evo_status evo_hip_sample(evo_hip_dtype dtype, const void *logits, size_t rows,
+                                  size_t vocab, size_t row_stride, const float *temperature,
+                                  const int32_t *top_k, const float *top_p,
+                                  const float *min_p, const float *uniform,
+                                  uint32_t *tokens, void *workspace,
+                                  size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
