@@ -943,10 +943,11 @@ evo::Status paged_cache(const evo_hip_paged_cache *cache, evo::hip::PagedCache *
   if (page % 8 != 0 || head % 8 != 0 || token % 8 != 0 || token < cache->head_dim)
     return invalid("page, head and token strides must be multiples of 8, a token's of its head "
                    "at least");
-  // (A stride of pages * page_stride that overflows is no address.)
+  // (A kernel counts the 16 tokens of a step in 32 bits; a stride that overflows
+  // is no address.)
   if (page > std::numeric_limits<size_t>::max() / 4 / cache->pages ||
       head > std::numeric_limits<size_t>::max() / 4 / cache->kv_heads ||
-      token > std::numeric_limits<size_t>::max() / 4 / size)
+      token > (size_t{1} << 24))
     return invalid("strides out of range");
   *out = {static_cast<int>(cache->dtype), static_cast<uint16_t *>(cache->key_pages),
           static_cast<uint16_t *>(cache->value_pages), static_cast<int>(cache->pages),

@@ -44,7 +44,8 @@ struct AttendArgs {
   int prefix_chunk;   // shared keys per chunk
   int prefix_slots;   // chunks of the shared keys
   int slots;          // chunks of a row at most, the shared ones first
-  float *part;        // [tokens][heads][slots][2 + head_dim]
+  float *part;        // [tokens][heads][slots][head_dim], unnormalised outputs
+  float2 *state;      // [tokens][heads][slots] (maximum, sum)
 };
 
 template <typename T> struct Mfma;
@@ -53,11 +54,34 @@ template <> struct Mfma<__bf16> {
   static __device__ inline f32x4 run(const vec &a, const vec &b, const f32x4 &c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
+  static __device__ inline f32x16 run(const vec &a, const vec &b, const f32x16 &c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  // sum + the eight elements.
+  static __device__ inline float add(const vec &p, float sum) {
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    const pair one = {static_cast<__bf16>(1.0F), static_cast<__bf16>(1.0F)};
+    sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(p, p, 0, 1), one, sum, false);
+    sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(p, p, 2, 3), one, sum, false);
+    sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(p, p, 4, 5), one, sum, false);
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(p, p, 6, 7), one, sum, false);
+  }
 };
 template <> struct Mfma<_Float16> {
   typedef f16x8 vec;
   static __device__ inline f32x4 run(const vec &a, const vec &b, const f32x4 &c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ inline f32x16 run(const vec &a, const vec &b, const f32x16 &c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ inline float add(const vec &p, float sum) {
+    typedef _Float16 pair __attribute__((ext_vector_type(2)));
+    const pair one = {static_cast<_Float16>(1.0F), static_cast<_Float16>(1.0F)};
+    sum = __builtin_amdgcn_fdot2(__builtin_shufflevector(p, p, 0, 1), one, sum, false);
+    sum = __builtin_amdgcn_fdot2(__builtin_shufflevector(p, p, 2, 3), one, sum, false);
+    sum = __builtin_amdgcn_fdot2(__builtin_shufflevector(p, p, 4, 5), one, sum, false);
+    return __builtin_amdgcn_fdot2(__builtin_shufflevector(p, p, 6, 7), one, sum, false);
   }
 };
 
@@ -100,6 +124,53 @@ __device__ inline bool find_tile(const AttendArgs &a, int tile, int *sequence, i
     base += __shfl(through, 63, 64);
   }
   return false;
+}
+
+// The rows a block works on: rows row0 .. of `rows` (a sequence's, or with
+// `prefix` the batch's), row r being token first_token + r / group; the positions
+// of the tile's first and last row (prefix: the last shared one, which all see).
+struct RowTile {
+  int sequence, row0, rows, first_token, first_position, last_position;
+};
+template <int kRows>
+__device__ inline bool row_tile(const AttendArgs &a, bool prefix, int tile, RowTile *t) {
+  if (prefix) {
+    *t = {0, tile * kRows, a.batch.tokens * a.group, 0, a.batch.shared_length - 1,
+          a.batch.shared_length - 1};
+    return true;
+  }
+  int sequence, tile_in;
+  if (!find_tile<kRows>(a, tile, &sequence, &tile_in))
+    return false;
+  sequence = __builtin_amdgcn_readfirstlane(sequence);
+  const SequenceRows own = sequence_rows(a.batch, sequence);
+  const int row0 = __builtin_amdgcn_readfirstlane(tile_in) * kRows;
+  const int rows = own.count * a.group, position = own.length - own.count;
+  *t = {sequence, row0, rows, own.first, position + row0 / a.group,
+        position + (min(row0 + kRows, rows) - 1) / a.group};
+  return true;
+}
+
+// Block -> phase, key/value head, chunk and row tile. Heads vary fastest: with a
+// multiple of eight of them the blocks of a head share an XCD's L2. The last
+// tiles, which see the most keys, start first.
+struct BlockWork {
+  bool prefix;
+  int kv_head, chunk, tile;
+};
+__device__ inline BlockWork block_work(const AttendArgs &a, unsigned prefix_blocks,
+                                       unsigned tiles) {
+  BlockWork w;
+  w.prefix = blockIdx.x < prefix_blocks;
+  unsigned rest = w.prefix ? blockIdx.x : blockIdx.x - prefix_blocks;
+  w.kv_head = static_cast<int>(rest % a.cache.kv_heads);
+  rest /= a.cache.kv_heads;
+  const unsigned chunks = w.prefix ? a.prefix_slots : a.slots - a.prefix_slots;
+  w.chunk = static_cast<int>(rest % chunks);
+  w.tile = static_cast<int>(rest / chunks);
+  if (!w.prefix)
+    w.tile = static_cast<int>(tiles) - 1 - w.tile;
+  return w;
 }
 
 // Softmax state and output of 16 rows over the keys a wave has seen. Lane l:
@@ -236,53 +307,32 @@ __device__ inline void attend(const Step<T, kD> &step, const typename Mfma<T>::v
 // Blocks below prefix_blocks take the shared keys, rows of the whole batch.
 template <typename T, int kD>
 __global__ __launch_bounds__(256) void paged_stream_kernel(const AttendArgs a,
-                                                           unsigned prefix_blocks) {
+                                                           unsigned prefix_blocks,
+                                                           unsigned tiles) {
   constexpr int kRows = 16, kWaves = 4, kVec = kD / 16, kSteps = kD / 32;
   typedef typename Mfma<T>::vec vec;
   __shared__ float top_s[kWaves][kRows], sum_s[kWaves][kRows];
   __shared__ __attribute__((aligned(16))) float out_s[kWaves][kRows][kD + 4];
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const bool prefix = blockIdx.x < prefix_blocks;
-  const int kv = a.cache.kv_heads;
-  unsigned rest = prefix ? blockIdx.x : blockIdx.x - prefix_blocks;
-  const int kv_head = static_cast<int>(rest % kv);
-  rest /= kv;
-  const int chunks = prefix ? a.prefix_slots : a.slots - a.prefix_slots;
-  const int chunk = static_cast<int>(rest % chunks);
-  const int tile = static_cast<int>(rest / chunks);
-
   if (blockIdx.x == prefix_blocks)
     report_bad_sequences(a.batch);
-
-  // Rows of the tile: `row` of `rows` at this lane, token and query head.
-  int row0, rows, first_token, first_position, last_position, sequence = 0;
-  if (prefix) {
-    row0 = tile * kRows;
-    rows = a.batch.tokens * a.group;
-    first_token = 0;
-    first_position = last_position = a.batch.shared_length - 1;
-  } else {
-    int tile_in;
-    if (!find_tile<kRows>(a, tile, &sequence, &tile_in))
-      return;
-    sequence = __builtin_amdgcn_readfirstlane(sequence);
-    const SequenceRows own = sequence_rows(a.batch, sequence);
-    row0 = __builtin_amdgcn_readfirstlane(tile_in) * kRows;
-    rows = own.count * a.group;
-    first_token = own.first;
-    first_position = own.length - own.count + row0 / a.group;
-    last_position = own.length - own.count + (min(row0 + kRows, rows) - 1) / a.group;
-  }
-  const int row = row0 + col;
-  const bool active = row < rows;
-  const int token_in = (active ? row : row0) / a.group;
-  const int token = first_token + token_in;
-  const int head = kv_head * a.group + (active ? row : row0) % a.group;
-  const int position = prefix ? last_position : first_position + token_in - row0 / a.group;
+  const BlockWork work = block_work(a, prefix_blocks, tiles);
+  const bool prefix = work.prefix;
+  const int kv_head = work.kv_head, chunk = work.chunk;
+  RowTile tile;
+  if (!row_tile<kRows>(a, prefix, work.tile, &tile))
+    return;
+  const int row = tile.row0 + col;
+  const bool active = row < tile.rows;
+  const int token_in = (active ? row : tile.row0) / a.group;
+  const int token = tile.first_token + token_in;
+  const int head = kv_head * a.group + (active ? row : tile.row0) % a.group;
+  const int position =
+      prefix ? tile.last_position : tile.first_position + token_in - tile.row0 / a.group;
 
   const int key0 = prefix ? chunk * a.prefix_chunk : a.batch.shared_length + chunk * a.chunk;
-  const int key1 = min(last_position + 1, key0 + (prefix ? a.prefix_chunk : a.chunk));
+  const int key1 = min(tile.last_position + 1, key0 + (prefix ? a.prefix_chunk : a.chunk));
   if (key0 >= key1 && (prefix || chunk > 0 || a.slots > 1))
     return;
 
@@ -302,7 +352,7 @@ __global__ __launch_bounds__(256) void paged_stream_kernel(const AttendArgs a,
     state.out[t] = f32x4{0.0F, 0.0F, 0.0F, 0.0F};
 
   const int32_t *table = prefix ? a.batch.shared_table
-                                : a.batch.page_table + sequence * a.batch.table_stride;
+                                : a.batch.page_table + tile.sequence * a.batch.table_stride;
   for (int k0 = key0 + 32 * wave; k0 < key1; k0 += 32 * kWaves) {
     int page[2];
 #pragma unroll
@@ -317,7 +367,7 @@ __global__ __launch_bounds__(256) void paged_stream_kernel(const AttendArgs a,
     }
     Step<T, kD> step;
     load_step<T, kD>(a, kv_head, k0, page, step);
-    const bool masked = page[0] < 0 || page[1] < 0 || k0 + 31 > first_position || k0 + 32 > key1;
+    const bool masked = page[0] < 0 || page[1] < 0 || k0 + 31 > tile.first_position || k0 + 32 > key1;
     int visible[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -352,7 +402,7 @@ __global__ __launch_bounds__(256) void paged_stream_kernel(const AttendArgs a,
   __syncthreads();
   // Thread: row tid / 16, elements kVec * (tid % 16) ...
   const int r = threadIdx.x >> 4, d = kVec * (threadIdx.x & 15);
-  if (row0 + r >= rows)
+  if (tile.row0 + r >= tile.rows)
     return;
   float top = top_s[0][r];
 #pragma unroll
@@ -368,8 +418,8 @@ __global__ __launch_bounds__(256) void paged_stream_kernel(const AttendArgs a,
     for (int e = 0; e < kVec; ++e)
       o[e] = fmaf(out_s[w][r][d + e], scale, o[e]);
   }
-  const size_t out_token = first_token + (row0 + r) / a.group;
-  const int out_head = kv_head * a.group + (row0 + r) % a.group;
+  const size_t out_token = tile.first_token + (tile.row0 + r) / a.group;
+  const int out_head = kv_head * a.group + (tile.row0 + r) % a.group;
   if (a.slots == 1) {
     // The row's only chunk. A row without keys is zero.
     const float inverse = total > 0.0F ? 1.0F / total : total == 0.0F ? 0.0F : total;
@@ -379,15 +429,272 @@ __global__ __launch_bounds__(256) void paged_stream_kernel(const AttendArgs a,
       dst[e] = bits_of<T>(o[e] * inverse);
     return;
   }
-  const int slot = prefix ? chunk : a.prefix_slots + chunk;
-  float *dst = a.part + ((out_token * a.heads + out_head) * a.slots + slot) * (kD + 2);
-  if (d == 0) {
-    dst[0] = top;
-    dst[1] = total;
-  }
+  const size_t slot = (out_token * a.heads + out_head) * a.slots +
+                      (prefix ? chunk : a.prefix_slots + chunk);
+  if (d == 0)
+    a.state[slot] = make_float2(top, total);
+  float *dst = a.part + slot * kD + d;
 #pragma unroll
   for (int e = 0; e < kVec; e += 2)
-    *reinterpret_cast<float2 *>(dst + 2 + d + e) = make_float2(o[e], o[e + 1]);
+    *reinterpret_cast<float2 *>(dst + e) = make_float2(o[e], o[e + 1]);
+}
+
+// ------------------------------------------------------------ many rows
+// 128 rows of a key/value head, 32 a wave, over tiles of 64 keys: K and V rows
+// are copied to LDS by DMA, double buffered, wave w bringing the tile's 16 keys
+// 16w .. (one page) of both. S^T = K Q^T on v_mfma_f32_32x32x16: lane l owns row l
+// % 32 and, with h = l / 32, keys 8j + 4h + i of each 32. V^T fragments in that
+// order come out of V's rows by ds_read_b64_tr_b16, which hands lane c of 16 the
+// column c of a block of 4 keys x 16 elements.
+// LDS rows are swizzled in 16-byte units: K so that 8 rows read at one unit hit
+// distinct banks, V so that 4 rows read at one pair of units do.
+template <int kUnits> __device__ inline int swizzle_k(int row, int unit) {
+  return unit ^ ((row * kUnits / 16) & (kUnits - 1));
+}
+template <int kUnits> __device__ inline int swizzle_v(int row, int unit) {
+  return unit ^ ((2 * (row * kUnits / 16)) & (kUnits - 1));
+}
+
+// Four keys of this lane's column: the 16 lanes of a group give the addresses of 4
+// rows of 16 elements, 4 lanes a row.
+template <typename Q> __device__ inline Q transposed(const uint16_t *from) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  return __builtin_bit_cast(Q, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(from)));
+}
+
+// A weight may exceed the running maximum's by 2^8 before the maximum follows.
+constexpr float kSlack = 8.0F;
+
+template <typename T, int kD>
+__global__ __launch_bounds__(256, 2) void paged_tile_kernel(const AttendArgs a,
+                                                            unsigned prefix_blocks,
+                                                            unsigned tiles) {
+  constexpr int kRows = 128, kKeys = 64, kUnits = kD / 8;
+  constexpr int kSteps = kD / 16, kTiles = kD / 32;   // K-steps of S^T, 32-row tiles of O^T
+  constexpr int kPlane = kKeys * kD;                  // elements of K or V in a stage
+  constexpr int kOps = kD / 32;                       // DMAs of 16 keys
+  constexpr int kOpRows = 512 / kD;                   // keys of a DMA
+  typedef typename Mfma<T>::vec vec;
+  extern __shared__ __attribute__((aligned(16))) uint16_t tile_lds[];  // [2][K, V][plane]
+
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (blockIdx.x == prefix_blocks)
+    report_bad_sequences(a.batch);
+  const BlockWork work = block_work(a, prefix_blocks, tiles);
+  const bool prefix = work.prefix;
+  RowTile tile;
+  if (!row_tile<kRows>(a, prefix, work.tile, &tile))
+    return;
+  const int row = tile.row0 + 32 * wave + col;
+  const bool active = row < tile.rows;
+  const int row_in = active ? row : tile.row0;
+  const int token_in = row_in / a.group;
+  const size_t token = tile.first_token + token_in;
+  const int head = work.kv_head * a.group + row_in % a.group;
+  const int first_token_in = tile.row0 / a.group;
+  const int position =
+      prefix ? tile.last_position : tile.first_position + token_in - first_token_in;
+  // Lowest and highest position of the wave's rows (wave_rows: it has some).
+  const bool wave_rows = tile.row0 + 32 * wave < tile.rows;
+  int wave_first = tile.last_position, wave_last = tile.last_position;
+  if (!prefix && wave_rows) {
+    const int last_row = min(tile.row0 + 32 * wave + 31, tile.rows - 1);
+    wave_first = tile.first_position + (tile.row0 + 32 * wave) / a.group - first_token_in;
+    wave_last = tile.first_position + last_row / a.group - first_token_in;
+  }
+
+  const int key0 = prefix ? work.chunk * a.prefix_chunk
+                          : a.batch.shared_length + work.chunk * a.chunk;
+  const int key1 = min(tile.last_position + 1, key0 + (prefix ? a.prefix_chunk : a.chunk));
+  if (key0 >= key1 && (prefix || work.chunk > 0 || a.slots > 1))
+    return;
+
+  vec q[kSteps];
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    q[s] = *reinterpret_cast<const vec *>(a.query + token * a.query_stride + head * kD + 16 * s +
+                                          8 * half);
+    if (!active)
+      q[s] = vec{};
+  }
+  f32x16 out[kTiles];
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      out[t][e] = 0.0F;
+  float top = -INFINITY, sum = 0.0F;
+
+  const int32_t *table = prefix ? a.batch.shared_table
+                                : a.batch.page_table + tile.sequence * a.batch.table_stride;
+  // Pages of the tile's four 16-key groups in lanes 0 .. 3 (-1: none).
+  auto pages_at = [&](int k0) {
+    int page = -1;
+    const int key = k0 + 16 * lane;
+    if (lane < 4 && key < key1) {
+      page = checked_page(table, key >> a.cache.page_shift, a.cache.pages);
+      if (page < 0)
+        report(a.batch, kBadPage);
+    }
+    return page;
+  };
+  // This lane's source offset inside a DMA, in bytes (K and V: other swizzles).
+  uint32_t k_offset[kOps], v_offset[kOps];
+#pragma unroll
+  for (int i = 0; i < kOps; ++i) {
+    const int r = 16 * wave + kOpRows * i + lane / kUnits;
+    const uint32_t down = static_cast<uint32_t>((r & 15) * a.cache.token_stride);
+    k_offset[i] = 2 * (down + 8 * swizzle_k<kUnits>(r, lane % kUnits));
+    v_offset[i] = 2 * (down + 8 * swizzle_v<kUnits>(r, lane % kUnits));
+  }
+  const unsigned lds = lds_address(tile_lds) + wave * 16 * kD * 2;
+  const int slot_mask = (1 << a.cache.page_shift) - 1;
+  auto issue = [&](int k0, int stage, int pages) {
+    const int page = __builtin_amdgcn_readlane(pages, wave);
+    if (page < 0)
+      return;
+    const size_t at = page * a.cache.page_stride + work.kv_head * a.cache.head_stride +
+                      ((k0 + 16 * wave) & slot_mask) * a.cache.token_stride;
+    const unsigned to = lds + stage * (4 * kPlane);
+#pragma unroll
+    for (int i = 0; i < kOps; ++i) {
+      dma16_at(a.cache.keys + at, k_offset[i], to + 1024 * i);
+      dma16_at(a.cache.values + at, v_offset[i], to + 2 * kPlane + 1024 * i);
+    }
+  };
+
+  int pages = key0 < key1 ? pages_at(key0) : -1, next_pages = -1;
+  issue(key0, 0, pages);
+  if (key0 + kKeys < key1)
+    next_pages = pages_at(key0 + kKeys);
+  int stage = 0;
+  for (int k0 = key0; k0 < key1; k0 += kKeys, stage ^= 1) {
+    wait_dma<0>();
+    // Values that no row sees (behind the last key, or of no page) may be
+    // anything, and 0 * NaN is NaN: their rows in LDS are zeroed.
+    const uint64_t missing = ~__ballot(pages >= 0) & 15;
+    if (missing != 0 || k0 + kKeys > key1) {
+      const int own = k0 + 16 * wave;
+      const int good = (missing >> wave & 1) != 0 ? 0 : min(16, max(0, key1 - own));
+      uint16_t *v = tile_lds + stage * 2 * kPlane + kPlane + 16 * wave * kD;
+      for (int i = good * kUnits + lane; i < 16 * kUnits; i += 64)
+        *reinterpret_cast<uint4 *>(v + 8 * i) = make_uint4(0, 0, 0, 0);
+    }
+    __syncthreads();
+    if (k0 + kKeys < key1) {
+      issue(k0 + kKeys, stage ^ 1, next_pages);
+      pages = next_pages;
+      if (k0 + 2 * kKeys < key1)
+        next_pages = pages_at(k0 + 2 * kKeys);
+    }
+    if (!wave_rows || k0 > wave_last)
+      continue;
+    const uint16_t *k_s = tile_lds + stage * 2 * kPlane, *v_s = k_s + kPlane;
+
+    f32x16 score[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        score[u][e] = 0.0F;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int r = 32 * u + col;
+        const vec k = *reinterpret_cast<const vec *>(
+            k_s + r * kD + 8 * swizzle_k<kUnits>(r, 2 * s + half));
+        score[u] = Mfma<T>::run(k, q[s], score[u]);
+      }
+    }
+    if (missing != 0 || k0 + kKeys - 1 > wave_first || k0 + kKeys > key1) {
+      const int visible = min(position + 1, key1) - k0;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int key = 32 * u + (e >> 2) * 8 + 4 * half + (e & 3);
+          score[u][e] = key < visible && (missing >> (2 * u + e / 8) & 1) == 0 ? score[u][e]
+                                                                               : -INFINITY;
+        }
+    }
+    float tile_top = score[0][0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e)
+      tile_top = fmaxf(tile_top, score[0][e]);
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      tile_top = fmaxf(tile_top, score[1][e]);
+    tile_top = fmaxf(tile_top, __shfl_xor(tile_top, 32, 64)) * a.scale2;
+    if (__any(tile_top > top + kSlack)) {
+      const float next = fmaxf(top, tile_top);
+      const float shrink = next == -INFINITY ? 1.0F : __builtin_amdgcn_exp2f(top - next);
+      sum *= shrink;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          out[t][e] *= shrink;
+      top = next;
+    }
+    const float base = top == -INFINITY ? 0.0F : top;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      vec p;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        p[j] = static_cast<T>(
+            __builtin_amdgcn_exp2f(fmaf(score[kk / 2][8 * (kk % 2) + j], a.scale2, -base)));
+      sum = Mfma<T>::add(p, sum);
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        // Keys 16kk + 4 half + (0 .. 3) and 8 more; elements 32t + 16 * (lane / 16 % 2) ..
+        typedef T quad __attribute__((ext_vector_type(4)));
+        quad part[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int r = 16 * kk + 8 * j + 4 * half + (lane & 15) / 4;
+          const int d = 32 * t + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+          const uint16_t *from = v_s + r * kD + 8 * swizzle_v<kUnits>(r, d / 8) + d % 8;
+          part[j] = transposed<quad>(from);
+        }
+        const vec v = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        out[t] = Mfma<T>::run(v, p, out[t]);
+      }
+    }
+  }
+
+  const float total = sum + __shfl_xor(sum, 32, 64);
+  if (!active)
+    return;
+  // Entry e of tile t: element 32t + 8 * (e / 4) + 4 half + e % 4 of row `row`.
+  if (a.slots == 1) {
+    // The row's only chunk. A row without keys is zero.
+    const float inverse = total > 0.0F ? 1.0F / total : total == 0.0F ? 0.0F : total;
+    uint16_t *dst = a.out + token * a.out_stride + head * kD + 4 * half;
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        uint16_t bits[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          bits[j] = bits_of<T>(out[t][e + j] * inverse);
+        *reinterpret_cast<uint2 *>(dst + 32 * t + 2 * e) = __builtin_bit_cast(uint2, bits);
+      }
+    return;
+  }
+  const size_t slot =
+      (token * a.heads + head) * a.slots + (prefix ? work.chunk : a.prefix_slots + work.chunk);
+  if (half == 0)
+    a.state[slot] = make_float2(top, total);
+  float *dst = a.part + slot * kD + 4 * half;
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4)
+      *reinterpret_cast<float4 *>(dst + 32 * t + 2 * e) =
+          make_float4(out[t][e], out[t][e + 1], out[t][e + 2], out[t][e + 3]);
 }
 
 // Rows whose keys lay in several chunks: a wave per row and head rescales the
@@ -410,17 +717,17 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const AttendArgs a) 
   // (Own keys and shared ones: a row behind the prefix has both, a padding row
   // neither.)
   const int count = position < 0 ? 0 : a.prefix_slots + own;
-  const float *src = a.part + index * a.slots * (kD + 2);
+  const float *src = a.part + index * a.slots * kD + 2 * lane;
+  const float2 *state = a.state + index * a.slots;
   float top = -INFINITY;
   for (int c = 0; c < count; ++c)
-    top = fmaxf(top, src[c * (kD + 2)]);
+    top = fmaxf(top, state[c].x);
   float total = 0.0F, o0 = 0.0F, o1 = 0.0F;
 #pragma unroll 4
   for (int c = 0; c < count; ++c) {
-    const float *from = src + c * (kD + 2);
-    const float scale = from[0] == -INFINITY ? 0.0F : __builtin_amdgcn_exp2f(from[0] - top);
-    const float2 o = *reinterpret_cast<const float2 *>(from + 2 + 2 * lane);
-    total = fmaf(from[1], scale, total);
+    const float2 from = state[c], o = *reinterpret_cast<const float2 *>(src + c * kD);
+    const float scale = from.x == -INFINITY ? 0.0F : __builtin_amdgcn_exp2f(from.x - top);
+    total = fmaf(from.y, scale, total);
     o0 = fmaf(o.x, scale, o0);
     o1 = fmaf(o.y, scale, o1);
   }
@@ -431,35 +738,42 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const AttendArgs a) 
 }
 
 struct AttendPlan {
-  size_t tiles, prefix_tiles;  // row tiles of the own keys, of the shared ones
+  bool own_stream, prefix_stream;  // 16-row blocks, else 128-row ones
+  size_t tiles, prefix_tiles;      // row tiles of the own keys, of the shared ones
   int chunk, prefix_chunk, prefix_slots, slots;
 };
 
 // Chunks of a launch: enough blocks for a few per CU, chunks of 128 keys and
 // more (32 for each wave), at most 64 of a row.
-int chunk_keys(size_t keys, size_t blocks) {
-  const size_t wanted = std::max<size_t>(1, 2048 / std::max<size_t>(1, blocks));
-  const size_t chunks = std::min<size_t>({wanted, (keys + 127) / 128, 64});
-  return static_cast<int>((keys + chunks * 128 - 1) / (chunks * 128) * 128);
+int chunk_keys(size_t keys, size_t blocks, size_t wanted_blocks, size_t least) {
+  const size_t wanted = std::max<size_t>(1, wanted_blocks / std::max<size_t>(1, blocks));
+  const size_t chunks = std::min<size_t>({wanted, (keys + least - 1) / least, 64});
+  return static_cast<int>((keys + chunks * least - 1) / (chunks * least) * least);
 }
 
 AttendPlan plan_attention(const PagedCache &cache, const PagedBatch &batch, size_t heads) {
-  constexpr size_t kRows = 16;
   const size_t kv = static_cast<size_t>(cache.kv_heads), group = heads / kv;
   const size_t sequences = static_cast<size_t>(batch.sequences);
   const size_t tokens = static_cast<size_t>(batch.tokens);
   const size_t most = static_cast<size_t>(batch.max_tokens) * group;
   AttendPlan plan{};
+  plan.own_stream = most <= 16;
+  plan.prefix_stream = tokens * group <= 16;
+  const size_t rows = plan.own_stream ? 16 : 128;
   // A tile each for the rows that fill one, and one more for each sequence's rest.
-  plan.tiles = std::min(sequences * ((most + kRows - 1) / kRows),
-                        tokens * group / kRows + std::min(sequences, tokens));
-  const size_t own = static_cast<size_t>(batch.max_length - batch.shared_length);
-  plan.chunk = chunk_keys(std::max<size_t>(own, 1), plan.tiles * kv);
-  int own_slots = static_cast<int>((std::max<size_t>(own, 1) + plan.chunk - 1) / plan.chunk);
+  plan.tiles = std::min(sequences * ((most + rows - 1) / rows),
+                        tokens * group / rows + std::min(sequences, tokens));
+  const size_t own = std::max(1, batch.max_length - batch.shared_length);
+  plan.chunk = plan.own_stream ? chunk_keys(own, plan.tiles * kv, 2048, 128)
+                               : chunk_keys(own, plan.tiles * kv, 1024, 512);
+  const int own_slots = static_cast<int>((own + plan.chunk - 1) / plan.chunk);
   if (batch.shared_length > 0) {
     const size_t shared = static_cast<size_t>(batch.shared_length);
-    plan.prefix_tiles = (tokens * group + kRows - 1) / kRows;
-    plan.prefix_chunk = chunk_keys(shared, plan.prefix_tiles * kv);
+    const size_t prefix_rows = plan.prefix_stream ? 16 : 128;
+    plan.prefix_tiles = (tokens * group + prefix_rows - 1) / prefix_rows;
+    plan.prefix_chunk = plan.prefix_stream
+                            ? chunk_keys(shared, plan.prefix_tiles * kv, 2048, 128)
+                            : chunk_keys(shared, plan.prefix_tiles * kv, 1024, 512);
     plan.prefix_slots =
         static_cast<int>((shared + plan.prefix_chunk - 1) / plan.prefix_chunk);
   }
@@ -474,16 +788,40 @@ size_t plan_bytes(const AttendPlan &plan, const PagedCache &cache, const PagedBa
                                (cache.head_dim + 2) * sizeof(float);
 }
 
+// One launch of the blocks of a kind: shared keys first, then own ones.
+template <typename T, int kD>
+Status launch_blocks(const AttendArgs &args, bool stream_kernel, size_t prefix_blocks,
+                     size_t own_blocks, size_t tiles, hipStream_t stream) {
+  if (prefix_blocks + own_blocks == 0)
+    return Status::Ok();
+  if (prefix_blocks + own_blocks >= (size_t{1} << 31))
+    return {ErrorCode::kInvalidArgument, "paged_attention: grid too large"};
+  const dim3 grid(static_cast<unsigned>(prefix_blocks + own_blocks));
+  const unsigned first = static_cast<unsigned>(prefix_blocks);
+  if (stream_kernel) {
+    hipLaunchKernelGGL((paged_stream_kernel<T, kD>), grid, dim3(256), 0, stream, args, first,
+                       static_cast<unsigned>(tiles));
+    return launch_status("paged_stream_kernel");
+  }
+  constexpr size_t kLdsBytes = 2 * 2 * 64 * kD * sizeof(uint16_t);
+  static_assert(kLdsBytes <= 64 * 1024, "default LDS limit, two blocks per CU");
+  hipLaunchKernelGGL((paged_tile_kernel<T, kD>), grid, dim3(256), kLdsBytes, stream, args, first,
+                     static_cast<unsigned>(tiles));
+  return launch_status("paged_tile_kernel");
+}
+
 template <typename T, int kD>
 Status launch_attention(const AttendArgs &args, const AttendPlan &plan, hipStream_t stream) {
   const size_t kv = static_cast<size_t>(args.cache.kv_heads);
   const size_t prefix_blocks = plan.prefix_tiles * kv * plan.prefix_slots;
-  const size_t blocks = prefix_blocks + plan.tiles * kv * (plan.slots - plan.prefix_slots);
-  if (blocks >= (size_t{1} << 31))
-    return {ErrorCode::kInvalidArgument, "paged_attention: grid too large"};
-  hipLaunchKernelGGL((paged_stream_kernel<T, kD>), dim3(static_cast<unsigned>(blocks)), dim3(256),
-                     0, stream, args, static_cast<unsigned>(prefix_blocks));
-  EVO_TRY(launch_status("paged_stream_kernel"));
+  const size_t own_blocks = plan.tiles * kv * (plan.slots - plan.prefix_slots);
+  if (plan.own_stream == plan.prefix_stream || prefix_blocks == 0) {
+    EVO_TRY((launch_blocks<T, kD>(args, plan.own_stream, prefix_blocks, own_blocks, plan.tiles,
+                                  stream)));
+  } else {
+    EVO_TRY((launch_blocks<T, kD>(args, plan.prefix_stream, prefix_blocks, 0, 0, stream)));
+    EVO_TRY((launch_blocks<T, kD>(args, plan.own_stream, 0, own_blocks, plan.tiles, stream)));
+  }
   if (plan.slots == 1)
     return Status::Ok();
   const size_t rows = static_cast<size_t>(args.batch.tokens) * args.heads;
@@ -539,7 +877,10 @@ Status paged_attention(const PagedCache &cache, const PagedBatch &batch, const v
                         static_cast<uint16_t *>(out), out_stride, static_cast<int>(heads),
                         static_cast<int>(heads / kv), 1.4426950408889634F * scale, plan.chunk,
                         plan.prefix_chunk, plan.prefix_slots, plan.slots,
-                        static_cast<float *>(workspace)};
+                        static_cast<float *>(workspace),
+                        reinterpret_cast<float2 *>(static_cast<float *>(workspace) +
+                                                   static_cast<size_t>(batch.tokens) * heads *
+                                                       plan.slots * dim)};
   return cache.dtype == kElementBF16 ? launch_dim<__bf16>(args, plan, stream)
                                      : launch_dim<_Float16>(args, plan, stream);
 }

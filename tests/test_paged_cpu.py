@@ -47,6 +47,7 @@ BAD_CACHES = [dict(struct_size=8), dict(dtype=N.DTYPE_F32), dict(dtype=7), dict(
               dict(page_stride=4096, head_stride=1024, token_stride=60),
               dict(page_stride=4096, head_stride=1024, token_stride=56),
               dict(page_stride=4100, head_stride=1024, token_stride=64),
+              dict(page_stride=4096, head_stride=1024, token_stride=(1 << 24) + 8),
               dict(page_stride=2 ** 62, head_stride=1024, token_stride=64)]
 BAD_BATCHES = [dict(struct_size=0), dict(sequences=0), dict(sequences=(1 << 20) + 1),
                dict(tokens=0), dict(tokens=(1 << 24) + 1), dict(max_tokens=0), dict(max_tokens=7),
