@@ -126,7 +126,36 @@ template <typename T> struct Row {
   float top, reach, bin_scale;
   double unit;  // 64 / (ln 2 * temperature)
   int bins;
+  bool vector;  // the row starts on 16 bytes
   __device__ float at(int i) const { return static_cast<float>(logits[i]); }
+  // f(value, index) over the tokens first .. end - 1 (first a multiple of 8),
+  // 16 bytes a load and four loads ahead where the row is aligned.
+  template <int kThreads, typename F> __device__ void each(int first, int end, F &&f) const {
+    constexpr int kPer = 16 / sizeof(T), kAhead = 4;
+    typedef T wide __attribute__((ext_vector_type(kPer)));
+    int tail = first;
+    if (vector) {
+      const int whole = (end - first) / kPer;
+      const wide *src = reinterpret_cast<const wide *>(logits + first);
+      for (int c0 = threadIdx.x; c0 < whole; c0 += kThreads * kAhead) {
+        wide v[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+          if (c0 + a * kThreads < whole)
+            v[a] = src[c0 + a * kThreads];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+          if (c0 + a * kThreads < whole) {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e)
+              f(static_cast<float>(v[a][e]), first + (c0 + a * kThreads) * kPer + e);
+          }
+      }
+      tail = first + whole * kPer;
+    }
+    for (int i = tail + threadIdx.x; i < end; i += kThreads)
+      f(at(i), i);
+  }
   // Bin of a value, -1 for one without weight. Every step is monotonic.
   __device__ int bin(float v) const {
     const float below = top - v;
@@ -217,18 +246,17 @@ __device__ inline void find_in_bin(const Row<T> &row, SampleShared<kThreads, kBi
       s.sub_mass[i] = 0;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < row.vocab; i += kThreads) {
-      const float v = row.at(i);
+    row.template each<kThreads>(0, row.vocab, [&](float v, int i) {
       if (row.bin(v) != bin)
-        continue;
+        return;
       const uint64_t p = place(v, i);
       if (p >> (shift + 8) != prefix)
-        continue;
+        return;
       const int digit = 255 - static_cast<int>((p >> shift) & 255);  // earlier first
       atomicAdd(&s.sub_count[digit], 1U);
       atomicAdd(reinterpret_cast<unsigned long long *>(&s.sub_mass[digit]),
                 static_cast<unsigned long long>(row.weight(v, s.powers)));
-    }
+    });
     __syncthreads();
     scan_bins<kThreads>(s.sub_count, s.sub_mass, 256, s.wave_count, s.wave_mass);
     // Equal entries: the last of them is the one with tokens behind it.
@@ -245,17 +273,16 @@ __device__ inline void find_in_bin(const Row<T> &row, SampleShared<kThreads, kBi
   if (threadIdx.x == 0)
     s.fill = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < row.vocab; i += kThreads) {
-    const float v = row.at(i);
+  row.template each<kThreads>(0, row.vocab, [&](float v, int i) {
     if (row.bin(v) != bin)
-      continue;
+      return;
     const uint64_t p = place(v, i);
     if (p >> shift != prefix)
-      continue;
+      return;
     const uint32_t slot = atomicAdd(&s.fill, 1U);
     s.list_place[slot] = p;
     s.list_mass[slot] = row.weight(v, s.powers);
-  }
+  });
   __syncthreads();
   // Rank by comparison: the one token whose range holds the target.
   const uint32_t size = s.fill;
@@ -290,6 +317,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a) {
   Row<T> row;
   row.logits = static_cast<const T *>(a.logits) + r * a.row_stride;
   row.vocab = a.vocab;
+  row.vector = reinterpret_cast<uintptr_t>(row.logits) % 16 == 0;
   row.bins = kBins;
   const float temperature = a.temperature == nullptr ? 1.0F : a.temperature[r];
   const int top_k = a.top_k == nullptr ? 0 : a.top_k[r];
@@ -306,12 +334,11 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a) {
 
   float top = -INFINITY, low = INFINITY;
   int bad = 0;
-  for (int i = threadIdx.x; i < a.vocab; i += kThreads) {
-    const float v = row.at(i);
+  row.template each<kThreads>(0, a.vocab, [&](float v, int) {
     bad |= !(v < INFINITY);
     top = fmaxf(top, v);
     low = v > -INFINITY ? fminf(low, v) : low;
-  }
+  });
   const auto most = [](float x, float y) { return fmaxf(x, y); };
   const auto least = [](float x, float y) { return fminf(x, y); };
   top = block_reduce<kThreads>(top, scratch_f, most);
@@ -326,9 +353,10 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a) {
   }
   if (temperature == 0.0F || top_k == 1) {
     int first = a.vocab;
-    for (int i = threadIdx.x; i < a.vocab; i += kThreads)
-      if (row.at(i) == top)
+    row.template each<kThreads>(0, a.vocab, [&](float v, int i) {
+      if (v == top)
         first = min(first, i);
+    });
     first = block_reduce<kThreads>(first, scratch_i, [](int x, int y) { return min(x, y); });
     if (threadIdx.x == 0)
       a.tokens[r] = static_cast<uint32_t>(first);
@@ -344,17 +372,16 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a) {
   // of the order too, as the weight falls along it).
   const double least_weight = static_cast<double>(min_p) * 4398046511104.0;
   uint64_t kept = 0;
-  for (int i = threadIdx.x; i < a.vocab; i += kThreads) {
-    const float v = row.at(i);
+  row.template each<kThreads>(0, a.vocab, [&](float v, int) {
     const int bin = row.bin(v);
     if (bin < 0)
-      continue;
+      return;
     const uint64_t w = row.weight(v, s.powers);
     atomicAdd(&s.count[bin], 1U);
     atomicAdd(reinterpret_cast<unsigned long long *>(&s.mass[bin]),
               static_cast<unsigned long long>(w));
     kept += static_cast<double>(w) >= least_weight ? w : 0;
-  }
+  });
   kept = block_reduce<kThreads>(kept, scratch_u, [](uint64_t x, uint64_t y) { return x + y; });
   __syncthreads();
   uint32_t total_count = 0;
