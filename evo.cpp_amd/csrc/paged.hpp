@@ -56,6 +56,10 @@ __host__ __device__ inline SequenceRows sequence_rows(const PagedBatch &batch, i
 // The sequence that owns row `token`, or -1. token_start is searched as if it
 // ascended; the answer is checked, so an unordered array gives -1 at worst.
 __host__ __device__ inline int sequence_of(const PagedBatch &batch, int token) {
+  // Row i of sequence i: a decode step.
+  const int same = token < 0 ? 0 : token < batch.sequences ? token : batch.sequences - 1;
+  if (batch.token_start[same] <= token && token < batch.token_start[same + 1])
+    return same;
   int low = 0, high = batch.sequences;  // the answer lies in [low, high)
   while (high - low > 1) {
     const int middle = low + (high - low) / 2;

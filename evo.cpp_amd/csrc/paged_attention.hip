@@ -44,6 +44,7 @@ struct AttendArgs {
   int prefix_chunk;   // shared keys per chunk
   int prefix_slots;   // chunks of the shared keys
   int slots;          // chunks of a row at most, the shared ones first
+  int direct;         // a row tile is a sequence
   float *part;        // [tokens][heads][slots][head_dim], unnormalised outputs
   float2 *state;      // [tokens][heads][slots] (maximum, sum)
 };
@@ -89,10 +90,15 @@ template <typename T> __device__ inline uint16_t bits_of(float v) {
   return __builtin_bit_cast(uint16_t, static_cast<T>(v));
 }
 
-// Chunks of a row at `position` (-1 and below: it sees nothing).
+// Chunks of own keys of a row at `position` (-1 and below: it sees nothing).
 __device__ inline int own_chunks(const AttendArgs &a, int position) {
   const int keys = position + 1 - a.batch.shared_length;
   return keys <= 0 ? 0 : (keys + a.chunk - 1) / a.chunk;
+}
+// Whether a row is finished by the block of its first chunk, not joined: it has
+// no other.
+__device__ inline bool single_chunk(const AttendArgs &a, int position) {
+  return a.prefix_slots == 0 && position < a.chunk;
 }
 
 // Row tile `tile` of the batch's own-key phase: the tiles of its sequences in
@@ -139,11 +145,13 @@ __device__ inline bool row_tile(const AttendArgs &a, bool prefix, int tile, RowT
           a.batch.shared_length - 1};
     return true;
   }
-  int sequence, tile_in;
-  if (!find_tile<kRows>(a, tile, &sequence, &tile_in))
+  int sequence = tile, tile_in = 0;
+  if (!a.direct && !find_tile<kRows>(a, tile, &sequence, &tile_in))
     return false;
   sequence = __builtin_amdgcn_readfirstlane(sequence);
   const SequenceRows own = sequence_rows(a.batch, sequence);
+  if (!own.valid || own.count == 0)
+    return false;
   const int row0 = __builtin_amdgcn_readfirstlane(tile_in) * kRows;
   const int rows = own.count * a.group, position = own.length - own.count;
   *t = {sequence, row0, rows, own.first, position + row0 / a.group,
@@ -173,6 +181,9 @@ __device__ inline BlockWork block_work(const AttendArgs &a, unsigned prefix_bloc
   return w;
 }
 
+// A weight may exceed the running maximum's by 2^8 before the maximum follows.
+constexpr float kSlack = 8.0F;
+
 // Softmax state and output of 16 rows over the keys a wave has seen. Lane l:
 // row l % 16, output elements kVec * (4 * (l / 16) + i) + t for i < 4, t < kVec.
 template <int kD> struct RowState {
@@ -182,12 +193,10 @@ template <int kD> struct RowState {
 };
 
 // One 32-key step. k[u][s]: K operand of keys 16u .., elements 32s ..; v[j]: this
-// lane's 8 keys, kVec elements each.
+// lane's 8 keys, kD / 16 elements each.
 template <typename T, int kD> struct Step {
-  static constexpr int kVec = kD / 16, kSteps = kD / 32;
-  typedef typename Mfma<T>::vec vec;
-  vec k[2][kSteps];
-  uint32_t v[8][kVec / 2];
+  typename Mfma<T>::vec k[2][kD / 32];
+  uint32_t v[8][kD / 32];
 };
 
 template <int kWords>
@@ -203,64 +212,55 @@ __device__ inline void load_words(const uint16_t *src, uint32_t (&w)[kWords]) {
   }
 }
 
-// Loads the keys k0 .. k0 + 31 (pages page[0], page[1] of 16 each; -1: none, the
-// registers are zeroed). k0 is a multiple of 16, so 16 keys share a page.
+// K and V of 16 keys from k0 (a multiple of 16) in page `page`: the keys share it.
 template <typename T, int kD>
-__device__ inline void load_step(const AttendArgs &a, int kv_head, int k0, const int (&page)[2],
-                                 Step<T, kD> &step) {
-  using S = Step<T, kD>;
-  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-  const int mask = (1 << a.cache.page_shift) - 1;
+__device__ inline void load_keys(const AttendArgs &a, int kv_head, int k0, int page,
+                                 typename Mfma<T>::vec (&k)[kD / 32]) {
+  const int lane = threadIdx.x & 63;
+  const uint16_t *base = a.cache.keys + (page * a.cache.page_stride +
+                                         kv_head * a.cache.head_stride +
+                                         (k0 & ((1 << a.cache.page_shift) - 1)) *
+                                             a.cache.token_stride);
+  const uint32_t offset =
+      (lane & 15) * static_cast<uint32_t>(a.cache.token_stride) + 8 * (lane >> 4);
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    if (page[u] < 0) {
+  for (int s = 0; s < kD / 32; ++s)
+    k[s] = *reinterpret_cast<const typename Mfma<T>::vec *>(base + offset + 32 * s);
+}
+template <int kD>
+__device__ inline void load_values(const AttendArgs &a, int kv_head, int k0, int page,
+                                   uint32_t (*v)[kD / 32]) {
+  const int lane = threadIdx.x & 63;
+  const uint16_t *base = a.cache.values + (page * a.cache.page_stride +
+                                           kv_head * a.cache.head_stride +
+                                           (k0 & ((1 << a.cache.page_shift) - 1)) *
+                                               a.cache.token_stride);
+  const uint32_t stride = static_cast<uint32_t>(a.cache.token_stride);
+  const uint32_t offset = 4 * (lane >> 4) * stride + kD / 16 * (lane & 15);
 #pragma unroll
-      for (int s = 0; s < S::kSteps; ++s)
-        step.k[u][s] = typename S::vec{};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int w = 0; w < S::kVec / 2; ++w)
-          step.v[4 * u + i][w] = 0;
-      continue;
-    }
-    const size_t base = page[u] * a.cache.page_stride + kv_head * a.cache.head_stride +
-                        ((k0 + 16 * u) & mask) * a.cache.token_stride;
-    const uint16_t *k = a.cache.keys + base + col * a.cache.token_stride + 8 * g;
-#pragma unroll
-    for (int s = 0; s < S::kSteps; ++s)
-      step.k[u][s] = *reinterpret_cast<const typename S::vec *>(k + 32 * s);
-    const uint16_t *v = a.cache.values + base + 4 * g * a.cache.token_stride + S::kVec * col;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      load_words(v + i * a.cache.token_stride, step.v[4 * u + i]);
-  }
+  for (int i = 0; i < 4; ++i)
+    load_words(base + offset + i * stride, v[i]);
 }
 
-// Adds a step's keys to 16 rows. visible: keys of the step this lane's row sees
-// (of each 16: its number may be over 16 or below 0); limit: keys of the step that
-// any row sees, whose values alone may be read.
+// S^T of a step for 16 rows: entry i of score[u] is key 16u + 4 * (lane / 16) + i.
 template <typename T, int kD>
-__device__ inline void attend(const Step<T, kD> &step, const typename Mfma<T>::vec *q,
-                              float scale2, bool masked, const int (&visible)[2],
-                              RowState<kD> &state) {
-  using S = Step<T, kD>;
-  const int g = (threadIdx.x & 63) >> 4;
-  f32x4 score[2];
+__device__ inline void scores(const Step<T, kD> &step, const typename Mfma<T>::vec *q,
+                              f32x4 (&score)[2]) {
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     score[u] = f32x4{0.0F, 0.0F, 0.0F, 0.0F};
 #pragma unroll
-    for (int s = 0; s < S::kSteps; ++s)
+    for (int s = 0; s < kD / 32; ++s)
       score[u] = Mfma<T>::run(step.k[u][s], q[s], score[u]);
   }
-  if (masked) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        score[u][i] = 4 * g + i < visible[u] ? score[u][i] : -INFINITY;
-  }
+}
+
+// Adds a step's scores and values to the rows' state.
+template <typename T, int kD>
+__device__ inline void attend(const f32x4 (&score)[2], const uint32_t (&v)[8][kD / 32],
+                              float scale2, RowState<kD> &state) {
+  constexpr int kVec = kD / 16;
+  typedef typename Mfma<T>::vec vec;
   float top = -INFINITY;
 #pragma unroll
   for (int u = 0; u < 2; ++u)
@@ -269,57 +269,68 @@ __device__ inline void attend(const Step<T, kD> &step, const typename Mfma<T>::v
       top = fmaxf(top, score[u][i]);
   top = fmaxf(top, __shfl_xor(top, 16, 64));
   top = fmaxf(top, __shfl_xor(top, 32, 64)) * scale2;
-  const float next = fmaxf(state.top, top);
-  if (__any(next != state.top)) {
+  if (__any(top > state.top + kSlack)) {
+    const float next = fmaxf(state.top, top);
     const float shrink = next == -INFINITY ? 1.0F : __builtin_amdgcn_exp2f(state.top - next);
     state.sum *= shrink;
 #pragma unroll
-    for (int t = 0; t < S::kVec; ++t)
+    for (int t = 0; t < kVec; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         state.out[t][i] *= shrink;
     state.top = next;
   }
-  const float base = next == -INFINITY ? 0.0F : next;
-  typename S::vec p;
+  const float base = state.top == -INFINITY ? 0.0F : state.top;
+  vec p;
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const T w = static_cast<T>(__builtin_amdgcn_exp2f(fmaf(score[u][i], scale2, -base)));
-      p[4 * u + i] = w;
-      state.sum += static_cast<float>(w);
-    }
+    for (int i = 0; i < 4; ++i)
+      p[4 * u + i] =
+          static_cast<T>(__builtin_amdgcn_exp2f(fmaf(score[u][i], scale2, -base)));
+  state.sum = Mfma<T>::add(p, state.sum);
 #pragma unroll
-  for (int t = 0; t < S::kVec; ++t) {
+  for (int t = 0; t < kVec; ++t) {
     // Element t of this lane's kVec of each of its 8 keys.
     uint32_t word[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      word[j] = __builtin_amdgcn_perm(step.v[2 * j + 1][t / 2], step.v[2 * j][t / 2],
+      word[j] = __builtin_amdgcn_perm(v[2 * j + 1][t / 2], v[2 * j][t / 2],
                                       t % 2 == 0 ? 0x05040100U : 0x07060302U);
-    state.out[t] = Mfma<T>::run(__builtin_bit_cast(typename S::vec, word), p, state.out[t]);
+    state.out[t] = Mfma<T>::run(__builtin_bit_cast(vec, word), p, state.out[t]);
   }
 }
 
 // 16 rows of a key/value head and a chunk of their keys per block; its four
 // waves take every fourth 32-key step and join their states through LDS.
 // Blocks below prefix_blocks take the shared keys, rows of the whole batch.
+template <int kD> struct StreamShared {
+  float top[4][16], sum[4][16];
+  __attribute__((aligned(16))) float out[4][16][kD + 4];
+};
 template <typename T, int kD>
-__global__ __launch_bounds__(256) void paged_stream_kernel(const AttendArgs a,
-                                                           unsigned prefix_blocks,
-                                                           unsigned tiles) {
+__device__ inline void stream_block(const AttendArgs &a, const BlockWork &work,
+                                    StreamShared<kD> &shared) {
   constexpr int kRows = 16, kWaves = 4, kVec = kD / 16, kSteps = kD / 32;
   typedef typename Mfma<T>::vec vec;
-  __shared__ float top_s[kWaves][kRows], sum_s[kWaves][kRows];
-  __shared__ __attribute__((aligned(16))) float out_s[kWaves][kRows][kD + 4];
+  auto &top_s = shared.top, &sum_s = shared.sum;
+  auto &out_s = shared.out;
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (blockIdx.x == prefix_blocks)
-    report_bad_sequences(a.batch);
-  const BlockWork work = block_work(a, prefix_blocks, tiles);
   const bool prefix = work.prefix;
   const int kv_head = work.kv_head, chunk = work.chunk;
+  const int key0 = prefix ? chunk * a.prefix_chunk : a.batch.shared_length + chunk * a.chunk;
+  int k0 = key0 + 32 * wave;
+  // The first step's table entries, requested beside the rows' own description
+  // where the table's row is known without it.
+  const bool early = prefix || a.direct;
+  int entries = -1;
+  if (early && lane < 2 &&
+      k0 + 16 * lane < (prefix ? a.batch.shared_length : a.batch.max_length)) {
+    const int32_t *row = prefix ? a.batch.shared_table
+                                : a.batch.page_table + work.tile * a.batch.table_stride;
+    entries = row[(k0 + 16 * lane) >> a.cache.page_shift];
+  }
   RowTile tile;
   if (!row_tile<kRows>(a, prefix, work.tile, &tile))
     return;
@@ -331,9 +342,9 @@ __global__ __launch_bounds__(256) void paged_stream_kernel(const AttendArgs a,
   const int position =
       prefix ? tile.last_position : tile.first_position + token_in - tile.row0 / a.group;
 
-  const int key0 = prefix ? chunk * a.prefix_chunk : a.batch.shared_length + chunk * a.chunk;
+  // (The first chunk of a sequence without keys goes on: its rows are zero.)
   const int key1 = min(tile.last_position + 1, key0 + (prefix ? a.prefix_chunk : a.chunk));
-  if (key0 >= key1 && (prefix || chunk > 0 || a.slots > 1))
+  if (key0 >= key1 && (prefix || chunk > 0))
     return;
 
   vec q[kSteps];
@@ -353,38 +364,68 @@ __global__ __launch_bounds__(256) void paged_stream_kernel(const AttendArgs a,
 
   const int32_t *table = prefix ? a.batch.shared_table
                                 : a.batch.page_table + tile.sequence * a.batch.table_stride;
-  for (int k0 = key0 + 32 * wave; k0 < key1; k0 += 32 * kWaves) {
-    int page[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      page[u] = -1;
-      if (k0 + 16 * u < key1) {
-        page[u] = checked_page(table, (k0 + 16 * u) >> a.cache.page_shift, a.cache.pages);
-        if (page[u] < 0 && lane == 0)
-          report(a.batch, kBadPage);
-      }
-      page[u] = __builtin_amdgcn_readfirstlane(page[u]);
-    }
+  // Pages of a step's two 16-key groups in lanes 0 and 1 (-1: none).
+  auto entries_at = [&](int k) {
+    const int key = k + 16 * lane;
+    return lane < 2 && key < key1 ? table[key >> a.cache.page_shift] : -1;
+  };
+  auto pages_of = [&](int entry, int k) {
+    const bool needed = lane < 2 && k + 16 * lane < key1;
+    const bool good = needed && entry >= 0 && entry < a.cache.pages;
+    if (needed && !good)
+      report(a.batch, kBadPage);
+    return good ? entry : -1;
+  };
+  // V of a step is requested before its scores, K of the next one as soon as the
+  // scores are done and the page after that with it, so that loads are always in
+  // flight with one set of registers. Without a page the loads go to page 0.
+  constexpr int kStride = 32 * kWaves;
+  if (k0 < key1) {
+    int pages = pages_of(early ? entries : entries_at(k0), k0);
+    int page[2] = {__builtin_amdgcn_readlane(pages, 0), __builtin_amdgcn_readlane(pages, 1)};
     Step<T, kD> step;
-    load_step<T, kD>(a, kv_head, k0, page, step);
-    const bool masked = page[0] < 0 || page[1] < 0 || k0 + 31 > tile.first_position || k0 + 32 > key1;
-    int visible[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int from = k0 + 16 * u;
-      visible[u] = page[u] < 0 ? 0 : min(position + 1, key1) - from;
-      // Values no row of the tile sees may be anything, and 0 * NaN is NaN.
-      if (masked && from + 16 > key1) {
+    for (int u = 0; u < 2; ++u)
+      load_keys<T, kD>(a, kv_head, k0 + 16 * u, max(page[u], 0), step.k[u]);
+    entries = entries_at(k0 + kStride);
+    for (;;) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (from + 4 * g + i >= key1) {
+      for (int u = 0; u < 2; ++u)
+        load_values<kD>(a, kv_head, k0 + 16 * u, max(page[u], 0), step.v + 4 * u);
+      f32x4 score[2];
+      scores<T, kD>(step, q, score);
+      const int here[2] = {page[0], page[1]}, k_here = k0;
+      k0 += kStride;
+      const bool more = k0 < key1;
+      if (more) {
+        pages = pages_of(entries, k0);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          page[u] = __builtin_amdgcn_readlane(pages, u);
+          load_keys<T, kD>(a, kv_head, k0 + 16 * u, max(page[u], 0), step.k[u]);
+        }
+        entries = entries_at(k0 + kStride);
+      }
+      if (here[0] < 0 || here[1] < 0 || k_here + 31 > tile.first_position ||
+          k_here + 32 > key1) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int from = k_here + 16 * u + 4 * g;
+          const int end = here[u] < 0 ? 0 : key1, visible = min(position + 1, end);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            score[u][i] = from + i < visible ? score[u][i] : -INFINITY;
+            // Values no row of the tile sees may be anything, and 0 * NaN is NaN.
 #pragma unroll
             for (int w = 0; w < kVec / 2; ++w)
-              step.v[4 * u + i][w] = 0;
+              step.v[4 * u + i][w] = from + i < end ? step.v[4 * u + i][w] : 0;
           }
+        }
       }
+      attend<T, kD>(score, step.v, a.scale2, state);
+      if (!more)
+        break;
     }
-    attend<T, kD>(step, q, a.scale2, masked, visible, state);
   }
 
   // Join the four waves: each leaves its rows' maximum, sum and output.
@@ -418,17 +459,32 @@ __global__ __launch_bounds__(256) void paged_stream_kernel(const AttendArgs a,
     for (int e = 0; e < kVec; ++e)
       o[e] = fmaf(out_s[w][r][d + e], scale, o[e]);
   }
-  const size_t out_token = tile.first_token + (tile.row0 + r) / a.group;
-  const int out_head = kv_head * a.group + (tile.row0 + r) % a.group;
-  if (a.slots == 1) {
-    // The row's only chunk. A row without keys is zero.
+  const int out_row = tile.row0 + r;
+  const size_t out_token = tile.first_token + out_row / a.group;
+  const int out_head = kv_head * a.group + out_row % a.group;
+  const int out_position =
+      prefix ? tile.last_position
+             : tile.first_position + out_row / a.group - tile.row0 / a.group;
+  if (!prefix && single_chunk(a, out_position)) {
+    if (chunk > 0)
+      return;
+    // A row without keys is zero.
     const float inverse = total > 0.0F ? 1.0F / total : total == 0.0F ? 0.0F : total;
     uint16_t *dst = a.out + out_token * a.out_stride + out_head * kD + d;
+    uint16_t bits[kVec];
 #pragma unroll
     for (int e = 0; e < kVec; ++e)
-      dst[e] = bits_of<T>(o[e] * inverse);
+      bits[e] = bits_of<T>(o[e] * inverse);
+    if constexpr (kVec == 8)
+      *reinterpret_cast<uint4 *>(dst) = __builtin_bit_cast(uint4, bits);
+    else if constexpr (kVec == 4)
+      *reinterpret_cast<uint2 *>(dst) = __builtin_bit_cast(uint2, bits);
+    else
+      *reinterpret_cast<uint32_t *>(dst) = __builtin_bit_cast(uint32_t, bits);
     return;
   }
+  if (key0 > out_position)
+    return;  // no key of the chunk is the row's, and no one reads its slot
   const size_t slot = (out_token * a.heads + out_head) * a.slots +
                       (prefix ? chunk : a.prefix_slots + chunk);
   if (d == 0)
@@ -463,26 +519,18 @@ template <typename Q> __device__ inline Q transposed(const uint16_t *from) {
   return __builtin_bit_cast(Q, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(from)));
 }
 
-// A weight may exceed the running maximum's by 2^8 before the maximum follows.
-constexpr float kSlack = 8.0F;
-
 template <typename T, int kD>
-__global__ __launch_bounds__(256, 2) void paged_tile_kernel(const AttendArgs a,
-                                                            unsigned prefix_blocks,
-                                                            unsigned tiles) {
+__device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
+                                  uint16_t *tile_lds) {  // [2][K, V][plane]
   constexpr int kRows = 128, kKeys = 64, kUnits = kD / 8;
   constexpr int kSteps = kD / 16, kTiles = kD / 32;   // K-steps of S^T, 32-row tiles of O^T
   constexpr int kPlane = kKeys * kD;                  // elements of K or V in a stage
   constexpr int kOps = kD / 32;                       // DMAs of 16 keys
   constexpr int kOpRows = 512 / kD;                   // keys of a DMA
   typedef typename Mfma<T>::vec vec;
-  extern __shared__ __attribute__((aligned(16))) uint16_t tile_lds[];  // [2][K, V][plane]
 
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (blockIdx.x == prefix_blocks)
-    report_bad_sequences(a.batch);
-  const BlockWork work = block_work(a, prefix_blocks, tiles);
   const bool prefix = work.prefix;
   RowTile tile;
   if (!row_tile<kRows>(a, prefix, work.tile, &tile))
@@ -508,7 +556,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const AttendArgs a,
   const int key0 = prefix ? work.chunk * a.prefix_chunk
                           : a.batch.shared_length + work.chunk * a.chunk;
   const int key1 = min(tile.last_position + 1, key0 + (prefix ? a.prefix_chunk : a.chunk));
-  if (key0 >= key1 && (prefix || work.chunk > 0 || a.slots > 1))
+  if (key0 >= key1 && (prefix || work.chunk > 0))
     return;
 
   vec q[kSteps];
@@ -668,8 +716,10 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const AttendArgs a,
   if (!active)
     return;
   // Entry e of tile t: element 32t + 8 * (e / 4) + 4 half + e % 4 of row `row`.
-  if (a.slots == 1) {
-    // The row's only chunk. A row without keys is zero.
+  if (!prefix && single_chunk(a, position)) {
+    if (work.chunk > 0)
+      return;
+    // A row without keys is zero.
     const float inverse = total > 0.0F ? 1.0F / total : total == 0.0F ? 0.0F : total;
     uint16_t *dst = a.out + token * a.out_stride + head * kD + 4 * half;
 #pragma unroll
@@ -684,6 +734,8 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const AttendArgs a,
       }
     return;
   }
+  if (key0 > position)
+    return;  // no key of the chunk is the row's, and no one reads its slot
   const size_t slot =
       (token * a.heads + head) * a.slots + (prefix ? work.chunk : a.prefix_slots + work.chunk);
   if (half == 0)
@@ -697,44 +749,129 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const AttendArgs a,
           make_float4(out[t][e], out[t][e + 1], out[t][e + 2], out[t][e + 3]);
 }
 
-// Rows whose keys lay in several chunks: a wave per row and head rescales the
-// chunks to their common maximum and sums them in order, two elements a lane.
-template <typename T, int kD>
-__global__ __launch_bounds__(256) void paged_combine_kernel(const AttendArgs a) {
-  const size_t index = blockIdx.x * 4ULL + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (index >= static_cast<size_t>(a.batch.tokens) * a.heads)
-    return;
-  const int token = static_cast<int>(index / a.heads), head = static_cast<int>(index % a.heads);
+// ------------------------------------------------------------- launches
+constexpr size_t kTileLds = 2 * 2 * 64 * sizeof(uint16_t);  // per element of a head
+static_assert(kTileLds * 128 <= 64 * 1024, "default LDS limit, two blocks per CU");
+
+// kKind 0: 16-row blocks; 1: 128-row blocks; 2: 128-row blocks on the shared keys
+// beside 16-row ones on each sequence's own, in one launch.
+template <typename T, int kD, int kKind>
+__global__ __launch_bounds__(256, kKind == 0 ? 3 : 2) void paged_attention_kernel(
+    const AttendArgs a, unsigned prefix_blocks, unsigned tiles) {
+  extern __shared__ __attribute__((aligned(16))) uint16_t attend_lds[];
+  if (blockIdx.x == prefix_blocks)
+    report_bad_sequences(a.batch);
+  const BlockWork work = block_work(a, prefix_blocks, tiles);
+  if (kKind == 1 || (kKind == 2 && work.prefix))
+    tile_block<T, kD>(a, work, attend_lds);
+  else
+    stream_block<T, kD>(a, work, *reinterpret_cast<StreamShared<kD> *>(attend_lds));
+}
+
+// Rows whose keys lay in several chunks: the chunks rescaled to their common
+// maximum and summed in a fixed order. A wave's lanes hold four elements of a row
+// each, its groups of kD / 4 lanes every kGroups-th chunk, and lane l the states of
+// chunks l, 64 + l, .. (256 at most). kSplit: a block per row and head, its four
+// waves sharing the chunks; else a block takes `heads` heads of one row, a wave
+// every fourth of them, so that a batch of many rows looks a row up once.
+template <typename T, int kD, bool kSplit>
+__global__ __launch_bounds__(256) void paged_combine_kernel(const AttendArgs a, int heads) {
+  constexpr int kLanes = kD / 4, kGroups = 64 / kLanes, kStates = kSplit ? 4 : 1;
+  constexpr int kWaves = kSplit ? 4 : 1;  // of a row and head
+  __shared__ float4 out_s[4][kLanes];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int head_blocks = (a.heads + heads - 1) / heads;
+  const int token = static_cast<int>(blockIdx.x / head_blocks);
+  const int head0 = static_cast<int>(blockIdx.x % head_blocks) * heads;
+  const int sub = kSplit ? wave : 0, group = lane / kLanes, l = lane % kLanes;
   const int sequence = sequence_of(a.batch, token);
   if (sequence < 0)
     return;
   const SequenceRows rows = sequence_rows(a.batch, sequence);
-  if (!rows.valid || lane >= kD / 2)
-    return;
   const int position = rows.length - rows.count + token - rows.first;
-  const int own = own_chunks(a, position);
-  // (Own keys and shared ones: a row behind the prefix has both, a padding row
-  // neither.)
-  const int count = position < 0 ? 0 : a.prefix_slots + own;
-  const float *src = a.part + index * a.slots * kD + 2 * lane;
-  const float2 *state = a.state + index * a.slots;
-  float top = -INFINITY;
-  for (int c = 0; c < count; ++c)
-    top = fmaxf(top, state[c].x);
-  float total = 0.0F, o0 = 0.0F, o1 = 0.0F;
-#pragma unroll 4
-  for (int c = 0; c < count; ++c) {
-    const float2 from = state[c], o = *reinterpret_cast<const float2 *>(src + c * kD);
-    const float scale = from.x == -INFINITY ? 0.0F : __builtin_amdgcn_exp2f(from.x - top);
-    total = fmaf(from.y, scale, total);
-    o0 = fmaf(o.x, scale, o0);
-    o1 = fmaf(o.y, scale, o1);
+  if (!rows.valid || single_chunk(a, position))
+    return;
+  // (A row behind the prefix sees it all, a padding row nothing.)
+  const int count = position < 0 ? 0 : a.prefix_slots + own_chunks(a, position);
+  for (int head = head0 + (kSplit ? 0 : wave); head < min(a.heads, head0 + heads);
+       head += kSplit ? 1 : 4) {
+    const size_t at = static_cast<size_t>(token) * a.heads + head;
+    const float *src = a.part + at * a.slots * kD + 4 * l;
+    float top[kStates], total = 0.0F, all = -INFINITY;
+    float part_sum[kStates];
+#pragma unroll
+    for (int i = 0; i < kStates; ++i) {
+      const bool has = 64 * i + lane < count;
+      const float2 s = has ? a.state[at * a.slots + 64 * i + lane] : make_float2(-INFINITY, 0.0F);
+      top[i] = s.x;
+      part_sum[i] = s.y;
+      all = fmaxf(all, top[i]);
+    }
+#pragma unroll
+    for (int offset = 32; offset > 0; offset >>= 1)
+      all = fmaxf(all, __shfl_xor(all, offset, 64));
+#pragma unroll
+    for (int i = 0; i < kStates; ++i) {
+      // (A chunk without visible keys has no weight.)
+      top[i] = top[i] == -INFINITY ? 0.0F : __builtin_amdgcn_exp2f(top[i] - all);
+      total = fmaf(part_sum[i], top[i], total);
+    }
+#pragma unroll
+    for (int offset = 32; offset > 0; offset >>= 1)
+      total += __shfl_xor(total, offset, 64);
+    float4 o = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+#pragma unroll
+    for (int i = 0; i < kStates; ++i) {
+      const int end = min(64, count - 64 * i);
+      for (int c0 = kGroups * sub; c0 < end; c0 += 4 * kGroups * kWaves) {
+        float scale[4];
+        float4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int c = c0 + kGroups * kWaves * u + group;
+          scale[u] = __shfl(top[i], c & 63, 64);
+          v[u] = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+          if (c < end)
+            v[u] = *reinterpret_cast<const float4 *>(src + (64 * i + c) * kD);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          o.x = fmaf(v[u].x, scale[u], o.x);
+          o.y = fmaf(v[u].y, scale[u], o.y);
+          o.z = fmaf(v[u].z, scale[u], o.z);
+          o.w = fmaf(v[u].w, scale[u], o.w);
+        }
+      }
+    }
+#pragma unroll
+    for (int offset = kLanes; offset < 64; offset <<= 1) {
+      o.x += __shfl_xor(o.x, offset, 64);
+      o.y += __shfl_xor(o.y, offset, 64);
+      o.z += __shfl_xor(o.z, offset, 64);
+      o.w += __shfl_xor(o.w, offset, 64);
+    }
+    if constexpr (kSplit) {
+      if (lane < kLanes)
+        out_s[wave][l] = o;
+      __syncthreads();
+      if (wave != 0)
+        return;
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) {
+        const float4 v = out_s[w][l];
+        o.x += v.x;
+        o.y += v.y;
+        o.z += v.z;
+        o.w += v.w;
+      }
+    }
+    const float inverse = total > 0.0F ? 1.0F / total : total == 0.0F ? 0.0F : total;
+    const uint16_t bits[4] = {bits_of<T>(o.x * inverse), bits_of<T>(o.y * inverse),
+                              bits_of<T>(o.z * inverse), bits_of<T>(o.w * inverse)};
+    if (lane < kLanes)
+      *reinterpret_cast<uint2 *>(a.out + token * a.out_stride + head * kD + 4 * l) =
+          __builtin_bit_cast(uint2, bits);
   }
-  const float inverse = total > 0.0F ? 1.0F / total : total == 0.0F ? 0.0F : total;
-  uint16_t *dst = a.out + token * a.out_stride + head * kD + 2 * lane;
-  dst[0] = bits_of<T>(o0 * inverse);
-  dst[1] = bits_of<T>(o1 * inverse);
 }
 
 struct AttendPlan {
@@ -742,38 +879,106 @@ struct AttendPlan {
   size_t tiles, prefix_tiles;      // row tiles of the own keys, of the shared ones
   int chunk, prefix_chunk, prefix_slots, slots;
 };
+constexpr size_t kMostSlots = 128;  // of each phase (256 in the combining kernel)
 
-// Chunks of a launch: enough blocks for a few per CU, chunks of 128 keys and
-// more (32 for each wave), at most 64 of a row.
-int chunk_keys(size_t keys, size_t blocks, size_t wanted_blocks, size_t least) {
-  const size_t wanted = std::max<size_t>(1, wanted_blocks / std::max<size_t>(1, blocks));
-  const size_t chunks = std::min<size_t>({wanted, (keys + least - 1) / least, 64});
-  return static_cast<int>((keys + chunks * least - 1) / (chunks * least) * least);
+int chunk_of(size_t keys, size_t chunks, size_t granule) {
+  return static_cast<int>((keys + chunks * granule - 1) / (chunks * granule) * granule);
+}
+
+// Keys per block of the 16-row kernel: enough blocks that the last ones to run do
+// not show, chunks of 128 keys (32 for each wave) and more.
+int stream_chunk(size_t keys, size_t blocks) {
+  const size_t wanted = std::max<size_t>(1, 8192 / std::max<size_t>(1, blocks));
+  return chunk_of(keys, std::min<size_t>({wanted, (keys + 127) / 128, kMostSlots}), 128);
+}
+
+// The 128-row blocks of a phase: `tiles` of them see `least` .. `most` keys each,
+// evenly spread, and all together read kv_bytes of keys and values and leave a part
+// of part_bytes in each chunk.
+struct TilePhase {
+  size_t tiles, least, most;
+  double other_keys;  // keys of further blocks, all together
+  double kv_bytes, part_bytes;
+};
+
+// Keys per block: the split of least modelled time. 64 keys of head_dim 128 take a
+// block 2.17 us where two share a CU and 1.3 alone; up to three rounds of 512
+// blocks are counted whole. Keys and values stream at 5 TB/s from 512 blocks, at 3.6
+// from one a CU. A part is written and read again, 4.5 TB/s, and joined by a further launch.
+int tile_chunk(const TilePhase &phase, size_t head_dim) {
+  const double key_us = 2.17 / 64.0 * static_cast<double>(head_dim) / 128.0;
+  constexpr size_t kSamples = 16;
+  int best = 0;
+  double best_us = 0.0;
+  for (size_t half_chunks = 2; half_chunks <= 2 * kMostSlots; half_chunks += half_chunks / 16 + 1) {
+    // chunks of the longest rows: 1, 1.5, 2, ..
+    const size_t keys = (2 * phase.most + half_chunks - 1) / half_chunks;
+    const int chunk = static_cast<int>((keys + 63) / 64 * 64);
+    if (best != 0 && (chunk < 256 || phase.most > kMostSlots * static_cast<size_t>(chunk)))
+      break;
+    double chunks = 0.0;
+    for (size_t i = 0; i < kSamples; ++i)
+      chunks += static_cast<double>(
+          (phase.least + (phase.most - phase.least) * (2 * i + 1) / (2 * kSamples) + chunk - 1) /
+          chunk);
+    chunks = std::max(1.0, chunks / kSamples);
+    const double blocks = chunks * static_cast<double>(phase.tiles);
+    const double longest = static_cast<double>(std::min<size_t>(chunk, phase.most)) * key_us;
+    double us = blocks <= 256.0    ? 0.6 * longest
+                : blocks <= 1536.0 ? std::ceil(blocks / 512.0) * longest
+                                   : (blocks / 512.0 + 0.3) * longest;
+    us = std::max(us, phase.kv_bytes /
+                          (3.6e6 + 1.4e6 * std::clamp(blocks / 256.0 - 1.0, 0.0, 1.0)));
+    us += phase.other_keys * key_us / 512.0;
+    if (chunks > 1.0)
+      us += 5.0 + 2.0 * phase.part_bytes * chunks / 4.5e6;
+    if (best == 0 || us < best_us) {
+      best = chunk;
+      best_us = us;
+    }
+  }
+  return best;
 }
 
 AttendPlan plan_attention(const PagedCache &cache, const PagedBatch &batch, size_t heads) {
   const size_t kv = static_cast<size_t>(cache.kv_heads), group = heads / kv;
   const size_t sequences = static_cast<size_t>(batch.sequences);
   const size_t tokens = static_cast<size_t>(batch.tokens);
+  const size_t dim = static_cast<size_t>(cache.head_dim);
   const size_t most = static_cast<size_t>(batch.max_tokens) * group;
   AttendPlan plan{};
   plan.own_stream = most <= 16;
   plan.prefix_stream = tokens * group <= 16;
   const size_t rows = plan.own_stream ? 16 : 128;
   // A tile each for the rows that fill one, and one more for each sequence's rest.
-  plan.tiles = std::min(sequences * ((most + rows - 1) / rows),
-                        tokens * group / rows + std::min(sequences, tokens));
+  plan.tiles = plan.own_stream ? sequences
+                               : std::min(sequences * ((most + rows - 1) / rows),
+                                          tokens * group / rows + std::min(sequences, tokens));
   const size_t own = std::max(1, batch.max_length - batch.shared_length);
-  plan.chunk = plan.own_stream ? chunk_keys(own, plan.tiles * kv, 2048, 128)
-                               : chunk_keys(own, plan.tiles * kv, 1024, 512);
+  const double part_bytes = static_cast<double>(tokens * heads * dim * sizeof(float));
+  if (plan.own_stream) {
+    plan.chunk = stream_chunk(own, plan.tiles * kv);
+  } else {
+    // The longest sequence is taken to bring the most rows too; the others' lengths
+    // are not known here and count as a third of its.
+    const size_t longest_tiles = (most + rows - 1) / rows;
+    const double share = static_cast<double>(batch.max_tokens) / static_cast<double>(tokens);
+    plan.chunk = tile_chunk({longest_tiles * kv, own - std::min(own, most / group) + 1, own,
+                             static_cast<double>((plan.tiles - longest_tiles) * kv * own) / 3.0,
+                             4.0 * static_cast<double>(own * kv * dim), part_bytes * share},
+                            dim);
+  }
   const int own_slots = static_cast<int>((own + plan.chunk - 1) / plan.chunk);
   if (batch.shared_length > 0) {
     const size_t shared = static_cast<size_t>(batch.shared_length);
     const size_t prefix_rows = plan.prefix_stream ? 16 : 128;
     plan.prefix_tiles = (tokens * group + prefix_rows - 1) / prefix_rows;
-    plan.prefix_chunk = plan.prefix_stream
-                            ? chunk_keys(shared, plan.prefix_tiles * kv, 2048, 128)
-                            : chunk_keys(shared, plan.prefix_tiles * kv, 1024, 512);
+    plan.prefix_chunk =
+        plan.prefix_stream
+            ? stream_chunk(shared, plan.prefix_tiles * kv)
+            : tile_chunk({plan.prefix_tiles * kv, shared, shared, 0.0,
+                          4.0 * static_cast<double>(shared * kv * dim), part_bytes},
+                         dim);
     plan.prefix_slots =
         static_cast<int>((shared + plan.prefix_chunk - 1) / plan.prefix_chunk);
   }
@@ -788,45 +993,38 @@ size_t plan_bytes(const AttendPlan &plan, const PagedCache &cache, const PagedBa
                                (cache.head_dim + 2) * sizeof(float);
 }
 
-// One launch of the blocks of a kind: shared keys first, then own ones.
-template <typename T, int kD>
-Status launch_blocks(const AttendArgs &args, bool stream_kernel, size_t prefix_blocks,
-                     size_t own_blocks, size_t tiles, hipStream_t stream) {
-  if (prefix_blocks + own_blocks == 0)
-    return Status::Ok();
-  if (prefix_blocks + own_blocks >= (size_t{1} << 31))
-    return {ErrorCode::kInvalidArgument, "paged_attention: grid too large"};
-  const dim3 grid(static_cast<unsigned>(prefix_blocks + own_blocks));
-  const unsigned first = static_cast<unsigned>(prefix_blocks);
-  if (stream_kernel) {
-    hipLaunchKernelGGL((paged_stream_kernel<T, kD>), grid, dim3(256), 0, stream, args, first,
-                       static_cast<unsigned>(tiles));
-    return launch_status("paged_stream_kernel");
-  }
-  constexpr size_t kLdsBytes = 2 * 2 * 64 * kD * sizeof(uint16_t);
-  static_assert(kLdsBytes <= 64 * 1024, "default LDS limit, two blocks per CU");
-  hipLaunchKernelGGL((paged_tile_kernel<T, kD>), grid, dim3(256), kLdsBytes, stream, args, first,
-                     static_cast<unsigned>(tiles));
-  return launch_status("paged_tile_kernel");
-}
-
 template <typename T, int kD>
 Status launch_attention(const AttendArgs &args, const AttendPlan &plan, hipStream_t stream) {
   const size_t kv = static_cast<size_t>(args.cache.kv_heads);
   const size_t prefix_blocks = plan.prefix_tiles * kv * plan.prefix_slots;
-  const size_t own_blocks = plan.tiles * kv * (plan.slots - plan.prefix_slots);
-  if (plan.own_stream == plan.prefix_stream || prefix_blocks == 0) {
-    EVO_TRY((launch_blocks<T, kD>(args, plan.own_stream, prefix_blocks, own_blocks, plan.tiles,
-                                  stream)));
-  } else {
-    EVO_TRY((launch_blocks<T, kD>(args, plan.prefix_stream, prefix_blocks, 0, 0, stream)));
-    EVO_TRY((launch_blocks<T, kD>(args, plan.own_stream, 0, own_blocks, plan.tiles, stream)));
+  const size_t blocks = prefix_blocks + plan.tiles * kv * (plan.slots - plan.prefix_slots);
+  if (blocks >= (size_t{1} << 31))
+    return {ErrorCode::kInvalidArgument, "paged_attention: grid too large"};
+  auto kernel = paged_attention_kernel<T, kD, 1>;
+  size_t lds = kTileLds * kD;
+  if (plan.own_stream && (plan.prefix_stream || prefix_blocks == 0)) {
+    kernel = paged_attention_kernel<T, kD, 0>;
+    lds = sizeof(StreamShared<kD>);
+  } else if (plan.own_stream) {
+    kernel = paged_attention_kernel<T, kD, 2>;
+    lds = std::max(lds, sizeof(StreamShared<kD>));
   }
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), lds, stream, args,
+                     static_cast<unsigned>(prefix_blocks), static_cast<unsigned>(plan.tiles));
+  EVO_TRY(launch_status("paged_attention_kernel"));
   if (plan.slots == 1)
     return Status::Ok();
-  const size_t rows = static_cast<size_t>(args.batch.tokens) * args.heads;
-  hipLaunchKernelGGL((paged_combine_kernel<T, kD>), dim3(ceil_div(rows, 4)), dim3(256), 0, stream,
-                     args);
+  const size_t tokens = static_cast<size_t>(args.batch.tokens), heads = args.heads;
+  if (plan.slots > 8) {
+    hipLaunchKernelGGL((paged_combine_kernel<T, kD, true>),
+                       dim3(static_cast<unsigned>(tokens * heads)), dim3(256), 0, stream, args, 1);
+  } else {
+    // Four heads of a row per block, all of them where the rows fill the chip.
+    const size_t of_block = std::min(heads, 4 * std::max<size_t>(1, tokens * heads / 8192));
+    hipLaunchKernelGGL((paged_combine_kernel<T, kD, false>),
+                       dim3(static_cast<unsigned>(tokens * ceil_div(heads, of_block))), dim3(256),
+                       0, stream, args, static_cast<int>(of_block));
+  }
   return launch_status("paged_combine_kernel");
 }
 
@@ -877,6 +1075,7 @@ Status paged_attention(const PagedCache &cache, const PagedBatch &batch, const v
                         static_cast<uint16_t *>(out), out_stride, static_cast<int>(heads),
                         static_cast<int>(heads / kv), 1.4426950408889634F * scale, plan.chunk,
                         plan.prefix_chunk, plan.prefix_slots, plan.slots,
+                        plan.own_stream ? 1 : 0,
                         static_cast<float *>(workspace),
                         reinterpret_cast<float2 *>(static_cast<float *>(workspace) +
                                                    static_cast<size_t>(batch.tokens) * heads *

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from functools import lru_cache
+from functools import lru_cache, partial
 
 PACKAGE_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIBRARY_PATH = os.path.join(PACKAGE_DIR, "lib", "libevo_hip.so")
@@ -24,28 +24,27 @@ FP8_MFMA_K32, FP8_MFMA_K128, FP8_EXACT = 0, 1, 2
 PAGED_BAD_SEQUENCE, PAGED_BAD_PAGE = 1, 2  # bits of PagedBatch.error
 
 
-class _Sized(ctypes.Structure):
-    """A parameter struct that knows its struct_size; fields not given are 0 or NULL."""
-
-    def __init__(self, **fields):
-        super().__init__(struct_size=ctypes.sizeof(self), **fields)
-
-
-class PagedCache(_Sized):
+class PagedCacheStruct(ctypes.Structure):
     _fields_ = [("struct_size", c_size), ("dtype", c_int), ("key_pages", c_void),
                 ("value_pages", c_void), ("pages", c_size), ("page_size", c_size),
                 ("kv_heads", c_size), ("head_dim", c_size), ("page_stride", c_size),
                 ("head_stride", c_size), ("token_stride", c_size)]
 
 
-class PagedBatch(_Sized):
+class PagedBatchStruct(ctypes.Structure):
     _fields_ = [("struct_size", c_size), ("sequences", c_size), ("tokens", c_size),
                 ("max_tokens", c_size), ("max_length", c_size), ("token_start", c_void),
                 ("lengths", c_void), ("page_table", c_void), ("table_stride", c_size),
                 ("shared_length", c_size), ("shared_table", c_void), ("error", c_void)]
 
 
-_paged = [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedBatch)]
+# PagedCache(dtype=.., ...): the struct with its struct_size; fields not given are 0
+# or NULL. (A decode step makes them for each call: an __init__ of their own would
+# take as long as the rest.)
+PagedCache = partial(PagedCacheStruct, ctypes.sizeof(PagedCacheStruct))
+PagedBatch = partial(PagedBatchStruct, ctypes.sizeof(PagedBatchStruct))
+
+_paged = [ctypes.POINTER(PagedCacheStruct), ctypes.POINTER(PagedBatchStruct)]
 
 # name -> (restype, argtypes) for include/evo/hip_ops.h
 _OPS = {
@@ -130,10 +129,7 @@ def load(path: str = LIBRARY_PATH) -> ctypes.CDLL:
 
 def call(name: str, *args) -> int:
     """Call an operator entry point; raise OpError on a non-OK status."""
-    lib = load()
-    status = getattr(lib, name)(*args)
-    if name.endswith("_bytes"):
-        return status
-    if status != 0:
-        raise OpError(f"{name}: {lib.evo_last_error().decode()}")
+    status = getattr(load(), name)(*args)
+    if status != 0 and not name.endswith("_bytes"):
+        raise OpError(f"{name}: {load().evo_last_error().decode()}")
     return status
