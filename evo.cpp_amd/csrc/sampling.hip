@@ -16,6 +16,7 @@
 #include "common.hpp"
 #include "ops.hpp"
 
+#include <algorithm>
 #include <cmath>
 
 namespace evo::hip {
@@ -43,6 +44,11 @@ __device__ inline uint32_t ordered(float v) {
 // Place of a token in the order: larger is earlier. 56 bits, vocab <= 2^20.
 __device__ inline uint64_t place(float v, int index) {
   return static_cast<uint64_t>(ordered(v)) << 24 | static_cast<uint32_t>(0xffffff - index);
+}
+
+__device__ inline float value_of(uint64_t place) {
+  const uint32_t bits = static_cast<uint32_t>(place >> 24);
+  return __builtin_bit_cast(float, (bits & 0x80000000U) != 0 ? bits & 0x7fffffffU : ~bits);
 }
 
 // 2^(i / 64).
@@ -76,12 +82,13 @@ __device__ inline uint64_t weight_units(double z, const double *powers) {
   e = fma(e, f, 5.86490495505617e-05);
   e = fma(e, f, 0.010830424696249145);
   e = fma(e, f, 1.0);
+  // powers[] is the table times 2^42; whole / 64 goes into the exponent.
   const int whole = static_cast<int>(n);
   const uint64_t bits = __builtin_bit_cast(uint64_t, e * powers[whole & 63]) +
-                        (static_cast<uint64_t>(static_cast<int64_t>((whole >> 6) + 42)) << 52);
+                        (static_cast<uint64_t>(static_cast<uint32_t>(whole & ~63) << 14) << 32);
   // Adding 2^52 rounds to a whole number in the low bits.
   const double shifted = __builtin_bit_cast(double, bits) + 4503599627370496.0;
-  return __builtin_bit_cast(uint64_t, shifted) & 0xfffffffffffffULL;
+  return __builtin_bit_cast(uint64_t, shifted) - 0x4330000000000000ULL;
 }
 
 template <typename V, typename F> __device__ inline V wave_reduce(V v, F &&f) {
@@ -89,6 +96,11 @@ template <typename V, typename F> __device__ inline V wave_reduce(V v, F &&f) {
   for (int offset = 32; offset > 0; offset >>= 1)
     v = f(v, __shfl_xor(v, offset, 64));
   return v;
+}
+__device__ inline uint64_t lane_value(uint64_t v, int lane) {
+  const uint32_t low = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), lane);
+  const uint32_t high = __builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), lane);
+  return static_cast<uint64_t>(high) << 32 | low;
 }
 template <int kThreads, typename V, typename F>
 __device__ inline V block_reduce(V v, V *scratch, F &&f) {
@@ -98,9 +110,11 @@ __device__ inline V block_reduce(V v, V *scratch, F &&f) {
     if ((threadIdx.x & 63) == 0)
       scratch[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = scratch[0];
-    for (int w = 1; w < kThreads / 64; ++w)
-      v = f(v, scratch[w]);
+    constexpr int kWaves = kThreads / 64;
+    v = scratch[(threadIdx.x & 63) % kWaves];
+#pragma unroll
+    for (int offset = kWaves / 2; offset > 0; offset >>= 1)
+      v = f(v, __shfl_xor(v, offset, 64));
   }
   return v;
 }
@@ -127,6 +141,9 @@ struct Cuts {
     return temperature >= 0.0F && temperature < INFINITY && top_k >= 0 && top_p > 0.0F &&
            top_p <= 1.0F && min_p >= 0.0F && min_p <= 1.0F && uniform == uniform;
   }
+  // Whether a row of this largest logit can be sampled.
+  __device__ bool samples(float top) const { return valid() && top < INFINITY && top > -INFINITY; }
+  __device__ bool has_k(int vocab) const { return top_k > 0 && top_k < vocab; }
   __device__ bool greedy() const { return temperature == 0.0F || top_k == 1; }
   // Least weight that min-p keeps.
   __device__ uint64_t least() const {
@@ -149,6 +166,17 @@ struct Cuts {
   }
 };
 
+// Values low <= v < high.
+struct Values {
+  float low, high;
+  __device__ bool has(float v) const { return v >= low && v < high; }
+  // Their places, the first in order and the last.
+  __device__ uint64_t first() const {
+    return high == INFINITY ? ~0ULL : (static_cast<uint64_t>(ordered(high)) << 24) - 1;
+  }
+  __device__ uint64_t last() const { return static_cast<uint64_t>(ordered(low)) << 24; }
+};
+
 // How a row's values map to bins and weights, given its largest and lowest value.
 struct Scale {
   float top, reach, bin_scale;
@@ -161,31 +189,179 @@ struct Scale {
     // A little less than bins / range: the last value stays inside.
     bin_scale = range > 0.0F ? fminf(static_cast<float>(bins) * 0.999999F / range, 3.0e38F) : 0.0F;
   }
-  // Bin of a value, -1 for one without weight. Every step is monotonic.
+  // Bin of a value, -1 for one without weight. Every step is monotonic, so a bin is a
+  // range of values.
   __device__ int bin(float v) const {
     const float below = top - v;
     return below <= reach ? static_cast<int>(below * bin_scale) : -1;
   }
-  __device__ bool in_bin(float v, float first) const {  // bin(v) == first
-    const float at = (top - v) * bin_scale;
-    return at >= first && at < first + 1.0F && top - v <= reach;
+  // Lowest value of the bins 0 .. `bin`: a search of 64 values at a time over the
+  // values' order. All lanes of a wave call it, with the same bin.
+  __device__ float lowest(int bin) const {
+    const float end = static_cast<float>(bin + 1);
+    uint32_t below = 0x007fffffU;  // -infinity, in no bin
+#pragma unroll 1
+    for (int shift = 26; shift >= 0; shift = shift == 2 ? 0 : shift - 6) {
+      const uint64_t key = below + ((static_cast<uint64_t>(threadIdx.x & 63) + 1) << shift);
+      bool in = true;
+      if (key < 0xff800000U) {
+        const float v = value_of(key << 24);
+        in = (top - v) * bin_scale < end && top - v <= reach;
+      }
+      const uint64_t inside = __ballot(in);
+      below += static_cast<uint32_t>(inside == 0 ? 64 : __builtin_ctzll(inside)) << shift;
+    }
+    return value_of(static_cast<uint64_t>(below + 1) << 24);
   }
-  __device__ uint64_t weight(float v, const double *powers) const {
-    const double z = (static_cast<double>(v) - static_cast<double>(top)) * unit;
-    return z < -2862.0 ? 0 : weight_units(z, powers);
+  __device__ Values values(int first, int last) const {  // of a run of bins
+    return {lowest(last), first == 0 ? INFINITY : lowest(first - 1)};
+  }
+  __device__ uint64_t weight(float v, const double *powers) const {  // of one in reach
+    return weight_units((static_cast<double>(v) - static_cast<double>(top)) * unit, powers);
   }
 };
 
+// ------------------------------------------------------- one wave's search
+// Between a wave's own writes to LDS and its reads of them.
+__device__ inline void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// 256 bins of counts and weights in LDS, four a lane.
+struct WaveBins {
+  uint64_t *mass;
+  uint32_t *count;
+  __device__ void clear() const {
+    const int lane = threadIdx.x & 63;
+    reinterpret_cast<uint4 *>(mass)[2 * lane] = make_uint4(0, 0, 0, 0);
+    reinterpret_cast<uint4 *>(mass)[2 * lane + 1] = make_uint4(0, 0, 0, 0);
+    reinterpret_cast<uint4 *>(count)[lane] = make_uint4(0, 0, 0, 0);
+    wave_sync();
+  }
+  __device__ void add(int bin, uint64_t w) const {
+    atomicAdd(&count[bin], 1U);
+    atomicAdd(reinterpret_cast<unsigned long long *>(&mass[bin]),
+              static_cast<unsigned long long>(w));
+  }
+};
+// The lane's four bins, and what lies before them.
+struct LaneBins {
+  uint64_t mass[4], mass_before, mass_total;
+  uint32_t count[4], count_before, count_total;
+  __device__ explicit LaneBins(const WaveBins &bins) {
+    const int lane = threadIdx.x & 63;
+    wave_sync();
+    uint64_t m = 0;
+    uint32_t c = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      mass[j] = bins.mass[4 * lane + j];
+      count[j] = bins.count[4 * lane + j];
+      m += mass[j];
+      c += count[j];
+    }
+    const uint64_t own_m = m;
+    const uint32_t own_c = c;
+#pragma unroll
+    for (int offset = 1; offset < 64; offset <<= 1) {
+      const uint64_t up_m = __shfl_up(m, offset, 64);
+      const uint32_t up_c = __shfl_up(c, offset, 64);
+      m += lane >= offset ? up_m : 0;
+      c += lane >= offset ? up_c : 0;
+    }
+    mass_before = m - own_m;
+    count_before = c - own_c;
+    mass_total = lane_value(m, 63);
+    count_total = __builtin_amdgcn_readlane(c, 63);
+  }
+};
+// The bin in which the running count or weight passes a target, what lies before it,
+// and how many tokens it has.
+struct Hit {
+  int bin;
+  uint64_t mass_before;
+  uint32_t count_before, members;
+};
+__device__ inline Hit locate(const LaneBins &b, bool by_count, uint64_t target) {
+  uint64_t at_m = b.mass_before;
+  uint32_t at_c = b.count_before;
+  Hit h{-1, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint64_t from = by_count ? at_c : at_m;
+    const uint64_t size = by_count ? b.count[j] : b.mass[j];
+    if (target >= from && target - from < size)
+      h = {4 * static_cast<int>(threadIdx.x & 63) + j, at_m, at_c, b.count[j]};
+    at_m += b.mass[j];
+    at_c += b.count[j];
+  }
+  const uint64_t owner = __ballot(h.bin >= 0);
+  const int from = owner == 0 ? 0 : __builtin_ctzll(owner);
+  return Hit{__builtin_amdgcn_readlane(h.bin, from), lane_value(h.mass_before, from),
+             static_cast<uint32_t>(__builtin_amdgcn_readlane(h.count_before, from)),
+             static_cast<uint32_t>(__builtin_amdgcn_readlane(h.members, from))};
+}
+
+// Among the tokens that the lanes hold (spot[e] != 0: a place; w[e]: its weight;
+// `members` of them), the one, in order, at which the running count or weight passes
+// the target: its place; `before` grows by the weight up to it, itself included. A
+// histogram over the range of the places leaves the few that are taken one by one.
+template <int kPer>
+__device__ inline uint64_t wave_find(uint64_t (&spot)[kPer], const uint64_t (&w)[kPer],
+                                     uint32_t members, const WaveBins &bins, bool by_count,
+                                     uint64_t target, uint64_t &before) {
+  while (members > 6) {
+    uint64_t last = ~0ULL, first = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      first = first > spot[e] ? first : spot[e];
+      last = spot[e] != 0 && spot[e] < last ? spot[e] : last;
+    }
+    first = wave_reduce(first, Most{});
+    last = wave_reduce(last, Least{});
+    const int shift = max(0, 56 - static_cast<int>(__builtin_clzll(first - last)));
+    bins.clear();
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      if (spot[e] != 0)
+        bins.add(static_cast<int>((first - spot[e]) >> shift), w[e]);
+    const Hit h = locate(LaneBins(bins), by_count, target);
+    before += h.mass_before;
+    target -= by_count ? h.count_before : h.mass_before;
+    members = h.members;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      if (spot[e] != 0 && static_cast<int>((first - spot[e]) >> shift) != h.bin)
+        spot[e] = 0;
+  }
+  uint64_t token = 0;
+  for (uint32_t i = 0; i < members; ++i) {
+    uint64_t first = 0, own = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      own = spot[e] > first ? w[e] : own;
+      first = spot[e] > first ? spot[e] : first;
+    }
+    token = wave_reduce(first, Most{});
+    own = lane_value(own, __builtin_ctzll(__ballot(first == token)));
+    before += own;
+    if (by_count ? target == i : target < own)
+      break;
+    target -= by_count ? 0 : own;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      spot[e] = spot[e] == token ? 0 : spot[e];
+  }
+  return token;
+}
+
 // ------------------------------------------------------- small vocabularies
-// A wave per row, kPer values a lane in registers. A border's bin is found in the
-// scanned histogram that the lanes hold, four bins each; a bin of more than a few
-// tokens is histogrammed again over the range of its places; the last few are taken
-// one by one.
+// A wave per row, kPer values a lane in registers.
 template <typename T, int kPer>
 __global__ __launch_bounds__(64) void sample_wave_kernel(const SampleArgs a) {
-  constexpr int kBins = 256;
-  __shared__ __attribute__((aligned(16))) uint64_t mass_s[kBins];
-  __shared__ __attribute__((aligned(16))) uint32_t count_s[kBins];
+  __shared__ __attribute__((aligned(16))) uint64_t mass_s[256];
+  __shared__ __attribute__((aligned(16))) uint32_t count_s[256];
   __shared__ double powers[64];
   const int lane = threadIdx.x;
   const size_t r = blockIdx.x;
@@ -195,13 +371,9 @@ __global__ __launch_bounds__(64) void sample_wave_kernel(const SampleArgs a) {
   for (int e = 0; e < kPer; ++e)
     v[e] = 64 * e + lane < a.vocab ? static_cast<float>(logits[64 * e + lane]) : -INFINITY;
   const Cuts cuts(a, r);
-  powers[lane] = kPowers[lane];
-  auto clear = [&] {
-    reinterpret_cast<uint4 *>(mass_s)[2 * lane] = make_uint4(0, 0, 0, 0);
-    reinterpret_cast<uint4 *>(mass_s)[2 * lane + 1] = make_uint4(0, 0, 0, 0);
-    reinterpret_cast<uint4 *>(count_s)[lane] = make_uint4(0, 0, 0, 0);
-  };
-  clear();
+  powers[lane] = kPowers[lane] * 4398046511104.0;
+  const WaveBins bins{mass_s, count_s};
+  bins.clear();
   float top = -INFINITY, low = INFINITY;
   bool bad = false;
 #pragma unroll
@@ -212,7 +384,7 @@ __global__ __launch_bounds__(64) void sample_wave_kernel(const SampleArgs a) {
   }
   top = wave_reduce(top, Most{});
   low = wave_reduce(low, Least{});
-  if (__any(bad) || top == -INFINITY || !cuts.valid()) {
+  if (__any(bad) || !cuts.samples(top)) {
     if (lane == 0)
       a.tokens[r] = kNoToken;
     return;
@@ -227,201 +399,129 @@ __global__ __launch_bounds__(64) void sample_wave_kernel(const SampleArgs a) {
       a.tokens[r] = static_cast<uint32_t>(first);
     return;
   }
-  const Scale scale(top, low, cuts.temperature, kBins);
-  __syncthreads();
-  uint64_t w[kPer];
+  const Scale scale(top, low, cuts.temperature, 256);
+  uint64_t w[kPer], kept = 0;
   int bin[kPer];
   const uint64_t least = cuts.least();
-  uint64_t kept = 0;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
     bin[e] = scale.bin(v[e]);
     w[e] = bin[e] >= 0 ? scale.weight(v[e], powers) : 0;
     kept += w[e] >= least ? w[e] : 0;
-    if (bin[e] >= 0) {
-      atomicAdd(&count_s[bin[e]], 1U);
-      atomicAdd(reinterpret_cast<unsigned long long *>(&mass_s[bin[e]]),
-                static_cast<unsigned long long>(w[e]));
-    }
+    if (bin[e] >= 0)
+      bins.add(bin[e], w[e]);
   }
-  // The lane's four bins, and what lies before them.
-  struct Bins {
-    uint64_t mass[4], mass_before, mass_total;
-    uint32_t count[4], count_before, count_total;
-  };
-  auto scanned = [&] {
-    Bins b;
-    __syncthreads();
-    uint64_t m = 0;
-    uint32_t c = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      b.mass[j] = mass_s[4 * lane + j];
-      b.count[j] = count_s[4 * lane + j];
-      m += b.mass[j];
-      c += b.count[j];
+  const LaneBins all(bins);
+  // The top-k border, the nucleus' border, the draw: one after the other through the
+  // same code (three copies of it cost more to fetch than to run).
+  uint64_t total = all.mass_total, token = 0;
+#pragma unroll 1
+  for (int border = 0; border < 3; ++border) {
+    uint64_t target;
+    if (border == 0) {
+      if (cuts.top_k == 0 || static_cast<uint32_t>(cuts.top_k) >= all.count_total)
+        continue;
+      target = static_cast<uint64_t>(cuts.top_k) - 1;
+    } else if (border == 1) {
+      if (cuts.top_p >= 1.0F)
+        continue;
+      target = cuts.nucleus(total);
+    } else {
+      if (cuts.min_p > 0.0F) {
+        kept = wave_reduce(kept, Sum{});
+        total = Least{}(total, kept);
+      }
+      target = cuts.draw(total);
     }
-    const uint64_t own_m = m;
-    const uint32_t own_c = c;
-#pragma unroll
-    for (int offset = 1; offset < 64; offset <<= 1) {
-      const uint64_t up_m = __shfl_up(m, offset, 64);
-      const uint32_t up_c = __shfl_up(c, offset, 64);
-      m += lane >= offset ? up_m : 0;
-      c += lane >= offset ? up_c : 0;
-    }
-    b.mass_before = m - own_m;
-    b.count_before = c - own_c;
-    b.mass_total = __shfl(m, 63, 64);
-    b.count_total = __shfl(c, 63, 64);
-    __syncthreads();
-    return b;
-  };
-  // The bin in which the running count or weight passes the target, what lies before
-  // it, and how many tokens it has.
-  struct Hit {
-    int bin;
-    uint64_t mass_before;
-    uint32_t count_before, members;
-  };
-  auto locate = [&](const Bins &b, bool by_count, uint64_t target) {
-    uint64_t at_m = b.mass_before;
-    uint32_t at_c = b.count_before;
-    Hit h{-1, 0, 0, 0};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint64_t from = by_count ? at_c : at_m;
-      const uint64_t size = by_count ? b.count[j] : b.mass[j];
-      if (target >= from && target - from < size)
-        h = {4 * lane + j, at_m, at_c, b.count[j]};
-      at_m += b.mass[j];
-      at_c += b.count[j];
-    }
-    const uint64_t owner = __ballot(h.bin >= 0);
-    const int from = owner == 0 ? 0 : __builtin_ctzll(owner);
-    return Hit{__shfl(h.bin, from, 64), __shfl(h.mass_before, from, 64),
-               static_cast<uint32_t>(__shfl(h.count_before, from, 64)),
-               static_cast<uint32_t>(__shfl(h.members, from, 64))};
-  };
-  const Bins all = scanned();
-  // The token at which the running count or weight of the order passes the target,
-  // and the weight up to it, itself included.
-  auto find = [&](bool by_count, uint64_t target, uint64_t *mass) {
-    Hit h = locate(all, by_count, target);
-    uint64_t before = h.mass_before;
-    target -= by_count ? h.count_before : h.mass_before;
-    uint64_t spot[kPer];  // the candidates' places, else 0
+    const Hit h = locate(all, border == 0, target);
+    uint64_t spot[kPer];
 #pragma unroll
     for (int e = 0; e < kPer; ++e)
       spot[e] = bin[e] == h.bin ? place(v[e], 64 * e + lane) : 0;
-    uint32_t members = h.members;
-    while (members > 6) {
-      uint64_t last = ~0ULL, first = 0;
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        first = first > spot[e] ? first : spot[e];
-        last = spot[e] != 0 && spot[e] < last ? spot[e] : last;
-      }
-      first = wave_reduce(first, Most{});
-      last = wave_reduce(last, Least{});
-      const int shift = max(0, 56 - static_cast<int>(__builtin_clzll(first - last)));
-      clear();
-      __syncthreads();
-#pragma unroll
-      for (int e = 0; e < kPer; ++e)
-        if (spot[e] != 0) {
-          const int sub = static_cast<int>((first - spot[e]) >> shift);
-          atomicAdd(&count_s[sub], 1U);
-          atomicAdd(reinterpret_cast<unsigned long long *>(&mass_s[sub]),
-                    static_cast<unsigned long long>(w[e]));
-        }
-      h = locate(scanned(), by_count, target);
-      before += h.mass_before;
-      target -= by_count ? h.count_before : h.mass_before;
-      members = h.members;
-#pragma unroll
-      for (int e = 0; e < kPer; ++e)
-        if (spot[e] != 0 && static_cast<int>((first - spot[e]) >> shift) != h.bin)
-          spot[e] = 0;
-    }
-    uint64_t token = 0;
-    for (uint32_t i = 0; i < members; ++i) {
-      uint64_t first = 0, own = 0;
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        own = spot[e] > first ? w[e] : own;
-        first = spot[e] > first ? spot[e] : first;
-      }
-      token = wave_reduce(first, Most{});
-      own = __shfl(own, __builtin_ctzll(__ballot(first == token)), 64);
-      before += own;
-      if (by_count ? target == i : target < own)
-        break;
-      target -= by_count ? 0 : own;
-#pragma unroll
-      for (int e = 0; e < kPer; ++e)
-        spot[e] = spot[e] == token ? 0 : spot[e];
-    }
-    *mass = before;
-    return 0xffffffU - static_cast<uint32_t>(token & 0xffffff);
-  };
-  uint64_t total = all.mass_total;
-  if (cuts.top_k > 0 && static_cast<uint32_t>(cuts.top_k) < all.count_total)
-    find(true, static_cast<uint64_t>(cuts.top_k) - 1, &total);
-  if (cuts.top_p < 1.0F)
-    find(false, cuts.nucleus(total), &total);
-  if (cuts.min_p > 0.0F) {
-    kept = wave_reduce(kept, Sum{});
-    total = total < kept ? total : kept;
+    total = h.mass_before;
+    token = wave_find<kPer>(spot, w, h.members, bins, border == 0,
+                            target - (border == 0 ? h.count_before : h.mass_before), total);
   }
-  uint64_t through;
-  const uint32_t token = find(false, cuts.draw(total), &through);
   if (lane == 0)
-    a.tokens[r] = token;
+    a.tokens[r] = 0xffffffU - static_cast<uint32_t>(token & 0xffffff);
 }
 
 // ------------------------------------------------------- large vocabularies
-template <typename T> struct Row {
+template <typename T> struct Row {  // or a part of one, from token `first`
   const T *logits;
-  int vocab;
-  bool vector;  // the row starts on 16 bytes
-  // f(value, index) over the tokens, 16 bytes a load and four loads ahead where the
-  // row is aligned.
-  template <int kThreads, typename F> __device__ void each(F &&f) const {
-    constexpr int kPer = 16 / sizeof(T), kAhead = 4;
+  int vocab, first;
+  bool vector;  // it starts on 16 bytes
+  __device__ Row(const SampleArgs &a, size_t r, int first_, int count)
+      : logits(static_cast<const T *>(a.logits) + r * a.row_stride + first_), vocab(count),
+        first(first_), vector(reinterpret_cast<uintptr_t>(logits) % 16 == 0) {}
+  // f(value, index) over the tokens, 16 bytes a load where the row is aligned, kLoads
+  // of them at a time and as many ahead. kLoads 1 where f is long: code of more copies
+  // is fetched more slowly than it runs; 4 where it is short and the loads are what
+  // takes the time.
+  // Only values that `wanted` has reach f; where it is given, the values of a load are
+  // looked over together first.
+  struct All {
+    __device__ bool operator()(float) const { return true; }
+  };
+  template <int kThreads, int kLoads, typename F> __device__ void each(F &&f) const {
+    each<kThreads, kLoads>(All{}, f);
+  }
+  template <int kThreads, int kLoads, typename W, typename F>
+  __device__ void each(W &&wanted, F &&f) const {
+    constexpr int kPer = 16 / sizeof(T);
     typedef T wide __attribute__((ext_vector_type(kPer)));
     int tail = 0;
     if (vector) {
       const int whole = vocab / kPer;
       const wide *src = reinterpret_cast<const wide *>(logits);
-      for (int c0 = threadIdx.x; c0 < whole; c0 += kThreads * kAhead) {
-        wide v[kAhead];
+      wide now[kLoads], next[kLoads];
+      const auto load = [&](wide(&to)[kLoads], int c) {
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a)
-          if (c0 + a * kThreads < whole)
-            v[a] = src[c0 + a * kThreads];
+        for (int a = 0; a < kLoads; ++a)
+          if (c + a * kThreads < whole)
+            to[a] = src[c + a * kThreads];
+      };
+      int c = threadIdx.x;
+      load(now, c);
+#pragma unroll 1
+      for (; c < whole; c += kThreads * kLoads) {
+        load(next, c + kThreads * kLoads);
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a)
-          if (c0 + a * kThreads < whole) {
+        for (int a = 0; a < kLoads; ++a)
+          if (a == 0 || c + a * kThreads < whole) {
+            bool any = false;
 #pragma unroll
             for (int e = 0; e < kPer; ++e)
-              f(static_cast<float>(v[a][e]), (c0 + a * kThreads) * kPer + e);
+              any |= wanted(static_cast<float>(now[a][e]));
+            if (any) {
+#pragma unroll
+              for (int e = 0; e < kPer; ++e)
+                if (wanted(static_cast<float>(now[a][e])))
+                  f(static_cast<float>(now[a][e]), first + (c + a * kThreads) * kPer + e);
+            }
           }
+#pragma unroll
+        for (int a = 0; a < kLoads; ++a)
+          now[a] = next[a];
       }
       tail = whole * kPer;
     }
+#pragma unroll 1
     for (int i = tail + threadIdx.x; i < vocab; i += kThreads)
-      f(static_cast<float>(logits[i]), i);
+      if (wanted(static_cast<float>(logits[i])))
+        f(static_cast<float>(logits[i]), first + i);
   }
 };
 
 // A row's histogram and a list of tokens.
+constexpr int kFew = 512;  // tokens that one wave searches
 template <int kThreads, int kBins, int kList> struct SampleShared {
   uint64_t mass[kBins];   // before the scan a bin's own, then of the bins before it
   uint32_t count[kBins];
   uint64_t list_place[kList], list_mass[kList];
-  uint64_t sub_mass[256], few_place[64], few_mass[64];
-  uint32_t sub_count[256];
+  __attribute__((aligned(16))) uint64_t sub_mass[256];
+  __attribute__((aligned(16))) uint32_t sub_count[256];
+  uint64_t few_place[kFew], few_mass[kFew];
   uint64_t wave_mass[kThreads / 64];
   uint32_t wave_count[kThreads / 64];
   double powers[64];
@@ -485,17 +585,17 @@ template <typename V> __device__ inline int last_at_most(const V *a, int size, V
   return low;
 }
 
-// The listed token, in order, at which the running count (by_count) or weight of the
-// list's `members` passes the target: its place, and the weight up to it, itself
-// included. More than 64 are narrowed by histograms over the range of their places.
+// Among the list's `size` tokens the `members` whose places lie in last .. first: the
+// one, in order, at which their running count (by_count) or weight passes the target.
+// Its place, and in *mass the weight up to it, itself included. More than one wave
+// searches are narrowed by histograms over the range of their places.
 template <int kThreads, int kBins, int kList>
-__device__ inline void find_in_list(SampleShared<kThreads, kBins, kList> &s, uint32_t members,
-                                    bool by_count, uint64_t target, uint64_t *at,
-                                    uint64_t *mass) {
+__device__ inline uint64_t find_in_list(SampleShared<kThreads, kBins, kList> &s, uint32_t size,
+                                        uint64_t last, uint64_t first, uint32_t members,
+                                        bool by_count, uint64_t target, uint64_t *mass) {
   __shared__ uint64_t scratch[kThreads / 64];
-  const uint32_t size = members;
-  uint64_t last = 0, first = ~0ULL, before = 0;  // places taken into account
-  while (members > 64) {
+  uint64_t before = 0;
+  while (members > kFew) {
     uint64_t lo = ~0ULL, hi = 0;
     for (uint32_t i = threadIdx.x; i < size; i += kThreads) {
       const uint64_t p = s.list_place[i];
@@ -514,12 +614,9 @@ __device__ inline void find_in_list(SampleShared<kThreads, kBins, kList> &s, uin
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < size; i += kThreads) {
       const uint64_t p = s.list_place[i];
-      if (p >= last && p <= first) {
-        const int sub = static_cast<int>((hi - p) >> shift);
-        atomicAdd(&s.sub_count[sub], 1U);
-        atomicAdd(reinterpret_cast<unsigned long long *>(&s.sub_mass[sub]),
-                  static_cast<unsigned long long>(s.list_mass[i]));
-      }
+      if (p >= last && p <= first)
+        WaveBins{s.sub_mass, s.sub_count}.add(static_cast<int>((hi - p) >> shift),
+                                              s.list_mass[i]);
     }
     __syncthreads();
     scan_bins<kThreads>(s.sub_count, s.sub_mass, 256, s.wave_count, s.wave_mass);
@@ -546,53 +643,61 @@ __device__ inline void find_in_list(SampleShared<kThreads, kBins, kList> &s, uin
     }
   }
   __syncthreads();
-  if (threadIdx.x < members) {
-    const uint64_t p = s.few_place[threadIdx.x], own = s.few_mass[threadIdx.x];
-    uint64_t ahead = 0;
-    uint32_t rank = 0;
-    for (uint32_t j = 0; j < members; ++j)
-      if (s.few_place[j] > p) {
-        ahead += s.few_mass[j];
-        ++rank;
-      }
-    if (by_count ? rank == target : ahead <= target && target < ahead + own) {
-      s.found_place = p;
-      s.found_mass = before + ahead + own;
+  if (threadIdx.x < 64) {
+    constexpr int kPer = kFew / 64;
+    uint64_t spot[kPer], w[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const uint32_t i = 64 * e + threadIdx.x;
+      spot[e] = i < members ? s.few_place[i] : 0;
+      w[e] = i < members ? s.few_mass[i] : 0;
+    }
+    const uint64_t place = wave_find<kPer>(spot, w, members,
+                                           WaveBins{s.sub_mass, s.sub_count}, by_count, target,
+                                           before);
+    if (threadIdx.x == 0) {
+      s.found_place = place;
+      s.found_mass = before;
     }
   }
   __syncthreads();
-  *at = s.found_place;
   *mass = s.found_mass;
-  __syncthreads();
+  return s.found_place;
 }
 
-// Lists the tokens that `take` wants, and their weights.
-template <typename T, int kThreads, int kBins, int kList, typename F>
+// Lists the tokens whose values lie in `one` or `other` and whose place begins with
+// `prefix` above `shift` bits, and their weights.
+template <typename T, int kThreads, int kBins, int kList>
 __device__ inline void gather(const Row<T> &row, const Scale &scale,
-                              SampleShared<kThreads, kBins, kList> &s, F &&take) {
+                              SampleShared<kThreads, kBins, kList> &s, const Values &one,
+                              const Values &other, int shift, uint64_t prefix) {
   if (threadIdx.x == 0)
     s.fill = 0;
   __syncthreads();
-  row.template each<kThreads>([&](float v, int i) {
-    if (!take(v, i))
-      return;
-    const uint32_t slot = atomicAdd(&s.fill, 1U);
-    s.list_place[slot] = place(v, i);
-    s.list_mass[slot] = scale.weight(v, s.powers);
+  const auto wanted = [&](float v) { return one.has(v) || other.has(v); };
+  row.template each<kThreads, 4>(wanted, [&](float v, int i) {
+    const uint64_t p = place(v, i);
+    if (p >> shift == prefix)
+      s.list_place[atomicAdd(&s.fill, 1U)] = p;
   });
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < s.fill; i += kThreads)
+    s.list_mass[i] = scale.weight(value_of(s.list_place[i]), s.powers);
   __syncthreads();
 }
 
-// find_in_list over the `members` tokens of a bin.
+// Lists the `members` tokens of a bin, or, where they are more than the list holds,
+// those of them among which the target is passed; members, target and the weight
+// before them follow.
 template <typename T, int kThreads, int kBins, int kList>
-__device__ inline void find_in_bin(const Row<T> &row, const Scale &scale,
-                                   SampleShared<kThreads, kBins, kList> &s, int bin,
-                                   uint32_t members, bool by_count, uint64_t target,
-                                   uint64_t *at, uint64_t *mass) {
-  // Tokens whose place begins with `prefix` in its bits above `shift`; mass before.
-  uint64_t prefix = 0, before = 0;
+__device__ inline void list_bin(const Row<T> &row, const Scale &scale,
+                                SampleShared<kThreads, kBins, kList> &s, int bin,
+                                bool by_count, uint32_t &members, uint64_t &target,
+                                uint64_t &before) {
+  // Tokens whose place begins with `prefix` in its bits above `shift`.
+  uint64_t prefix = 0;
   int shift = 56;
-  const float first_bin = static_cast<float>(bin);
+  const Values values = scale.values(bin, bin);
   while (members > kList) {
     // More than the list holds (many equal logits): 8 bits of the place at a time.
     shift -= 8;
@@ -601,9 +706,7 @@ __device__ inline void find_in_bin(const Row<T> &row, const Scale &scale,
       s.sub_mass[i] = 0;
     }
     __syncthreads();
-    row.template each<kThreads>([&](float v, int i) {
-      if (!scale.in_bin(v, first_bin))
-        return;
+    row.template each<kThreads, 1>([&](float v) { return values.has(v); }, [&](float v, int i) {
       const uint64_t p = place(v, i);
       if (p >> (shift + 8) != prefix)
         return;
@@ -625,51 +728,183 @@ __device__ inline void find_in_bin(const Row<T> &row, const Scale &scale,
     prefix = prefix << 8 | static_cast<uint64_t>(255 - digit);
     __syncthreads();
   }
-  gather(row, scale, s, [&](float v, int i) {
-    return scale.in_bin(v, first_bin) && place(v, i) >> shift == prefix;
+  gather(row, scale, s, values, values, shift, prefix);
+}
+
+// Largest and lowest value of a row (its part); +infinity for NaN too, which no
+// row is sampled with.
+template <int kThreads, typename T>
+__device__ inline float2 row_range(const Row<T> &row, float *scratch) {
+  float top = -INFINITY, low = INFINITY;
+  bool bad = false;
+  row.template each<kThreads, 4>([&](float v, int) {
+    bad |= v != v;
+    top = fmaxf(top, v);
+    low = fminf(low, v);
   });
-  find_in_list(s, members, by_count, target, at, mass);
-  *mass += before;
+  top = block_reduce<kThreads>(bad ? INFINITY : top, scratch, Most{});
+  low = block_reduce<kThreads>(low, scratch, Least{});
+  return make_float2(top, low);
+}
+
+// Adds a row's (its part's) tokens to the histogram in LDS; weights only where
+// `weighted`. Returns this thread's weight of what min-p keeps (a beginning of the
+// order too, as the weight falls along it).
+template <int kThreads, typename T>
+__device__ inline uint64_t fill_bins(const Row<T> &row, const Scale &scale, bool weighted,
+                                     uint64_t least, uint32_t *count, uint64_t *mass,
+                                     const double *powers) {
+  uint64_t kept = 0;
+  const auto add = [&](float v, bool keep) {
+    const int bin = scale.bin(v);
+    if (bin < 0)
+      return;
+    const uint64_t w = scale.weight(v, powers);
+    atomicAdd(&count[bin], 1U);
+    atomicAdd(reinterpret_cast<unsigned long long *>(&mass[bin]),
+              static_cast<unsigned long long>(w));
+    if (keep)
+      kept += w >= least ? w : 0;
+  };
+  if (!weighted)
+    row.template each<kThreads, 4>([&](float v, int) {
+      const int bin = scale.bin(v);
+      if (bin >= 0)
+        atomicAdd(&count[bin], 1U);
+    });
+  else if (least > 0)
+    row.template each<kThreads, 1>([&](float v, int) { add(v, true); });
+  else
+    row.template each<kThreads, 1>([&](float v, int) { add(v, false); });
+  return kept;
+}
+
+// Few rows of a large vocabulary run in three launches: ranges of a row's parts,
+// their histograms, and a block per row that joins them and finds the borders.
+// Histograms are integers: the split does not show in them.
+constexpr int kSplitBins = 1024;
+struct SplitRows {
+  int parts, part;   // of a row; tokens of a part, a multiple of 8
+  float2 *range;     // [rows][parts]
+  uint64_t *kept;    // [rows][parts]
+  uint64_t *mass;    // [rows][parts][kSplitBins]
+  uint32_t *count;
+  __device__ float2 whole_range(size_t r) const {
+    float2 all = range[r * parts];
+    for (int i = 1; i < parts; ++i) {
+      const float2 v = range[r * parts + i];
+      all = make_float2(fmaxf(all.x, v.x), fminf(all.y, v.y));
+    }
+    return all;
+  }
+};
+
+template <typename T, int kThreads>
+__global__ __launch_bounds__(kThreads) void sample_range_kernel(const SampleArgs a,
+                                                                const SplitRows split) {
+  __shared__ float scratch[kThreads / 64];
+  const size_t r = blockIdx.x / split.parts;
+  const int first = static_cast<int>(blockIdx.x % split.parts) * split.part;
+  const Row<T> row(a, r, first, min(split.part, a.vocab - first));
+  const float2 range = row_range<kThreads>(row, scratch);
+  if (threadIdx.x == 0)
+    split.range[blockIdx.x] = range;
+}
+
+template <typename T, int kThreads>
+__global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs a,
+                                                               const SplitRows split) {
+  __shared__ uint64_t mass[kSplitBins];
+  __shared__ uint32_t count[kSplitBins];
+  __shared__ uint64_t scratch[kThreads / 64];
+  __shared__ double powers[64];
+  const size_t r = blockIdx.x / split.parts;
+  const int first = static_cast<int>(blockIdx.x % split.parts) * split.part;
+  const Row<T> row(a, r, first, min(split.part, a.vocab - first));
+  const Cuts cuts(a, r);
+  const float2 range = split.whole_range(r);
+  if (!cuts.samples(range.x) || cuts.greedy())
+    return;
+  const bool weighted = !cuts.has_k(a.vocab);
+  for (int i = threadIdx.x; i < kSplitBins; i += kThreads) {
+    count[i] = 0;
+    mass[i] = 0;
+  }
+  if (threadIdx.x < 64)
+    powers[threadIdx.x] = kPowers[threadIdx.x] * 4398046511104.0;
+  __syncthreads();
+  const Scale scale(range.x, range.y, cuts.temperature, kSplitBins);
+  uint64_t kept =
+      fill_bins<kThreads>(row, scale, weighted, cuts.least(), count, mass, powers);
+  kept = block_reduce<kThreads>(kept, scratch, Sum{});
+  __syncthreads();
+  const size_t at = static_cast<size_t>(blockIdx.x) * kSplitBins;
+  for (int i = threadIdx.x; i < kSplitBins; i += kThreads) {
+    split.count[at + i] = count[i];
+    if (weighted)
+      split.mass[at + i] = mass[i];
+  }
+  if (threadIdx.x == 0)
+    split.kept[blockIdx.x] = kept;
 }
 
 // A block per row. A row with top-k counts its bins first: where the tokens up to
 // the k-th one's bin fit the list, everything else happens there.
-template <typename T, int kThreads, int kBins, int kList>
-__global__ __launch_bounds__(kThreads) void sample_block_kernel(const SampleArgs a) {
+template <typename T, int kThreads, int kBins, int kList, bool kSplit>
+__global__ __launch_bounds__(kThreads) void sample_block_kernel(const SampleArgs a,
+                                                                const SplitRows split) {
+  static_assert(!kSplit || kBins == kSplitBins, "the parts' histograms");
   __shared__ SampleShared<kThreads, kBins, kList> s;
   __shared__ float scratch_f[kThreads / 64];
   __shared__ int scratch_i[kThreads / 64];
   __shared__ uint64_t scratch_u[kThreads / 64];
   const size_t r = blockIdx.x;
-  Row<T> row;
-  row.logits = static_cast<const T *>(a.logits) + r * a.row_stride;
-  row.vocab = a.vocab;
-  row.vector = reinterpret_cast<uintptr_t>(row.logits) % 16 == 0;
+  const Row<T> row(a, r, 0, a.vocab);
   const Cuts cuts(a, r);
-  for (int i = threadIdx.x; i < kBins; i += kThreads) {
-    s.count[i] = 0;
-    s.mass[i] = 0;
-  }
+  // (With its parts' histograms at hand a row starts from their sums.)
+  const auto sum_parts = [&](bool weighted) {
+    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+      uint32_t c = 0;
+      uint64_t m = 0;
+      const size_t at = r * split.parts * kBins + i;
+      for (int p0 = 0; p0 < split.parts; p0 += 8) {  // eight loads at a time
+        uint32_t cs[8];
+        uint64_t ms[8];
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+          const bool has = p0 + p < split.parts;
+          const size_t from = at + static_cast<size_t>(has ? p0 + p : 0) * kBins;
+          cs[p] = has ? split.count[from] : 0;
+          ms[p] = has && weighted ? split.mass[from] : 0;
+        }
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+          c += cs[p];
+          m += ms[p];
+        }
+      }
+      s.count[i] = c;
+      s.mass[i] = m;
+    }
+  };
+  const auto clear = [&] {
+    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+      s.count[i] = 0;
+      s.mass[i] = 0;
+    }
+  };
   if (threadIdx.x < 64)
-    s.powers[threadIdx.x] = kPowers[threadIdx.x];
-
-  float top = -INFINITY, low = INFINITY;
-  bool bad = false;
-  row.template each<kThreads>([&](float v, int) {
-    bad |= v != v;
-    top = fmaxf(top, v);
-    low = fminf(low, v);
-  });
-  top = block_reduce<kThreads>(top, scratch_f, Most{});
-  low = block_reduce<kThreads>(low, scratch_f, Least{});
-  if (__syncthreads_or(bad) || !(top < INFINITY) || top == -INFINITY || !cuts.valid()) {
+    s.powers[threadIdx.x] = kPowers[threadIdx.x] * 4398046511104.0;
+  const float2 range = kSplit ? split.whole_range(r) : row_range<kThreads>(row, scratch_f);
+  const float top = range.x;
+  if (!cuts.samples(top)) {
     if (threadIdx.x == 0)
       a.tokens[r] = kNoToken;
     return;
   }
   if (cuts.greedy()) {
     int first = a.vocab;
-    row.template each<kThreads>([&](float v, int i) {
+    row.template each<kThreads, 4>([&](float v, int i) {
       first = v == top ? min(first, i) : first;
     });
     first = block_reduce<kThreads>(first, scratch_i, Least{});
@@ -677,17 +912,21 @@ __global__ __launch_bounds__(kThreads) void sample_block_kernel(const SampleArgs
       a.tokens[r] = static_cast<uint32_t>(first);
     return;
   }
-  const Scale scale(top, low, cuts.temperature, kBins);
+  const Scale scale(top, range.y, cuts.temperature, kBins);
   const uint64_t least = cuts.least();
-  const bool has_k = cuts.top_k > 0 && cuts.top_k < a.vocab;
+  const bool has_k = cuts.has_k(a.vocab);
   const uint32_t rank = static_cast<uint32_t>(cuts.top_k) - 1;
-  uint64_t at = 0, mass = 0, total = 0, kept = 0;
+  uint64_t total = 0, kept = 0;
+  uint32_t count = 0;  // tokens of weight, or listed
+  bool listed = false;
   if (has_k) {
-    row.template each<kThreads>([&](float v, int) {
-      const int bin = scale.bin(v);
-      if (bin >= 0)
-        atomicAdd(&s.count[bin], 1U);
-    });
+    if (kSplit) {
+      sum_parts(false);
+    } else {
+      clear();
+      __syncthreads();
+      fill_bins<kThreads>(row, scale, false, least, s.count, s.mass, s.powers);
+    }
     __syncthreads();
     const uint32_t last = s.count[kBins - 1];
     __syncthreads();
@@ -695,100 +934,159 @@ __global__ __launch_bounds__(kThreads) void sample_block_kernel(const SampleArgs
     const uint32_t all = s.count[kBins - 1] + last;
     // (Tokens without weight are not counted: with fewer than k, all are kept.)
     const int bin = last_at_most(s.count, kBins, min(rank, all - 1));
-    const uint32_t through = bin == kBins - 1 ? all : s.count[bin + 1];
-    if (through <= kList) {
-      const float end = static_cast<float>(bin + 1);
-      gather(row, scale, s, [&](float v, int) {
-        return (top - v) * scale.bin_scale < end && top - v <= scale.reach;
-      });
-      if (rank < all - 1) {
-        find_in_list(s, through, true, rank, &at, &total);
-      } else {
-        uint64_t sum = 0;
-        for (uint32_t i = threadIdx.x; i < through; i += kThreads)
-          sum += s.list_mass[i];
-        total = block_reduce<kThreads>(sum, scratch_u, Sum{});
+    count = bin == kBins - 1 ? all : s.count[bin + 1];
+    if (count <= kList) {
+      listed = true;
+      const Values all_kept = scale.values(0, bin);
+      gather(row, scale, s, all_kept, all_kept, 56, 0);
+      for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
+        total += s.list_mass[i];
+        kept += s.list_mass[i] >= least ? s.list_mass[i] : 0;
       }
-      if (cuts.top_p < 1.0F)
-        find_in_list(s, through, false, cuts.nucleus(total), &at, &total);
-      if (cuts.min_p > 0.0F) {
-        for (uint32_t i = threadIdx.x; i < through; i += kThreads)
-          kept += s.list_mass[i] >= least ? s.list_mass[i] : 0;
-        kept = block_reduce<kThreads>(kept, scratch_u, Sum{});
-        total = Least{}(total, kept);
-      }
-      find_in_list(s, through, false, cuts.draw(total), &at, &mass);
-      if (threadIdx.x == 0)
-        a.tokens[r] = 0xffffffU - static_cast<uint32_t>(at & 0xffffff);
-      return;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kThreads) {
-      s.count[i] = 0;
-      s.mass[i] = 0;
+      total = block_reduce<kThreads>(total, scratch_u, Sum{});
     }
     __syncthreads();
   }
-  // Counts and weights by bin, and the weight of what min-p keeps (a beginning of the
-  // order too, as the weight falls along it).
-  row.template each<kThreads>([&](float v, int) {
-    const int bin = scale.bin(v);
-    if (bin < 0)
-      return;
-    const uint64_t w = scale.weight(v, s.powers);
-    atomicAdd(&s.count[bin], 1U);
-    atomicAdd(reinterpret_cast<unsigned long long *>(&s.mass[bin]),
-              static_cast<unsigned long long>(w));
-    if (least > 0)
-      kept += w >= least ? w : 0;
-  });
-  __syncthreads();
-  const uint32_t last_count = s.count[kBins - 1];
-  const uint64_t last_mass = s.mass[kBins - 1];
-  __syncthreads();
-  scan_bins<kThreads>(s.count, s.mass, kBins, s.wave_count, s.wave_mass);
-  const uint32_t total_count = s.count[kBins - 1] + last_count;
-  total = s.mass[kBins - 1] + last_mass;
-  const auto members = [&](int bin) {
-    return (bin == kBins - 1 ? total_count : s.count[bin + 1]) - s.count[bin];
-  };
-  if (has_k && rank < total_count - 1) {
-    const int bin = last_at_most(s.count, kBins, rank);
-    find_in_bin(row, scale, s, bin, members(bin), true, rank - s.count[bin], &at, &mass);
-    total = s.mass[bin] + mass;
-  }
-  if (cuts.top_p < 1.0F) {
-    const uint64_t target = cuts.nucleus(total);
-    const int bin = last_at_most(s.mass, kBins, target);
-    find_in_bin(row, scale, s, bin, members(bin), false, target - s.mass[bin], &at, &mass);
-    total = s.mass[bin] + mass;
+  if (!listed) {
+    if (kSplit && !has_k) {
+      sum_parts(true);
+      for (int p = threadIdx.x; p < split.parts; p += kThreads)
+        kept += split.kept[r * split.parts + p];
+    } else {
+      clear();
+      __syncthreads();
+      kept = fill_bins<kThreads>(row, scale, true, least, s.count, s.mass, s.powers);
+    }
+    __syncthreads();
+    const uint32_t last_count = s.count[kBins - 1];
+    const uint64_t last_mass = s.mass[kBins - 1];
+    __syncthreads();
+    scan_bins<kThreads>(s.count, s.mass, kBins, s.wave_count, s.wave_mass);
+    count = s.count[kBins - 1] + last_count;
+    total = s.mass[kBins - 1] + last_mass;
   }
   if (cuts.min_p > 0.0F)
-    total = Least{}(total, block_reduce<kThreads>(kept, scratch_u, Sum{}));
-  const uint64_t target = cuts.draw(total);
-  const int bin = last_at_most(s.mass, kBins, target);
-  find_in_bin(row, scale, s, bin, members(bin), false, target - s.mass[bin], &at, &mass);
+    kept = block_reduce<kThreads>(kept, scratch_u, Sum{});
+  const auto in_bins = [&](int first, int last) {  // their tokens
+    return (last == kBins - 1 ? count : s.count[last + 1]) - s.count[first];
+  };
+  const auto drawn = [&](uint64_t of) {
+    return cuts.draw(cuts.min_p > 0.0F ? Least{}(of, kept) : of);
+  };
+  // The top-k border, the nucleus' border, the draw: one after the other through the
+  // same code. The draw's bin depends on the nucleus' border only by that border's
+  // place inside its own bin: the bins it may be in are listed along with that one.
+  uint64_t at = 0;
+  bool joint = false;
+  uint32_t size = count;
+#pragma unroll 1
+  for (int border = 0; border < 3; ++border) {
+    const bool by_count = border == 0;
+    uint64_t target, before = 0;
+    if (border == 0) {
+      if (!has_k || rank >= count - 1)
+        continue;
+      target = rank;
+    } else if (border == 1) {
+      if (cuts.top_p >= 1.0F)
+        continue;
+      target = cuts.nucleus(total);
+    } else {
+      target = drawn(total);
+    }
+    uint32_t members = count;
+    uint64_t last = 0, first = ~0ULL;
+    if (!listed) {
+      const int bin = by_count ? last_at_most(s.count, kBins, static_cast<uint32_t>(target))
+                               : last_at_most(s.mass, kBins, target);
+      members = in_bins(bin, bin);
+      before = s.mass[bin];
+      target -= by_count ? s.count[bin] : before;
+      if (border == 1) {
+        const uint64_t through = bin == kBins - 1 ? total : Least{}(total, s.mass[bin + 1]);
+        const int low = last_at_most(s.mass, kBins, drawn(before + 1));
+        const int high = last_at_most(s.mass, kBins, drawn(through));
+        joint = members + in_bins(low, high) <= kList;
+        if (joint) {
+          gather(row, scale, s, scale.values(bin, bin), scale.values(low, high), 56, 0);
+          size = s.fill;
+          __syncthreads();
+        }
+      }
+      if (joint) {
+        const Values values = scale.values(bin, bin);
+        last = values.last();
+        first = values.first();
+      } else {
+        list_bin(row, scale, s, bin, by_count, members, target, before);
+        size = members;
+      }
+    }
+    at = find_in_list(s, size, last, first, members, by_count, target, &total);
+    total += before;
+    __syncthreads();
+  }
   if (threadIdx.x == 0)
     a.tokens[r] = 0xffffffU - static_cast<uint32_t>(at & 0xffffff);
 }
 
+// Parts of a row: none below 16384 tokens (a block's own passes are short) and from
+// 512 rows on (they fill the chip); else enough for four blocks a CU, of 8192 tokens
+// and more.
+int parts_of(size_t rows, size_t vocab) {
+  if (vocab <= 16384 || rows >= 512)
+    return 1;
+  return static_cast<int>(std::min<size_t>((1024 + rows - 1) / rows, (vocab + 8191) / 8192));
+}
+size_t split_bytes(size_t rows, size_t parts) {
+  return rows * parts * (kSplitBins * (sizeof(uint64_t) + sizeof(uint32_t)) + sizeof(uint64_t) +
+                         sizeof(float2));
+}
+
 template <typename T>
-void launch_sample(const SampleArgs &args, size_t rows, hipStream_t stream) {
+Status launch_sample(const SampleArgs &args, size_t rows, void *workspace, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(rows));
-  if (args.vocab <= 512)
+  const size_t vocab = static_cast<size_t>(args.vocab);
+  SplitRows split{};
+  split.parts = workspace == nullptr ? 1 : parts_of(rows, vocab);
+  if (args.vocab <= 512) {
     hipLaunchKernelGGL((sample_wave_kernel<T, 8>), grid, dim3(64), 0, stream, args);
-  else if (args.vocab <= 1024)
+  } else if (args.vocab <= 1024) {
     hipLaunchKernelGGL((sample_wave_kernel<T, 16>), grid, dim3(64), 0, stream, args);
-  else if (args.vocab <= 16384)
-    hipLaunchKernelGGL((sample_block_kernel<T, 256, 1024, 512>), grid, dim3(256), 0, stream, args);
-  else
-    hipLaunchKernelGGL((sample_block_kernel<T, 1024, 2048, 2048>), grid, dim3(1024), 0, stream,
-                       args);
+  } else if (args.vocab <= 16384) {
+    hipLaunchKernelGGL((sample_block_kernel<T, 256, 1024, 512, false>), grid, dim3(256), 0,
+                       stream, args, split);
+  } else if (split.parts == 1) {
+    hipLaunchKernelGGL((sample_block_kernel<T, 1024, 1024, 2048, false>), grid, dim3(1024), 0,
+                       stream, args, split);
+  } else {
+    const size_t parts = static_cast<size_t>(split.parts);
+    split.part = static_cast<int>(((vocab + parts - 1) / parts + 7) / 8 * 8);
+    // (Rounded up, fewer parts may do.)
+    split.parts = static_cast<int>((vocab + split.part - 1) / split.part);
+    split.mass = static_cast<uint64_t *>(workspace);
+    split.kept = split.mass + rows * parts * kSplitBins;
+    split.range = reinterpret_cast<float2 *>(split.kept + rows * parts);
+    split.count = reinterpret_cast<uint32_t *>(split.range + rows * parts);
+    const dim3 blocks(static_cast<unsigned>(rows * split.parts));
+    hipLaunchKernelGGL((sample_range_kernel<T, 512>), blocks, dim3(512), 0, stream, args, split);
+    EVO_TRY(launch_status("sample_range_kernel"));
+    hipLaunchKernelGGL((sample_bins_kernel<T, 512>), blocks, dim3(512), 0, stream, args, split);
+    EVO_TRY(launch_status("sample_bins_kernel"));
+    hipLaunchKernelGGL((sample_block_kernel<T, 1024, 1024, 2048, true>), grid, dim3(1024), 0,
+                       stream, args, split);
+  }
+  return launch_status("sample_kernel");
 }
 
 }  // namespace
 
-size_t sample_workspace_bytes(size_t, size_t) { return 0; }
+size_t sample_workspace_bytes(size_t rows, size_t vocab) {
+  if (rows == 0 || rows > (size_t{1} << 30) || vocab == 0 || vocab > (size_t{1} << 20))
+    return 0;
+  const int parts = parts_of(rows, vocab);
+  return parts == 1 ? 0 : split_bytes(rows, static_cast<size_t>(parts));
+}
 
 Status sample_tokens(int dtype, const void *logits, size_t rows, size_t vocab, size_t row_stride,
                      const float *temperature, const int32_t *top_k, const float *top_p,
@@ -802,15 +1100,16 @@ Status sample_tokens(int dtype, const void *logits, size_t rows, size_t vocab, s
     return {ErrorCode::kInvalidArgument, "sample: logits are F32, BF16 or F16"};
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == kElementF32 ? 4 : 2) != 0)
     return {ErrorCode::kInvalidArgument, "sample: misaligned logits"};
+  if (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||
+                               workspace_bytes < sample_workspace_bytes(rows, vocab)))
+    return {ErrorCode::kInvalidArgument, "sample: workspace too small or not 16-byte aligned"};
   const SampleArgs args{logits, static_cast<int>(vocab), row_stride, temperature, top_k,
                         top_p, min_p, uniform, tokens};
   if (dtype == kElementF32)
-    launch_sample<float>(args, rows, stream);
-  else if (dtype == kElementBF16)
-    launch_sample<__bf16>(args, rows, stream);
-  else
-    launch_sample<_Float16>(args, rows, stream);
-  return launch_status("sample_kernel");
+    return launch_sample<float>(args, rows, workspace, stream);
+  if (dtype == kElementBF16)
+    return launch_sample<__bf16>(args, rows, workspace, stream);
+  return launch_sample<_Float16>(args, rows, workspace, stream);
 }
 
 }  // namespace evo::hip

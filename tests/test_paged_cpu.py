@@ -128,6 +128,16 @@ def test_sample_refused(bad):
                None, None, None, v["uniform"], v["tokens"], None, 0, None)
 
 
+def test_sample_workspace_refused():
+    need = N.call("evo_hip_sample_workspace_bytes", 4, 100000)
+    assert need > 0
+    assert N.call("evo_hip_sample_workspace_bytes", 4, 512) == 0
+    for workspace, size in ((C, need - 1), (C + 8, need)):
+        with pytest.raises(N.OpError, match="workspace"):
+            N.call("evo_hip_sample", N.DTYPE_F32, A, 4, 100000, 100000, None, None, None, None, A,
+                   B, workspace, size, None)
+
+
 # ------------------------------------------------------------ index rules
 @pytest.fixture(scope="module")
 def rules():
