@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace evo::hip {
 
@@ -91,42 +92,75 @@ __device__ inline uint64_t weight_units(double z, const double *powers) {
   return __builtin_bit_cast(uint64_t, shifted) - 0x4330000000000000ULL;
 }
 
-template <typename V, typename F> __device__ inline V wave_reduce(V v, F &&f) {
-#pragma unroll
-  for (int offset = 32; offset > 0; offset >>= 1)
-    v = f(v, __shfl_xor(v, offset, 64));
-  return v;
-}
-__device__ inline uint64_t lane_value(uint64_t v, int lane) {
-  const uint32_t low = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), lane);
-  const uint32_t high = __builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), lane);
-  return static_cast<uint64_t>(high) << 32 | low;
-}
-template <int kThreads, typename V, typename F>
-__device__ inline V block_reduce(V v, V *scratch, F &&f) {
-  v = wave_reduce(v, f);
-  if constexpr (kThreads > 64) {
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0)
-      scratch[threadIdx.x >> 6] = v;
-    __syncthreads();
-    constexpr int kWaves = kThreads / 64;
-    v = scratch[(threadIdx.x & 63) % kWaves];
-#pragma unroll
-    for (int offset = kWaves / 2; offset > 0; offset >>= 1)
-      v = f(v, __shfl_xor(v, offset, 64));
-  }
-  return v;
-}
 struct Most {
   template <typename V> __device__ V operator()(V x, V y) const { return x > y ? x : y; }
+  template <typename V> static __device__ V identity() {
+    return std::is_same_v<V, float> ? static_cast<V>(-INFINITY) : static_cast<V>(0);
+  }
 };
 struct Least {
   template <typename V> __device__ V operator()(V x, V y) const { return x < y ? x : y; }
+  template <typename V> static __device__ V identity() {
+    return std::is_same_v<V, float> ? static_cast<V>(INFINITY)
+           : std::is_same_v<V, int> ? static_cast<V>(0x7fffffff)
+                                    : static_cast<V>(~0ULL);
+  }
 };
 struct Sum {
   template <typename V> __device__ V operator()(V x, V y) const { return x + y; }
+  template <typename V> static __device__ V identity() { return 0; }
 };
+
+// v of another lane, by the DPP control kCtrl; `other` in lanes it has none for.
+template <int kCtrl, int kRows, typename V> __device__ inline V dpp(V other, V v) {
+  constexpr int kWords = sizeof(V) / 4;
+  uint32_t from[kWords], to[kWords];
+  __builtin_memcpy(from, &v, sizeof(V));
+  __builtin_memcpy(to, &other, sizeof(V));
+#pragma unroll
+  for (int i = 0; i < kWords; ++i)
+    to[i] = __builtin_amdgcn_update_dpp(to[i], from[i], kCtrl, kRows, 0xf, false);
+  __builtin_memcpy(&v, to, sizeof(V));
+  return v;
+}
+// f over the lanes 0 .. this one: rows of 16 lanes, then row to row, in registers
+// (shuffles go through LDS: six of them take a microsecond of a lone wave).
+template <typename F, typename V> __device__ inline V wave_scan(V v) {
+  const F f;
+  const V none = F::template identity<V>();
+  v = f(v, dpp<0x111, 0xf>(none, v));  // row_shr 1, 2, 4, 8
+  v = f(v, dpp<0x112, 0xf>(none, v));
+  v = f(v, dpp<0x114, 0xf>(none, v));
+  v = f(v, dpp<0x118, 0xf>(none, v));
+  v = f(v, dpp<0x142, 0xa>(none, v));  // row_bcast 15: into rows 1 and 3
+  return f(v, dpp<0x143, 0xc>(none, v));  // row_bcast 31: into rows 2 and 3
+}
+template <typename V> __device__ inline V lane_value(V v, int lane) {
+  constexpr int kWords = sizeof(V) / 4;
+  uint32_t words[kWords];
+  __builtin_memcpy(words, &v, sizeof(V));
+#pragma unroll
+  for (int i = 0; i < kWords; ++i)
+    words[i] = __builtin_amdgcn_readlane(words[i], lane);
+  __builtin_memcpy(&v, words, sizeof(V));
+  return v;
+}
+template <typename V, typename F> __device__ inline V wave_reduce(V v, F) {
+  return lane_value(wave_scan<F>(v), 63);
+}
+template <int kThreads, typename V, typename F>
+__device__ inline V block_reduce(V v, V *scratch, F f) {
+  v = wave_reduce(v, f);
+  if constexpr (kThreads > 64) {
+    const int lane = threadIdx.x & 63;
+    __syncthreads();
+    if (lane == 0)
+      scratch[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = wave_reduce(lane < kThreads / 64 ? scratch[lane] : F::template identity<V>(), f);
+  }
+  return v;
+}
 
 // A row's parameters.
 struct Cuts {
@@ -195,23 +229,29 @@ struct Scale {
     const float below = top - v;
     return below <= reach ? static_cast<int>(below * bin_scale) : -1;
   }
-  // Lowest value of the bins 0 .. `bin`: a search of 64 values at a time over the
-  // values' order. All lanes of a wave call it, with the same bin.
+  // Lowest value of the bins 0 .. `bin`: the 64 values around the one that the bin's
+  // end maps back to are tried, then, 64 at a time, all. All lanes of a wave call it,
+  // with the same bin.
   __device__ float lowest(int bin) const {
     const float end = static_cast<float>(bin + 1);
-    uint32_t below = 0x007fffffU;  // -infinity, in no bin
+    const auto inside = [&](uint64_t key) {
+      const float v = value_of(key << 24);
+      return key >= 0xff800000U || ((top - v) * bin_scale < end && top - v <= reach);
+    };
+    const uint64_t lane = threadIdx.x & 63;
+    uint64_t below = ordered(fmaxf(top - end / bin_scale, -3.0e38F)) - 33;
+    const uint64_t tried = __ballot(inside(below + lane));
+    if (tried != 0 && (tried & 1) == 0) {
+      below += __builtin_ctzll(tried) - 1;
+    } else {
+      below = 0x007fffffU;  // -infinity, in no bin
 #pragma unroll 1
-    for (int shift = 26; shift >= 0; shift = shift == 2 ? 0 : shift - 6) {
-      const uint64_t key = below + ((static_cast<uint64_t>(threadIdx.x & 63) + 1) << shift);
-      bool in = true;
-      if (key < 0xff800000U) {
-        const float v = value_of(key << 24);
-        in = (top - v) * bin_scale < end && top - v <= reach;
+      for (int shift = 26; shift >= 0; shift = shift == 2 ? 0 : shift - 6) {
+        const uint64_t in = __ballot(inside(below + ((lane + 1) << shift)));
+        below += static_cast<uint64_t>(in == 0 ? 64 : __builtin_ctzll(in)) << shift;
       }
-      const uint64_t inside = __ballot(in);
-      below += static_cast<uint32_t>(inside == 0 ? 64 : __builtin_ctzll(inside)) << shift;
     }
-    return value_of(static_cast<uint64_t>(below + 1) << 24);
+    return value_of((below + 1) << 24);
   }
   __device__ Values values(int first, int last) const {  // of a run of bins
     return {lowest(last), first == 0 ? INFINITY : lowest(first - 1)};
@@ -263,17 +303,12 @@ struct LaneBins {
     }
     const uint64_t own_m = m;
     const uint32_t own_c = c;
-#pragma unroll
-    for (int offset = 1; offset < 64; offset <<= 1) {
-      const uint64_t up_m = __shfl_up(m, offset, 64);
-      const uint32_t up_c = __shfl_up(c, offset, 64);
-      m += lane >= offset ? up_m : 0;
-      c += lane >= offset ? up_c : 0;
-    }
+    m = wave_scan<Sum>(m);
+    c = wave_scan<Sum>(c);
     mass_before = m - own_m;
     count_before = c - own_c;
     mass_total = lane_value(m, 63);
-    count_total = __builtin_amdgcn_readlane(c, 63);
+    count_total = lane_value(c, 63);
   }
 };
 // The bin in which the running count or weight passes a target, what lies before it,
@@ -298,9 +333,8 @@ __device__ inline Hit locate(const LaneBins &b, bool by_count, uint64_t target) 
   }
   const uint64_t owner = __ballot(h.bin >= 0);
   const int from = owner == 0 ? 0 : __builtin_ctzll(owner);
-  return Hit{__builtin_amdgcn_readlane(h.bin, from), lane_value(h.mass_before, from),
-             static_cast<uint32_t>(__builtin_amdgcn_readlane(h.count_before, from)),
-             static_cast<uint32_t>(__builtin_amdgcn_readlane(h.members, from))};
+  return Hit{lane_value(h.bin, from), lane_value(h.mass_before, from),
+             lane_value(h.count_before, from), lane_value(h.members, from)};
 }
 
 // Among the tokens that the lanes hold (spot[e] != 0: a place; w[e]: its weight;
@@ -458,16 +492,18 @@ template <typename T> struct Row {  // or a part of one, from token `first`
   // of them at a time and as many ahead. kLoads 1 where f is long: code of more copies
   // is fetched more slowly than it runs; 4 where it is short and the loads are what
   // takes the time.
-  // Only values that `wanted` has reach f; where it is given, the values of a load are
-  // looked over together first.
-  struct All {
-    __device__ bool operator()(float) const { return true; }
-  };
   template <int kThreads, int kLoads, typename F> __device__ void each(F &&f) const {
-    each<kThreads, kLoads>(All{}, f);
+    each_load<kThreads, kLoads>(
+        [&](const auto &values, int i) {
+#pragma unroll
+          for (int e = 0; e < 16 / static_cast<int>(sizeof(T)); ++e)
+            f(static_cast<float>(values[e]), i + e);
+        },
+        f);
   }
+  // The same with whole(values of a load, index of the first) for the 16-byte loads.
   template <int kThreads, int kLoads, typename W, typename F>
-  __device__ void each(W &&wanted, F &&f) const {
+  __device__ void each_load(W &&whole_load, F &&f) const {
     constexpr int kPer = 16 / sizeof(T);
     typedef T wide __attribute__((ext_vector_type(kPer)));
     int tail = 0;
@@ -488,18 +524,8 @@ template <typename T> struct Row {  // or a part of one, from token `first`
         load(next, c + kThreads * kLoads);
 #pragma unroll
         for (int a = 0; a < kLoads; ++a)
-          if (a == 0 || c + a * kThreads < whole) {
-            bool any = false;
-#pragma unroll
-            for (int e = 0; e < kPer; ++e)
-              any |= wanted(static_cast<float>(now[a][e]));
-            if (any) {
-#pragma unroll
-              for (int e = 0; e < kPer; ++e)
-                if (wanted(static_cast<float>(now[a][e])))
-                  f(static_cast<float>(now[a][e]), first + (c + a * kThreads) * kPer + e);
-            }
-          }
+          if (a == 0 || c + a * kThreads < whole)
+            whole_load(now[a], first + (c + a * kThreads) * kPer);
 #pragma unroll
         for (int a = 0; a < kLoads; ++a)
           now[a] = next[a];
@@ -508,8 +534,7 @@ template <typename T> struct Row {  // or a part of one, from token `first`
     }
 #pragma unroll 1
     for (int i = tail + threadIdx.x; i < vocab; i += kThreads)
-      if (wanted(static_cast<float>(logits[i])))
-        f(static_cast<float>(logits[i]), first + i);
+      f(static_cast<float>(logits[i]), first + i);
   }
 };
 
@@ -543,13 +568,8 @@ __device__ inline void scan_bins(uint32_t *count, uint64_t *mass, int size, uint
   const uint32_t own_c = c;
   const uint64_t own_m = m;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int offset = 1; offset < 64; offset <<= 1) {
-    const uint32_t up_c = __shfl_up(c, offset, 64);
-    const uint64_t up_m = __shfl_up(m, offset, 64);
-    c += lane >= offset ? up_c : 0;
-    m += lane >= offset ? up_m : 0;
-  }
+  c = wave_scan<Sum>(c);
+  m = wave_scan<Sum>(m);
   if (lane == 63) {
     wave_count[wave] = c;
     wave_mass[wave] = m;
@@ -674,15 +694,33 @@ __device__ inline void gather(const Row<T> &row, const Scale &scale,
   if (threadIdx.x == 0)
     s.fill = 0;
   __syncthreads();
+  const auto push = [&](int i) {
+    if (shift < 56 && place(static_cast<float>(row.logits[i]), i) >> shift != prefix)
+      return;
+    s.list_place[atomicAdd(&s.fill, 1U)] = static_cast<uint64_t>(i);
+  };
   const auto wanted = [&](float v) { return one.has(v) || other.has(v); };
-  row.template each<kThreads, 4>(wanted, [&](float v, int i) {
-    const uint64_t p = place(v, i);
-    if (p >> shift == prefix)
-      s.list_place[atomicAdd(&s.fill, 1U)] = p;
-  });
+  // Few of the tokens are wanted: a load's make a mask without a branch.
+  row.template each_load<kThreads, 4>(
+      [&](const auto &values, int i) {
+        uint32_t mask = 0;
+#pragma unroll
+        for (int e = 0; e < 16 / static_cast<int>(sizeof(T)); ++e)
+          mask |= wanted(static_cast<float>(values[e])) ? 1U << e : 0;
+        for (; mask != 0; mask &= mask - 1)
+          push(i + __builtin_ctz(mask));
+      },
+      [&](float v, int i) {
+        if (wanted(v))
+          push(i);
+      });
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < s.fill; i += kThreads)
-    s.list_mass[i] = scale.weight(value_of(s.list_place[i]), s.powers);
+  for (uint32_t i = threadIdx.x; i < s.fill; i += kThreads) {
+    const int token = static_cast<int>(s.list_place[i]);
+    const float v = static_cast<float>(row.logits[token]);
+    s.list_place[i] = place(v, token);
+    s.list_mass[i] = scale.weight(v, s.powers);
+  }
   __syncthreads();
 }
 
@@ -706,7 +744,9 @@ __device__ inline void list_bin(const Row<T> &row, const Scale &scale,
       s.sub_mass[i] = 0;
     }
     __syncthreads();
-    row.template each<kThreads, 1>([&](float v) { return values.has(v); }, [&](float v, int i) {
+    row.template each<kThreads, 1>([&](float v, int i) {
+      if (!values.has(v))
+        return;
       const uint64_t p = place(v, i);
       if (p >> (shift + 8) != prefix)
         return;
