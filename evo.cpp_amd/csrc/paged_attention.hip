@@ -26,6 +26,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace evo::hip {
 
@@ -255,6 +256,15 @@ __device__ inline void scores(const Step<T, kD> &step, const typename Mfma<T>::v
   }
 }
 
+// Infinities and NaN in a word of two elements.
+template <typename T> __device__ inline bool nonfinite(uint32_t word) {
+  constexpr uint32_t kExponent = std::is_same_v<T, __bf16> ? 0x7f80U : 0x7c00U;
+  return (word & kExponent) == kExponent || (word >> 16 & kExponent) == kExponent;
+}
+template <typename T> __device__ inline float element(uint16_t bits) {
+  return static_cast<float>(__builtin_bit_cast(T, bits));
+}
+
 // Adds a step's scores and values to the rows' state.
 template <typename T, int kD>
 __device__ inline void attend(const f32x4 (&score)[2], const uint32_t (&v)[8][kD / 32],
@@ -301,17 +311,42 @@ __device__ inline void attend(const f32x4 (&score)[2], const uint32_t (&v)[8][kD
   }
 }
 
-// 16 rows of a key/value head and a chunk of their keys per block; its four
-// waves take every fourth 32-key step and join their states through LDS.
+// The keys of a step (bit 16u + 4 * (lane / 16) + i) with an infinity or NaN among
+// their values, which are zeroed.
+template <typename T, int kD>
+__device__ inline uint32_t odd_keys(uint32_t (&v)[8][kD / 32]) {
+  const int g = (threadIdx.x & 63) >> 4;
+  uint32_t keys = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    bool odd = false;
+#pragma unroll
+    for (int w = 0; w < kD / 32; ++w)
+      odd |= nonfinite<T>(v[j][w]);
+    const uint64_t lanes = __ballot(odd);
+#pragma unroll
+    for (int other = 0; other < 4; ++other)
+      keys |= (lanes >> (16 * other) & 0xffff) != 0 ? 1U << (j / 4 * 16 + 4 * other + j % 4) : 0;
+    if ((lanes >> (16 * g) & 0xffff) != 0) {
+#pragma unroll
+      for (int w = 0; w < kD / 32; ++w)
+        v[j][w] = 0;
+    }
+  }
+  return keys;
+}
+
+// 16 rows of a key/value head and a chunk of their keys per block; its kWaves waves
+// take every kWaves-th 32-key step and join their states through LDS.
 // Blocks below prefix_blocks take the shared keys, rows of the whole batch.
 template <int kD> struct StreamShared {
   float top[4][16], sum[4][16];
   __attribute__((aligned(16))) float out[4][16][kD + 4];
 };
-template <typename T, int kD>
+template <typename T, int kD, int kWaves>
 __device__ inline void stream_block(const AttendArgs &a, const BlockWork &work,
                                     StreamShared<kD> &shared) {
-  constexpr int kRows = 16, kWaves = 4, kVec = kD / 16, kSteps = kD / 32;
+  constexpr int kRows = 16, kVec = kD / 16, kSteps = kD / 32;
   typedef typename Mfma<T>::vec vec;
   auto &top_s = shared.top, &sum_s = shared.sum;
   auto &out_s = shared.out;
@@ -397,6 +432,7 @@ __device__ inline void stream_block(const AttendArgs &a, const BlockWork &work,
       const int here[2] = {page[0], page[1]}, k_here = k0;
       k0 += kStride;
       const bool more = k0 < key1;
+      uint32_t apart = 0;  // keys of the step
       if (more) {
         pages = pages_of(entries, k0);
 #pragma unroll
@@ -421,37 +457,89 @@ __device__ inline void stream_block(const AttendArgs &a, const BlockWork &work,
               step.v[4 * u + i][w] = from + i < end ? step.v[4 * u + i][w] : 0;
           }
         }
+        // An infinity or NaN among the values of a key that some rows of the tile see
+        // and others do not: the key's values go through the products as zeros, and
+        // to the rows that see it one by one.
+        if (tile.first_position != tile.last_position)
+          apart = odd_keys<T, kD>(step.v);
       }
       attend<T, kD>(score, step.v, a.scale2, state);
+      for (; apart != 0; apart &= apart - 1) {
+        const int key = __builtin_ctz(apart), u = key / 16;
+        const float base = state.top == -INFINITY ? 0.0F : state.top;
+        float s = score[0][0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j)
+          s = 4 * u + key % 4 == j ? score[j / 4][j % 4] : s;
+        s = __shfl(s, 16 * (key % 16 / 4) + col, 64);
+        const uint16_t *v =
+            a.cache.values + (here[u] * a.cache.page_stride + kv_head * a.cache.head_stride +
+                              ((k_here + key) & ((1 << a.cache.page_shift) - 1)) *
+                                  a.cache.token_stride);
+        const float weight = __builtin_amdgcn_exp2f(fmaf(s, a.scale2, -base));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int t = 0; t < kVec; ++t)
+            if (s != -INFINITY)
+              state.out[t][i] =
+                  fmaf(weight, element<T>(v[kVec * (4 * g + i) + t]), state.out[t][i]);
+      }
       if (!more)
         break;
     }
   }
 
-  // Join the four waves: each leaves its rows' maximum, sum and output.
-  float sum = state.sum + __shfl_xor(state.sum, 16, 64);
-  sum += __shfl_xor(sum, 32, 64);
-  if (g == 0) {
-    top_s[wave][col] = state.top;
-    sum_s[wave][col] = sum;
+  // Join the waves: each leaves its rows' maximum, sum and output, of eight the last
+  // four to the first.
+  state.sum += __shfl_xor(state.sum, 16, 64);
+  state.sum += __shfl_xor(state.sum, 32, 64);
+  const auto leave = [&](int at) {
+    if (g == 0) {
+      top_s[at][col] = state.top;
+      sum_s[at][col] = state.sum;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int t = 0; t < kVec; ++t)
+        out_s[at][col][kVec * (4 * g + i) + t] = state.out[t][i];
+  };
+  if constexpr (kWaves == 8) {
+    if (wave >= 4)
+      leave(wave - 4);
+    __syncthreads();
+    if (wave < 4) {
+      const float top = fmaxf(state.top, top_s[wave][col]), base = top == -INFINITY ? 0.0F : top;
+      const float mine = __builtin_amdgcn_exp2f(state.top - base);
+      const float theirs = __builtin_amdgcn_exp2f(top_s[wave][col] - base);
+      state.top = top;
+      state.sum = state.sum * mine + sum_s[wave][col] * theirs;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int t = 0; t < kVec; ++t)
+          state.out[t][i] =
+              state.out[t][i] * mine + out_s[wave][col][kVec * (4 * g + i) + t] * theirs;
+    }
+    __syncthreads();
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int t = 0; t < kVec; ++t)
-      out_s[wave][col][kVec * (4 * g + i) + t] = state.out[t][i];
+  if (wave < 4)
+    leave(wave);
   __syncthreads();
+  if (wave >= 4)
+    return;
   // Thread: row tid / 16, elements kVec * (tid % 16) ...
   const int r = threadIdx.x >> 4, d = kVec * (threadIdx.x & 15);
   if (tile.row0 + r >= tile.rows)
     return;
   float top = top_s[0][r];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w)
+  for (int w = 1; w < 4; ++w)
     top = fmaxf(top, top_s[w][r]);
   float total = 0.0F, o[kVec] = {};
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < 4; ++w) {
     const float scale = top_s[w][r] == -INFINITY ? 0.0F
                                                  : __builtin_amdgcn_exp2f(top_s[w][r] - top);
     total = fmaf(sum_s[w][r], scale, total);
@@ -519,9 +607,41 @@ template <typename Q> __device__ inline Q transposed(const uint16_t *from) {
   return __builtin_bit_cast(Q, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(from)));
 }
 
+// out += V^T P over a tile's 64 keys, P = exp2(score * scale2 - base).
+template <typename T, int kD>
+__device__ inline void add_values(const uint16_t *v_s, const f32x16 (&score)[2], float scale2,
+                                  float base, float &sum, f32x16 (&out)[kD / 32]) {
+  constexpr int kUnits = kD / 8;
+  typedef typename Mfma<T>::vec vec;
+  typedef T quad __attribute__((ext_vector_type(4)));
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk) {
+    vec p;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      p[j] = static_cast<T>(
+          __builtin_amdgcn_exp2f(fmaf(score[kk / 2][8 * (kk % 2) + j], scale2, -base)));
+    sum = Mfma<T>::add(p, sum);
+#pragma unroll
+    for (int t = 0; t < kD / 32; ++t) {
+      // Keys 16kk + 4 half + (0 .. 3) and 8 more; elements 32t + 16 * (lane / 16 % 2) ..
+      quad part[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = 16 * kk + 8 * j + 4 * half + (lane & 15) / 4;
+        const int d = 32 * t + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+        part[j] = transposed<quad>(v_s + r * kD + 8 * swizzle_v<kUnits>(r, d / 8) + d % 8);
+      }
+      const vec v = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      out[t] = Mfma<T>::run(v, p, out[t]);
+    }
+  }
+}
+
 template <typename T, int kD>
 __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
-                                  uint16_t *tile_lds) {  // [2][K, V][plane]
+                                  uint16_t *tile_lds) {  // [2][K, V][plane], odd keys
   constexpr int kRows = 128, kKeys = 64, kUnits = kD / 8;
   constexpr int kSteps = kD / 16, kTiles = kD / 32;   // K-steps of S^T, 32-row tiles of O^T
   constexpr int kPlane = kKeys * kD;                  // elements of K or V in a stage
@@ -617,7 +737,8 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
   issue(key0, 0, pages);
   if (key0 + kKeys < key1)
     next_pages = pages_at(key0 + kKeys);
-  int stage = 0;
+  int stage = 0, odd_tiles = 0, odd_first = 0;
+  uint16_t *odd_s = tile_lds + 4 * kPlane;  // [tile][wave], 16 keys a bit each
   for (int k0 = key0; k0 < key1; k0 += kKeys, stage ^= 1) {
     wait_dma<0>();
     // Values that no row sees (behind the last key, or of no page) may be
@@ -629,6 +750,33 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
       uint16_t *v = tile_lds + stage * 2 * kPlane + kPlane + 16 * wave * kD;
       for (int i = good * kUnits + lane; i < 16 * kUnits; i += 64)
         *reinterpret_cast<uint4 *>(v + 8 * i) = make_uint4(0, 0, 0, 0);
+    }
+    // Keys with an infinity or NaN among their values that some rows of the block see
+    // and others do not: 0 * NaN again. Their values are zeroed too, and added at the
+    // end to the rows that see them.
+    if (!prefix && tile.first_position != tile.last_position &&
+        k0 + kKeys - 1 > tile.first_position) {
+      uint16_t *v = tile_lds + stage * 2 * kPlane + kPlane + 16 * wave * kD;
+      uint32_t odd_rows = 0;
+#pragma unroll
+      for (int i = 0; i < kOps; ++i) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(v + 8 * (64 * i + lane));
+        const uint64_t odd = __ballot(nonfinite<T>(x.x) || nonfinite<T>(x.y) ||
+                                      nonfinite<T>(x.z) || nonfinite<T>(x.w));
+        if (odd != 0) {
+#pragma unroll
+          for (int r = 0; r < kOpRows; ++r)
+            if ((odd >> (r * kUnits) & ((uint64_t{1} << kUnits) - 1)) != 0)
+              odd_rows |= 1U << (kOpRows * i + r);
+          if ((odd_rows >> (kOpRows * i + lane / kUnits) & 1) != 0)
+            *reinterpret_cast<uint4 *>(v + 8 * (64 * i + lane)) = make_uint4(0, 0, 0, 0);
+        }
+      }
+      if (odd_tiles == 0)
+        odd_first = k0;
+      if (lane == 0)
+        odd_s[4 * odd_tiles + wave] = static_cast<uint16_t>(odd_rows);
+      ++odd_tiles;
     }
     __syncthreads();
     if (k0 + kKeys < key1) {
@@ -686,30 +834,35 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
       top = next;
     }
     const float base = top == -INFINITY ? 0.0F : top;
+    add_values<T, kD>(v_s, score, a.scale2, base, sum, out);
+  }
+
+  // The odd keys' values, to the rows that see them (their weights are in the sum).
+  if (odd_tiles > 0) {
+    __syncthreads();
+    for (int i = 0; i < 4 * odd_tiles; ++i)
+      for (uint32_t bits = odd_s[i]; bits != 0; bits &= bits - 1) {
+        const int key = odd_first + 16 * i + __builtin_ctz(bits);
+        const size_t at = table[key >> a.cache.page_shift] * a.cache.page_stride +
+                          work.kv_head * a.cache.head_stride +
+                          (key & slot_mask) * a.cache.token_stride;
+        const uint16_t *k = a.cache.keys + at + 8 * half, *v = a.cache.values + at + 4 * half;
+        float dot = 0.0F;
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      vec p;
+        for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        p[j] = static_cast<T>(
-            __builtin_amdgcn_exp2f(fmaf(score[kk / 2][8 * (kk % 2) + j], a.scale2, -base)));
-      sum = Mfma<T>::add(p, sum);
+          for (int e = 0; e < 8; ++e)
+            dot = fmaf(static_cast<float>(q[s][e]), element<T>(k[16 * s + e]), dot);
+        dot += __shfl_xor(dot, 32, 64);
+        const float weight = __builtin_amdgcn_exp2f(fmaf(dot, a.scale2, -top));
+        if (key <= position) {
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        // Keys 16kk + 4 half + (0 .. 3) and 8 more; elements 32t + 16 * (lane / 16 % 2) ..
-        typedef T quad __attribute__((ext_vector_type(4)));
-        quad part[2];
+          for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int r = 16 * kk + 8 * j + 4 * half + (lane & 15) / 4;
-          const int d = 32 * t + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
-          const uint16_t *from = v_s + r * kD + 8 * swizzle_v<kUnits>(r, d / 8) + d % 8;
-          part[j] = transposed<quad>(from);
+            for (int e = 0; e < 16; ++e)
+              out[t][e] = fmaf(weight, element<T>(v[32 * t + (e >> 2) * 8 + (e & 3)]), out[t][e]);
         }
-        const vec v = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
-        out[t] = Mfma<T>::run(v, p, out[t]);
       }
-    }
   }
 
   const float total = sum + __shfl_xor(sum, 32, 64);
@@ -750,22 +903,28 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
 }
 
 // ------------------------------------------------------------- launches
-constexpr size_t kTileLds = 2 * 2 * 64 * sizeof(uint16_t);  // per element of a head
-static_assert(kTileLds * 128 <= 64 * 1024, "default LDS limit, two blocks per CU");
+// LDS of a 128-row block: two stages of K and V, and a word for each 16 keys of the
+// tiles that only some of its rows see (four: 128 positions and a tile's rest).
+constexpr size_t tile_lds_bytes(size_t head_dim) {
+  return 2 * 2 * 64 * head_dim * sizeof(uint16_t) + 16 * sizeof(uint16_t);
+}
+static_assert(2 * tile_lds_bytes(128) <= 160 * 1024, "two blocks per CU");
 
-// kKind 0: 16-row blocks; 1: 128-row blocks; 2: 128-row blocks on the shared keys
-// beside 16-row ones on each sequence's own, in one launch.
+// Blocks of a launch. kSmall: 16 rows, 4 waves; kSmallWide: 16 rows, 8 waves; kLarge:
+// 128 rows; kMixed: 128 rows on the shared keys beside 16 rows on each sequence's own.
+enum BlockKind : int { kSmall, kSmallWide, kLarge, kMixed };
 template <typename T, int kD, int kKind>
-__global__ __launch_bounds__(256, kKind == 0 ? 3 : 2) void paged_attention_kernel(
-    const AttendArgs a, unsigned prefix_blocks, unsigned tiles) {
+__global__ __launch_bounds__(kKind == kSmallWide ? 512 : 256, kKind == kSmall ? 3 : 2) void
+paged_attention_kernel(const AttendArgs a, unsigned prefix_blocks, unsigned tiles) {
   extern __shared__ __attribute__((aligned(16))) uint16_t attend_lds[];
   if (blockIdx.x == prefix_blocks)
     report_bad_sequences(a.batch);
   const BlockWork work = block_work(a, prefix_blocks, tiles);
-  if (kKind == 1 || (kKind == 2 && work.prefix))
+  if (kKind == kLarge || (kKind == kMixed && work.prefix))
     tile_block<T, kD>(a, work, attend_lds);
   else
-    stream_block<T, kD>(a, work, *reinterpret_cast<StreamShared<kD> *>(attend_lds));
+    stream_block<T, kD, kKind == kSmallWide ? 8 : 4>(
+        a, work, *reinterpret_cast<StreamShared<kD> *>(attend_lds));
 }
 
 // Rows whose keys lay in several chunks: the chunks rescaled to their common
@@ -876,6 +1035,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const AttendArgs a, 
 
 struct AttendPlan {
   bool own_stream, prefix_stream;  // 16-row blocks, else 128-row ones
+  bool wide;                       // 16-row blocks of 8 waves
   size_t tiles, prefix_tiles;      // row tiles of the own keys, of the shared ones
   int chunk, prefix_chunk, prefix_slots, slots;
 };
@@ -956,7 +1116,11 @@ AttendPlan plan_attention(const PagedCache &cache, const PagedBatch &batch, size
                                           tokens * group / rows + std::min(sequences, tokens));
   const size_t own = std::max(1, batch.max_length - batch.shared_length);
   const double part_bytes = static_cast<double>(tokens * heads * dim * sizeof(float));
-  if (plan.own_stream) {
+  if (plan.own_stream && batch.shared_length == 0 && plan.tiles * kv <= 512 && own <= 512) {
+    // One block for all keys of a row: the launch that joins chunks would take longer.
+    plan.wide = own > 128;
+    plan.chunk = 512;
+  } else if (plan.own_stream) {
     plan.chunk = stream_chunk(own, plan.tiles * kv);
   } else {
     // The longest sequence is taken to bring the most rows too; the others' lengths
@@ -1000,16 +1164,18 @@ Status launch_attention(const AttendArgs &args, const AttendPlan &plan, hipStrea
   const size_t blocks = prefix_blocks + plan.tiles * kv * (plan.slots - plan.prefix_slots);
   if (blocks >= (size_t{1} << 31))
     return {ErrorCode::kInvalidArgument, "paged_attention: grid too large"};
-  auto kernel = paged_attention_kernel<T, kD, 1>;
-  size_t lds = kTileLds * kD;
+  auto kernel = paged_attention_kernel<T, kD, kLarge>;
+  size_t lds = tile_lds_bytes(kD);
   if (plan.own_stream && (plan.prefix_stream || prefix_blocks == 0)) {
-    kernel = paged_attention_kernel<T, kD, 0>;
+    kernel = plan.wide ? paged_attention_kernel<T, kD, kSmallWide>
+                       : paged_attention_kernel<T, kD, kSmall>;
     lds = sizeof(StreamShared<kD>);
   } else if (plan.own_stream) {
-    kernel = paged_attention_kernel<T, kD, 2>;
+    kernel = paged_attention_kernel<T, kD, kMixed>;
     lds = std::max(lds, sizeof(StreamShared<kD>));
   }
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), lds, stream, args,
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(plan.wide ? 512 : 256),
+                     lds, stream, args,
                      static_cast<unsigned>(prefix_blocks), static_cast<unsigned>(plan.tiles));
   EVO_TRY(launch_status("paged_attention_kernel"));
   if (plan.slots == 1)

@@ -8,8 +8,8 @@ import pytest
 import torch
 
 from evo_hip import native as N
-from paged_util import (CODES, DEVICE, KINDS, Paged, attend, check_attention, exact_rotation,
-                        half_step)
+from paged_util import (CODES, DEVICE, KINDS, Paged, attend, check_attention, exact_attention,
+                        exact_rotation, half_step)
 
 pytestmark = pytest.mark.gpu
 
@@ -201,6 +201,44 @@ def test_shared_prefix_matches_own_pages():
     p.table[:, :shared // p.page] = p.shared_table
     whole = attend(p, query, 0.09, shared_length=0, shared_table=None)
     check_attention(p, query, 0.09, whole)
+
+
+@pytest.mark.parametrize("heads,kv_heads,n,length,kind,dim", [
+    (4, 4, 7, 7, "bf16", 128), (4, 4, 9, 300, "f16", 128), (8, 2, 4, 40, "bf16", 64),
+    (2, 1, 8, 70, "f16", 32), (4, 4, 100, 100, "bf16", 128), (8, 2, 90, 700, "f16", 128),
+    (7, 1, 40, 41, "bf16", 64), (4, 2, 70, 130, "f16", 32)])
+@pytest.mark.parametrize("what", [float("inf"), float("-inf"), float("nan")])
+def test_nonfinite_values_reach_only_rows_that_see_them(heads, kv_heads, n, length, kind, dim,
+                                                        what):
+    """A value and then a key of a later row: the rows before it keep their bits, the
+    others get it where the definition puts it."""
+    p = Paged([(n, length), (3, 20)], heads=heads, kv_heads=kv_heads, dim=dim, kind=kind)
+    query = p.normal(p.tokens, heads * dim)
+    clean = attend(p, query, dim ** -0.5).view(-1, heads, dim)
+    for position in (length - n + 1, length - 2, length - 1):
+        row, kv, d = position - (length - n), kv_heads - 1, dim - 3
+        mine = slice(kv * (heads // kv_heads), heads)
+        at = p.page_of(0, position), kv, position % p.page, d
+        kept = p.values[at].clone()
+        p.values[at] = what
+        out = attend(p, query, dim ** -0.5).view(-1, heads, dim)
+        p.values[at] = kept
+        touched = out[row:n, mine]
+        assert torch.equal(out[:row], clean[:row]) and torch.equal(out[n:], clean[n:])
+        got = touched[..., d].float()
+        assert got.isnan().all() if what != what else (got == what).all()
+        p.values[at] = 0.0
+        expected, far = exact_attention(p, query, dim ** -0.5)
+        p.values[at] = kept
+        rest = [e for e in range(dim) if e != d]
+        assert ((touched[..., rest].double() - expected[row:n, mine][..., rest]).abs() <=
+                far[row:n, mine][..., rest]).all()
+        kept = p.keys[at].clone()
+        p.keys[at] = float("nan")
+        out = attend(p, query, dim ** -0.5).view(-1, heads, dim)
+        p.keys[at] = kept
+        assert torch.equal(out[:row], clean[:row]) and torch.equal(out[n:], clean[n:])
+        assert out[row:n, mine].isnan().all()
 
 
 def test_attention_rows_without_keys_are_zero():
