@@ -123,9 +123,10 @@ __device__ inline bool find_tile(const AttendArgs &a, int tile, int *sequence, i
     }
     const uint64_t found = __ballot(base + through > tile);
     if (found != 0) {
+      // A sequence's last tiles, which see the most keys, come first.
       const int at = __builtin_ctzll(found);
       *sequence = s0 + at;
-      *tile_in = tile - base - __shfl(through - tiles, at, 64);
+      *tile_in = base + __shfl(through, at, 64) - 1 - tile;
       return true;
     }
     base += __shfl(through, 63, 64);
@@ -161,14 +162,12 @@ __device__ inline bool row_tile(const AttendArgs &a, bool prefix, int tile, RowT
 }
 
 // Block -> phase, key/value head, chunk and row tile. Heads vary fastest: with a
-// multiple of eight of them the blocks of a head share an XCD's L2. The last
-// tiles, which see the most keys, start first.
+// multiple of eight of them the blocks of a head share an XCD's L2.
 struct BlockWork {
   bool prefix;
   int kv_head, chunk, tile;
 };
-__device__ inline BlockWork block_work(const AttendArgs &a, unsigned prefix_blocks,
-                                       unsigned tiles) {
+__device__ inline BlockWork block_work(const AttendArgs &a, unsigned prefix_blocks) {
   BlockWork w;
   w.prefix = blockIdx.x < prefix_blocks;
   unsigned rest = w.prefix ? blockIdx.x : blockIdx.x - prefix_blocks;
@@ -177,8 +176,6 @@ __device__ inline BlockWork block_work(const AttendArgs &a, unsigned prefix_bloc
   const unsigned chunks = w.prefix ? a.prefix_slots : a.slots - a.prefix_slots;
   w.chunk = static_cast<int>(rest % chunks);
   w.tile = static_cast<int>(rest / chunks);
-  if (!w.prefix)
-    w.tile = static_cast<int>(tiles) - 1 - w.tile;
   return w;
 }
 
@@ -915,11 +912,11 @@ static_assert(2 * tile_lds_bytes(128) <= 160 * 1024, "two blocks per CU");
 enum BlockKind : int { kSmall, kSmallWide, kLarge, kMixed };
 template <typename T, int kD, int kKind>
 __global__ __launch_bounds__(kKind == kSmallWide ? 512 : 256, kKind == kSmall ? 3 : 2) void
-paged_attention_kernel(const AttendArgs a, unsigned prefix_blocks, unsigned tiles) {
+paged_attention_kernel(const AttendArgs a, unsigned prefix_blocks) {
   extern __shared__ __attribute__((aligned(16))) uint16_t attend_lds[];
   if (blockIdx.x == prefix_blocks)
     report_bad_sequences(a.batch);
-  const BlockWork work = block_work(a, prefix_blocks, tiles);
+  const BlockWork work = block_work(a, prefix_blocks);
   if (kKind == kLarge || (kKind == kMixed && work.prefix))
     tile_block<T, kD>(a, work, attend_lds);
   else
@@ -1175,8 +1172,7 @@ Status launch_attention(const AttendArgs &args, const AttendPlan &plan, hipStrea
     lds = std::max(lds, sizeof(StreamShared<kD>));
   }
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(plan.wide ? 512 : 256),
-                     lds, stream, args,
-                     static_cast<unsigned>(prefix_blocks), static_cast<unsigned>(plan.tiles));
+                     lds, stream, args, static_cast<unsigned>(prefix_blocks));
   EVO_TRY(launch_status("paged_attention_kernel"));
   if (plan.slots == 1)
     return Status::Ok();
