@@ -277,7 +277,7 @@ Status paged_append(const PagedCache &cache, const PagedBatch &batch, int dtype,
   const size_t passes = ceil_div((heads + 2 * kv) * (dim / 16), 256);
   const size_t parts = batch.tokens >= 512 ? 1 : passes;
   const size_t blocks = parts * static_cast<size_t>(batch.tokens);
-  if (blocks > (size_t{1} << 31) - 1)
+  if (blocks > ((size_t{1} << 32) - 1) / 256)  // a launch counts its threads in 32 bits
     return {ErrorCode::kInvalidArgument, "paged_append: grid too large"};
   const AppendArgs args{cache, batch, projected, row_stride, static_cast<int>(heads),
                         column_split ? 1 : 0, rope.inv_freq, static_cast<int>(rope.rotary_dim),

@@ -1159,7 +1159,15 @@ Status launch_attention(const AttendArgs &args, const AttendPlan &plan, hipStrea
   const size_t kv = static_cast<size_t>(args.cache.kv_heads);
   const size_t prefix_blocks = plan.prefix_tiles * kv * plan.prefix_slots;
   const size_t blocks = prefix_blocks + plan.tiles * kv * (plan.slots - plan.prefix_slots);
-  if (blocks >= (size_t{1} << 31))
+  // A launch counts its threads in 32 bits.
+  const size_t tokens = static_cast<size_t>(args.batch.tokens), heads = args.heads;
+  const bool split_join = plan.slots > 64 || (plan.slots > 8 && tokens * heads < (1U << 16));
+  // Four heads of a row per joining block, all of them where the rows fill the chip.
+  const size_t of_block =
+      split_join ? 1 : std::min(heads, 4 * std::max<size_t>(1, tokens * heads / 8192));
+  const size_t join_blocks = plan.slots == 1 ? 0 : tokens * ceil_div(heads, of_block);
+  constexpr size_t kMostThreads = (size_t{1} << 32) - 1;
+  if (blocks > kMostThreads / (plan.wide ? 512 : 256) || join_blocks > kMostThreads / 256)
     return {ErrorCode::kInvalidArgument, "paged_attention: grid too large"};
   auto kernel = paged_attention_kernel<T, kD, kLarge>;
   size_t lds = tile_lds_bytes(kD);
@@ -1176,17 +1184,10 @@ Status launch_attention(const AttendArgs &args, const AttendPlan &plan, hipStrea
   EVO_TRY(launch_status("paged_attention_kernel"));
   if (plan.slots == 1)
     return Status::Ok();
-  const size_t tokens = static_cast<size_t>(args.batch.tokens), heads = args.heads;
-  if (plan.slots > 8) {
-    hipLaunchKernelGGL((paged_combine_kernel<T, kD, true>),
-                       dim3(static_cast<unsigned>(tokens * heads)), dim3(256), 0, stream, args, 1);
-  } else {
-    // Four heads of a row per block, all of them where the rows fill the chip.
-    const size_t of_block = std::min(heads, 4 * std::max<size_t>(1, tokens * heads / 8192));
-    hipLaunchKernelGGL((paged_combine_kernel<T, kD, false>),
-                       dim3(static_cast<unsigned>(tokens * ceil_div(heads, of_block))), dim3(256),
-                       0, stream, args, static_cast<int>(of_block));
-  }
+  const auto join = split_join ? paged_combine_kernel<T, kD, true>
+                               : paged_combine_kernel<T, kD, false>;
+  hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(join_blocks)), dim3(256), 0, stream, args,
+                     static_cast<int>(of_block));
   return launch_status("paged_combine_kernel");
 }
 

@@ -1121,8 +1121,10 @@ Status launch_sample(const SampleArgs &args, size_t rows, void *workspace, hipSt
 
 }  // namespace
 
+constexpr size_t kMostRows = size_t{1} << 20;  // a launch counts its threads in 32 bits
+
 size_t sample_workspace_bytes(size_t rows, size_t vocab) {
-  if (rows == 0 || rows > (size_t{1} << 30) || vocab == 0 || vocab > (size_t{1} << 20))
+  if (rows == 0 || rows > kMostRows || vocab == 0 || vocab > (size_t{1} << 20))
     return 0;
   const int parts = parts_of(rows, vocab);
   return parts == 1 ? 0 : split_bytes(rows, static_cast<size_t>(parts));
@@ -1133,9 +1135,9 @@ Status sample_tokens(int dtype, const void *logits, size_t rows, size_t vocab, s
                      const float *min_p, const float *uniform, uint32_t *tokens, void *workspace,
                      size_t workspace_bytes, hipStream_t stream) {
   if (logits == nullptr || uniform == nullptr || tokens == nullptr || rows == 0 ||
-      rows > (size_t{1} << 30) || vocab == 0 || vocab > (size_t{1} << 20) || row_stride < vocab)
+      rows > kMostRows || vocab == 0 || vocab > (size_t{1} << 20) || row_stride < vocab)
     return {ErrorCode::kInvalidArgument,
-            "sample: null tensor, no rows, or a vocabulary of none or more than 2^20"};
+            "sample: null tensor, rows outside 1 .. 2^20, or a vocabulary outside 1 .. 2^20"};
   if (dtype != kElementF32 && dtype != kElementBF16 && dtype != kElementF16)
     return {ErrorCode::kInvalidArgument, "sample: logits are F32, BF16 or F16"};
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == kElementF32 ? 4 : 2) != 0)

@@ -305,7 +305,9 @@ typedef struct evo_hip_paged_cache {
  * positions, the first ones are padding. Rows behind the last sequence's
  * (token_start[sequences] < tokens) belong to none and are left as they are.
  *   max_tokens, max_length: host bounds on a sequence's rows and positions
- *     (max_length <= table_stride * page_size).
+ *     (max_length <= table_stride * page_size, at most 2^30). They choose the
+ *     launches: close bounds run faster. tokens is below 2^24, sequences at
+ *     most 2^20.
  *   token_start, lengths, page_table: int32 device arrays, read by each call
  *     when it runs, so a captured graph follows their changes within the
  *     bounds; page_table [sequences][table_stride].
@@ -352,8 +354,8 @@ typedef struct evo_hip_paged_batch {
  *   query      [tokens][query_stride] in the cache's dtype, the rotated
  *              queries (rows of 16-byte aligned heads, query_stride a multiple
  *              of 8); padding rows are zeroed and append nothing.
- * Rounded once, to nearest even; a value beyond FP16 becomes infinity.
- * Two sequences must not append to the same slot. */
+ * Rounded once, to nearest even; a value beyond FP16 becomes infinity. query
+ * must not overlap projected, and two sequences must not append to one slot. */
 EVO_API evo_status evo_hip_paged_append(const evo_hip_paged_cache *cache,
                                         const evo_hip_paged_batch *batch,
                                         evo_hip_dtype dtype, const void *projected,
@@ -373,8 +375,8 @@ EVO_API evo_status evo_hip_paged_append(const evo_hip_paged_cache *cache,
  *   scale  positive (1 / sqrt(head_dim) as a rule).
  * With shared_length the prefix's keys are read once for the rows of all
  * sequences, not once for each.
- * Positions beyond a sequence's rows may hold anything; within them, values have
- * to be finite for the rows before them to be.
+ * What a row does not see has no effect on it, infinities and NaN included:
+ * positions behind its own, slots behind a sequence's length, other pages.
  * The workspace (16-byte aligned, no initial contents) takes the partial
  * results of keys that are split over blocks; its size depends on the host
  * fields of the structs and heads alone. Calls that overlap need one each. */
@@ -389,7 +391,7 @@ EVO_API evo_status evo_hip_paged_attention(const evo_hip_paged_cache *cache,
                                            size_t workspace_bytes, void *stream);
 
 /* tokens[r] = one token of row r of logits [rows][row_stride] (F32, BF16 or
- * F16, vocab <= 2^20), in the order and with the cuts of evo_sampler_sample:
+ * F16; rows and vocab at most 2^20), in the order and with the cuts of evo_sampler_sample:
  * tokens by descending logit, equal ones by ascending index; of these the first
  * top_k (0, or vocab and more: all); weights exp(logit / temperature) in 64 bits;
  * of these the shortest beginning whose weight reaches top_p of what top-k left

@@ -190,6 +190,24 @@ def test_attention_shared_prefix(shared, sequences, heads, kv_heads, kind, dim):
               trailing=2))
 
 
+@pytest.mark.parametrize("sequences,shared,heads,kv_heads", [
+    ([(1, 40000)], 0, 2, 1), ([(2, 20001), (1, 3)], 0, 3, 1), ([(1, 33000), (2, 40000)], 32768, 2, 2),
+    ([(40, 30000)], 0, 1, 1), ([(1, 16400)] * 9, 16384, 4, 4)])
+def test_attention_many_chunks(sequences, shared, heads, kv_heads):
+    """Rows of more chunks than a wave has lanes, and both ways of joining them."""
+    run(Paged(sequences, heads=heads, kv_heads=kv_heads, dim=64, page=128, shared=shared))
+
+
+@pytest.mark.parametrize("shared", [0, 64])
+def test_attention_many_sequences(shared):
+    """More sequences than a wave looks at together, single tokens among prompts."""
+    counts = [1 + (37 * i) % 5 if i % 7 else 30 + i for i in range(150)]
+    sequences = [(n, shared + n + (13 * i) % 50) for i, n in enumerate(counts)]
+    run(Paged(sequences, heads=4, kv_heads=2, dim=64, shared=shared, trailing=1))
+    run(Paged([(1, shared + 1 + (29 * i) % 90) for i in range(300)], heads=4, kv_heads=2, dim=32,
+              shared=shared))
+
+
 def test_shared_prefix_matches_own_pages():
     """The same batch with the prefix's pages in every table row: the same rows, within
     the bounds of both."""

@@ -97,6 +97,19 @@ def test_attention_refused(bad):
         attend(**bad)
 
 
+def test_launches_beyond_32_bit_threads_refused():
+    """Rows that a launch could not count."""
+    with pytest.raises(N.OpError, match="grid too large"):
+        append(b=batch(tokens=1 << 24, max_tokens=4))
+    with pytest.raises(N.OpError, match="too many rows|grid too large"):
+        attend(b=batch(tokens=1 << 24, max_tokens=1 << 24), heads=256, query_stride=256 * 64,
+               out_stride=256 * 64)
+    with pytest.raises(N.OpError, match="grid too large"):
+        attend(b=batch(sequences=1 << 20, tokens=1 << 20, max_tokens=1, max_length=1 << 16,
+                       table_stride=1 << 12), c=cache(kv_heads=32), heads=32, query_stride=2048,
+               out_stride=2048)
+
+
 def test_attention_workspace_refused():
     """A call whose keys are split needs all of its workspace."""
     b = batch(max_length=60, shared_length=32, shared_table=A)
@@ -118,7 +131,7 @@ def test_workspace_query_of_refused_structs_is_zero():
 
 @pytest.mark.parametrize("bad", [
     dict(dtype=N.DTYPE_SPLIT), dict(logits=None), dict(logits=A + 2), dict(rows=0),
-    dict(rows=(1 << 30) + 1), dict(vocab=0), dict(vocab=(1 << 20) + 1, stride=1 << 21),
+    dict(rows=(1 << 20) + 1), dict(vocab=0), dict(vocab=(1 << 20) + 1, stride=1 << 21),
     dict(stride=511), dict(uniform=None), dict(tokens=None)])
 def test_sample_refused(bad):
     v = {**dict(dtype=N.DTYPE_F32, logits=A, rows=3, vocab=512, stride=512, uniform=A, tokens=B),
