@@ -492,36 +492,43 @@ template <typename T> struct Row {  // or a part of one, from token `first`
   // of them at a time and as many ahead. kLoads 1 where f is long: code of more copies
   // is fetched more slowly than it runs; 4 where it is short and the loads are what
   // takes the time.
+  static constexpr int kPer = 16 / sizeof(T);
+  typedef T wide __attribute__((ext_vector_type(16 / sizeof(T))));
+  template <int kThreads, int kLoads>
+  __device__ void load(wide (&to)[kLoads], int c = threadIdx.x) const {
+    const wide *src = reinterpret_cast<const wide *>(logits);
+#pragma unroll
+    for (int a = 0; a < kLoads; ++a)
+      if (vector && c + a * kThreads < vocab / kPer)
+        to[a] = src[c + a * kThreads];
+  }
   template <int kThreads, int kLoads, typename F> __device__ void each(F &&f) const {
+    wide now[kLoads];
+    load<kThreads, kLoads>(now);
+    each<kThreads, kLoads>(now, f);
+  }
+  // The same where the caller has called load() already, ahead of other waits.
+  template <int kThreads, int kLoads, typename F>
+  __device__ void each(wide (&now)[kLoads], F &&f) const {
     each_load<kThreads, kLoads>(
+        now,
         [&](const auto &values, int i) {
 #pragma unroll
-          for (int e = 0; e < 16 / static_cast<int>(sizeof(T)); ++e)
+          for (int e = 0; e < kPer; ++e)
             f(static_cast<float>(values[e]), i + e);
         },
         f);
   }
-  // The same with whole(values of a load, index of the first) for the 16-byte loads.
+  // And with whole(values of a load, index of the first) for the 16-byte loads.
   template <int kThreads, int kLoads, typename W, typename F>
-  __device__ void each_load(W &&whole_load, F &&f) const {
-    constexpr int kPer = 16 / sizeof(T);
-    typedef T wide __attribute__((ext_vector_type(kPer)));
+  __device__ void each_load(wide (&now)[kLoads], W &&whole_load, F &&f) const {
     int tail = 0;
     if (vector) {
       const int whole = vocab / kPer;
-      const wide *src = reinterpret_cast<const wide *>(logits);
-      wide now[kLoads], next[kLoads];
-      const auto load = [&](wide(&to)[kLoads], int c) {
-#pragma unroll
-        for (int a = 0; a < kLoads; ++a)
-          if (c + a * kThreads < whole)
-            to[a] = src[c + a * kThreads];
-      };
-      int c = threadIdx.x;
-      load(now, c);
+      wide next[kLoads];
 #pragma unroll 1
-      for (; c < whole; c += kThreads * kLoads) {
-        load(next, c + kThreads * kLoads);
+      for (int c = threadIdx.x; c < whole; c += kThreads * kLoads) {
+        load<kThreads, kLoads>(next, c + kThreads * kLoads);
 #pragma unroll
         for (int a = 0; a < kLoads; ++a)
           if (a == 0 || c + a * kThreads < whole)
@@ -701,7 +708,10 @@ __device__ inline void gather(const Row<T> &row, const Scale &scale,
   };
   const auto wanted = [&](float v) { return one.has(v) || other.has(v); };
   // Few of the tokens are wanted: a load's make a mask without a branch.
+  typename Row<T>::wide now[4];
+  row.template load<kThreads, 4>(now);
   row.template each_load<kThreads, 4>(
+      now,
       [&](const auto &values, int i) {
         uint32_t mask = 0;
 #pragma unroll
@@ -791,9 +801,9 @@ __device__ inline float2 row_range(const Row<T> &row, float *scratch) {
 // `weighted`. Returns this thread's weight of what min-p keeps (a beginning of the
 // order too, as the weight falls along it).
 template <int kThreads, typename T>
-__device__ inline uint64_t fill_bins(const Row<T> &row, const Scale &scale, bool weighted,
-                                     uint64_t least, uint32_t *count, uint64_t *mass,
-                                     const double *powers) {
+__device__ inline uint64_t fill_bins(const Row<T> &row, typename Row<T>::wide (&now)[2],
+                                     const Scale &scale, bool weighted, uint64_t least,
+                                     uint32_t *count, uint64_t *mass, const double *powers) {
   uint64_t kept = 0;
   const auto add = [&](float v, bool keep) {
     const int bin = scale.bin(v);
@@ -807,15 +817,15 @@ __device__ inline uint64_t fill_bins(const Row<T> &row, const Scale &scale, bool
       kept += w >= least ? w : 0;
   };
   if (!weighted)
-    row.template each<kThreads, 4>([&](float v, int) {
+    row.template each<kThreads, 2>(now, [&](float v, int) {
       const int bin = scale.bin(v);
       if (bin >= 0)
         atomicAdd(&count[bin], 1U);
     });
   else if (least > 0)
-    row.template each<kThreads, 1>([&](float v, int) { add(v, true); });
+    row.template each<kThreads, 2>(now, [&](float v, int) { add(v, true); });
   else
-    row.template each<kThreads, 1>([&](float v, int) { add(v, false); });
+    row.template each<kThreads, 2>(now, [&](float v, int) { add(v, false); });
   return kept;
 }
 
@@ -829,13 +839,11 @@ struct SplitRows {
   uint64_t *kept;    // [rows][parts]
   uint64_t *mass;    // [rows][parts][kSplitBins]
   uint32_t *count;
+  // A lane a part (there are at most 64); all lanes of a wave call it.
   __device__ float2 whole_range(size_t r) const {
-    float2 all = range[r * parts];
-    for (int i = 1; i < parts; ++i) {
-      const float2 v = range[r * parts + i];
-      all = make_float2(fmaxf(all.x, v.x), fminf(all.y, v.y));
-    }
-    return all;
+    const int lane = threadIdx.x & 63;
+    const float2 v = lane < parts ? range[r * parts + lane] : make_float2(-INFINITY, INFINITY);
+    return make_float2(wave_reduce(v.x, Most{}), wave_reduce(v.y, Least{}));
   }
 };
 
@@ -861,6 +869,8 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs 
   const size_t r = blockIdx.x / split.parts;
   const int first = static_cast<int>(blockIdx.x % split.parts) * split.part;
   const Row<T> row(a, r, first, min(split.part, a.vocab - first));
+  typename Row<T>::wide now[2];
+  row.template load<kThreads, 2>(now);
   const Cuts cuts(a, r);
   const float2 range = split.whole_range(r);
   if (!cuts.samples(range.x) || cuts.greedy())
@@ -875,7 +885,7 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs 
   __syncthreads();
   const Scale scale(range.x, range.y, cuts.temperature, kSplitBins);
   uint64_t kept =
-      fill_bins<kThreads>(row, scale, weighted, cuts.least(), count, mass, powers);
+      fill_bins<kThreads>(row, now, scale, weighted, cuts.least(), count, mass, powers);
   kept = block_reduce<kThreads>(kept, scratch, Sum{});
   __syncthreads();
   const size_t at = static_cast<size_t>(blockIdx.x) * kSplitBins;
@@ -963,9 +973,11 @@ __global__ __launch_bounds__(kThreads) void sample_block_kernel(const SampleArgs
     if (kSplit) {
       sum_parts(false);
     } else {
+      typename Row<T>::wide now[2];
+      row.template load<kThreads, 2>(now);
       clear();
       __syncthreads();
-      fill_bins<kThreads>(row, scale, false, least, s.count, s.mass, s.powers);
+      fill_bins<kThreads>(row, now, scale, false, least, s.count, s.mass, s.powers);
     }
     __syncthreads();
     const uint32_t last = s.count[kBins - 1];
@@ -993,9 +1005,11 @@ __global__ __launch_bounds__(kThreads) void sample_block_kernel(const SampleArgs
       for (int p = threadIdx.x; p < split.parts; p += kThreads)
         kept += split.kept[r * split.parts + p];
     } else {
+      typename Row<T>::wide now[2];
+      row.template load<kThreads, 2>(now);
       clear();
       __syncthreads();
-      kept = fill_bins<kThreads>(row, scale, true, least, s.count, s.mass, s.powers);
+      kept = fill_bins<kThreads>(row, now, scale, true, least, s.count, s.mass, s.powers);
     }
     __syncthreads();
     const uint32_t last_count = s.count[kBins - 1];
@@ -1070,13 +1084,15 @@ __global__ __launch_bounds__(kThreads) void sample_block_kernel(const SampleArgs
     a.tokens[r] = 0xffffffU - static_cast<uint32_t>(at & 0xffffff);
 }
 
-// Parts of a row: none below 16384 tokens (a block's own passes are short) and from
-// 512 rows on (they fill the chip); else enough for four blocks a CU, of 8192 tokens
-// and more.
+// Parts of a row: several where rows are long and too few to fill the chip, enough
+// for four blocks a CU, of 8192 tokens and more. us in parts and whole, BF16: 1 row of
+// 32000 27 and 28, of 65536 31 and 41, of 131072 36 and 65; 64 rows of 65536 42 and 46,
+// 128 rows of 65536 48 and 47, of 131072 62 and 73; 256 rows of 131072 85 and 78.
 int parts_of(size_t rows, size_t vocab) {
-  if (vocab <= 16384 || rows >= 512)
+  if (vocab < 32768 || rows > vocab / 1024)
     return 1;
-  return static_cast<int>(std::min<size_t>((1024 + rows - 1) / rows, (vocab + 8191) / 8192));
+  return static_cast<int>(
+      std::min<size_t>({(1024 + rows - 1) / rows, (vocab + 8191) / 8192, 64}));
 }
 size_t split_bytes(size_t rows, size_t parts) {
   return rows * parts * (kSplitBins * (sizeof(uint64_t) + sizeof(uint32_t)) + sizeof(uint64_t) +
