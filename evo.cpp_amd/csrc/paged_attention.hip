@@ -1038,57 +1038,108 @@ struct AttendPlan {
 };
 constexpr size_t kMostSlots = 128;  // of each phase (256 in the combining kernel)
 
-int chunk_of(size_t keys, size_t chunks, size_t granule) {
-  return static_cast<int>((keys + chunks * granule - 1) / (chunks * granule) * granule);
-}
+// What the parts of one phase may take, in bytes: half of the last cache. One chunk
+// is always taken.
+constexpr double kMostPartBytes = 128e6;
 
-// Keys per block of the 16-row kernel: enough blocks that the last ones to run do
-// not show, chunks of 128 keys (32 for each wave) and more.
-int stream_chunk(size_t keys, size_t blocks) {
-  const size_t wanted = std::max<size_t>(1, 8192 / std::max<size_t>(1, blocks));
-  return chunk_of(keys, std::min<size_t>({wanted, (keys + 127) / 128, kMostSlots}), 128);
+// The 16-row blocks of a phase: `blocks` of them for each chunk of the longest row's
+// `most` keys; the rows see as many each, or, uneven, anything up to that.
+struct StreamPhase {
+  size_t most, blocks;
+  bool uneven;
+  bool joined;  // parts are joined in any case
+  double all_part_bytes;
+};
+
+// Keys per block of the 16-row kernel: the split of least modelled time, its constants
+// fitted to measured splits of 33 batches (3% on average behind the best split of each,
+// 14% at most). Keys and values stream at 5.8 TB/s from 256 blocks on; 1000 keys take
+// a block 8 us, and as long at the end, while the chip runs empty; a part's block
+// costs 2 ns and joining the parts 9 us. Chunks are 128 keys and more, 32 for each wave.
+int stream_chunk(const StreamPhase &phase, size_t head_dim) {
+  int best = 0;
+  double best_us = 0.0;
+  for (size_t slots = 1; slots <= kMostSlots; slots += slots / 16 + 1) {
+    const int chunk = static_cast<int>((phase.most + slots * 128 - 1) / (slots * 128) * 128);
+    if (best != 0 && static_cast<double>(slots) * phase.all_part_bytes > kMostPartBytes)
+      break;
+    constexpr size_t kSamples = 16;
+    double chunks = 0.0, keys = 0.0;
+    for (size_t i = 0; i < kSamples; ++i) {
+      const size_t seen =
+          phase.uneven ? std::max<size_t>(1, phase.most * (2 * i + 1) / (2 * kSamples))
+                       : phase.most;
+      chunks += static_cast<double>((seen + chunk - 1) / chunk);
+      keys += static_cast<double>(seen);
+    }
+    const double blocks = chunks / kSamples * static_cast<double>(phase.blocks);
+    const double bytes = keys / kSamples * static_cast<double>(4 * phase.blocks * head_dim);
+    const double full_us = 0.008 * static_cast<double>(std::min<size_t>(chunk, phase.most));
+    double us = std::max(bytes / (5.8e6 * std::min(1.0, blocks / 256.0)), full_us) +
+                full_us * std::min(1.0, blocks / 444.0);
+    if (static_cast<size_t>(chunk) < phase.most)
+      us += (phase.joined ? 0.0 : 9.0) + 0.002 * blocks;
+    if (best == 0 || us < best_us) {
+      best = chunk;
+      best_us = us;
+    }
+    if (chunk == 128)
+      break;
+  }
+  return best;
 }
 
 // The 128-row blocks of a phase: `tiles` of them see `least` .. `most` keys each,
 // evenly spread, and all together read kv_bytes of keys and values and leave a part
-// of part_bytes in each chunk.
+// of part_bytes in each chunk; all rows of the batch have all_part_bytes each.
 struct TilePhase {
   size_t tiles, least, most;
   double other_keys;  // keys of further blocks, all together
-  double kv_bytes, part_bytes;
+  double kv_bytes, part_bytes, all_part_bytes;
 };
 
-// Keys per block: the split of least modelled time. 64 keys of head_dim 128 take a
-// block 2.17 us where two share a CU and 1.3 alone; up to three rounds of 512
-// blocks are counted whole. Keys and values stream at 5 TB/s from 512 blocks, at 3.6
-// from one a CU. A part is written and read again, 4.5 TB/s, and joined by a further launch.
+// Keys per block: the split of least modelled time, its constants fitted to measured
+// splits of 34 batches (3% on average behind the best split of each, 23% at most).
+// 64 keys of head_dim 128 take a block 2.3 us where two share a CU and 2.1 alone;
+// 512 blocks run at a time, the longest start first, and the last ones leave part of
+// the chip idle. Keys and values stream at 5 TB/s from 512 blocks, at 3.6 from one
+// a CU. A part costs its bytes at 1.3 TB/s (written, read again, more tails), and all
+// parts one more launch.
 int tile_chunk(const TilePhase &phase, size_t head_dim) {
-  const double key_us = 2.17 / 64.0 * static_cast<double>(head_dim) / 128.0;
+  const double key_us = 2.3 / 64.0 * static_cast<double>(head_dim) / 128.0;
+  constexpr double kAlone = 0.9;
   constexpr size_t kSamples = 16;
   int best = 0;
   double best_us = 0.0;
   for (size_t half_chunks = 2; half_chunks <= 2 * kMostSlots; half_chunks += half_chunks / 16 + 1) {
     // chunks of the longest rows: 1, 1.5, 2, ..
-    const size_t keys = (2 * phase.most + half_chunks - 1) / half_chunks;
-    const int chunk = static_cast<int>((keys + 63) / 64 * 64);
-    if (best != 0 && (chunk < 256 || phase.most > kMostSlots * static_cast<size_t>(chunk)))
+    const size_t longest_keys = (2 * phase.most + half_chunks - 1) / half_chunks;
+    const int chunk = static_cast<int>((longest_keys + 63) / 64 * 64);
+    const size_t slots = (phase.most + chunk - 1) / chunk;
+    if (best != 0 && (chunk < 128 || slots > kMostSlots ||
+                      static_cast<double>(slots) * phase.all_part_bytes > kMostPartBytes))
       break;
-    double chunks = 0.0;
-    for (size_t i = 0; i < kSamples; ++i)
-      chunks += static_cast<double>(
-          (phase.least + (phase.most - phase.least) * (2 * i + 1) / (2 * kSamples) + chunk - 1) /
-          chunk);
+    double chunks = 0.0, keys = 0.0;
+    for (size_t i = 0; i < kSamples; ++i) {
+      const size_t seen =
+          phase.least + (phase.most - phase.least) * (2 * i + 1) / (2 * kSamples);
+      chunks += static_cast<double>((seen + chunk - 1) / chunk);
+      keys += static_cast<double>(seen);
+    }
     chunks = std::max(1.0, chunks / kSamples);
-    const double blocks = chunks * static_cast<double>(phase.tiles);
-    const double longest = static_cast<double>(std::min<size_t>(chunk, phase.most)) * key_us;
-    double us = blocks <= 256.0    ? 0.6 * longest
-                : blocks <= 1536.0 ? std::ceil(blocks / 512.0) * longest
-                                   : (blocks / 512.0 + 0.3) * longest;
+    keys = keys / kSamples * static_cast<double>(phase.tiles) + phase.other_keys;
+    const double full = static_cast<double>(std::min<size_t>(chunk, phase.most));
+    const double least = static_cast<double>(std::min<size_t>(chunk, phase.least));
+    const double own_blocks = chunks * static_cast<double>(phase.tiles);
+    const double rounds = (own_blocks + phase.other_keys / full) / 512.0;
+    const double pairs = std::clamp(2.0 * rounds - 1.0, 0.0, 1.0);  // CUs with two blocks
+    double us = full * key_us * (kAlone + (1.0 - kAlone) * pairs);
+    if (rounds > 0.5)
+      us = std::max(us, (keys / 512.0 + (std::ceil(rounds) - rounds) * least) * key_us);
     us = std::max(us, phase.kv_bytes /
-                          (3.6e6 + 1.4e6 * std::clamp(blocks / 256.0 - 1.0, 0.0, 1.0)));
-    us += phase.other_keys * key_us / 512.0;
+                          (3.6e6 + 1.4e6 * std::clamp(own_blocks / 256.0 - 1.0, 0.0, 1.0)));
     if (chunks > 1.0)
-      us += 5.0 + 2.0 * phase.part_bytes * chunks / 4.5e6;
+      us += 5.0 + phase.part_bytes * chunks / 1.3e6;
     if (best == 0 || us < best_us) {
       best = chunk;
       best_us = us;
@@ -1118,15 +1169,17 @@ AttendPlan plan_attention(const PagedCache &cache, const PagedBatch &batch, size
     plan.wide = own > 128;
     plan.chunk = 512;
   } else if (plan.own_stream) {
-    plan.chunk = stream_chunk(own, plan.tiles * kv);
+    plan.chunk = stream_chunk(
+        {own, plan.tiles * kv, sequences > 1, batch.shared_length > 0, part_bytes}, dim);
   } else {
     // The longest sequence is taken to bring the most rows too; the others' lengths
-    // are not known here and count as a third of its.
+    // are not known here and count as 0.6 of its.
     const size_t longest_tiles = (most + rows - 1) / rows;
     const double share = static_cast<double>(batch.max_tokens) / static_cast<double>(tokens);
     plan.chunk = tile_chunk({longest_tiles * kv, own - std::min(own, most / group) + 1, own,
-                             static_cast<double>((plan.tiles - longest_tiles) * kv * own) / 3.0,
-                             4.0 * static_cast<double>(own * kv * dim), part_bytes * share},
+                             static_cast<double>((plan.tiles - longest_tiles) * kv * own) * 0.6,
+                             4.0 * static_cast<double>(own * kv * dim), part_bytes * share,
+                             part_bytes},
                             dim);
   }
   const int own_slots = static_cast<int>((own + plan.chunk - 1) / plan.chunk);
@@ -1136,9 +1189,9 @@ AttendPlan plan_attention(const PagedCache &cache, const PagedBatch &batch, size
     plan.prefix_tiles = (tokens * group + prefix_rows - 1) / prefix_rows;
     plan.prefix_chunk =
         plan.prefix_stream
-            ? stream_chunk(shared, plan.prefix_tiles * kv)
+            ? stream_chunk({shared, plan.prefix_tiles * kv, false, true, part_bytes}, dim)
             : tile_chunk({plan.prefix_tiles * kv, shared, shared, 0.0,
-                          4.0 * static_cast<double>(shared * kv * dim), part_bytes},
+                          4.0 * static_cast<double>(shared * kv * dim), part_bytes, part_bytes},
                          dim);
     plan.prefix_slots =
         static_cast<int>((shared + plan.prefix_chunk - 1) / plan.prefix_chunk);
