@@ -1057,23 +1057,23 @@ struct StreamPhase {
 // a block 8 us, and as long at the end, while the chip runs empty; a part's block
 // costs 2 ns and joining the parts 9 us. Chunks are 128 keys and more, 32 for each wave.
 int stream_chunk(const StreamPhase &phase, size_t head_dim) {
+  const uint32_t most = static_cast<uint32_t>(phase.most);
+  const double bytes = (phase.uneven ? 2.0 : 4.0) * static_cast<double>(most) *
+                       static_cast<double>(phase.blocks * head_dim);
   int best = 0;
   double best_us = 0.0;
   for (size_t slots = 1; slots <= kMostSlots; slots += slots / 16 + 1) {
     const int chunk = static_cast<int>((phase.most + slots * 128 - 1) / (slots * 128) * 128);
     if (best != 0 && static_cast<double>(slots) * phase.all_part_bytes > kMostPartBytes)
       break;
-    constexpr size_t kSamples = 16;
-    double chunks = 0.0, keys = 0.0;
-    for (size_t i = 0; i < kSamples; ++i) {
-      const size_t seen =
-          phase.uneven ? std::max<size_t>(1, phase.most * (2 * i + 1) / (2 * kSamples))
-                       : phase.most;
-      chunks += static_cast<double>((seen + chunk - 1) / chunk);
-      keys += static_cast<double>(seen);
+    const uint32_t samples = phase.uneven ? 16 : 1;
+    uint32_t chunks = 0;
+    for (uint32_t i = 0; i < samples; ++i) {
+      const uint32_t seen =
+          phase.uneven ? static_cast<uint32_t>((uint64_t{most} * (2 * i + 1) + 31) / 32) : most;
+      chunks += (seen + chunk - 1) / chunk;
     }
-    const double blocks = chunks / kSamples * static_cast<double>(phase.blocks);
-    const double bytes = keys / kSamples * static_cast<double>(4 * phase.blocks * head_dim);
+    const double blocks = static_cast<double>(chunks) / samples * static_cast<double>(phase.blocks);
     const double full_us = 0.008 * static_cast<double>(std::min<size_t>(chunk, phase.most));
     double us = std::max(bytes / (5.8e6 * std::min(1.0, blocks / 256.0)), full_us) +
                 full_us * std::min(1.0, blocks / 444.0);
@@ -1108,7 +1108,7 @@ struct TilePhase {
 int tile_chunk(const TilePhase &phase, size_t head_dim) {
   const double key_us = 2.3 / 64.0 * static_cast<double>(head_dim) / 128.0;
   constexpr double kAlone = 0.9;
-  constexpr size_t kSamples = 16;
+  const uint32_t samples = phase.least == phase.most ? 1 : 16;
   int best = 0;
   double best_us = 0.0;
   for (size_t half_chunks = 2; half_chunks <= 2 * kMostSlots; half_chunks += half_chunks / 16 + 1) {
@@ -1119,15 +1119,14 @@ int tile_chunk(const TilePhase &phase, size_t head_dim) {
     if (best != 0 && (chunk < 128 || slots > kMostSlots ||
                       static_cast<double>(slots) * phase.all_part_bytes > kMostPartBytes))
       break;
-    double chunks = 0.0, keys = 0.0;
-    for (size_t i = 0; i < kSamples; ++i) {
-      const size_t seen =
-          phase.least + (phase.most - phase.least) * (2 * i + 1) / (2 * kSamples);
-      chunks += static_cast<double>((seen + chunk - 1) / chunk);
-      keys += static_cast<double>(seen);
+    uint32_t sum = 0;
+    for (uint32_t i = 0; i < samples; ++i) {
+      const size_t seen = phase.least + (phase.most - phase.least) * (2 * i + 1) / 32;
+      sum += (static_cast<uint32_t>(seen) + chunk - 1) / chunk;
     }
-    chunks = std::max(1.0, chunks / kSamples);
-    keys = keys / kSamples * static_cast<double>(phase.tiles) + phase.other_keys;
+    const double chunks = std::max(1.0, static_cast<double>(sum) / samples);
+    const double keys = 0.5 * static_cast<double>((phase.least + phase.most) * phase.tiles) +
+                        phase.other_keys;
     const double full = static_cast<double>(std::min<size_t>(chunk, phase.most));
     const double least = static_cast<double>(std::min<size_t>(chunk, phase.least));
     const double own_blocks = chunks * static_cast<double>(phase.tiles);
@@ -1177,7 +1176,8 @@ AttendPlan plan_attention(const PagedCache &cache, const PagedBatch &batch, size
     const size_t longest_tiles = (most + rows - 1) / rows;
     const double share = static_cast<double>(batch.max_tokens) / static_cast<double>(tokens);
     plan.chunk = tile_chunk({longest_tiles * kv, own - std::min(own, most / group) + 1, own,
-                             static_cast<double>((plan.tiles - longest_tiles) * kv * own) * 0.6,
+                             0.6 * static_cast<double>((plan.tiles - longest_tiles) * kv) *
+                                 static_cast<double>(own),
                              4.0 * static_cast<double>(own * kv * dim), part_bytes * share,
                              part_bytes},
                             dim);

@@ -379,7 +379,10 @@ EVO_API evo_status evo_hip_paged_append(const evo_hip_paged_cache *cache,
  * positions behind its own, slots behind a sequence's length, other pages.
  * The workspace (16-byte aligned, no initial contents) takes the partial
  * results of keys that are split over blocks; its size depends on the host
- * fields of the structs and heads alone. Calls that overlap need one each. */
+ * fields of the structs and heads alone. It does not grow with the batch (few
+ * rows are split more), but two phases (own keys, shared ones) take at most
+ * 136 MB each, or tokens * heads * (head_dim + 2) * 4 bytes where that is more.
+ * Calls that overlap need one each. */
 EVO_API size_t evo_hip_paged_attention_workspace_bytes(const evo_hip_paged_cache *cache,
                                                        const evo_hip_paged_batch *batch,
                                                        size_t heads);
@@ -393,7 +396,8 @@ EVO_API evo_status evo_hip_paged_attention(const evo_hip_paged_cache *cache,
 /* tokens[r] = one token of row r of logits [rows][row_stride] (F32, BF16 or
  * F16; rows and vocab at most 2^20), in the order and with the cuts of evo_sampler_sample:
  * tokens by descending logit, equal ones by ascending index; of these the first
- * top_k (0, or vocab and more: all); weights exp(logit / temperature) in 64 bits;
+ * top_k (0, or vocab and more: all); weights exp(logit / temperature) in 64 bits
+ * (one below 2^-43 of the largest counts as none);
  * of these the shortest beginning whose weight reaches top_p of what top-k left
  * (1: all); of these the ones of at least min_p times the largest weight (0: all);
  * then the first whose cumulative weight exceeds uniform times the weight left.

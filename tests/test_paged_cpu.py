@@ -121,6 +121,33 @@ def test_attention_workspace_refused():
             attend(b=b, workspace=workspace, workspace_bytes=size)
 
 
+@pytest.mark.parametrize("seed", range(4))
+def test_attention_workspace_bound(seed):
+    """Of any batch: whole slots of all rows, and two phases of at most 136 MB, or of
+    one slot where that is more."""
+    rng = np.random.default_rng(seed)
+    for _ in range(500):
+        def size(high, low=1):
+            return int(np.exp(rng.uniform(np.log(low), np.log(high))))
+        dim, page = int(rng.choice([32, 64, 128])), 16 << rng.integers(0, 8)
+        kv_heads = size(64)
+        heads = kv_heads * int(rng.choice([1, 2, 3, 4, 7, 8, 16, 32]))
+        max_tokens, sequences = size(16384), size(2000)
+        tokens = max(max_tokens, min(max_tokens * sequences, size(65536)))
+        shared = page * (size(1 << 20) // page) if rng.random() < 0.5 else 0
+        length = shared + max(max_tokens, size(1 << 21))
+        c = cache(head_dim=dim, page_size=page, kv_heads=kv_heads, pages=1 << 20)
+        b = batch(sequences=sequences, tokens=tokens, max_tokens=max_tokens, max_length=length,
+                  table_stride=length // page + 1, shared_length=shared,
+                  shared_table=A if shared else None)
+        need = N.call("evo_hip_paged_attention_workspace_bytes", ctypes.byref(c),
+                      ctypes.byref(b), heads)
+        slot = tokens * heads * (dim + 2) * 4
+        slots, rest = divmod(need, slot)
+        assert rest == 0 and slots != 1 and slots <= 256 and (not shared or slots >= 2)
+        assert need <= 2 * max(136e6, slot)
+
+
 def test_workspace_query_of_refused_structs_is_zero():
     query = "evo_hip_paged_attention_workspace_bytes"
     assert N.call(query, ctypes.byref(cache(page_size=3)), ctypes.byref(batch()), 4) == 0
