@@ -333,14 +333,16 @@ __device__ inline uint32_t odd_keys(uint32_t (&v)[8][kD / 32]) {
   return keys;
 }
 
-// 16 rows of a key/value head and a chunk of their keys per block; its kWaves waves
-// take every kWaves-th 32-key step and join their states through LDS.
+// 16 rows of a key/value head and a chunk of their keys per block; its four waves take
+// every fourth 32-key step and join their states through LDS. (Eight waves a block
+// took longer at every size: one sequence of 512 keys 9.7 us for 8.9, 60 of them 17.4
+// for 15.2.)
 // Blocks below prefix_blocks take the shared keys, rows of the whole batch.
 template <int kD> struct StreamShared {
   float top[4][16], sum[4][16];
   __attribute__((aligned(16))) float out[4][16][kD + 4];
 };
-template <typename T, int kD, int kWaves>
+template <typename T, int kD>
 __device__ inline void stream_block(const AttendArgs &a, const BlockWork &work,
                                     StreamShared<kD> &shared) {
   constexpr int kRows = 16, kVec = kD / 16, kSteps = kD / 32;
@@ -411,7 +413,7 @@ __device__ inline void stream_block(const AttendArgs &a, const BlockWork &work,
   // V of a step is requested before its scores, K of the next one as soon as the
   // scores are done and the page after that with it, so that loads are always in
   // flight with one set of registers. Without a page the loads go to page 0.
-  constexpr int kStride = 32 * kWaves;
+  constexpr int kStride = 32 * 4;
   if (k0 < key1) {
     int pages = pages_of(early ? entries : entries_at(k0), k0);
     int page[2] = {__builtin_amdgcn_readlane(pages, 0), __builtin_amdgcn_readlane(pages, 1)};
@@ -487,45 +489,19 @@ __device__ inline void stream_block(const AttendArgs &a, const BlockWork &work,
     }
   }
 
-  // Join the waves: each leaves its rows' maximum, sum and output, of eight the last
-  // four to the first.
+  // Join the waves: each leaves its rows' maximum, sum and output.
   state.sum += __shfl_xor(state.sum, 16, 64);
   state.sum += __shfl_xor(state.sum, 32, 64);
-  const auto leave = [&](int at) {
-    if (g == 0) {
-      top_s[at][col] = state.top;
-      sum_s[at][col] = state.sum;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int t = 0; t < kVec; ++t)
-        out_s[at][col][kVec * (4 * g + i) + t] = state.out[t][i];
-  };
-  if constexpr (kWaves == 8) {
-    if (wave >= 4)
-      leave(wave - 4);
-    __syncthreads();
-    if (wave < 4) {
-      const float top = fmaxf(state.top, top_s[wave][col]), base = top == -INFINITY ? 0.0F : top;
-      const float mine = __builtin_amdgcn_exp2f(state.top - base);
-      const float theirs = __builtin_amdgcn_exp2f(top_s[wave][col] - base);
-      state.top = top;
-      state.sum = state.sum * mine + sum_s[wave][col] * theirs;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int t = 0; t < kVec; ++t)
-          state.out[t][i] =
-              state.out[t][i] * mine + out_s[wave][col][kVec * (4 * g + i) + t] * theirs;
-    }
-    __syncthreads();
+  if (g == 0) {
+    top_s[wave][col] = state.top;
+    sum_s[wave][col] = state.sum;
   }
-  if (wave < 4)
-    leave(wave);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int t = 0; t < kVec; ++t)
+      out_s[wave][col][kVec * (4 * g + i) + t] = state.out[t][i];
   __syncthreads();
-  if (wave >= 4)
-    return;
   // Thread: row tid / 16, elements kVec * (tid % 16) ...
   const int r = threadIdx.x >> 4, d = kVec * (threadIdx.x & 15);
   if (tile.row0 + r >= tile.rows)
@@ -907,11 +883,11 @@ constexpr size_t tile_lds_bytes(size_t head_dim) {
 }
 static_assert(2 * tile_lds_bytes(128) <= 160 * 1024, "two blocks per CU");
 
-// Blocks of a launch. kSmall: 16 rows, 4 waves; kSmallWide: 16 rows, 8 waves; kLarge:
-// 128 rows; kMixed: 128 rows on the shared keys beside 16 rows on each sequence's own.
-enum BlockKind : int { kSmall, kSmallWide, kLarge, kMixed };
+// Blocks of a launch. kSmall: 16 rows; kLarge: 128 rows; kMixed: 128 rows on the shared
+// keys beside 16 rows on each sequence's own.
+enum BlockKind : int { kSmall, kLarge, kMixed };
 template <typename T, int kD, int kKind>
-__global__ __launch_bounds__(kKind == kSmallWide ? 512 : 256, kKind == kSmall ? 3 : 2) void
+__global__ __launch_bounds__(256, kKind == kSmall ? 3 : 2) void
 paged_attention_kernel(const AttendArgs a, unsigned prefix_blocks) {
   extern __shared__ __attribute__((aligned(16))) uint16_t attend_lds[];
   if (blockIdx.x == prefix_blocks)
@@ -920,8 +896,7 @@ paged_attention_kernel(const AttendArgs a, unsigned prefix_blocks) {
   if (kKind == kLarge || (kKind == kMixed && work.prefix))
     tile_block<T, kD>(a, work, attend_lds);
   else
-    stream_block<T, kD, kKind == kSmallWide ? 8 : 4>(
-        a, work, *reinterpret_cast<StreamShared<kD> *>(attend_lds));
+    stream_block<T, kD>(a, work, *reinterpret_cast<StreamShared<kD> *>(attend_lds));
 }
 
 // Rows whose keys lay in several chunks: the chunks rescaled to their common
@@ -1032,7 +1007,6 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const AttendArgs a, 
 
 struct AttendPlan {
   bool own_stream, prefix_stream;  // 16-row blocks, else 128-row ones
-  bool wide;                       // 16-row blocks of 8 waves
   size_t tiles, prefix_tiles;      // row tiles of the own keys, of the shared ones
   int chunk, prefix_chunk, prefix_slots, slots;
 };
@@ -1163,11 +1137,7 @@ AttendPlan plan_attention(const PagedCache &cache, const PagedBatch &batch, size
                                           tokens * group / rows + std::min(sequences, tokens));
   const size_t own = std::max(1, batch.max_length - batch.shared_length);
   const double part_bytes = static_cast<double>(tokens * heads * dim * sizeof(float));
-  if (plan.own_stream && batch.shared_length == 0 && plan.tiles * kv <= 512 && own <= 512) {
-    // One block for all keys of a row: the launch that joins chunks would take longer.
-    plan.wide = own > 128;
-    plan.chunk = 512;
-  } else if (plan.own_stream) {
+  if (plan.own_stream) {
     plan.chunk = stream_chunk(
         {own, plan.tiles * kv, sequences > 1, batch.shared_length > 0, part_bytes}, dim);
   } else {
@@ -1214,26 +1184,28 @@ Status launch_attention(const AttendArgs &args, const AttendPlan &plan, hipStrea
   const size_t blocks = prefix_blocks + plan.tiles * kv * (plan.slots - plan.prefix_slots);
   // A launch counts its threads in 32 bits.
   const size_t tokens = static_cast<size_t>(args.batch.tokens), heads = args.heads;
-  const bool split_join = plan.slots > 64 || (plan.slots > 8 && tokens * heads < (1U << 16));
+  // A block per row and head where there are more chunks than lanes, or many chunks of
+  // few rows: 512 rows of 31 chunks 4.0 us, else 6.4; 600 tokens' rows of few chunks 103
+  // us with the attention, else 81.
+  const bool split_join = plan.slots > 64 || (plan.slots > 16 && tokens * heads <= 2048);
   // Four heads of a row per joining block, all of them where the rows fill the chip.
   const size_t of_block =
       split_join ? 1 : std::min(heads, 4 * std::max<size_t>(1, tokens * heads / 8192));
   const size_t join_blocks = plan.slots == 1 ? 0 : tokens * ceil_div(heads, of_block);
   constexpr size_t kMostThreads = (size_t{1} << 32) - 1;
-  if (blocks > kMostThreads / (plan.wide ? 512 : 256) || join_blocks > kMostThreads / 256)
+  if (blocks > kMostThreads / 256 || join_blocks > kMostThreads / 256)
     return {ErrorCode::kInvalidArgument, "paged_attention: grid too large"};
   auto kernel = paged_attention_kernel<T, kD, kLarge>;
   size_t lds = tile_lds_bytes(kD);
   if (plan.own_stream && (plan.prefix_stream || prefix_blocks == 0)) {
-    kernel = plan.wide ? paged_attention_kernel<T, kD, kSmallWide>
-                       : paged_attention_kernel<T, kD, kSmall>;
+    kernel = paged_attention_kernel<T, kD, kSmall>;
     lds = sizeof(StreamShared<kD>);
   } else if (plan.own_stream) {
     kernel = paged_attention_kernel<T, kD, kMixed>;
     lds = std::max(lds, sizeof(StreamShared<kD>));
   }
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(plan.wide ? 512 : 256),
-                     lds, stream, args, static_cast<unsigned>(prefix_blocks));
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), lds,
+                     stream, args, static_cast<unsigned>(prefix_blocks));
   EVO_TRY(launch_status("paged_attention_kernel"));
   if (plan.slots == 1)
     return Status::Ok();

@@ -1105,11 +1105,16 @@ Status launch_sample(const SampleArgs &args, size_t rows, void *workspace, hipSt
   const size_t vocab = static_cast<size_t>(args.vocab);
   SplitRows split{};
   split.parts = workspace == nullptr ? 1 : parts_of(rows, vocab);
+  // A wave a row to 1024 values (us, with blocks of 256 threads in brackets: 1 row of
+  // 1024 8.5 (11.9), 2048 rows 15 (37)), then blocks of 256 threads or 1024. us of both:
+  // 256 rows of 9000 25 and 25, of 16000 32 and 29, of 32000 46 and 38; 512 rows of 16000
+  // 36 and 52, of 32000 55 and 68, of 65536 95 and 102, of 131072 235 and 172.
+  const bool narrow = vocab <= (rows <= 256 ? 8192 : 65536);
   if (args.vocab <= 512) {
     hipLaunchKernelGGL((sample_wave_kernel<T, 8>), grid, dim3(64), 0, stream, args);
   } else if (args.vocab <= 1024) {
     hipLaunchKernelGGL((sample_wave_kernel<T, 16>), grid, dim3(64), 0, stream, args);
-  } else if (args.vocab <= 16384) {
+  } else if (narrow) {
     hipLaunchKernelGGL((sample_block_kernel<T, 256, 1024, 512, false>), grid, dim3(256), 0,
                        stream, args, split);
   } else if (split.parts == 1) {

@@ -87,6 +87,16 @@ def test_tokens(vocab, rows, kind, workspace):
     compare(logits.to(DEVICE).to(kind), *parameters(rng, rows, vocab), workspace=workspace)
 
 
+@pytest.mark.parametrize("vocab,rows", [(8192, 257), (8193, 20), (8193, 257), (20000, 300),
+                                        (65536, 257), (65537, 257)])
+def test_many_rows(vocab, rows):
+    """More rows than the chip has CUs, which run in smaller blocks, with ties among
+    them: few bits of a logit."""
+    rng = np.random.default_rng(rows * vocab)
+    logits = (np.round(rng.normal(0, 2.5, (rows, vocab)) * 64) / 64).astype(np.float32)
+    compare(torch.from_numpy(logits).to(DEVICE), *parameters(rng, rows, vocab))
+
+
 @pytest.mark.parametrize("vocab", [512, 3000, 40000])
 @pytest.mark.parametrize("workspace", [True, False])
 def test_equal_logits(vocab, workspace):
