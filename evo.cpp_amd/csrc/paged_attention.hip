@@ -580,35 +580,24 @@ template <typename Q> __device__ inline Q transposed(const uint16_t *from) {
   return __builtin_bit_cast(Q, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(from)));
 }
 
-// out += V^T P over a tile's 64 keys, P = exp2(score * scale2 - base).
+// V^T operands of keys 16kk .. of a tile: keys 16kk + 4 half + (0 .. 3) and 8 more of
+// elements 32t + 16 * (lane / 16 % 2) ..
 template <typename T, int kD>
-__device__ inline void add_values(const uint16_t *v_s, const f32x16 (&score)[2], float scale2,
-                                  float base, float &sum, f32x16 (&out)[kD / 32]) {
+__device__ inline void read_values(const uint16_t *v_s, int kk,
+                                   typename Mfma<T>::vec (&v)[kD / 32]) {
   constexpr int kUnits = kD / 8;
-  typedef typename Mfma<T>::vec vec;
   typedef T quad __attribute__((ext_vector_type(4)));
   const int lane = threadIdx.x & 63, half = lane >> 5;
 #pragma unroll
-  for (int kk = 0; kk < 4; ++kk) {
-    vec p;
+  for (int t = 0; t < kD / 32; ++t) {
+    quad part[2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      p[j] = static_cast<T>(
-          __builtin_amdgcn_exp2f(fmaf(score[kk / 2][8 * (kk % 2) + j], scale2, -base)));
-    sum = Mfma<T>::add(p, sum);
-#pragma unroll
-    for (int t = 0; t < kD / 32; ++t) {
-      // Keys 16kk + 4 half + (0 .. 3) and 8 more; elements 32t + 16 * (lane / 16 % 2) ..
-      quad part[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int r = 16 * kk + 8 * j + 4 * half + (lane & 15) / 4;
-        const int d = 32 * t + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
-        part[j] = transposed<quad>(v_s + r * kD + 8 * swizzle_v<kUnits>(r, d / 8) + d % 8);
-      }
-      const vec v = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
-      out[t] = Mfma<T>::run(v, p, out[t]);
+    for (int j = 0; j < 2; ++j) {
+      const int r = 16 * kk + 8 * j + 4 * half + (lane & 15) / 4;
+      const int d = 32 * t + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+      part[j] = transposed<quad>(v_s + r * kD + 8 * swizzle_v<kUnits>(r, d / 8) + d % 8);
     }
+    v[t] = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
   }
 }
 
@@ -762,19 +751,35 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
       continue;
     const uint16_t *k_s = tile_lds + stage * 2 * kPlane, *v_s = k_s + kPlane;
 
+    // Operands are requested from LDS a part (a quarter of the tile's products) ahead of
+    // their products: left to the compiler, the wave waits for each.
+    constexpr int kPart = kSteps / 2;
+    vec k_part[2][kPart], v_part[2][kTiles];
+    const auto read_keys = [&](int kk) {
+      const int r = 32 * (kk / 2) + col;
+#pragma unroll
+      for (int s = 0; s < kPart; ++s)
+        k_part[kk % 2][s] = *reinterpret_cast<const vec *>(
+            k_s + r * kD + 8 * swizzle_k<kUnits>(r, 2 * (kPart * (kk % 2) + s) + half));
+    };
     f32x16 score[2];
+    read_keys(0);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int kk = 0; kk < 4; ++kk) {
+      if (kk < 3)
+        read_keys(kk + 1);
+      else
+        read_values<T, kD>(v_s, 0, v_part[0]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (kk % 2 == 0)
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        score[u][e] = 0.0F;
+        for (int e = 0; e < 16; ++e)
+          score[kk / 2][e] = 0.0F;
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const int r = 32 * u + col;
-        const vec k = *reinterpret_cast<const vec *>(
-            k_s + r * kD + 8 * swizzle_k<kUnits>(r, 2 * s + half));
-        score[u] = Mfma<T>::run(k, q[s], score[u]);
-      }
+      for (int s = 0; s < kPart; ++s)
+        score[kk / 2] = Mfma<T>::run(k_part[kk % 2][s], q[kPart * (kk % 2) + s], score[kk / 2]);
+      __builtin_amdgcn_sched_barrier(0);
     }
     if (missing != 0 || k0 + kKeys - 1 > wave_first || k0 + kKeys > key1) {
       const int visible = min(position + 1, key1) - k0;
@@ -807,7 +812,27 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
       top = next;
     }
     const float base = top == -INFINITY ? 0.0F : top;
-    add_values<T, kD>(v_s, score, a.scale2, base, sum, out);
+    vec p[2];
+    const auto weights = [&](int kk) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        p[kk % 2][j] = static_cast<T>(
+            __builtin_amdgcn_exp2f(fmaf(score[kk / 2][8 * (kk % 2) + j], a.scale2, -base)));
+      sum = Mfma<T>::add(p[kk % 2], sum);
+    };
+    weights(0);
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      if (kk < 3)
+        read_values<T, kD>(v_s, kk + 1, v_part[(kk + 1) % 2]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+        out[t] = Mfma<T>::run(v_part[kk % 2][t], p[kk % 2], out[t]);
+      if (kk < 3)
+        weights(kk + 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
 
   // The odd keys' values, to the rows that see them (their weights are in the sum).
