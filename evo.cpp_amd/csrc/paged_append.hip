@@ -4,7 +4,10 @@
 //
 // x' = x cos a - y sin a, y' = y cos a + x sin a over the rotated pairs of a
 // query or key head, a = (position / scale) * inv_freq[i]; the rest and the
-// values pass through. Bound by bytes: each value is read and written once.
+// values pass through. Bound by bytes: each value is read and written once. 8 prompts
+// of up to 2048 tokens (F32 rows of 32 query, key and value heads of 128, 521 MB in
+// all) take 101 us, 5.2 TB/s, the rate of a copy; one token takes 4.3 us, a launch and
+// three loads that wait for each other (sequence, length, page).
 #include "common.hpp"
 #include "ops.hpp"
 #include "paged.hpp"
@@ -273,9 +276,11 @@ Status paged_append(const PagedCache &cache, const PagedBatch &batch, int dtype,
     return {ErrorCode::kInvalidArgument, "paged_append: invalid rotation"};
   const bool vector = reinterpret_cast<uintptr_t>(projected) % 16 == 0 &&
                       row_stride * size % 16 == 0;
-  // A block's pass over the heads; few rows are split over them.
+  // A block's pass over the heads; few rows are split over them. us split and whole, 32
+  // heads of each kind: 1 row 4.3 and 4.7, 27 rows 5.5 and 6.1, 103 rows 6.3 and 6.6, 264
+  // rows 8.2 and 8.0, 428 rows 10.5 and 9.5.
   const size_t passes = ceil_div((heads + 2 * kv) * (dim / 16), 256);
-  const size_t parts = batch.tokens >= 512 ? 1 : passes;
+  const size_t parts = batch.tokens > 128 ? 1 : passes;
   const size_t blocks = parts * static_cast<size_t>(batch.tokens);
   if (blocks > ((size_t{1} << 32) - 1) / 256)  // a launch counts its threads in 32 bits
     return {ErrorCode::kInvalidArgument, "paged_append: grid too large"};

@@ -13,6 +13,13 @@
 // histogram nor a split of a row can change a token, and a border is off by less
 // than 1e-11 of the row's largest weight. A weight below 2^-43 (30 below the top,
 // in units of the temperature) counts as none.
+//
+// What bounds it: 2048 rows of 512 values 10.4 us, one round of waves, each a chain of
+// reductions, LDS atomics and two or three searches; 128 rows of 131072 BF16 values 64
+// us, of which their ranges take 7.6 (34 MB, 4.4 TB/s),
+// the histograms 21 (the weights' 64-bit arithmetic), and the borders 35 (a block a row:
+// 13 to read the row again for the borders' bins, the rest scans and searches of one
+// wave after another).
 #include "common.hpp"
 #include "ops.hpp"
 

@@ -180,6 +180,43 @@ def test_defaults_and_strides():
                                 for r in range(40)]
 
 
+def test_captured_rows_split_over_blocks():
+    """A large vocabulary in a graph, on a stream of its own: each replay samples the
+    logits and parameters it finds, like the eager call."""
+    rng = np.random.default_rng(11)
+    rows, vocab = 3, 70000
+    need = N.call("evo_hip_sample_workspace_bytes", rows, vocab)
+    assert need > 0
+    logits = torch.zeros(rows, vocab, dtype=torch.bfloat16, device=DEVICE)
+    values = [f32([0.0] * rows) for _ in range(4)]  # uniform, temperature, top_p, min_p
+    top_k, tokens = i32([0] * rows), i32([0] * rows)
+    scratch = torch.full((need,), 255, dtype=torch.uint8, device=DEVICE)
+
+    def draw(stream):
+        N.call("evo_hip_sample", CODES[logits.dtype], logits.data_ptr(), rows, vocab, vocab,
+               values[1].data_ptr(), top_k.data_ptr(), values[2].data_ptr(),
+               values[3].data_ptr(), values[0].data_ptr(), tokens.data_ptr(),
+               scratch.data_ptr(), need, stream.cuda_stream)
+
+    stream = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        draw(stream)
+    for _ in range(5):
+        logits.copy_(torch.from_numpy(rng.normal(0, 3, (rows, vocab)).astype(np.float32)))
+        given = parameters(rng, rows, vocab)
+        for to, value in zip((values[0], values[1], top_k, values[2], values[3]), given):
+            to.copy_(torch.tensor(value))
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = tokens.cpu()
+        compare(logits, *given)
+        draw(torch.cuda.current_stream())
+        torch.cuda.synchronize()
+        assert torch.equal(replayed, tokens.cpu())
+
+
 def test_same_tokens_as_the_host_sampler():
     """evo_sampler_sample's token, for the draw that its generator makes."""
     import ctypes
