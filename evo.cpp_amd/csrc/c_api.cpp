@@ -1012,11 +1012,15 @@ evo_status evo_hip_paged_append(const evo_hip_paged_cache *cache, const evo_hip_
 
 size_t evo_hip_paged_attention_workspace_bytes(const evo_hip_paged_cache *cache,
                                                const evo_hip_paged_batch *batch, size_t heads) {
-  evo::hip::PagedCache pages;
-  evo::hip::PagedBatch rows;
-  if (!paged_call(cache, batch, &pages, &rows).ok())
+  try {
+    evo::hip::PagedCache pages;
+    evo::hip::PagedBatch rows;
+    if (!paged_call(cache, batch, &pages, &rows).ok())
+      return 0;
+    return evo::hip::paged_attention_workspace_bytes(pages, rows, heads);
+  } catch (...) {
     return 0;
-  return evo::hip::paged_attention_workspace_bytes(pages, rows, heads);
+  }
 }
 
 evo_status evo_hip_paged_attention(const evo_hip_paged_cache *cache,

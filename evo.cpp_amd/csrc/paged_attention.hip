@@ -51,7 +51,7 @@ struct AttendArgs {
   size_t out_stride;
   int heads, group;   // query heads, and how many share a key/value head
   float scale2;       // log2(e) * scale
-  int chunk;          // own keys per chunk (a multiple of 128)
+  int chunk;          // own keys per chunk (a multiple of 64)
   int prefix_chunk;   // shared keys per chunk
   int prefix_slots;   // chunks of the shared keys
   int slots;          // chunks of a row at most, the shared ones first
@@ -851,8 +851,10 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
     for (int i = 0; i < 4 * odd_tiles; ++i)
       for (uint32_t bits = odd_s[i]; bits != 0; bits &= bits - 1) {
         const int key = odd_first + 16 * i + __builtin_ctz(bits);
-        const size_t at = table[key >> a.cache.page_shift] * a.cache.page_stride +
-                          work.kv_head * a.cache.head_stride +
+        const int page = checked_page(table, key >> a.cache.page_shift, a.cache.pages);
+        if (page < 0)
+          continue;
+        const size_t at = page * a.cache.page_stride + work.kv_head * a.cache.head_stride +
                           (key & slot_mask) * a.cache.token_stride;
         const uint16_t *k = a.cache.keys + at + 8 * half, *v = a.cache.values + at + 4 * half;
         float dot = 0.0F;
@@ -1049,6 +1051,14 @@ struct AttendPlan {
 };
 constexpr size_t kMostSlots = 128;  // of each phase (256 in the combining kernel)
 
+// Chunks of a row of least .. most keys, every number as likely, on average: the sum
+// over k of the chance that it has more than k * chunk.
+double mean_chunks(double least, double most, double chunk) {
+  const double all = std::ceil(least / chunk), any = std::ceil(most / chunk);
+  return any <= all ? all
+                    : all + (any - all) * (most - 0.5 * (all + any - 1.0) * chunk) / (most - least);
+}
+
 // What the parts of one phase may take, in bytes: half of the last cache. One chunk
 // is always taken.
 constexpr double kMostPartBytes = 128e6;
@@ -1068,23 +1078,15 @@ struct StreamPhase {
 // a block 8 us, and as long at the end, while the chip runs empty; a part's block
 // costs 2 ns and joining the parts 9 us. Chunks are 128 keys and more, 32 for each wave.
 int stream_chunk(const StreamPhase &phase, size_t head_dim) {
-  const uint32_t most = static_cast<uint32_t>(phase.most);
-  const double bytes = (phase.uneven ? 2.0 : 4.0) * static_cast<double>(most) *
-                       static_cast<double>(phase.blocks * head_dim);
+  const double most = static_cast<double>(phase.most), least = phase.uneven ? 0.0 : most;
+  const double bytes = 2.0 * (least + most) * static_cast<double>(phase.blocks * head_dim);
   int best = 0;
   double best_us = 0.0;
   for (size_t slots = 1; slots <= kMostSlots; slots += slots / 16 + 1) {
     const int chunk = static_cast<int>((phase.most + slots * 128 - 1) / (slots * 128) * 128);
     if (best != 0 && static_cast<double>(slots) * phase.all_part_bytes > kMostPartBytes)
       break;
-    const uint32_t samples = phase.uneven ? 16 : 1;
-    uint32_t chunks = 0;
-    for (uint32_t i = 0; i < samples; ++i) {
-      const uint32_t seen =
-          phase.uneven ? static_cast<uint32_t>((uint64_t{most} * (2 * i + 1) + 31) / 32) : most;
-      chunks += (seen + chunk - 1) / chunk;
-    }
-    const double blocks = static_cast<double>(chunks) / samples * static_cast<double>(phase.blocks);
+    const double blocks = mean_chunks(least, most, chunk) * static_cast<double>(phase.blocks);
     const double full_us = 0.008 * static_cast<double>(std::min<size_t>(chunk, phase.most));
     double us = std::max(bytes / (5.8e6 * std::min(1.0, blocks / 256.0)), full_us) +
                 full_us * std::min(1.0, blocks / 444.0);
@@ -1119,7 +1121,6 @@ struct TilePhase {
 int tile_chunk(const TilePhase &phase, size_t head_dim) {
   const double key_us = 2.3 / 64.0 * static_cast<double>(head_dim) / 128.0;
   constexpr double kAlone = 0.9;
-  const uint32_t samples = phase.least == phase.most ? 1 : 16;
   int best = 0;
   double best_us = 0.0;
   for (size_t half_chunks = 2; half_chunks <= 2 * kMostSlots; half_chunks += half_chunks / 16 + 1) {
@@ -1130,12 +1131,8 @@ int tile_chunk(const TilePhase &phase, size_t head_dim) {
     if (best != 0 && (chunk < 128 || slots > kMostSlots ||
                       static_cast<double>(slots) * phase.all_part_bytes > kMostPartBytes))
       break;
-    uint32_t sum = 0;
-    for (uint32_t i = 0; i < samples; ++i) {
-      const size_t seen = phase.least + (phase.most - phase.least) * (2 * i + 1) / 32;
-      sum += (static_cast<uint32_t>(seen) + chunk - 1) / chunk;
-    }
-    const double chunks = std::max(1.0, static_cast<double>(sum) / samples);
+    const double chunks = mean_chunks(static_cast<double>(phase.least),
+                                      static_cast<double>(phase.most), chunk);
     const double keys = 0.5 * static_cast<double>((phase.least + phase.most) * phase.tiles) +
                         phase.other_keys;
     const double full = static_cast<double>(std::min<size_t>(chunk, phase.most));
@@ -1285,9 +1282,13 @@ Status paged_attention(const PagedCache &cache, const PagedBatch &batch, const v
       out_stride < heads * dim)
     return {ErrorCode::kInvalidArgument,
             "paged_attention: rows have to start on 16 bytes and hold every head"};
+  if (out == query && out_stride != query_stride)
+    return {ErrorCode::kInvalidArgument,
+            "paged_attention: in place, out_stride has to be query_stride"};
   if (!(scale > 0.0F) || !std::isfinite(scale))
     return {ErrorCode::kInvalidArgument, "paged_attention: scale must be positive and finite"};
-  if (static_cast<size_t>(batch.tokens) * heads >= (size_t{1} << 31))
+  // (Rows are counted in 32 bits, up to the end of their last tile.)
+  if (static_cast<size_t>(batch.tokens) * heads >= (size_t{1} << 31) - 128)
     return {ErrorCode::kInvalidArgument, "paged_attention: too many rows"};
   const AttendPlan plan = plan_attention(cache, batch, heads);
   const size_t bytes = plan_bytes(plan, cache, batch, heads);

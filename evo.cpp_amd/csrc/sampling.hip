@@ -672,8 +672,10 @@ __device__ inline uint64_t find_in_list(SampleShared<kThreads, kBins, kList> &s,
     const uint64_t p = s.list_place[i];
     if (p >= last && p <= first) {
       const uint32_t slot = atomicAdd(&s.fill, 1U);
-      s.few_place[slot] = p;
-      s.few_mass[slot] = s.list_mass[i];
+      if (slot < kFew) {
+        s.few_place[slot] = p;
+        s.few_mass[slot] = s.list_mass[i];
+      }
     }
   }
   __syncthreads();
@@ -711,7 +713,9 @@ __device__ inline void gather(const Row<T> &row, const Scale &scale,
   const auto push = [&](int i) {
     if (shift < 56 && place(static_cast<float>(row.logits[i]), i) >> shift != prefix)
       return;
-    s.list_place[atomicAdd(&s.fill, 1U)] = static_cast<uint64_t>(i);
+    const uint32_t slot = atomicAdd(&s.fill, 1U);
+    if (slot < kList)  // (there are no more, unless someone writes the logits meanwhile)
+      s.list_place[slot] = static_cast<uint64_t>(i);
   };
   const auto wanted = [&](float v) { return one.has(v) || other.has(v); };
   // Few of the tokens are wanted: a load's make a mask without a branch.
@@ -732,7 +736,7 @@ __device__ inline void gather(const Row<T> &row, const Scale &scale,
           push(i);
       });
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < s.fill; i += kThreads) {
+  for (uint32_t i = threadIdx.x; i < min(s.fill, static_cast<uint32_t>(kList)); i += kThreads) {
     const int token = static_cast<int>(s.list_place[i]);
     const float v = static_cast<float>(row.logits[token]);
     s.list_place[i] = place(v, token);
@@ -1070,7 +1074,7 @@ __global__ __launch_bounds__(kThreads) void sample_block_kernel(const SampleArgs
         joint = members + in_bins(low, high) <= kList;
         if (joint) {
           gather(row, scale, s, scale.values(bin, bin), scale.values(low, high), 56, 0);
-          size = s.fill;
+          size = min(s.fill, static_cast<uint32_t>(kList));
           __syncthreads();
         }
       }

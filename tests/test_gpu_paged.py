@@ -259,6 +259,14 @@ def test_nonfinite_values_reach_only_rows_that_see_them(heads, kv_heads, n, leng
         assert out[row:n, mine].isnan().all()
 
 
+@pytest.mark.parametrize("heads,kv_heads,n,length,kind,dim", [
+    (2, 1, 40, 6000, "bf16", 64), (4, 4, 3, 5000, "f16", 128), (1, 1, 150, 9000, "bf16", 32)])
+@pytest.mark.parametrize("what", [float("inf"), float("-inf"), float("nan")])
+def test_nonfinite_values_in_rows_of_many_chunks(heads, kv_heads, n, length, kind, dim, what):
+    test_nonfinite_values_reach_only_rows_that_see_them(heads, kv_heads, n, length, kind, dim,
+                                                        what)
+
+
 def test_attention_rows_without_keys_are_zero():
     p = Paged([(3, 0), (5, 2), (1, 1), (40, 7), (0, 0)], dim=64, trailing=4)
     run(p)

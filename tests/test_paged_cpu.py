@@ -97,6 +97,12 @@ def test_attention_refused(bad):
         attend(**bad)
 
 
+def test_in_place_with_another_stride_refused():
+    """A row's output would lie on another row's query."""
+    with pytest.raises(N.OpError, match="in place"):
+        attend(query=B, out=B, query_stride=256, out_stride=264)
+
+
 def test_launches_beyond_32_bit_threads_refused():
     """Rows that a launch could not count."""
     with pytest.raises(N.OpError, match="grid too large"):
@@ -108,6 +114,14 @@ def test_launches_beyond_32_bit_threads_refused():
         attend(b=batch(sequences=1 << 20, tokens=1 << 20, max_tokens=1, max_length=1 << 16,
                        table_stride=1 << 12), c=cache(kv_heads=32), heads=32, query_stride=2048,
                out_stride=2048)
+
+
+def test_rows_up_to_the_end_of_their_tile_refused():
+    """2^31 - 128 rows of one key/value head: the end of the last tile is counted too."""
+    with pytest.raises(N.OpError, match="too many rows"):
+        attend(c=cache(kv_heads=1, head_dim=32),
+               b=batch(tokens=(1 << 24) - 1, max_tokens=(1 << 24) - 1, max_length=40), heads=128,
+               query_stride=128 * 32, out_stride=128 * 32)
 
 
 def test_attention_workspace_refused():
