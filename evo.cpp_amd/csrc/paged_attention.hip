@@ -651,6 +651,25 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
   if (key0 >= key1 && (prefix || work.chunk > 0))
     return;
 
+  const int32_t *table = prefix ? a.batch.shared_table
+                                : a.batch.page_table + tile.sequence * a.batch.table_stride;
+  // Table entries of the tile's four 16-key groups in lanes 0 .. 3, and their pages
+  // (-1: none). An entry is looked at a tile after its load: to wait for it is to wait
+  // for every DMA before it.
+  auto entries_at = [&](int k0) {
+    const int key = k0 + 16 * lane;
+    return lane < 4 && key < key1 ? table[key >> a.cache.page_shift] : -1;
+  };
+  auto pages_of = [&](int entry, int k0) {
+    const bool needed = lane < 4 && k0 + 16 * lane < key1;
+    const bool good = needed && entry >= 0 && entry < a.cache.pages;
+    if (needed && !good)
+      report(a.batch, kBadPage);
+    return good ? entry : -1;
+  };
+  const int first_entries = entries_at(key0);
+  int entries = entries_at(key0 + kKeys);  // of the next tile
+
   vec q[kSteps];
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
@@ -667,19 +686,6 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
       out[t][e] = 0.0F;
   float top = -INFINITY, sum = 0.0F;
 
-  const int32_t *table = prefix ? a.batch.shared_table
-                                : a.batch.page_table + tile.sequence * a.batch.table_stride;
-  // Pages of the tile's four 16-key groups in lanes 0 .. 3 (-1: none).
-  auto pages_at = [&](int k0) {
-    int page = -1;
-    const int key = k0 + 16 * lane;
-    if (lane < 4 && key < key1) {
-      page = checked_page(table, key >> a.cache.page_shift, a.cache.pages);
-      if (page < 0)
-        report(a.batch, kBadPage);
-    }
-    return page;
-  };
   // This lane's source offset inside a DMA, in bytes (K and V: other swizzles).
   uint32_t k_offset[kOps], v_offset[kOps];
 #pragma unroll
@@ -705,10 +711,8 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
     }
   };
 
-  int pages = key0 < key1 ? pages_at(key0) : -1, next_pages = -1;
+  int pages = pages_of(first_entries, key0);
   issue(key0, 0, pages);
-  if (key0 + kKeys < key1)
-    next_pages = pages_at(key0 + kKeys);
   int stage = 0, odd_tiles = 0, odd_first = 0;
   uint16_t *odd_s = tile_lds + 4 * kPlane;  // [tile][wave], 16 keys a bit each
   for (int k0 = key0; k0 < key1; k0 += kKeys, stage ^= 1) {
@@ -752,10 +756,9 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
     }
     __syncthreads();
     if (k0 + kKeys < key1) {
-      issue(k0 + kKeys, stage ^ 1, next_pages);
-      pages = next_pages;
-      if (k0 + 2 * kKeys < key1)
-        next_pages = pages_at(k0 + 2 * kKeys);
+      pages = pages_of(entries, k0 + kKeys);
+      issue(k0 + kKeys, stage ^ 1, pages);
+      entries = entries_at(k0 + 2 * kKeys);
     }
     if (!wave_rows || k0 > wave_last)
       continue;
