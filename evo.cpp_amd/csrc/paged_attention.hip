@@ -24,7 +24,7 @@
 // 16 rows a block (one query's group of heads) are bound by the bytes of keys and
 // values: 64 sequences of up to 8190 positions, 8 key/value heads of 128, 644 MB, take
 // 126 us, 5.1 TB/s, and 5.4 to join their parts. 128 rows a block are bound by issue:
-// 4096 tokens on 12288 cached ones, 32 heads over 8, 962 GFLOP, take 940 us, 1.02
+// 4096 tokens on 12288 cached ones, 32 heads over 8, 962 GFLOP, take 930 us, 1.03
 // PFLOP/s, the matrix cores busy 45% of the cycles and the vector units 40%, at the
 // 1.76 GHz that the card's power leaves; an 8192-cubed product of the library reaches
 // 1.22 PFLOP/s. Rows of up to 16 take the first form (us with it and with the second: 64
