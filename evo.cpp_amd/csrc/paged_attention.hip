@@ -1076,10 +1076,10 @@ struct StreamPhase {
 };
 
 // Keys per block of the 16-row kernel: the split of least modelled time, its constants
-// fitted to measured splits of 33 batches (3% on average behind the best split of each,
-// 14% at most). Keys and values stream at 5.8 TB/s from 256 blocks on; 1000 keys take
-// a block 8 us, and as long at the end, while the chip runs empty; a part's block
-// costs 2 ns and joining the parts 9 us. Chunks are 128 keys and more, 32 for each wave.
+// fitted to measured splits of 48 batches (3% on average behind the best split of each,
+// 25% at most). Keys and values stream at 5.8 TB/s from 160 blocks on; 1000 keys take
+// a block 10 us, and 8 at the end, while the chip runs empty; a part's block costs
+// 3 ns and joining the parts 9 us. Chunks are 128 keys and more, 32 for each wave.
 int stream_chunk(const StreamPhase &phase, size_t head_dim) {
   const double most = static_cast<double>(phase.most), least = phase.uneven ? 0.0 : most;
   const double bytes = 2.0 * (least + most) * static_cast<double>(phase.blocks * head_dim);
@@ -1090,11 +1090,11 @@ int stream_chunk(const StreamPhase &phase, size_t head_dim) {
     if (best != 0 && static_cast<double>(slots) * phase.all_part_bytes > kMostPartBytes)
       break;
     const double blocks = mean_chunks(least, most, chunk) * static_cast<double>(phase.blocks);
-    const double full_us = 0.008 * static_cast<double>(std::min<size_t>(chunk, phase.most));
-    double us = std::max(bytes / (5.8e6 * std::min(1.0, blocks / 256.0)), full_us) +
-                full_us * std::min(1.0, blocks / 444.0);
+    const double full = static_cast<double>(std::min<size_t>(chunk, phase.most));
+    double us = std::max(bytes / (5.8e6 * std::min(1.0, blocks / 160.0)), 0.010 * full) +
+                0.008 * full * std::min(1.0, blocks / 444.0);
     if (static_cast<size_t>(chunk) < phase.most)
-      us += (phase.joined ? 0.0 : 9.0) + 0.002 * blocks;
+      us += (phase.joined ? 0.0 : 9.0) + 0.003 * blocks;
     if (best == 0 || us < best_us) {
       best = chunk;
       best_us = us;

@@ -282,8 +282,8 @@ EVO_API evo_status evo_hip_attention_ws(const float *projected, size_t rows,
  * dtype: EVO_HIP_BF16 or EVO_HIP_F16. page_size: a power of two from 16 to
  * 32768. head_dim: 32, 64 or 128. The strides count elements and are
  * multiples of 8, token_stride at most 2^24; all three 0 means dense
- * [pages][kv_heads][page_size][head_dim]. Both bases are 16-byte aligned. Slots that no sequence has
- * written may hold anything. */
+ * [pages][kv_heads][page_size][head_dim]. Both bases are 16-byte aligned. Slots that no
+ * sequence has written may hold anything. */
 typedef struct evo_hip_paged_cache {
   size_t struct_size;
   evo_hip_dtype dtype;
