@@ -192,11 +192,25 @@ __device__ inline BlockWork block_work(const AttendArgs &a, unsigned prefix_bloc
 // A weight may exceed the running maximum's by 2^8 before the maximum follows.
 constexpr float kSlack = 8.0F;
 
+// Weight of a score where that of `base` is 1. The difference is scaled, not the two
+// scores: their products' roundings would leave 2^(+-256) of it at scores of 2^32.
+__device__ inline float weight(float score, float base, float scale2) {
+  return __builtin_amdgcn_exp2f((score - base) * scale2);
+}
+// 128-row blocks form exp2(score * scale2 - base * scale2) all the same, with one
+// instruction less a score (4096 tokens on 12288 cached ones 938 us, else 963), where
+// the base's product is below this, so that its rounding is below 2^-14. A row beyond
+// has its base taken from its scores first.
+constexpr float kNear = 1024.0F;
+__device__ inline bool is_far(float top, float scale2) {
+  return top != -INFINITY && !(fabsf(top * scale2) < kNear);
+}
+
 // Softmax state and output of 16 rows over the keys a wave has seen. Lane l:
 // row l % 16, output elements kVec * (4 * (l / 16) + i) + t for i < 4, t < kVec.
 template <int kD> struct RowState {
   static constexpr int kVec = kD / 16;
-  float top, sum;  // log2 domain; the sum of this lane's own keys
+  float top, sum;  // a score as it is; the sum of this lane's own keys
   f32x4 out[kVec];
 };
 
@@ -285,10 +299,10 @@ __device__ inline void attend(const f32x4 (&score)[2], const uint32_t (&v)[8][kD
     for (int i = 0; i < 4; ++i)
       top = fmaxf(top, score[u][i]);
   top = fmaxf(top, __shfl_xor(top, 16, 64));
-  top = fmaxf(top, __shfl_xor(top, 32, 64)) * scale2;
-  if (__any(top > state.top + kSlack)) {
+  top = fmaxf(top, __shfl_xor(top, 32, 64));
+  if (__any((top - state.top) * scale2 > kSlack)) {
     const float next = fmaxf(state.top, top);
-    const float shrink = next == -INFINITY ? 1.0F : __builtin_amdgcn_exp2f(state.top - next);
+    const float shrink = next == -INFINITY ? 1.0F : weight(state.top, next, scale2);
     state.sum *= shrink;
 #pragma unroll
     for (int t = 0; t < kVec; ++t)
@@ -303,8 +317,7 @@ __device__ inline void attend(const f32x4 (&score)[2], const uint32_t (&v)[8][kD
   for (int u = 0; u < 2; ++u)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      p[4 * u + i] =
-          static_cast<T>(__builtin_amdgcn_exp2f(fmaf(score[u][i], scale2, -base)));
+      p[4 * u + i] = static_cast<T>(weight(score[u][i], base, scale2));
   state.sum = Mfma<T>::add(p, state.sum);
 #pragma unroll
   for (int t = 0; t < kVec; ++t) {
@@ -485,14 +498,14 @@ __device__ inline void stream_block(const AttendArgs &a, const BlockWork &work,
             a.cache.values + (here[u] * a.cache.page_stride + kv_head * a.cache.head_stride +
                               ((k_here + key) & ((1 << a.cache.page_shift) - 1)) *
                                   a.cache.token_stride);
-        const float weight = __builtin_amdgcn_exp2f(fmaf(s, a.scale2, -base));
+        const float w = weight(s, base, a.scale2);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int t = 0; t < kVec; ++t)
             if (s != -INFINITY)
               state.out[t][i] =
-                  fmaf(weight, element<T>(v[kVec * (4 * g + i) + t]), state.out[t][i]);
+                  fmaf(w, element<T>(v[kVec * (4 * g + i) + t]), state.out[t][i]);
       }
       if (!more)
         break;
@@ -523,8 +536,7 @@ __device__ inline void stream_block(const AttendArgs &a, const BlockWork &work,
   float total = 0.0F, o[kVec] = {};
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    const float scale = top_s[w][r] == -INFINITY ? 0.0F
-                                                 : __builtin_amdgcn_exp2f(top_s[w][r] - top);
+    const float scale = top_s[w][r] == -INFINITY ? 0.0F : weight(top_s[w][r], top, a.scale2);
     total = fmaf(sum_s[w][r], scale, total);
 #pragma unroll
     for (int e = 0; e < kVec; ++e)
@@ -685,6 +697,8 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
     for (int e = 0; e < 16; ++e)
       out[t][e] = 0.0F;
   float top = -INFINITY, sum = 0.0F;
+  float shift = 0.0F;      // a weight is exp2(score * scale2 + shift)
+  bool far_rows = false;   // some of the wave's
 
   // This lane's source offset inside a DMA, in bytes (K and V: other swizzles).
   uint32_t k_offset[kOps], v_offset[kOps];
@@ -812,10 +826,10 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
 #pragma unroll
     for (int e = 0; e < 16; ++e)
       tile_top = fmaxf(tile_top, score[1][e]);
-    tile_top = fmaxf(tile_top, __shfl_xor(tile_top, 32, 64)) * a.scale2;
-    if (__any(tile_top > top + kSlack)) {
+    tile_top = fmaxf(tile_top, __shfl_xor(tile_top, 32, 64));
+    if (__any((tile_top - top) * a.scale2 > kSlack)) {
       const float next = fmaxf(top, tile_top);
-      const float shrink = next == -INFINITY ? 1.0F : __builtin_amdgcn_exp2f(top - next);
+      const float shrink = next == -INFINITY ? 1.0F : weight(top, next, a.scale2);
       sum *= shrink;
 #pragma unroll
       for (int t = 0; t < kTiles; ++t)
@@ -823,14 +837,24 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
         for (int e = 0; e < 16; ++e)
           out[t][e] *= shrink;
       top = next;
+      const bool far = is_far(top, a.scale2);
+      far_rows = __any(far);
+      shift = far || top == -INFINITY ? 0.0F : -top * a.scale2;
     }
-    const float base = top == -INFINITY ? 0.0F : top;
+    if (far_rows) {
+      const float base = is_far(top, a.scale2) ? top : 0.0F;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          score[u][e] -= base;
+    }
     vec p[2];
     const auto weights = [&](int kk) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         p[kk % 2][j] = static_cast<T>(
-            __builtin_amdgcn_exp2f(fmaf(score[kk / 2][8 * (kk % 2) + j], a.scale2, -base)));
+            __builtin_amdgcn_exp2f(fmaf(score[kk / 2][8 * (kk % 2) + j], a.scale2, shift)));
       sum = Mfma<T>::add(p[kk % 2], sum);
     };
     weights(0);
@@ -867,13 +891,13 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
           for (int e = 0; e < 8; ++e)
             dot = fmaf(static_cast<float>(q[s][e]), element<T>(k[16 * s + e]), dot);
         dot += __shfl_xor(dot, 32, 64);
-        const float weight = __builtin_amdgcn_exp2f(fmaf(dot, a.scale2, -top));
+        const float w = weight(dot, top, a.scale2);
         if (key <= position) {
 #pragma unroll
           for (int t = 0; t < kTiles; ++t)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              out[t][e] = fmaf(weight, element<T>(v[32 * t + (e >> 2) * 8 + (e & 3)]), out[t][e]);
+              out[t][e] = fmaf(w, element<T>(v[32 * t + (e >> 2) * 8 + (e & 3)]), out[t][e]);
         }
       }
   }
@@ -986,7 +1010,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const AttendArgs a, 
 #pragma unroll
     for (int i = 0; i < kStates; ++i) {
       // (A chunk without visible keys has no weight.)
-      top[i] = top[i] == -INFINITY ? 0.0F : __builtin_amdgcn_exp2f(top[i] - all);
+      top[i] = top[i] == -INFINITY ? 0.0F : weight(top[i], all, a.scale2);
       total = fmaf(part_sum[i], top[i], total);
     }
 #pragma unroll

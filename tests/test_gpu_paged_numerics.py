@@ -1,0 +1,75 @@
+"""Paged attention at the ends of its numeric range: scores far beyond 2^24."""
+import math
+
+import pytest
+import torch
+
+from paged_util import DEVICE, Paged, attend, exact_attention, half_step
+
+pytestmark = pytest.mark.gpu
+
+# Batches of 16-row and of 128-row blocks, of one chunk and of several, and behind a prefix.
+BATCHES = [([(1, 700), (2, 90)], 0, 4, 2), ([(1, 9000)], 0, 2, 1), ([(40, 300), (7, 50)], 0, 4, 2),
+           ([(150, 3000)], 0, 1, 1), ([(1, 100), (1, 90)], 64, 4, 4),
+           ([(20, 1200), (1, 600)], 512, 4, 1)]
+
+
+def whole_numbers(p, *shape):
+    return torch.randint(-3, 4, shape, generator=p.gen, device=DEVICE).float()
+
+
+@pytest.mark.parametrize("sequences,shared,heads,kv_heads", BATCHES)
+@pytest.mark.parametrize("kind,dim,power", [("bf16", 64, 4), ("bf16", 64, 8), ("bf16", 128, 11),
+                                            ("bf16", 64, 14), ("bf16", 32, 30), ("f16", 64, 4),
+                                            ("f16", 64, 8), ("f16", 128, 9)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_far_scores(sequences, shared, heads, kv_heads, kind, dim, power, sign):
+    """Scores of 2^17 to 2^70 (FP16: 2^25 to 2^35) and all of one sign, exact in F32: products of whole numbers
+    times 2^(2 power), 4096 of them in the first element and at most 9 in each other one. Two
+    scores are equal or at least 2^(2 power) * scale apart, 22, and the keys are copies of
+    six, so that the largest score is met in many steps and chunks. Equal weights are exact
+    in 16 bits, the others are below 2^-32, 2^-18 for all 9000 keys at most. A row is off by
+    them, by its F32 sums (a lane adds less than 2^10 values, the rest is a tree: below
+    2^-13 of the values' size) and by one rounding of the output."""
+    p = Paged(sequences, heads=heads, kv_heads=kv_heads, dim=dim, kind=kind, shared=shared)
+    few, query = whole_numbers(p, 6, kv_heads, dim), whole_numbers(p, p.tokens, heads, dim)
+    few[..., 0], query[..., 0] = 64.0 * sign, 64.0
+    none = p.keys.isnan()
+    which = torch.randint(0, 6, (p.pages, p.page), generator=p.gen, device=DEVICE)
+    p.keys.copy_((few * 2.0 ** power)[which].transpose(1, 2).to(p.kind))
+    p.keys.masked_fill_(none, math.nan)
+    query = (query * 2.0 ** power).view(p.tokens, heads * dim).to(p.kind)
+    scale = dim ** -0.5 * (256 if kind == "f16" else 1)
+    out = attend(p, query, scale).view(p.tokens, heads, dim).double()
+    expected, _ = exact_attention(p, query, scale)
+    room = p.values.nan_to_num().abs().max().double() * 2.0 ** -12 + \
+        expected.abs() * half_step(p.kind)
+    assert torch.isfinite(out).all()
+    assert ((out - expected).abs() <= room).all()
+
+
+@pytest.mark.parametrize("sequences,shared,heads,kv_heads", BATCHES)
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_around_a_thousand(sequences, shared, heads, kv_heads, sign):
+    """Largest scores of a row on both sides of 1024 in units of ln 2 (1012 and 1044, 71 more
+    or less), exact in F32, and a softmax over many keys: 128-row blocks form a weight in
+    another way beyond it. Its exponent is off by one rounding at 1115 (2^-14), where chunks
+    of both ways meet by twice that: below 2^-13 of a weight, and as much in the sum. The weights' rounding counts twice, as the rounded ones are summed."""
+    dim = 32
+    p = Paged(sequences, heads=heads, kv_heads=kv_heads, dim=dim, shared=shared)
+    query = whole_numbers(p, p.tokens, heads, dim)
+    none = p.keys.isnan()
+    keys = whole_numbers(p, *p.keys.shape)
+    keys[..., 0], query[..., 0] = 64.0 * sign, 62.0 if sign > 0 else 64.0
+    p.keys.copy_(keys.to(p.kind))
+    p.keys.masked_fill_(none, math.nan)
+    query = query.view(p.tokens, heads * dim).to(p.kind)
+    scale = dim ** -0.5
+    out = attend(p, query, scale).view(p.tokens, heads, dim).double()
+    expected, _ = exact_attention(p, query, scale)
+    values, p.values = p.values, p.values.abs()
+    size, _ = exact_attention(p, query, scale)  # sum of p |v|
+    p.values = values
+    u = half_step(p.kind)
+    room = size * (2 * u * (1 + 4 * u) + 2.0 ** -12) + expected.abs() * u
+    assert ((out - expected).abs() <= room * (1 + u)).all()
