@@ -189,7 +189,9 @@ __device__ inline BlockWork block_work(const AttendArgs &a, unsigned prefix_bloc
   return w;
 }
 
-// A weight may exceed the running maximum's by 2^8 before the maximum follows.
+// A weight may exceed the running maximum's by 2^8 before the maximum follows. The wave
+// branches as one, but each row follows by its own scores alone: another base rounds its
+// weights differently, and its bits must not depend on what other rows see.
 constexpr float kSlack = 8.0F;
 
 // Weight of a score where that of `base` is 1. The difference is scaled, not the two
@@ -300,9 +302,10 @@ __device__ inline void attend(const f32x4 (&score)[2], const uint32_t (&v)[8][kD
       top = fmaxf(top, score[u][i]);
   top = fmaxf(top, __shfl_xor(top, 16, 64));
   top = fmaxf(top, __shfl_xor(top, 32, 64));
-  if (__any((top - state.top) * scale2 > kSlack)) {
-    const float next = fmaxf(state.top, top);
-    const float shrink = next == -INFINITY ? 1.0F : weight(state.top, next, scale2);
+  const bool follows = (top - state.top) * scale2 > kSlack;
+  if (__any(follows)) {
+    const float next = follows ? top : state.top;
+    const float shrink = follows ? weight(state.top, next, scale2) : 1.0F;
     state.sum *= shrink;
 #pragma unroll
     for (int t = 0; t < kVec; ++t)
@@ -827,9 +830,10 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
     for (int e = 0; e < 16; ++e)
       tile_top = fmaxf(tile_top, score[1][e]);
     tile_top = fmaxf(tile_top, __shfl_xor(tile_top, 32, 64));
-    if (__any((tile_top - top) * a.scale2 > kSlack)) {
-      const float next = fmaxf(top, tile_top);
-      const float shrink = next == -INFINITY ? 1.0F : weight(top, next, a.scale2);
+    const bool follows = (tile_top - top) * a.scale2 > kSlack;
+    if (__any(follows)) {
+      const float next = follows ? tile_top : top;
+      const float shrink = follows ? weight(top, next, a.scale2) : 1.0F;
       sum *= shrink;
 #pragma unroll
       for (int t = 0; t < kTiles; ++t)

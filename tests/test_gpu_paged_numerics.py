@@ -73,3 +73,43 @@ def test_scores_around_a_thousand(sequences, shared, heads, kv_heads, sign):
     u = half_step(p.kind)
     room = size * (2 * u * (1 + 4 * u) + 2.0 ** -12) + expected.abs() * u
     assert ((out - expected).abs() <= room * (1 + u)).all()
+
+
+@pytest.mark.parametrize("heads,kv_heads,n,length,kind,dim", [
+    (2, 2, 12, 300, "bf16", 64), (8, 2, 4, 900, "f16", 128), (4, 4, 100, 500, "bf16", 128),
+    (8, 2, 40, 700, "f16", 64), (2, 1, 40, 5000, "bf16", 32), (1, 1, 10, 5000, "f16", 64)])
+def test_large_later_key_leaves_earlier_rows(heads, kv_heads, n, length, kind, dim):
+    """A key that one row and those after it see gets far larger scores than any other:
+    the rows before it keep their bits, and another sequence's."""
+    p = Paged([(n, length), (3, 20)], heads=heads, kv_heads=kv_heads, dim=dim, kind=kind)
+    query = p.normal(p.tokens, heads * dim, std=1.5)
+    clean = attend(p, query, dim ** -0.5)
+    for position in (length - 1, length - 2, length - n // 2):
+        row = position - (length - n)
+        at = p.page_of(0, position), slice(None), position % p.page
+        kept = p.keys[at].clone()
+        own = query[row:n].view(n - row, kv_heads, heads // kv_heads, dim).float().sum((0, 2))
+        p.keys[at] = (own * (60.0 / own.norm(dim=-1, keepdim=True))).to(p.kind)
+        out = attend(p, query, dim ** -0.5)
+        p.keys[at] = kept
+        assert torch.equal(out[:row], clean[:row]) and torch.equal(out[n:], clean[n:])
+        assert not torch.equal(out[row:n], clean[row:n])
+
+
+@pytest.mark.parametrize("sequences,shared,heads,kv_heads", [
+    ([(1, 330), (1, 400), (1, 321)], 320, 2, 2), ([(2, 900)] * 3, 640, 4, 2),
+    ([(30, 400), (25, 500), (9, 900)], 320, 4, 4), ([(1, 2100)] * 150, 2048, 4, 2)])
+@pytest.mark.parametrize("kind,dim", [("bf16", 64), ("f16", 128)])
+def test_other_sequences_queries_leave_a_row(sequences, shared, heads, kv_heads, kind, dim):
+    """Behind a shared prefix rows of all sequences share a block: one sequence's queries
+    ten times as large change no bit of another's rows."""
+    p = Paged(sequences, heads=heads, kv_heads=kv_heads, dim=dim, kind=kind, shared=shared)
+    query = p.normal(p.tokens, heads * dim, std=1.5)
+    clean = attend(p, query, dim ** -0.5)
+    n, other = sequences[0][0], query.clone()
+    other[n:n + sequences[1][0]] *= 10.0
+    out = attend(p, other, dim ** -0.5)
+    rest = torch.ones(p.tokens, dtype=torch.bool)
+    rest[n:n + sequences[1][0]] = False
+    assert torch.equal(out[rest], clean[rest])
+    assert not torch.equal(out[~rest], clean[~rest])
