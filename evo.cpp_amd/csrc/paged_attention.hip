@@ -189,15 +189,26 @@ __device__ inline BlockWork block_work(const AttendArgs &a, unsigned prefix_bloc
   return w;
 }
 
-// A weight may exceed the running maximum's by 2^8 before the maximum follows. The wave
-// branches as one, but each row follows by its own scores alone: another base rounds its
-// weights differently, and its bits must not depend on what other rows see.
-constexpr float kSlack = 8.0F;
+// A weight may exceed the running maximum's by 2^kSlack before the maximum follows. The
+// wave branches as one, but each row follows by its own scores alone: another base rounds
+// its weights differently, and its bits must not depend on what other rows see.
+// The maximum's own weight is 2^kLift, in the sum and the outputs alike. FP16 spans few
+// powers of two: unlifted, weights below 2^-14 lost bits and those below 2^-25 were
+// nothing, all of a row's output where its leading key has small values. Lifted by 9 it
+// holds weights down to 2^-23 of the largest in full and every one to 2^-34. The slack
+// leaves room below 2^16; less slack and more lift costs prompts (4096 tokens, us: slack
+// 2 180, 4 173, 5 167, 6 and 8 165).
+template <typename T> constexpr float kSlack = std::is_same_v<T, _Float16> ? 6.0F : 8.0F;
+template <typename T> constexpr float kLift = std::is_same_v<T, _Float16> ? 9.0F : 0.0F;
 
 // Weight of a score where that of `base` is 1. The difference is scaled, not the two
 // scores: their products' roundings would leave 2^(+-256) of it at scores of 2^32.
 __device__ inline float weight(float score, float base, float scale2) {
   return __builtin_amdgcn_exp2f((score - base) * scale2);
+}
+// The same lifted, for the cache's type T.
+template <typename T> __device__ inline float lifted(float score, float base, float scale2) {
+  return __builtin_amdgcn_exp2f(fmaf(score - base, scale2, kLift<T>));
 }
 // 128-row blocks form exp2(score * scale2 - base * scale2) all the same, with one
 // instruction less a score (4096 tokens on 12288 cached ones 938 us, else 963), where
@@ -302,7 +313,7 @@ __device__ inline void attend(const f32x4 (&score)[2], const uint32_t (&v)[8][kD
       top = fmaxf(top, score[u][i]);
   top = fmaxf(top, __shfl_xor(top, 16, 64));
   top = fmaxf(top, __shfl_xor(top, 32, 64));
-  const bool follows = (top - state.top) * scale2 > kSlack;
+  const bool follows = (top - state.top) * scale2 > kSlack<T>;
   if (__any(follows)) {
     const float next = follows ? top : state.top;
     const float shrink = follows ? weight(state.top, next, scale2) : 1.0F;
@@ -320,7 +331,7 @@ __device__ inline void attend(const f32x4 (&score)[2], const uint32_t (&v)[8][kD
   for (int u = 0; u < 2; ++u)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      p[4 * u + i] = static_cast<T>(weight(score[u][i], base, scale2));
+      p[4 * u + i] = static_cast<T>(lifted<T>(score[u][i], base, scale2));
   state.sum = Mfma<T>::add(p, state.sum);
 #pragma unroll
   for (int t = 0; t < kVec; ++t) {
@@ -501,7 +512,7 @@ __device__ inline void stream_block(const AttendArgs &a, const BlockWork &work,
             a.cache.values + (here[u] * a.cache.page_stride + kv_head * a.cache.head_stride +
                               ((k_here + key) & ((1 << a.cache.page_shift) - 1)) *
                                   a.cache.token_stride);
-        const float w = weight(s, base, a.scale2);
+        const float w = lifted<T>(s, base, a.scale2);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -700,7 +711,7 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
     for (int e = 0; e < 16; ++e)
       out[t][e] = 0.0F;
   float top = -INFINITY, sum = 0.0F;
-  float shift = 0.0F;      // a weight is exp2(score * scale2 + shift)
+  float shift = kLift<T>;  // a weight is exp2(score * scale2 + shift)
   bool far_rows = false;   // some of the wave's
 
   // This lane's source offset inside a DMA, in bytes (K and V: other swizzles).
@@ -830,7 +841,7 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
     for (int e = 0; e < 16; ++e)
       tile_top = fmaxf(tile_top, score[1][e]);
     tile_top = fmaxf(tile_top, __shfl_xor(tile_top, 32, 64));
-    const bool follows = (tile_top - top) * a.scale2 > kSlack;
+    const bool follows = (tile_top - top) * a.scale2 > kSlack<T>;
     if (__any(follows)) {
       const float next = follows ? tile_top : top;
       const float shrink = follows ? weight(top, next, a.scale2) : 1.0F;
@@ -843,7 +854,7 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
       top = next;
       const bool far = is_far(top, a.scale2);
       far_rows = __any(far);
-      shift = far || top == -INFINITY ? 0.0F : -top * a.scale2;
+      shift = far || top == -INFINITY ? kLift<T> : fmaf(-top, a.scale2, kLift<T>);
     }
     if (far_rows) {
       const float base = is_far(top, a.scale2) ? top : 0.0F;
@@ -895,7 +906,7 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
           for (int e = 0; e < 8; ++e)
             dot = fmaf(static_cast<float>(q[s][e]), element<T>(k[16 * s + e]), dot);
         dot += __shfl_xor(dot, 32, 64);
-        const float w = weight(dot, top, a.scale2);
+        const float w = lifted<T>(dot, top, a.scale2);
         if (key <= position) {
 #pragma unroll
           for (int t = 0; t < kTiles; ++t)

@@ -113,3 +113,36 @@ def test_other_sequences_queries_leave_a_row(sequences, shared, heads, kv_heads,
     rest[n:n + sequences[1][0]] = False
     assert torch.equal(out[rest], clean[rest])
     assert not torch.equal(out[~rest], clean[~rest])
+
+
+@pytest.mark.parametrize("step", [13.5, 15.5, 20, 23.5, 26, 28.5])
+@pytest.mark.parametrize("first", [True, False])
+@pytest.mark.parametrize("rows,length,heads,shared", [
+    (1, 16000, 1, 0), (40, 16000, 1, 0), (1, 300, 4, 0), (100, 400, 2, 0), (2, 4200, 2, 4096),
+    (70, 4300, 2, 4096)])
+def test_many_small_fp16_weights(step, first, rows, length, heads, shared):
+    """One key takes 2^step times the weight of every other, and its values are small: the
+    others, down to 2^-28.5, make the row. Scores are exact: (step, 0, ..) times ln 2. The
+    bound counts the weights' rounding twice, as the rounded ones are summed: relative, or
+    for each key half the spacing of FP16's smallest values, 2^-25, where the largest weight
+    is 2^9 and more; F32 sums, below 2^-14; the output's rounding."""
+    dim = 64
+    p = Paged([(rows, length)], heads=heads, kv_heads=1, dim=dim, kind="f16", shared=shared)
+    query = torch.zeros(rows, heads, dim, device=DEVICE)
+    query[..., 0] = 1.0
+    query = query.view(rows, heads * dim).to(p.kind)
+    none = p.keys.isnan()
+    p.keys.zero_()
+    # (Every row sees both places.)
+    place = 0 if first else length - rows
+    at = p.page_of(0, place), slice(None), place % p.page
+    p.keys[at + (0,)] = float(step)
+    p.keys.masked_fill_(none, math.nan)
+    p.values.copy_((p.values.abs() + 0.5) * 512.0)
+    p.values[at] = 2.0 ** -10
+    scale = math.log(2.0)
+    out = attend(p, query, scale).view(rows, heads, dim).double()
+    expected, _ = exact_attention(p, query, scale)
+    u, most = half_step(p.kind), p.values.nan_to_num().double().abs().max()
+    room = expected * (2 * u * (1 + 4 * u) + 2.0 ** -14 + u) + 2 * length * 2.0 ** -34 * most
+    assert ((out - expected).abs() <= room + torch.finfo(p.kind).smallest_normal * u * 2).all()
