@@ -1327,8 +1327,9 @@ Status paged_attention(const PagedCache &cache, const PagedBatch &batch, const v
   if (out == query && out_stride != query_stride)
     return {ErrorCode::kInvalidArgument,
             "paged_attention: in place, out_stride has to be query_stride"};
-  if (!(scale > 0.0F) || !std::isfinite(scale))
-    return {ErrorCode::kInvalidArgument, "paged_attention: scale must be positive and finite"};
+  const float scale2 = 1.4426950408889634F * scale;
+  if (!(scale > 0.0F) || !std::isfinite(scale2))
+    return {ErrorCode::kInvalidArgument, "paged_attention: scale must be positive, and its multiple by log2(e) finite"};
   // (Rows are counted in 32 bits, up to the end of their last tile.)
   if (static_cast<size_t>(batch.tokens) * heads >= (size_t{1} << 31) - 128)
     return {ErrorCode::kInvalidArgument, "paged_attention: too many rows"};
@@ -1341,7 +1342,7 @@ Status paged_attention(const PagedCache &cache, const PagedBatch &batch, const v
                 " bytes needed) or not 16-byte aligned"};
   const AttendArgs args{cache, batch, static_cast<const uint16_t *>(query), query_stride,
                         static_cast<uint16_t *>(out), out_stride, static_cast<int>(heads),
-                        static_cast<int>(heads / kv), 1.4426950408889634F * scale, plan.chunk,
+                        static_cast<int>(heads / kv), scale2, plan.chunk,
                         plan.prefix_chunk, plan.prefix_slots, plan.slots,
                         plan.own_stream ? 1 : 0,
                         static_cast<float *>(workspace),

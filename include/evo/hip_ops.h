@@ -372,7 +372,7 @@ EVO_API evo_status evo_hip_paged_append(const evo_hip_paged_cache *cache,
  *   query  [tokens][query_stride] and out [tokens][out_stride], the cache's
  *          dtype, heads side by side, 16-byte aligned, strides multiples of 8;
  *          out may be query, with the same stride.
- *   scale  positive (1 / sqrt(head_dim) as a rule).
+ *   scale  positive and below 2.3e38 (1 / sqrt(head_dim) as a rule).
  * With shared_length the prefix's keys are read once for the rows of all
  * sequences, not once for each.
  * What a row does not see has no effect on it, infinities and NaN included:

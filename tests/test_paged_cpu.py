@@ -240,3 +240,10 @@ def test_sequence_of_row(rules, starts):
 @pytest.mark.parametrize("entry,page", [(0, 0), (7, 7), (8, -1), (-1, -1), (LOW, -1), (HIGH, -1)])
 def test_page_of_table(rules, entry, page):
     assert rules.evo_test_paged_page(ints([3, entry]), 1, 8) == page
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 3.4e38])
+def test_scale_beyond_its_binary_form_refused(scale):
+    """A finite scale whose multiple by log2(e) is infinite: every weight would be NaN."""
+    with pytest.raises(N.OpError, match="scale"):
+        attend(scale=scale)
