@@ -9,10 +9,12 @@
 // border, and only that bin's tokens are ranked.
 //
 // The weights exp((logit - top) / temperature) are 64-bit and summed as
-// integers of 2^-42: such a sum has no order, so neither the atomics of the
-// histogram nor a split of a row can change a token, and a border is off by less
-// than 1e-11 of the row's largest weight. A weight below 2^-43 (30 below the top,
-// in units of the temperature) counts as none.
+// integers of 2^-B: such a sum has no order, so neither the atomics of the
+// histogram nor a split of a row can change a token. B = 63 - ceil(log2(vocab)),
+// 51 at most, is what 64-bit sums leave room for: each weight is rounded by up to
+// 2^-(B+1) of the largest, so a border is off by vocab * 2^-(B+1) at most (512
+// values 1.1e-13, 131072 9.3e-10, 2^20 6.0e-8). A weight below 2^-(B+1) counts as
+// none.
 //
 // What bounds it: 2048 rows of 512 values 10.4 us, one round of waves, each a chain of
 // reductions, LDS atomics and two or three searches; 128 rows of 131072 BF16 values 64
@@ -31,7 +33,6 @@ namespace evo::hip {
 
 namespace {
 
-constexpr double kReach = 31.0;  // exp(-31) < 2^-43
 constexpr uint32_t kNoToken = 0xffffffffU;
 
 struct SampleArgs {
@@ -42,6 +43,8 @@ struct SampleArgs {
   const int32_t *top_k;
   const float *top_p, *min_p, *uniform;
   uint32_t *tokens;
+  double units;  // 2^B, the largest weight
+  double reach;  // exp(-reach) = 2^-(B+2)
 };
 
 // Order of the values as integers; -0 and 0 are one value.
@@ -79,9 +82,9 @@ __device__ const double kPowers[64] = {
     0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0,
 };
 
-// exp(x) in units of 2^-42, rounded, for x = z * ln(2) / 64 in [-32, 0]: with
+// exp(x) in units of 2^-B, B <= 51, rounded, for x = z * ln(2) / 64 in [-37, 0]: with
 // z = n + f, 2^(n / 64) from a table and a shift, exp(f ln(2) / 64) by its
-// series to the fifth power in f (the next term is below 2^-60).
+// series to the fifth power in f (the next term is below 2^-54).
 __device__ inline uint64_t weight_units(double z, const double *powers) {
   const double n = __builtin_rint(z), f = z - n;
   double e = 1.2417843701716925e-12;
@@ -90,7 +93,7 @@ __device__ inline uint64_t weight_units(double z, const double *powers) {
   e = fma(e, f, 5.86490495505617e-05);
   e = fma(e, f, 0.010830424696249145);
   e = fma(e, f, 1.0);
-  // powers[] is the table times 2^42; whole / 64 goes into the exponent.
+  // powers[] is the table times 2^B; whole / 64 goes into the exponent.
   const int whole = static_cast<int>(n);
   const uint64_t bits = __builtin_bit_cast(uint64_t, e * powers[whole & 63]) +
                         (static_cast<uint64_t>(static_cast<uint32_t>(whole & ~63) << 14) << 32);
@@ -173,11 +176,12 @@ __device__ inline V block_reduce(V v, V *scratch, F f) {
 struct Cuts {
   float temperature, top_p, min_p, uniform;
   int top_k;
+  double units;
   __device__ Cuts(const SampleArgs &a, size_t r)
       : temperature(a.temperature == nullptr ? 1.0F : a.temperature[r]),
         top_p(a.top_p == nullptr ? 1.0F : a.top_p[r]),
         min_p(a.min_p == nullptr ? 0.0F : a.min_p[r]), uniform(a.uniform[r]),
-        top_k(a.top_k == nullptr ? 0 : a.top_k[r]) {}
+        top_k(a.top_k == nullptr ? 0 : a.top_k[r]), units(a.units) {}
   __device__ bool valid() const {
     return temperature >= 0.0F && temperature < INFINITY && top_k >= 0 && top_p > 0.0F &&
            top_p <= 1.0F && min_p >= 0.0F && min_p <= 1.0F && uniform == uniform;
@@ -188,7 +192,7 @@ struct Cuts {
   __device__ bool greedy() const { return temperature == 0.0F || top_k == 1; }
   // Least weight that min-p keeps.
   __device__ uint64_t least() const {
-    return static_cast<uint64_t>(__builtin_ceil(static_cast<double>(min_p) * 4398046511104.0));
+    return static_cast<uint64_t>(__builtin_ceil(static_cast<double>(min_p) * units));
   }
   // The nucleus keeps tokens while the weight before them is below top_p * total: up
   // to the first at which the weight, itself included, passes this.
@@ -222,9 +226,9 @@ struct Values {
 struct Scale {
   float top, reach, bin_scale;
   double unit;  // 64 / (ln 2 * temperature)
-  __device__ Scale(float top_, float low, float temperature, int bins)
+  __device__ Scale(const SampleArgs &a, float top_, float low, float temperature, int bins)
       : top(top_), reach(static_cast<float>(
-                       fmin(kReach * static_cast<double>(temperature), 3.0e38))),
+                       fmin(a.reach * static_cast<double>(temperature), 3.0e38))),
         unit(92.33248261893106 / static_cast<double>(temperature)) {
     const float range = fminf(reach, top - low);
     // A little less than bins / range: the last value stays inside.
@@ -412,7 +416,7 @@ __global__ __launch_bounds__(64) void sample_wave_kernel(const SampleArgs a) {
   for (int e = 0; e < kPer; ++e)
     v[e] = 64 * e + lane < a.vocab ? static_cast<float>(logits[64 * e + lane]) : -INFINITY;
   const Cuts cuts(a, r);
-  powers[lane] = kPowers[lane] * 4398046511104.0;
+  powers[lane] = kPowers[lane] * a.units;
   const WaveBins bins{mass_s, count_s};
   bins.clear();
   float top = -INFINITY, low = INFINITY;
@@ -440,7 +444,7 @@ __global__ __launch_bounds__(64) void sample_wave_kernel(const SampleArgs a) {
       a.tokens[r] = static_cast<uint32_t>(first);
     return;
   }
-  const Scale scale(top, low, cuts.temperature, 256);
+  const Scale scale(a, top, low, cuts.temperature, 256);
   uint64_t w[kPer], kept = 0;
   int bin[kPer];
   const uint64_t least = cuts.least();
@@ -892,9 +896,9 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs 
     mass[i] = 0;
   }
   if (threadIdx.x < 64)
-    powers[threadIdx.x] = kPowers[threadIdx.x] * 4398046511104.0;
+    powers[threadIdx.x] = kPowers[threadIdx.x] * a.units;
   __syncthreads();
-  const Scale scale(range.x, range.y, cuts.temperature, kSplitBins);
+  const Scale scale(a, range.x, range.y, cuts.temperature, kSplitBins);
   uint64_t kept =
       fill_bins<kThreads>(row, now, scale, weighted, cuts.least(), count, mass, powers);
   kept = block_reduce<kThreads>(kept, scratch, Sum{});
@@ -955,7 +959,7 @@ __global__ __launch_bounds__(kThreads) void sample_block_kernel(const SampleArgs
     }
   };
   if (threadIdx.x < 64)
-    s.powers[threadIdx.x] = kPowers[threadIdx.x] * 4398046511104.0;
+    s.powers[threadIdx.x] = kPowers[threadIdx.x] * a.units;
   const float2 range = kSplit ? split.whole_range(r) : row_range<kThreads>(row, scratch_f);
   const float top = range.x;
   if (!cuts.samples(top)) {
@@ -973,7 +977,7 @@ __global__ __launch_bounds__(kThreads) void sample_block_kernel(const SampleArgs
       a.tokens[r] = static_cast<uint32_t>(first);
     return;
   }
-  const Scale scale(top, range.y, cuts.temperature, kBins);
+  const Scale scale(a, top, range.y, cuts.temperature, kBins);
   const uint64_t least = cuts.least();
   const bool has_k = cuts.has_k(a.vocab);
   const uint32_t rank = static_cast<uint32_t>(cuts.top_k) - 1;
@@ -1177,8 +1181,13 @@ Status sample_tokens(int dtype, const void *logits, size_t rows, size_t vocab, s
   if (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||
                                workspace_bytes < sample_workspace_bytes(rows, vocab)))
     return {ErrorCode::kInvalidArgument, "sample: workspace too small or not 16-byte aligned"};
-  const SampleArgs args{logits, static_cast<int>(vocab), row_stride, temperature, top_k,
-                        top_p, min_p, uniform, tokens};
+  int log2_vocab = 0;  // rounded up
+  while ((size_t{1} << log2_vocab) < vocab)
+    ++log2_vocab;
+  const int bits = std::min(51, 63 - log2_vocab);
+  const SampleArgs args{logits, static_cast<int>(vocab), row_stride, temperature, top_k, top_p,
+                        min_p, uniform, tokens, std::ldexp(1.0, bits),
+                        0.6931471805599453 * (bits + 2)};
   if (dtype == kElementF32)
     return launch_sample<float>(args, rows, workspace, stream);
   if (dtype == kElementBF16)

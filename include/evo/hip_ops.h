@@ -396,8 +396,9 @@ EVO_API evo_status evo_hip_paged_attention(const evo_hip_paged_cache *cache,
 /* tokens[r] = one token of row r of logits [rows][row_stride] (F32, BF16 or
  * F16; rows and vocab at most 2^20), in the order and with the cuts of evo_sampler_sample:
  * tokens by descending logit, equal ones by ascending index; of these the first
- * top_k (0, or vocab and more: all); weights exp(logit / temperature) in 64 bits
- * (one below 2^-43 of the largest counts as none);
+ * top_k (0, or vocab and more: all); weights exp(logit / temperature) in 64 bits,
+ * held to 2^-(B+1) of the largest, B = 63 - ceil(log2(vocab)) and 51 at most (one
+ * below that counts as none, and a border is off by vocab times that at most);
  * of these the shortest beginning whose weight reaches top_p of what top-k left
  * (1: all); of these the ones of at least min_p times the largest weight (0: all);
  * then the first whose cumulative weight exceeds uniform times the weight left.

@@ -260,3 +260,34 @@ def mt19937_64(seed):
     y ^= (y << 37) & 0xFFF7EEE000000000
     y ^= y >> 43
     return (y & mask) >> 11
+
+
+@pytest.mark.parametrize("vocab,least,most", [(512, 5, 10), (1000, 6, 11), (5000, 8, 14),
+                                              (131072, 20, 27), (2 ** 20, 22, 28)])
+@pytest.mark.parametrize("workspace", [True, False])
+def test_draws_in_a_flat_tail(vocab, least, most, workspace):
+    """One token and many equal ones far below it, and draws among those. A weight is held to
+    2^-(B+1) of the largest, B = min(51, 63 - ceil(log2(vocab))): the cumulative weights on
+    both sides of the token pass the draw but for vocab times that, in the running weight and
+    in the total each, and for the definition's own sums in 64 bits (vocab additions of 2^-53
+    of a total that is below 2, four times)."""
+    rng = np.random.default_rng(vocab)
+    rows = 40
+    below = np.linspace(least, most, rows).astype(np.float32)
+    leader = rng.integers(0, vocab, rows)
+    logits = np.repeat(-below[:, None], vocab, 1)
+    logits[np.arange(rows), leader] = 0.0
+    weight = np.exp(-below.astype(np.float64))
+    total = 1.0 + weight * (vocab - 1)
+    # Steps of 2^-24 below 1 that lie in the tail.
+    steps = np.maximum(1, np.floor(rng.random(rows) * (1 - 1 / total) * 2 ** 24))
+    uniform = (1.0 - steps * 2.0 ** -24).astype(np.float32)
+    got = sample(torch.from_numpy(logits).to(DEVICE), f32(uniform.tolist()),
+                 workspace=workspace).numpy()
+    bits = min(51, 63 - math.ceil(math.log2(vocab)))
+    room = 2 * vocab * 2.0 ** -(bits + 1) + vocab * 2.0 ** -51
+    rank = np.where(got == leader, 0, np.where(got < leader, got + 1, got))
+    drawn = uniform.astype(np.float64) * total
+    assert (rank > 0).all()
+    assert (1.0 + (rank - 1) * weight <= drawn + room).all()
+    assert (1.0 + rank * weight >= drawn - room).all()
