@@ -405,7 +405,10 @@ EVO_API evo_status evo_hip_paged_attention(const evo_hip_paged_cache *cache,
  * temperature 0, or top_k 1: the first token.
  *   temperature, top_p, min_p (F32), top_k (int32): device [rows], or NULL for
  *     1, 1, 0 and 0.
- *   uniform: device F32 [rows], in [0, 1) (beyond: its nearer end).
+ *   uniform: device F32 [rows], in [0, 1) (beyond: its nearer end). Its 24 bits are
+ *     the draw's resolution: evo_sampler_sample draws 53, so the two agree where
+ *     no border lies between its draw and the F32 one, and tokens of less than 2^-24
+ *     of the weight are met in steps of that.
  * The device arrays are read when the call runs. A row gets UINT32_MAX where its
  * logits hold NaN or +infinity or nothing above -infinity, or its parameters are
  * out of range (temperature negative or not finite, top_k negative, top_p outside

@@ -291,3 +291,31 @@ def test_draws_in_a_flat_tail(vocab, least, most, workspace):
     assert (rank > 0).all()
     assert (1.0 + (rank - 1) * weight <= drawn + room).all()
     assert (1.0 + rank * weight >= drawn - room).all()
+
+
+@pytest.mark.parametrize("vocab", [512, 5000, 50257, 131072])
+def test_draws_beside_borders(vocab):
+    """The two F32 draws nearest to the end of a token's share, one before it and one not:
+    that token and the next. (They are no nearer than the borders are held, in the definition's
+    64-bit sums too.)"""
+    rng = np.random.default_rng(vocab + 1)
+    rows = 64
+    logits = rng.normal(0, 2.5, (rows, vocab)).astype(np.float32)
+    bits = min(51, 63 - math.ceil(math.log2(vocab)))
+    uniform, expected = [], []
+    for r in range(rows):
+        order = np.argsort(-logits[r], kind="stable")
+        share = np.exp(logits[r, order].astype(np.float64) - float(logits[r, order[0]]))
+        total = share.sum()
+        ahead = np.cumsum(share) / total
+        room = vocab * (2.0 ** -bits + 2.0 ** -51)  # of the weight before the draw and the total
+        # A token early in the order: its neighbours' shares are wider than F32's steps.
+        rank = int(rng.integers(0, min(60, vocab // 8)))
+        near = np.float32(ahead[rank])
+        step = np.float32(np.inf if r % 2 else -np.inf)
+        while (near >= ahead[rank]) != (r % 2 == 1) or abs(near - ahead[rank]) * total < room:
+            near = np.nextafter(near, step)
+        uniform.append(float(near))
+        expected.append(int(order[rank + r % 2]))
+    got = sample(torch.from_numpy(logits).to(DEVICE), f32(uniform))
+    assert got.tolist() == expected
