@@ -146,3 +146,42 @@ def test_many_small_fp16_weights(step, first, rows, length, heads, shared):
     u, most = half_step(p.kind), p.values.nan_to_num().double().abs().max()
     room = expected * (2 * u * (1 + 4 * u) + 2.0 ** -14 + u) + 2 * length * 2.0 ** -34 * most
     assert ((out - expected).abs() <= room + torch.finfo(p.kind).smallest_normal * u * 2).all()
+
+
+@pytest.mark.parametrize("n,length,heads,kv_heads", [(3, 200, 4, 2), (40, 300, 2, 2), (1, 3000, 1, 1)])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_scores_of_minus_infinity(n, length, heads, kv_heads, kind):
+    """Keys whose scores are -infinity have no weight; rows that see no other are zero."""
+    p = Paged([(n, length)], heads=heads, kv_heads=kv_heads, dim=64, kind=kind)
+    query = p.normal(n, heads, 64)
+    query[..., 0] = 1.0
+    query = query.view(n, -1).contiguous()
+    first = length - n + 1  # The first row sees only what lies before this position.
+    for position in range(length):
+        if position < first - 1 or position % 3 == 0:
+            p.keys[p.page_of(0, position), :, position % p.page, 0] = -math.inf
+    out = attend(p, query, 0.125)
+    everything = p.keys.clone()
+    p.keys[..., 0].masked_fill_(~p.keys[..., 0].isnan(), -math.inf)
+    assert (attend(p, query, 0.125) == 0).all()
+    p.keys.copy_(everything)
+    seen = [i for i in range(length) if not (i < first - 1 or i % 3 == 0)]
+    rows = query.view(n, heads, 64).double()
+    if not seen:
+        assert (out == 0).all()
+        return
+    at = torch.tensor(seen, device=DEVICE)
+    pages = torch.tensor([p.page_of(0, i) for i in seen], device=DEVICE)
+    k, v = (pool[pages, :, at % p.page].double().repeat_interleave(heads // kv_heads, 1)
+            for pool in (p.keys, p.values))
+    for row in range(n):
+        mine = at <= length - n + row
+        if not mine.any():
+            assert (out[row] == 0).all()
+            continue
+        w = torch.softmax(torch.einsum("hd,khd->hk", rows[row], k[mine]) * 0.125, 1)
+        expected, size = (torch.einsum("hk,khd->hd", w, x[mine]) for x in (v, v.abs()))
+        u = half_step(p.kind)
+        # (Scores: sums of 64 products of size 64 at most in all, 72 roundings, felt twice.)
+        room = size * (2 * u * (1 + 4 * u) + 2 * 72 * 64 * 2.0 ** -24) + expected.abs() * u
+        assert ((out[row].view(heads, 64).double() - expected).abs() <= room * (1 + u) + 1e-6).all()
