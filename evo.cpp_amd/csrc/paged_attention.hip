@@ -17,19 +17,19 @@
 // that order as long as V does. K and V go from memory to registers without LDS:
 // a K operand is 16 bytes of a key's row as it lies, and a lane loads 8 keys x 8
 // elements of V and transposes them with v_perm (one per output word).
-// Scores, maxima, sums and outputs are F32; the weights p <= 1 are rounded to the
-// cache's type for the second product, and the sum is taken of the rounded ones,
-// so that the weights applied add up to one.
+// Scores, maxima, sums and outputs are F32; the weights (at most 2^8 before the maximum
+// follows, in FP16 2^15) are rounded to the cache's type for the second product, and
+// the sum is taken of the rounded ones, so that the weights applied add up to one.
 //
 // 16 rows a block (one query's group of heads) are bound by the bytes of keys and
 // values: 64 sequences of up to 8190 positions, 8 key/value heads of 128, 644 MB, take
-// 126 us, 5.1 TB/s, and 5.4 to join their parts. 128 rows a block are bound by issue:
-// 4096 tokens on 12288 cached ones, 32 heads over 8, 962 GFLOP, take 930 us, 1.03
-// PFLOP/s, the matrix cores busy 45% of the cycles and the vector units 40%, at the
-// 1.76 GHz that the card's power leaves; an 8192-cubed product of the library reaches
-// 1.22 PFLOP/s. Rows of up to 16 take the first form (us with it and with the second: 64
-// sequences of 2000, one token 45 and 59, four tokens 53 and 69; 32 sequences of 16
-// tokens, one head a key/value head, 94 and 110).
+// 126 us, 5.1 TB/s, and 5.3 to join their parts. 128 rows a block are bound by issue:
+// 4096 tokens on 12288 cached ones, 32 heads over 8, 962 GFLOP, take 905 to 935 us (two
+// cards), 1.06 to 1.03 PFLOP/s, the matrix cores busy 51% of the cycles and the vector
+// units 44%, at the 1.76 GHz that the card's power leaves; an 8192-cubed product of the
+// library reaches 1.22 PFLOP/s. Rows of up to 16 take the first form (us with it and with
+// the second: 64 sequences of 2000, one token 49 and 56, four tokens 50 and 65; 32
+// sequences of 16 tokens, one head a key/value head, 94 and 108).
 #include "common.hpp"
 #include "ops.hpp"
 #include "paged.hpp"
@@ -1115,8 +1115,8 @@ struct StreamPhase {
 };
 
 // Keys per block of the 16-row kernel: the split of least modelled time, its constants
-// fitted to measured splits of 48 batches (3% on average behind the best split of each,
-// 25% at most). Keys and values stream at 5.8 TB/s from 160 blocks on; 1000 keys take
+// fitted to measured splits (3% on average behind the best split of each of 49 batches,
+// 26% at most: 4 sequences of up to 6000 keys, 21.6 us for 17.1). Keys and values stream at 5.8 TB/s from 160 blocks on; 1000 keys take
 // a block 10 us, and 8 at the end, while the chip runs empty; a part's block costs
 // 3 ns and joining the parts 9 us. Chunks are 128 keys and more, 32 for each wave.
 int stream_chunk(const StreamPhase &phase, size_t head_dim) {
@@ -1154,8 +1154,10 @@ struct TilePhase {
 };
 
 // Keys per block: the split of least modelled time, its constants fitted to measured
-// splits of 34 batches (3% on average behind the best split of each, 23% at most).
-// 64 keys of head_dim 128 take a block 2.3 us where two share a CU and 2.1 alone;
+// splits (4% on average behind the best split of each of 40 batches, 28% at most: 16
+// ragged sequences of up to 64 tokens on 2000, 46 us for 36). 64 keys of head_dim 128
+// take a block 2.3 us where two share a CU and 2.1 alone (in the middle of a long
+// chunk the kernel now measures 2.1 and 1.2: of a lone block the model is least true);
 // 512 blocks run at a time, the longest start first, and the last ones leave part of
 // the chip idle. Keys and values stream at 5 TB/s from 512 blocks, at 3.6 from one
 // a CU. A part costs its bytes at 1.3 TB/s (written, read again, more tails), and all

@@ -306,8 +306,10 @@ typedef struct evo_hip_paged_cache {
  * (token_start[sequences] < tokens) belong to none and are left as they are.
  *   max_tokens, max_length: host bounds on a sequence's rows and positions
  *     (max_length <= table_stride * page_size, at most 2^30). They choose the
- *     launches: close bounds run faster. tokens is below 2^24, sequences at
- *     most 2^20.
+ *     launches: close bounds run faster. tokens is at most 2^24, sequences at
+ *     most 2^20, and a launch 2^24 blocks: a call that would need more is refused
+ *     (attention takes a block for each key/value head of each sequence and of each
+ *     16 or 128 rows, times the chunks of its keys; tokens * heads is below 2^31 - 128).
  *   token_start, lengths, page_table: int32 device arrays, read by each call
  *     when it runs, so a captured graph follows their changes within the
  *     bounds; page_table [sequences][table_stride].
@@ -376,7 +378,11 @@ EVO_API evo_status evo_hip_paged_append(const evo_hip_paged_cache *cache,
  * With shared_length the prefix's keys are read once for the rows of all
  * sequences, not once for each.
  * What a row does not see has no effect on it, infinities and NaN included:
- * positions behind its own, slots behind a sequence's length, other pages.
+ * positions behind its own, slots behind a sequence's length, other pages, other rows.
+ * Scores and sums are F32. Weights are rounded to the cache's type for their product
+ * with the values: BF16 to 2^-8 of each, FP16 to 2^-11 of each that is at least 2^-23
+ * of the row's largest, the others to 2^-34 of the largest. A row whose every score is
+ * -infinity is zero.
  * The workspace (16-byte aligned, no initial contents) takes the partial
  * results of keys that are split over blocks; its size depends on the host
  * fields of the structs and heads alone. It does not grow with the batch (few
