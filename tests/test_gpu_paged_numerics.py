@@ -185,3 +185,20 @@ def test_scores_of_minus_infinity(n, length, heads, kv_heads, kind):
         # (Scores: sums of 64 products of size 64 at most in all, 72 roundings, felt twice.)
         room = size * (2 * u * (1 + 4 * u) + 2 * 72 * 64 * 2.0 ** -24) + expected.abs() * u
         assert ((out[row].view(heads, 64).double() - expected).abs() <= room * (1 + u) + 1e-6).all()
+
+
+@pytest.mark.parametrize("sequences,shared,heads,kv_heads", BATCHES)
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("what", [1000.0, 1e30, math.inf, math.nan])
+def test_one_rows_query_leaves_the_others(sequences, shared, heads, kv_heads, kind, what):
+    """A row of far larger scores, of infinite ones, or of NaN, in a block of others."""
+    p = Paged(sequences, heads=heads, kv_heads=kv_heads, dim=64, kind=kind, shared=shared)
+    query = p.normal(p.tokens, heads * 64, std=1.5)
+    clean = attend(p, query, 0.125)
+    row = p.tokens // 2
+    other = query.clone()
+    other[row] = (query[row].float() * what).to(p.kind)
+    out = attend(p, other, 0.125)
+    rest = torch.arange(p.tokens) != row
+    assert torch.equal(out[rest], clean[rest])
+    assert not torch.equal(out[row], clean[row])
