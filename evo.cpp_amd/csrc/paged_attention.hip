@@ -899,14 +899,16 @@ __device__ inline void tile_block(const AttendArgs &a, const BlockWork &work,
         const size_t at = page * a.cache.page_stride + work.kv_head * a.cache.head_stride +
                           (key & slot_mask) * a.cache.token_stride;
         const uint16_t *k = a.cache.keys + at + 8 * half, *v = a.cache.values + at + 4 * half;
-        float dot = 0.0F;
+        // The score as it was: the same instructions, the key in all of their 32 rows. (A
+        // sum in another order is another one, by any factor in the weight of a far score.)
+        f32x16 score;
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          score[e] = 0.0F;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            dot = fmaf(static_cast<float>(q[s][e]), element<T>(k[16 * s + e]), dot);
-        dot += __shfl_xor(dot, 32, 64);
-        const float w = lifted<T>(dot, top, a.scale2);
+          score = Mfma<T>::run(*reinterpret_cast<const vec *>(k + 16 * s), q[s], score);
+        const float w = lifted<T>(score[0], top, a.scale2);
         if (key <= position) {
 #pragma unroll
           for (int t = 0; t < kTiles; ++t)

@@ -202,3 +202,24 @@ def test_one_rows_query_leaves_the_others(sequences, shared, heads, kv_heads, ki
     rest = torch.arange(p.tokens) != row
     assert torch.equal(out[rest], clean[rest])
     assert not torch.equal(out[row], clean[row])
+
+
+@pytest.mark.parametrize("n,length,heads,kv_heads,dim", [
+    (10, 300, 2, 2, 64), (40, 300, 2, 2, 64), (100, 900, 4, 2, 128), (70, 5000, 1, 1, 32)])
+def test_leading_key_of_far_scores_with_an_infinite_value(n, length, heads, kv_heads, dim):
+    """Scores near 2^34 that are not exact in F32, and a key that leads every row which sees
+    it by 2^30 and more: these rows are its values, one of them infinite."""
+    p = Paged([(n, length), (3, 20)], heads=heads, kv_heads=kv_heads, dim=dim)
+    query = p.normal(p.tokens, heads, dim, std=2e4)
+    query[..., 0] = 2.0 ** 17
+    query = query.view(p.tokens, -1)
+    none = p.keys.isnan()
+    p.keys.copy_(p.keys.float() * 2e4).masked_fill_(none, math.nan)
+    position = length - n + 1
+    at = p.page_of(0, position), slice(None), position % p.page
+    p.keys[at + (0,)] = 2.0 ** 19
+    p.values[at + (dim - 3,)] = math.inf
+    out = attend(p, query, dim ** -0.5).view(p.tokens, kv_heads, heads // kv_heads, dim)
+    expected = p.values[at][None, :, None].expand_as(out[1:n])
+    assert torch.isfinite(out[0]).all() and torch.isfinite(out[n:]).all()
+    assert torch.equal(out[1:n], expected)
