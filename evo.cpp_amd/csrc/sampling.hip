@@ -16,6 +16,10 @@
 // values 1.1e-13, 131072 9.3e-10, 2^20 6.0e-8). A weight below 2^-(B+1) counts as
 // none.
 //
+// A row is read two or three times. Every index and every loop is bounded whatever
+// the later reads find, so that logits or a workspace that someone else writes
+// meanwhile cost the row its token and no more.
+//
 // What bounds it: 2048 rows of 512 values 10.4 us, one round of waves, each a chain of
 // reductions, LDS atomics and two or three searches; 128 rows of 131072 BF16 values 64
 // us, of which their ranges take 7.6 (34 MB, 4.4 TB/s),
@@ -57,6 +61,9 @@ __device__ inline uint64_t place(float v, int index) {
   return static_cast<uint64_t>(ordered(v)) << 24 | static_cast<uint32_t>(0xffffff - index);
 }
 
+__device__ inline uint32_t token_of(uint64_t place) {
+  return place == 0 ? kNoToken : 0xffffffU - static_cast<uint32_t>(place & 0xffffff);
+}
 __device__ inline float value_of(uint64_t place) {
   const uint32_t bits = static_cast<uint32_t>(place >> 24);
   return __builtin_bit_cast(float, (bits & 0x80000000U) != 0 ? bits & 0x7fffffffU : ~bits);
@@ -225,10 +232,12 @@ struct Values {
 // How a row's values map to bins and weights, given its largest and lowest value.
 struct Scale {
   float top, reach, bin_scale;
+  int last_bin;
   double unit;  // 64 / (ln 2 * temperature)
   __device__ Scale(const SampleArgs &a, float top_, float low, float temperature, int bins)
       : top(top_), reach(static_cast<float>(
                        fmin(a.reach * static_cast<double>(temperature), 3.0e38))),
+        last_bin(bins - 1),
         unit(92.33248261893106 / static_cast<double>(temperature)) {
     const float range = fminf(reach, top - low);
     // A little less than bins / range: the last value stays inside.
@@ -238,7 +247,7 @@ struct Scale {
   // range of values.
   __device__ int bin(float v) const {
     const float below = top - v;
-    return below <= reach ? static_cast<int>(below * bin_scale) : -1;
+    return below <= reach ? min(static_cast<int>(below * bin_scale), last_bin) : -1;
   }
   // Lowest value of the bins 0 .. `bin`: the 64 values around the one that the bin's
   // end maps back to are tried, then, 64 at a time, all. All lanes of a wave call it,
@@ -351,12 +360,13 @@ __device__ inline Hit locate(const LaneBins &b, bool by_count, uint64_t target) 
 // Among the tokens that the lanes hold (spot[e] != 0: a place; w[e]: its weight;
 // `members` of them), the one, in order, at which the running count or weight passes
 // the target: its place; `before` grows by the weight up to it, itself included. A
-// histogram over the range of the places leaves the few that are taken one by one.
+// histogram over the range of the places leaves the few that are taken one by one: seven
+// of them at most, as each leaves eight of 56 bits less. 0 where there is none.
 template <int kPer>
 __device__ inline uint64_t wave_find(uint64_t (&spot)[kPer], const uint64_t (&w)[kPer],
                                      uint32_t members, const WaveBins &bins, bool by_count,
                                      uint64_t target, uint64_t &before) {
-  while (members > 6) {
+  for (int pass = 0; members > 6 && pass < 7; ++pass) {
     uint64_t last = ~0ULL, first = 0;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
@@ -488,7 +498,7 @@ __global__ __launch_bounds__(64) void sample_wave_kernel(const SampleArgs a) {
                             target - (border == 0 ? h.count_before : h.mass_before), total);
   }
   if (lane == 0)
-    a.tokens[r] = 0xffffffU - static_cast<uint32_t>(token & 0xffffff);
+    a.tokens[r] = token_of(token);
 }
 
 // ------------------------------------------------------- large vocabularies
@@ -633,7 +643,7 @@ __device__ inline uint64_t find_in_list(SampleShared<kThreads, kBins, kList> &s,
                                         bool by_count, uint64_t target, uint64_t *mass) {
   __shared__ uint64_t scratch[kThreads / 64];
   uint64_t before = 0;
-  while (members > kFew) {
+  for (int pass = 0; members > kFew && pass < 7; ++pass) {
     uint64_t lo = ~0ULL, hi = 0;
     for (uint32_t i = threadIdx.x; i < size; i += kThreads) {
       const uint64_t p = s.list_place[i];
@@ -684,6 +694,7 @@ __device__ inline uint64_t find_in_list(SampleShared<kThreads, kBins, kList> &s,
   }
   __syncthreads();
   if (threadIdx.x < 64) {
+    members = min(members, min(s.fill, static_cast<uint32_t>(kFew)));
     constexpr int kPer = kFew / 64;
     uint64_t spot[kPer], w[kPer];
 #pragma unroll
@@ -706,9 +717,9 @@ __device__ inline uint64_t find_in_list(SampleShared<kThreads, kBins, kList> &s,
 }
 
 // Lists the tokens whose values lie in `one` or `other` and whose place begins with
-// `prefix` above `shift` bits, and their weights.
+// `prefix` above `shift` bits, and their weights. Returns how many the list holds.
 template <typename T, int kThreads, int kBins, int kList>
-__device__ inline void gather(const Row<T> &row, const Scale &scale,
+__device__ inline uint32_t gather(const Row<T> &row, const Scale &scale,
                               SampleShared<kThreads, kBins, kList> &s, const Values &one,
                               const Values &other, int shift, uint64_t prefix) {
   if (threadIdx.x == 0)
@@ -740,20 +751,22 @@ __device__ inline void gather(const Row<T> &row, const Scale &scale,
           push(i);
       });
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < min(s.fill, static_cast<uint32_t>(kList)); i += kThreads) {
+  const uint32_t held = min(s.fill, static_cast<uint32_t>(kList));
+  for (uint32_t i = threadIdx.x; i < held; i += kThreads) {
     const int token = static_cast<int>(s.list_place[i]);
     const float v = static_cast<float>(row.logits[token]);
     s.list_place[i] = place(v, token);
     s.list_mass[i] = scale.weight(v, s.powers);
   }
   __syncthreads();
+  return held;
 }
 
 // Lists the `members` tokens of a bin, or, where they are more than the list holds,
 // those of them among which the target is passed; members, target and the weight
-// before them follow.
+// before them follow. Returns how many the list holds.
 template <typename T, int kThreads, int kBins, int kList>
-__device__ inline void list_bin(const Row<T> &row, const Scale &scale,
+__device__ inline uint32_t list_bin(const Row<T> &row, const Scale &scale,
                                 SampleShared<kThreads, kBins, kList> &s, int bin,
                                 bool by_count, uint32_t &members, uint64_t &target,
                                 uint64_t &before) {
@@ -761,7 +774,7 @@ __device__ inline void list_bin(const Row<T> &row, const Scale &scale,
   uint64_t prefix = 0;
   int shift = 56;
   const Values values = scale.values(bin, bin);
-  while (members > kList) {
+  while (members > kList && shift > 0) {
     // More than the list holds (many equal logits): 8 bits of the place at a time.
     shift -= 8;
     for (int i = threadIdx.x; i < 256; i += kThreads) {
@@ -793,7 +806,7 @@ __device__ inline void list_bin(const Row<T> &row, const Scale &scale,
     prefix = prefix << 8 | static_cast<uint64_t>(255 - digit);
     __syncthreads();
   }
-  gather(row, scale, s, values, values, shift, prefix);
+  return gather(row, scale, s, values, values, shift, prefix);
 }
 
 // Largest and lowest value of a row (its part); +infinity for NaN too, which no
@@ -1005,7 +1018,7 @@ __global__ __launch_bounds__(kThreads) void sample_block_kernel(const SampleArgs
     if (count <= kList) {
       listed = true;
       const Values all_kept = scale.values(0, bin);
-      gather(row, scale, s, all_kept, all_kept, 56, 0);
+      count = gather(row, scale, s, all_kept, all_kept, 56, 0);
       for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
         total += s.list_mass[i];
         kept += s.list_mass[i] >= least ? s.list_mass[i] : 0;
@@ -1077,9 +1090,7 @@ __global__ __launch_bounds__(kThreads) void sample_block_kernel(const SampleArgs
         const int high = last_at_most(s.mass, kBins, drawn(through));
         joint = members + in_bins(low, high) <= kList;
         if (joint) {
-          gather(row, scale, s, scale.values(bin, bin), scale.values(low, high), 56, 0);
-          size = min(s.fill, static_cast<uint32_t>(kList));
-          __syncthreads();
+          size = gather(row, scale, s, scale.values(bin, bin), scale.values(low, high), 56, 0);
         }
       }
       if (joint) {
@@ -1087,8 +1098,7 @@ __global__ __launch_bounds__(kThreads) void sample_block_kernel(const SampleArgs
         last = values.last();
         first = values.first();
       } else {
-        list_bin(row, scale, s, bin, by_count, members, target, before);
-        size = members;
+        size = list_bin(row, scale, s, bin, by_count, members, target, before);
       }
     }
     at = find_in_list(s, size, last, first, members, by_count, target, &total);
@@ -1096,7 +1106,7 @@ __global__ __launch_bounds__(kThreads) void sample_block_kernel(const SampleArgs
     __syncthreads();
   }
   if (threadIdx.x == 0)
-    a.tokens[r] = 0xffffffU - static_cast<uint32_t>(at & 0xffffff);
+    a.tokens[r] = token_of(at);
 }
 
 // Parts of a row: several where rows are long and too few to fill the chip, enough

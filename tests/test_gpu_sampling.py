@@ -319,3 +319,30 @@ def test_draws_beside_borders(vocab):
         expected.append(int(order[rank + r % 2]))
     got = sample(torch.from_numpy(logits).to(DEVICE), f32(uniform))
     assert got.tolist() == expected
+
+
+@pytest.mark.parametrize("vocab,rows", [(1500, 64), (20000, 16), (70000, 4)])
+def test_logits_that_change_meanwhile(vocab, rows):
+    """Another stream writes the logits while the call runs, flat, steep, equal and masked ones
+    in turn: it ends, and gives tokens of the vocabulary or none. What is written before a
+    call alone is sampled as ever."""
+    rng = np.random.default_rng(vocab)
+    flat = rng.normal(0, 0.1, (rows, vocab))
+    steep = rng.normal(0, 30.0, (rows, vocab))
+    equal = np.zeros((rows, vocab))
+    masked = np.where(rng.random((rows, vocab)) < 0.99, -math.inf, 1.0)
+    kinds = [torch.from_numpy(x.astype(np.float32)).to(DEVICE)
+             for x in (flat, steep, equal, masked)]
+    logits = kinds[0].clone()
+    given = parameters(rng, rows, vocab)
+    single = [f32(given[0]), f32(given[1]), i32(given[2]), f32(given[3]), f32(given[4])]
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i in range(12):
+        with torch.cuda.stream(other):
+            for j in range(6):
+                logits.copy_(kinds[(i + j) % 4])
+        got = sample(logits, *single, workspace=bool(i % 2))
+        assert ((got == NONE) | ((got >= 0) & (got < vocab))).all()
+    logits.copy_(kinds[1])
+    compare(logits, *given)
