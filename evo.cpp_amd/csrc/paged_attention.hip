@@ -24,8 +24,8 @@
 // 16 rows a block (one query's group of heads) are bound by the bytes of keys and
 // values: 64 sequences of up to 8190 positions, 8 key/value heads of 128, 644 MB, take
 // 126 us, 5.1 TB/s, and 5.3 to join their parts. 128 rows a block are bound by issue:
-// 4096 tokens on 12288 cached ones, 32 heads over 8, 962 GFLOP, take 905 to 935 us (two
-// cards), 1.06 to 1.03 PFLOP/s, the matrix cores busy 51% of the cycles and the vector
+// 4096 tokens on 12288 cached ones, 32 heads over 8, 962 GFLOP, take 905 to 967 us (by
+// card), 1.06 to 0.99 PFLOP/s, the matrix cores busy 51% of the cycles and the vector
 // units 44%, at the 1.76 GHz that the card's power leaves; an 8192-cubed product of the
 // library reaches 1.22 PFLOP/s. Rows of up to 16 take the first form (us with it and with
 // the second: 64 sequences of 2000, one token 49 and 56, four tokens 50 and 65; 32
