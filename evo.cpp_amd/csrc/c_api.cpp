@@ -1010,6 +1010,26 @@ evo_status evo_hip_paged_append(const evo_hip_paged_cache *cache, const evo_hip_
   });
 }
 
+evo_status evo_hip_paged_append_normed(
+    const evo_hip_paged_cache *cache, const evo_hip_paged_batch *batch, evo_hip_dtype dtype,
+    const void *projected, size_t row_stride, size_t heads, int column_split,
+    const float *query_scale, const float *key_scale, size_t scale_stride, float eps,
+    int eps_inside, const float *inv_freq, size_t rotary_dim, int interleaved, float rope_scale,
+    void *query, size_t query_stride, void *stream) {
+  return protect([&]() -> evo_status {
+    evo::hip::PagedCache pages;
+    evo::hip::PagedBatch rows;
+    const auto checked = paged_call(cache, batch, &pages, &rows);
+    if (!checked.ok())
+      return publish(checked);
+    const evo::hip::PagedRope rope{inv_freq, rotary_dim, interleaved != 0, rope_scale};
+    const evo::hip::HeadNorm norm{query_scale, key_scale, scale_stride, eps, eps_inside != 0};
+    return publish(evo::hip::paged_append(pages, rows, static_cast<int>(dtype), projected,
+                                          row_stride, heads, column_split != 0, rope, query,
+                                          query_stride, static_cast<hipStream_t>(stream), &norm));
+  });
+}
+
 size_t evo_hip_paged_attention_workspace_bytes(const evo_hip_paged_cache *cache,
                                                const evo_hip_paged_batch *batch, size_t heads) {
   try {

@@ -240,9 +240,19 @@ struct PagedRope {
   bool interleaved;
   float scale;
 };
+// RMS norm of each query and key head before it is rotated: x / (rms + eps), or
+// x / sqrt(rms^2 + eps) when inside, times the scale (F32 [head_dim], `stride` elements
+// from one head's to the next one's; null: 1).
+struct HeadNorm {
+  const float *query_scale, *key_scale;
+  size_t stride;
+  float eps;
+  int inside;
+};
 Status paged_append(const PagedCache &cache, const PagedBatch &batch, int dtype,
                     const void *projected, size_t row_stride, size_t heads, bool column_split,
-                    const PagedRope &rope, void *query, size_t query_stride, hipStream_t stream);
+                    const PagedRope &rope, void *query, size_t query_stride, hipStream_t stream,
+                    const HeadNorm *norm = nullptr);
 
 // Attention over the paged cache (paged_attention.hip).
 size_t paged_attention_workspace_bytes(const PagedCache &cache, const PagedBatch &batch,

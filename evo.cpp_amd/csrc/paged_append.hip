@@ -8,6 +8,10 @@
 // of up to 2048 tokens (F32 rows of 32 query, key and value heads of 128, 521 MB in
 // all) take 101 us, 5.2 TB/s, the rate of a copy; one token takes 4.3 us, a launch and
 // three loads that wait for each other (sequence, length, page).
+//
+// With norms, each query and key head x is first divided by its root mean square:
+// x / (rms + eps) or x / sqrt(rms^2 + eps), times a scale of each element. The kDim / 16
+// threads that hold a head add up its squares between themselves, in registers.
 #include "common.hpp"
 #include "ops.hpp"
 #include "paged.hpp"
@@ -79,6 +83,61 @@ __device__ inline void turn(double position, float inv_freq, float *cosine, floa
   sincospif(2.0F * static_cast<float>(turns - rint(turns)), sine, cosine);
 }
 
+// v of another lane of the wave, by the DPP control kCtrl: all lanes of a head run together.
+template <int kCtrl> __device__ inline float other_lane(float v) {
+  const int bits = __builtin_bit_cast(int, v);
+  return __builtin_bit_cast(float,
+                            __builtin_amdgcn_update_dpp(bits, bits, kCtrl, 0xf, 0xf, false));
+}
+// f over the 2, 4 or 8 neighbouring lanes that hold a head.
+template <int kLanes, typename F> __device__ inline float over_head(float v, F f) {
+  v = f(v, other_lane<0xb1>(v));  // quad_perm 1 0 3 2
+  if constexpr (kLanes > 2)
+    v = f(v, other_lane<0x4e>(v));  // quad_perm 2 3 0 1
+  if constexpr (kLanes > 4)
+    v = f(v, other_lane<0x141>(v));  // row_half_mirror: the other four of eight
+  return v;
+}
+
+// What a head's elements are multiplied with to be normalized, but for their scale:
+// first `lift` (a power of two, 1 but for squares that leave the range of F32), then
+// `inverse`.
+struct HeadSize {
+  float lift, inverse;
+};
+template <int kLanes>
+__device__ inline HeadSize head_size(const float (&u)[8], const float (&v)[8],
+                                     const HeadNorm &norm) {
+  constexpr float kMean = 1.0F / static_cast<float>(16 * kLanes);
+  const auto squares = [&](float lift) {
+    float sum = 0.0F;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = u[e] * lift, y = v[e] * lift;
+      sum = fmaf(x, x, sum);
+      sum = fmaf(y, y, sum);
+    }
+    return over_head<kLanes>(sum, [](float x, float y) { return x + y; });
+  };
+  const float sum = squares(1.0F);
+  if (sum > 0x1p-100F && sum < 0x1p120F) {
+    const float mean = sum * kMean;
+    return {1.0F, 1.0F / (norm.inside ? sqrtf(mean + norm.eps) : sqrtf(mean) + norm.eps)};
+  }
+  // Squares beyond the range, infinities, NaN and zeros. The largest element is
+  // brought near one; eps is at most 1, so it does not overflow.
+  float most = 0.0F;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    most = fmaxf(most, fmaxf(fabsf(u[e]), fabsf(v[e])));
+  most = over_head<kLanes>(most, [](float x, float y) { return fmaxf(x, y); });
+  const bool plain = most == 0.0F || !(most < INFINITY);
+  const float lift = plain ? 1.0F : ldexpf(1.0F, max(-126, min(-ilogbf(most), 120)));
+  const float rms = sqrtf(squares(lift) * kMean);
+  const float size = norm.inside ? hypotf(rms, sqrtf(norm.eps) * lift) : rms + norm.eps * lift;
+  return {lift, 1.0F / size};
+}
+
 // Which elements of a head a thread holds, in two groups of 8.
 enum Layout : int {
   kHalves = 0,       // pairs (i, rotary / 2 + i), rotary % 16 == 0
@@ -92,8 +151,9 @@ enum Layout : int {
 // 8j and rotary / 2 + 8j, and threads past the rotated pairs hold what passes
 // through; otherwise its groups lie side by side, and in halves of any size
 // the partner of an element is loaded beside it.
-template <typename S, typename T, int kDim, bool kVector, int kLayout>
-__global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
+template <typename S, typename T, int kDim, bool kVector, int kLayout, bool kNormed>
+__global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a,
+                                                           const HeadNorm norm) {
   constexpr int kLanes = kDim / 16, kHeadsPerPass = 256 / kLanes;
   constexpr int kAngles = kLayout == kAnyHalves ? 16 : 8;
   const int row = static_cast<int>(blockIdx.x / a.parts);
@@ -170,6 +230,29 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
     const S *from = src + (a.column_split ? (of_kind * 3 + kind) * kDim : head * kDim);
     load8<S, kVector>(from + first, u);
     load8<S, kVector>(from + second, v);
+    HeadSize size{1.0F, 1.0F};
+    const float *weight = nullptr;
+    if constexpr (kNormed) {
+      if (kind != 2) {
+        weight = kind == 0 ? norm.query_scale : norm.key_scale;
+        if (weight != nullptr)
+          weight += of_kind * norm.stride;
+        float g[8], h[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          g[e] = h[e] = 1.0F;
+        if (weight != nullptr) {
+          load8<float, true>(weight + first, g);
+          load8<float, true>(weight + second, h);
+        }
+        size = head_size<kLanes>(u, v, norm);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          u[e] = u[e] * size.lift * size.inverse * g[e];
+          v[e] = v[e] * size.lift * size.inverse * h[e];
+        }
+      }
+    }
     if (kind == 2 || !turns) {
       store8<T>(dst + first, u);
       store8<T>(dst + second, v);
@@ -196,8 +279,13 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
         const int d = first + e;
         const float self = e < 8 ? u[e % 8] : v[e % 8];
         float other = 0.0F;
-        if (d < a.rotary)
-          other = to_float(from[d < half ? d + half : d - half]);
+        if (d < a.rotary) {
+          const int partner = d < half ? d + half : d - half;
+          other = to_float(from[partner]);
+          if constexpr (kNormed)
+            other = other * size.lift * size.inverse *
+                    (weight != nullptr ? weight[partner] : 1.0F);
+        }
         const float turned = self * cosine[e % kAngles] +
                              (d < half ? -other : other) * sine[e % kAngles];
         (e < 8 ? x : y)[e % 8] = turned;
@@ -217,37 +305,49 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
   }
 }
 
-template <typename S, typename T, int kDim, bool kVector>
-void launch_layout(const AppendArgs &a, unsigned blocks, hipStream_t stream) {
-  auto kernel = paged_append_kernel<S, T, kDim, kVector, kAnyHalves>;
+struct Launch {
+  bool vector;
+  const HeadNorm *norm;
+  unsigned blocks;
+  hipStream_t stream;
+};
+
+template <typename S, typename T, int kDim, bool kVector, bool kNormed>
+void launch_layout(const AppendArgs &a, const Launch &l) {
+  auto kernel = paged_append_kernel<S, T, kDim, kVector, kAnyHalves, kNormed>;
   if (a.interleaved)
-    kernel = paged_append_kernel<S, T, kDim, kVector, kInterleaved>;
+    kernel = paged_append_kernel<S, T, kDim, kVector, kInterleaved, kNormed>;
   else if (a.rotary % 16 == 0)
-    kernel = paged_append_kernel<S, T, kDim, kVector, kHalves>;
-  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream, a);
+    kernel = paged_append_kernel<S, T, kDim, kVector, kHalves, kNormed>;
+  hipLaunchKernelGGL(kernel, dim3(l.blocks), dim3(256), 0, l.stream, a,
+                     kNormed ? *l.norm : HeadNorm{});
 }
 
-template <typename S, typename T>
-void launch_append(const AppendArgs &a, bool vector, unsigned blocks, hipStream_t stream) {
+template <typename S, typename T, int kDim>
+void launch_dim(const AppendArgs &a, const Launch &l) {
+  if (l.norm == nullptr)
+    return l.vector ? launch_layout<S, T, kDim, true, false>(a, l)
+                    : launch_layout<S, T, kDim, false, false>(a, l);
+  return l.vector ? launch_layout<S, T, kDim, true, true>(a, l)
+                  : launch_layout<S, T, kDim, false, true>(a, l);
+}
+
+template <typename S, typename T> void launch_append(const AppendArgs &a, const Launch &l) {
   switch (a.cache.head_dim) {
   case 32:
-    return vector ? launch_layout<S, T, 32, true>(a, blocks, stream)
-                  : launch_layout<S, T, 32, false>(a, blocks, stream);
+    return launch_dim<S, T, 32>(a, l);
   case 64:
-    return vector ? launch_layout<S, T, 64, true>(a, blocks, stream)
-                  : launch_layout<S, T, 64, false>(a, blocks, stream);
+    return launch_dim<S, T, 64>(a, l);
   default:
-    return vector ? launch_layout<S, T, 128, true>(a, blocks, stream)
-                  : launch_layout<S, T, 128, false>(a, blocks, stream);
+    return launch_dim<S, T, 128>(a, l);
   }
 }
 
-template <typename S>
-void launch_source(const AppendArgs &a, bool vector, unsigned blocks, hipStream_t stream) {
+template <typename S> void launch_source(const AppendArgs &a, const Launch &l) {
   if (a.cache.dtype == kElementBF16)
-    launch_append<S, __bf16>(a, vector, blocks, stream);
+    launch_append<S, __bf16>(a, l);
   else
-    launch_append<S, _Float16>(a, vector, blocks, stream);
+    launch_append<S, _Float16>(a, l);
 }
 
 }  // namespace
@@ -255,7 +355,7 @@ void launch_source(const AppendArgs &a, bool vector, unsigned blocks, hipStream_
 Status paged_append(const PagedCache &cache, const PagedBatch &batch, int dtype,
                     const void *projected, size_t row_stride, size_t heads, bool column_split,
                     const PagedRope &rope, void *query, size_t query_stride,
-                    hipStream_t stream) {
+                    hipStream_t stream, const HeadNorm *norm) {
   const size_t kv = static_cast<size_t>(cache.kv_heads), dim = static_cast<size_t>(cache.head_dim);
   if (projected == nullptr || query == nullptr || heads == 0 || heads > (1U << 16) ||
       heads % kv != 0 || (column_split && heads != kv))
@@ -274,6 +374,13 @@ Status paged_append(const PagedCache &cache, const PagedBatch &batch, int dtype,
       (rope.rotary_dim != 0 &&
        (rope.inv_freq == nullptr || !(rope.scale > 0.0F) || !std::isfinite(rope.scale))))
     return {ErrorCode::kInvalidArgument, "paged_append: invalid rotation"};
+  if (norm != nullptr &&
+      ((reinterpret_cast<uintptr_t>(norm->query_scale) |
+        reinterpret_cast<uintptr_t>(norm->key_scale)) % 16 != 0 ||
+       norm->stride % 4 != 0 || (norm->stride != 0 && norm->stride < dim) ||
+       norm->stride > (size_t{1} << 30) || !(norm->eps > 0.0F) || norm->eps > 1.0F))
+    return {ErrorCode::kInvalidArgument,
+            "paged_append: norm scales have to start on 16 bytes, eps is above 0 and at most 1"};
   const bool vector = reinterpret_cast<uintptr_t>(projected) % 16 == 0 &&
                       row_stride * size % 16 == 0;
   // A block's pass over the heads; few rows are split over them. us split and whole, 32
@@ -288,13 +395,13 @@ Status paged_append(const PagedCache &cache, const PagedBatch &batch, int dtype,
                         column_split ? 1 : 0, rope.inv_freq, static_cast<int>(rope.rotary_dim),
                         rope.interleaved ? 1 : 0, rope.rotary_dim != 0 ? rope.scale : 1.0F,
                         static_cast<uint16_t *>(query), query_stride, static_cast<int>(parts)};
-  const unsigned grid = static_cast<unsigned>(blocks);
+  const Launch launch{vector, norm, static_cast<unsigned>(blocks), stream};
   if (dtype == kElementF32)
-    launch_source<float>(args, vector, grid, stream);
+    launch_source<float>(args, launch);
   else if (dtype == kElementBF16)
-    launch_source<__bf16>(args, vector, grid, stream);
+    launch_source<__bf16>(args, launch);
   else
-    launch_source<_Float16>(args, vector, grid, stream);
+    launch_source<_Float16>(args, launch);
   return launch_status("paged_append_kernel");
 }
 

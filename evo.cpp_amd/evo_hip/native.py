@@ -89,6 +89,10 @@ _OPS = {
                                      c_size, c_void]),
     "evo_hip_paged_append": (c_int, _paged + [c_int, c_void, c_size, c_size, c_int, c_void,
                                               c_size, c_int, c_float, c_void, c_size, c_void]),
+    "evo_hip_paged_append_normed": (c_int, _paged + [c_int, c_void, c_size, c_size, c_int, c_void,
+                                                     c_void, c_size, c_float, c_int, c_void,
+                                                     c_size, c_int, c_float, c_void, c_size,
+                                                     c_void]),
     "evo_hip_paged_attention_workspace_bytes": (c_size, _paged + [c_size]),
     "evo_hip_paged_attention": (c_int, _paged + [c_void, c_size, c_size, c_float, c_void, c_size,
                                                  c_void, c_size, c_void]),

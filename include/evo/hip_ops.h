@@ -366,6 +366,25 @@ EVO_API evo_status evo_hip_paged_append(const evo_hip_paged_cache *cache,
                                         int interleaved, float rope_scale, void *query,
                                         size_t query_stride, void *stream);
 
+/* evo_hip_paged_append of query and key heads that are normalized before they are
+ * rotated, each by its own root mean square over head_dim:
+ *   y = x / (sqrt(mean(x^2)) + eps) * scale           (as evo_hip_rms_norm), or
+ *   y = x / sqrt(mean(x^2) + eps) * scale             with eps_inside.
+ * Values are stored as they are. Formed in F32 (a head whose squares would leave its
+ * range is brought near one first) and rounded once, after the rotation; a head that
+ * holds an infinity becomes what the formula gives: NaN there, zero elsewhere.
+ *   query_scale, key_scale  F32 [head_dim], one for all heads (scale_stride 0) or
+ *              [heads], [kv_heads][scale_stride] (a multiple of 4, head_dim at least);
+ *              16-byte aligned; NULL: 1.
+ *   eps        above 0, at most 1.
+ * The other arguments, and what they refuse, are evo_hip_paged_append's. */
+EVO_API evo_status evo_hip_paged_append_normed(
+    const evo_hip_paged_cache *cache, const evo_hip_paged_batch *batch, evo_hip_dtype dtype,
+    const void *projected, size_t row_stride, size_t heads, int column_split,
+    const float *query_scale, const float *key_scale, size_t scale_stride, float eps,
+    int eps_inside, const float *inv_freq, size_t rotary_dim, int interleaved, float rope_scale,
+    void *query, size_t query_stride, void *stream);
+
 /* Attention of a batch's rows over the cache: for each row and query head h
  *   out = sum_k softmax_k(scale * query . key[k]) * value[k]
  * over the positions k up to the row's own, of key/value head
