@@ -1077,4 +1077,21 @@ evo_status evo_hip_sample(evo_hip_dtype dtype, const void *logits, size_t rows, 
   });
 }
 
+size_t evo_hip_token_logprobs_workspace_bytes(size_t rows, size_t vocab, size_t alternatives) {
+  return evo::hip::token_logprobs_workspace_bytes(rows, vocab, alternatives);
+}
+
+evo_status evo_hip_token_logprobs(evo_hip_dtype dtype, const void *logits, size_t rows,
+                                  size_t vocab, size_t row_stride, const uint32_t *tokens,
+                                  float *logprob, uint32_t *rank, float *entropy,
+                                  size_t alternatives, uint32_t *top_tokens, float *top_logprobs,
+                                  void *workspace, size_t workspace_bytes, void *stream) {
+  return protect([&]() -> evo_status {
+    return publish(evo::hip::token_logprobs(static_cast<int>(dtype), logits, rows, vocab,
+                                            row_stride, tokens, logprob, rank, entropy,
+                                            alternatives, top_tokens, top_logprobs, workspace,
+                                            workspace_bytes, static_cast<hipStream_t>(stream)));
+  });
+}
+
 }  // extern "C"

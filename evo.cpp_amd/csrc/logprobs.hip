@@ -1,0 +1,559 @@
+// SPDX-License-Identifier: Apache-2.0
+// What a row of logits says of a given token: its log probability and its rank, the
+// row's entropy, and the first tokens of the order (logits descending, equal ones by
+// index) with theirs.
+//
+// With m the largest logit and d = x - m, others = sum exp(d) over all tokens but one of
+// the largest, t = sum d exp(d):
+//   log p(x) = d - log1p(others),  entropy = log1p(others) - t / (1 + others).
+// Without the largest token's own 1 in the sum, a row that is sure of its token keeps
+// what is left of it: both terms have one sign, so neither cancels.
+//
+// A wave takes a segment of 2048 logits in registers, so it reads them once and knows
+// its largest before it forms a weight. It leaves (m, sum, t, count of the largest) and
+// the largest of each group of 64 logits. The first k tokens are then found top down: the
+// first k segments, of their groups the first k, of these groups' logits the first k, each in
+// order of (largest, index). (A token outside them has k segments or groups before it,
+// each with a token that comes before it.) So the row is not read again but for k groups.
+// Vocabularies up to 2048 need one wave a row and one launch.
+#include "common.hpp"
+#include "lanes.hpp"
+#include "ops.hpp"
+
+#include <cmath>
+
+namespace evo::hip {
+
+namespace {
+
+constexpr uint32_t kNoToken = 0xffffffffU;
+constexpr int kSegment = 2048, kGroup = 64, kGroups = kSegment / kGroup;
+constexpr int kMostTop = 64;
+
+// Of one segment: its largest logit, how many are equal to it, and the sums of exp(d)
+// and of d exp(d) over the others. before: tokens in front of the given one.
+struct Segment {
+  float top, sum, spread;
+  uint32_t equal, before, unused[3];
+};
+
+struct LogprobArgs {
+  const void *logits;
+  int rows, vocab, segments;
+  size_t row_stride;
+  const uint32_t *tokens;
+  float *logprob;
+  uint32_t *rank;
+  float *entropy;
+  int alternatives;
+  uint32_t *top_tokens;
+  float *top_logprobs;
+  Segment *stats;  // [rows][segments]
+  float *groups;   // [rows][segments * kGroups], the largest of each
+};
+
+__device__ inline float value_of_order(uint32_t order) {
+  return __builtin_bit_cast(float, (order & 0x80000000U) != 0 ? order & 0x7fffffffU : ~order);
+}
+// A token's place: larger is earlier.
+__device__ inline uint64_t place(uint32_t order, uint32_t index) {
+  return static_cast<uint64_t>(order) << 32 | ~index;
+}
+__device__ inline uint32_t order_of(uint64_t place) { return static_cast<uint32_t>(place >> 32); }
+__device__ inline uint32_t index_of(uint64_t place) { return ~static_cast<uint32_t>(place); }
+
+// kPer logits a lane: 16 bytes at a time where rows start on them (kVec), one by one
+// otherwise.
+template <typename S, bool kVec, int kPer> struct Logits {
+  static constexpr int kEach = kVec ? 16 / static_cast<int>(sizeof(S)) : 1;
+  float x[kPer];
+
+  static __device__ int index(int first, int i) {
+    const int lane = threadIdx.x & 63;
+    return first + (i / kEach * 64 + lane) * kEach + i % kEach;
+  }
+  // Logits first .. of a row; -infinity behind its end.
+  __device__ void load(const S *row, int first, int vocab) {
+    if (first + kPer * 64 <= vocab) {
+#pragma unroll
+      for (int i = 0; i < kPer; i += kEach)
+        read(row + index(first, i), i);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; i += kEach) {
+      const int at = index(first, i);
+      if (at + kEach <= vocab) {
+        read(row + at, i);
+        continue;
+      }
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        x[i + e] = at + e < vocab ? static_cast<float>(row[at + e]) : -INFINITY;
+    }
+  }
+  __device__ void read(const S *from, int i) {
+    typedef S vector __attribute__((ext_vector_type(kEach)));
+    const vector v = *reinterpret_cast<const vector *>(from);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+      x[i + e] = static_cast<float>(v[e]);
+  }
+};
+
+__device__ inline float larger(float x, float y) { return __builtin_fmaxf(x, y); }
+
+constexpr float kLog2e = 1.44269504088896341F, kLog2eLow = 1.92596299e-8F;
+// exp(d) for d <= 0. Its argument's rounding is off by up to |d| * 2^-24; kExact adds
+// what the rounding lost.
+template <bool kExact> __device__ inline float weight(float d) {
+  const float scaled = d * kLog2e;
+  const float w = __builtin_amdgcn_exp2f(scaled);
+  if constexpr (!kExact)
+    return w;
+  const float lost = fmaf(d, kLog2eLow, fmaf(d, kLog2e, -scaled));
+  // (-infinity leaves no number.)
+  return w == 0.0F ? 0.0F : fmaf(w * lost, 0.693147180559945F, w);
+}
+
+// The sums of a segment. chunk: registers looked over at once for one that holds the
+// largest.
+template <bool kExact, int kPer>
+__device__ inline void sums(const float (&x)[kPer], float top, float &sum, float &spread,
+                            uint32_t &equal) {
+  constexpr int kChunk = 8;
+  const float base = top == -INFINITY ? 0.0F : top;
+  sum = spread = 0.0F;
+  equal = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; i += kChunk) {
+    float most = x[i];
+#pragma unroll
+    for (int e = 1; e < kChunk; ++e)
+      most = larger(most, x[i + e]);
+    if (__any(most == base)) {
+#pragma unroll
+      for (int e = 0; e < kChunk; ++e) {
+        const bool first = x[i + e] == base;
+        const float d = x[i + e] - base, w = first ? 0.0F : weight<kExact>(d);
+        equal += first ? 1U : 0U;
+        sum += w;
+        spread = fmaf(w, larger(d, -200.0F), spread);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kChunk; ++e) {
+        const float d = x[i + e] - base, w = weight<kExact>(d);
+        sum += w;
+        spread = fmaf(w, larger(d, -200.0F), spread);  // (a weight of 0 has d = -infinity)
+      }
+    }
+  }
+  sum = wave_reduce(sum, Sum());
+  spread = wave_reduce(spread, Sum());
+  equal = wave_reduce(equal, Sum());
+}
+
+// Largest logit and sums; every lane has them. Sums of a small total come from far
+// logits, whose arguments round worst: they are formed again, exactly.
+template <int kPer>
+__device__ inline Segment segment_of(const float (&x)[kPer]) {
+  Segment s{};
+  s.top = x[0];
+#pragma unroll
+  for (int i = 1; i < kPer; ++i)
+    s.top = larger(s.top, x[i]);
+  s.top = wave_reduce(s.top, Most());
+  sums<false>(x, s.top, s.sum, s.spread, s.equal);
+  if (s.sum < 0.0625F && s.sum > 0.0F)
+    sums<true>(x, s.top, s.sum, s.spread, s.equal);
+  return s;
+}
+
+// Tokens of the segment in front of `token`, whose logit is `given`.
+template <typename L, int kPer>
+__device__ inline uint32_t count_before(const float (&x)[kPer], int first, float given,
+                                        int token) {
+  // Those behind it in the row come before it only by a larger logit.
+  const float above = value_of_order(ordered(given) + 1);
+  uint32_t count = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; i += L::kEach) {
+    const int at = L::index(first, i);
+    if (L::kEach > 1 && !__any(at <= token && token < at + L::kEach)) {
+      const float least = at < token ? given : above;
+#pragma unroll
+      for (int e = 0; e < L::kEach; ++e)
+        count += __popcll(__ballot(x[i + e] >= least));
+    } else {
+#pragma unroll
+      for (int e = 0; e < L::kEach; ++e)
+        count += __popcll(__ballot(x[i + e] >= (at + e < token ? given : above)));
+    }
+  }
+  return count;
+}
+
+// A row's results from its whole sums.
+struct Row {
+  float top, log_total, entropy;
+  bool valid;  // a row with a logit above -infinity, and none that is NaN or +infinity
+  __device__ explicit Row(const Segment &s) : top(s.top) {
+    const float others = static_cast<float>(s.equal - 1) + s.sum;
+    valid = s.top > -INFINITY && s.top < INFINITY && s.sum == s.sum;
+    log_total = log1pf(others);
+    entropy = log_total - s.spread / (1.0F + others);
+  }
+  __device__ float logprob(float logit) const {
+    return valid ? logit - top - log_total : __builtin_nanf("");
+  }
+};
+__device__ inline void write_row(const LogprobArgs &a, int row, const Row &r, uint32_t before,
+                                 bool given, float logit) {
+  if (a.logprob != nullptr)
+    a.logprob[row] = given ? r.logprob(logit) : __builtin_nanf("");
+  if (a.rank != nullptr)
+    a.rank[row] = given && r.valid ? before : kNoToken;
+  if (a.entropy != nullptr)
+    a.entropy[row] = r.valid ? r.entropy : __builtin_nanf("");
+}
+__device__ inline void write_top(const LogprobArgs &a, int row, const Row &r, int rank,
+                                 uint64_t place) {
+  const size_t at = static_cast<size_t>(row) * a.alternatives + rank;
+  a.top_tokens[at] = r.valid ? index_of(place) : kNoToken;
+  a.top_logprobs[at] = r.logprob(value_of_order(order_of(place)));
+}
+
+// The k largest of n different places in LDS, moved to the list's beginning in any
+// order; returns how many (n, if there are no more). One wave calls it.
+__device__ inline int keep_best(uint64_t *list, int n, int k) {
+  const int lane = threadIdx.x & 63;
+  wave_sync();
+  if (n <= k)
+    return n;
+  uint64_t border = 0;
+#pragma unroll 1
+  for (int bit = 63; bit >= 0; --bit) {
+    const uint64_t tried = border | uint64_t{1} << bit;
+    int count = 0;
+    for (int i = 0; i < n; i += 64)
+      count += __popcll(__ballot(i + lane < n && list[i + lane] >= tried));
+    if (count >= k)
+      border = tried;
+    if (count == k)
+      break;
+  }
+  int kept = 0;
+  for (int i = 0; i < n; i += 64) {
+    const uint64_t own = i + lane < n ? list[i + lane] : 0;
+    const uint64_t in = __ballot(own >= border && i + lane < n);
+    if (in >> lane & 1)
+      list[kept + __popcll(in & ((uint64_t{1} << lane) - 1))] = own;
+    kept += __popcll(in);
+  }
+  wave_sync();
+  return kept;
+}
+// Writes the first tokens of a row from its best places, at most 64.
+__device__ inline void write_best(const LogprobArgs &a, int row, const Row &r,
+                                  const uint64_t *list, int n) {
+  const int lane = threadIdx.x & 63;
+  const uint64_t own = lane < n ? list[lane] : 0;
+  int rank = 0;
+  for (int i = 0; i < n; ++i)
+    rank += list[i] > own ? 1 : 0;
+  if (lane < n && rank < a.alternatives)
+    write_top(a, row, r, rank, own);
+}
+
+// ------------------------------------------------- one wave takes a row
+template <typename S, bool kVec, int kPer>
+__global__ __launch_bounds__(256) void row_kernel(const LogprobArgs a) {
+  typedef Logits<S, kVec, kPer> L;
+  extern __shared__ uint64_t lists[];  // [4][64 * kPer], where alternatives are asked for
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int row = blockIdx.x * 4 + wave;
+  if (row >= a.rows)
+    return;
+  const S *logits = static_cast<const S *>(a.logits) + row * a.row_stride;
+  const uint32_t token = a.tokens != nullptr ? a.tokens[row] : kNoToken;
+  L l;
+  l.load(logits, 0, a.vocab);
+  const bool given = token < static_cast<uint32_t>(a.vocab);
+  const float logit = given ? static_cast<float>(logits[token]) : 0.0F;
+  Segment s = segment_of(l.x);
+  if (given && a.rank != nullptr)
+    s.before = count_before<L>(l.x, 0, logit, static_cast<int>(token));
+  const Row r(s);
+  if (lane == 0)
+    write_row(a, row, r, s.before, given, logit);
+  const int k = a.alternatives;
+  if (k == 0)
+    return;
+
+  // The k-th largest of the lanes' largest (0: fewer lanes have one) bounds the k-th
+  // token from below.
+  uint32_t order[kPer], most = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    order[i] = L::index(0, i) < a.vocab ? ordered(l.x[i]) : 0;
+    most = max(most, order[i]);
+  }
+  uint32_t border = 0;
+#pragma unroll 1
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t tried = border | 1U << bit;
+    const int count = __popcll(__ballot(most >= tried));
+    if (count >= k)
+      border = tried;
+    if (count == k)
+      break;
+  }
+  border = max(border, 1U);
+  uint64_t *list = lists + wave * (64 * kPer);
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint64_t in = __ballot(order[i] >= border);
+    if (in == 0)
+      continue;
+    if (in >> lane & 1)
+      list[n + __popcll(in & ((uint64_t{1} << lane) - 1))] =
+          place(order[i], static_cast<uint32_t>(L::index(0, i)));
+    n += __popcll(in);
+  }
+  n = keep_best(list, n, n <= 64 ? 64 : k);
+  write_best(a, row, r, list, n);
+}
+
+// ------------------------------------------------- rows of several segments
+template <typename S, bool kVec>
+__global__ __launch_bounds__(256) void segment_kernel(const LogprobArgs a) {
+  typedef Logits<S, kVec, kSegment / 64> L;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const unsigned at = blockIdx.x * 4 + wave;
+  const int row = static_cast<int>(at / a.segments), segment = static_cast<int>(at % a.segments);
+  if (row >= a.rows)
+    return;
+  const S *logits = static_cast<const S *>(a.logits) + row * a.row_stride;
+  const uint32_t token = a.tokens != nullptr && a.rank != nullptr ? a.tokens[row] : kNoToken;
+  const int first = segment * kSegment;
+  L l;
+  l.load(logits, first, a.vocab);
+  const bool given = token < static_cast<uint32_t>(a.vocab);
+  const float logit = given ? static_cast<float>(logits[token]) : 0.0F;
+
+  if (a.alternatives > 0) {
+    // The largest of 64 neighbours: of kEach in each of 64 / kEach lanes.
+    constexpr int kLanes = kGroup / L::kEach, kRegisters = kSegment / 64 / L::kEach;
+    constexpr int kPerRegister = 64 / kLanes;  // groups
+    float mine = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kRegisters; ++j) {
+      float most = l.x[j * L::kEach];
+#pragma unroll
+      for (int e = 1; e < L::kEach; ++e)
+        most = larger(most, l.x[j * L::kEach + e]);
+      if constexpr (kLanes == 64) {
+        most = wave_reduce(most, Most());
+      } else {
+        most = larger(most, dpp<0xb1, 0xf>(most, most));   // quad_perm 1 0 3 2
+        most = larger(most, dpp<0x4e, 0xf>(most, most));   // quad_perm 2 3 0 1
+        most = larger(most, dpp<0x141, 0xf>(most, most));  // row_half_mirror
+        if constexpr (kLanes == 16)
+          most = larger(most, dpp<0x140, 0xf>(most, most));  // row_mirror
+      }
+      mine = lane % kLanes == j ? most : mine;
+    }
+    if (lane % kLanes < kRegisters)
+      a.groups[(static_cast<size_t>(row) * a.segments + segment) * kGroups +
+               lane % kLanes * kPerRegister + lane / kLanes] = mine;
+  }
+  Segment s = segment_of(l.x);
+  if (given)
+    s.before = count_before<L>(l.x, first, logit, static_cast<int>(token));
+  if (lane == 0)
+    a.stats[at] = s;
+}
+
+// A row's segments joined, and its first tokens.
+template <typename S> __global__ __launch_bounds__(256) void join_kernel(const LogprobArgs a) {
+  __shared__ uint64_t list[kMostTop * kGroup];
+  __shared__ uint32_t chosen[kMostTop];
+  __shared__ uint32_t scratch[4];
+  __shared__ float floats[4];
+  __shared__ int count;
+  __shared__ uint32_t least;
+  static_assert(kMostTop * kGroups <= kMostTop * kGroup, "groups of the best segments fit the list");
+  const int row = blockIdx.x;
+  const Segment *stats = a.stats + static_cast<size_t>(row) * a.segments;
+  const S *logits = static_cast<const S *>(a.logits) + row * a.row_stride;
+  const uint32_t token = a.tokens != nullptr ? a.tokens[row] : kNoToken;
+  const bool given = token < static_cast<uint32_t>(a.vocab);
+  const float logit = given ? static_cast<float>(logits[token]) : 0.0F;
+
+  Segment whole{};
+  whole.top = -INFINITY;
+  for (int i = threadIdx.x; i < a.segments; i += 256)
+    whole.top = larger(whole.top, stats[i].top);
+  whole.top = block_reduce<256>(whole.top, floats, Most());
+  for (int i = threadIdx.x; i < a.segments; i += 256) {
+    const Segment s = stats[i];
+    whole.before += s.before;
+    if (s.top == whole.top) {
+      whole.equal += s.equal;
+      whole.sum += s.sum;
+      whole.spread += s.spread;
+    } else {
+      // (Nothing above -infinity: its sum is zero, or NaN.)
+      const float away = larger(s.top - whole.top, -200.0F), shrink = expf(s.top - whole.top);
+      const float sum = s.sum + (s.top == -INFINITY ? 0.0F : static_cast<float>(s.equal));
+      whole.sum += shrink * sum;
+      whole.spread += shrink * fmaf(away, sum, s.spread);
+    }
+  }
+  whole.sum = block_reduce<256>(whole.sum, floats, Sum());
+  whole.spread = block_reduce<256>(whole.spread, floats, Sum());
+  whole.equal = block_reduce<256>(whole.equal, scratch, Sum());
+  whole.before = block_reduce<256>(whole.before, scratch, Sum());
+  const Row r(whole);
+  if (threadIdx.x == 0)
+    write_row(a, row, r, whole.before, given, logit);
+  const int k = a.alternatives;
+  if (k == 0)
+    return;
+
+  // The wave's k best of the list: their indexes to `chosen`, the order of the last
+  // one to `least` (0: there are fewer). The list is empty then.
+  const auto choose = [&](int n) {
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      const int kept = keep_best(list, n < 0 ? count : n, k);
+      const int lane = threadIdx.x;
+      const uint32_t order = lane < kept ? order_of(list[lane]) : 0xffffffffU;
+      if (lane < kept)
+        chosen[lane] = index_of(list[lane]);
+      const uint32_t last = ~wave_reduce(~order, Most());
+      if (lane == 0) {
+        least = kept < k ? 0 : last;
+        count = 0;
+      }
+    }
+    __syncthreads();
+  };
+  const auto add = [&](uint64_t place) { list[atomicAdd(&count, 1)] = place; };
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.segments; i += 256)
+    list[i] = place(ordered(stats[i].top), static_cast<uint32_t>(i));
+  choose(a.segments);
+  const int segments = min(k, a.segments);
+  const uint32_t border = least;
+  for (int i = threadIdx.x; i < segments * kGroups; i += 256) {
+    const uint32_t group = chosen[i / kGroups] * kGroups + i % kGroups;
+    if (group * kGroup >= static_cast<uint32_t>(a.vocab))
+      continue;
+    const uint32_t order =
+        ordered(a.groups[static_cast<size_t>(row) * a.segments * kGroups + group]);
+    if (order >= border)
+      add(place(order, group));
+  }
+  __syncthreads();
+  const int groups = min(k, count);
+  choose(-1);
+  const uint32_t group_border = least;
+  for (int i = threadIdx.x; i < groups * kGroup; i += 256) {
+    const uint32_t index = chosen[i / kGroup] * kGroup + i % kGroup;
+    if (index >= static_cast<uint32_t>(a.vocab))
+      continue;
+    const uint32_t order = ordered(static_cast<float>(logits[index]));
+    if (order >= group_border)
+      add(place(order, index));
+  }
+  __syncthreads();
+  if (threadIdx.x < 64)
+    write_best(a, row, r, list, keep_best(list, count, k));
+}
+
+template <typename S, bool kVec, int kPer>
+void launch_rows(const LogprobArgs &a, hipStream_t stream) {
+  const size_t lists = a.alternatives > 0 ? 4 * 64 * kPer * sizeof(uint64_t) : 0;
+  hipLaunchKernelGGL((row_kernel<S, kVec, kPer>), dim3(ceil_div(a.rows, 4)), dim3(256),
+                     static_cast<unsigned>(lists), stream, a);
+}
+
+template <typename S, bool kVec> void launch(const LogprobArgs &a, hipStream_t stream) {
+  if (a.vocab <= 512)
+    return launch_rows<S, kVec, 8>(a, stream);
+  if (a.vocab <= 1024)
+    return launch_rows<S, kVec, 16>(a, stream);
+  if (a.vocab <= kSegment)
+    return launch_rows<S, kVec, 32>(a, stream);
+  const size_t waves = static_cast<size_t>(a.rows) * a.segments;
+  hipLaunchKernelGGL((segment_kernel<S, kVec>), dim3(ceil_div(waves, 4)), dim3(256), 0, stream,
+                     a);
+  hipLaunchKernelGGL(join_kernel<S>, dim3(a.rows), dim3(256), 0, stream, a);
+}
+
+template <typename S>
+void launch_type(const LogprobArgs &a, bool vector, hipStream_t stream) {
+  if (vector)
+    launch<S, true>(a, stream);
+  else
+    launch<S, false>(a, stream);
+}
+
+constexpr size_t kMostRows = size_t{1} << 20;
+size_t segments_of(size_t vocab) { return (vocab + kSegment - 1) / kSegment; }
+
+}  // namespace
+
+size_t token_logprobs_workspace_bytes(size_t rows, size_t vocab, size_t alternatives) {
+  if (rows > kMostRows || vocab > kMostRows || vocab <= kSegment)
+    return 0;
+  return rows * segments_of(vocab) *
+         (sizeof(Segment) + (alternatives > 0 ? kGroups * sizeof(float) : 0));
+}
+
+Status token_logprobs(int dtype, const void *logits, size_t rows, size_t vocab, size_t row_stride,
+                      const uint32_t *tokens, float *logprob, uint32_t *rank, float *entropy,
+                      size_t alternatives, uint32_t *top_tokens, float *top_logprobs,
+                      void *workspace, size_t workspace_bytes, hipStream_t stream) {
+  if (dtype != kElementF32 && dtype != kElementBF16 && dtype != kElementF16)
+    return {ErrorCode::kInvalidArgument, "token_logprobs: logits are F32, BF16 or F16"};
+  const size_t size = dtype == kElementF32 ? 4 : 2;
+  if (logits == nullptr || rows == 0 || rows > kMostRows || vocab == 0 || vocab > kMostRows ||
+      row_stride < vocab || reinterpret_cast<uintptr_t>(logits) % size != 0)
+    return {ErrorCode::kInvalidArgument,
+            "token_logprobs: rows or vocab out of range, or row_stride below vocab"};
+  if (tokens == nullptr && (logprob != nullptr || rank != nullptr))
+    return {ErrorCode::kInvalidArgument, "token_logprobs: logprob and rank need tokens"};
+  if (alternatives > kMostTop || alternatives > vocab ||
+      (alternatives > 0 && (top_tokens == nullptr || top_logprobs == nullptr)))
+    return {ErrorCode::kInvalidArgument,
+            "token_logprobs: at most 64 alternatives, no more than vocab, with their outputs"};
+  if (logprob == nullptr && rank == nullptr && entropy == nullptr && alternatives == 0)
+    return {ErrorCode::kInvalidArgument, "token_logprobs: no output"};
+  const size_t need = token_logprobs_workspace_bytes(rows, vocab, alternatives);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need ||
+                   reinterpret_cast<uintptr_t>(workspace) % 16 != 0))
+    return {ErrorCode::kInvalidArgument, "token_logprobs: workspace too small or not aligned"};
+  const size_t segments = segments_of(vocab);
+  // (A launch counts its threads in 32 bits.)
+  if (ceil_div(rows * segments, 4) > ((size_t{1} << 32) - 1) / 256)
+    return {ErrorCode::kInvalidArgument, "token_logprobs: grid too large"};
+  Segment *const stats = static_cast<Segment *>(workspace);
+  const LogprobArgs args{logits, static_cast<int>(rows), static_cast<int>(vocab),
+                         static_cast<int>(segments), row_stride, tokens, logprob, rank, entropy,
+                         static_cast<int>(alternatives), top_tokens, top_logprobs, stats,
+                         need > 0 ? reinterpret_cast<float *>(stats + rows * segments) : nullptr};
+  const bool vector = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && row_stride * size % 16 == 0;
+  if (dtype == kElementF32)
+    launch_type<float>(args, vector, stream);
+  else if (dtype == kElementBF16)
+    launch_type<__bf16>(args, vector, stream);
+  else
+    launch_type<_Float16>(args, vector, stream);
+  return launch_status("token_logprobs kernels");
+}
+
+}  // namespace evo::hip

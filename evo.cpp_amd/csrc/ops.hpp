@@ -269,4 +269,11 @@ Status sample_tokens(int dtype, const void *logits, size_t rows, size_t vocab, s
                      const float *min_p, const float *uniform, uint32_t *tokens, void *workspace,
                      size_t workspace_bytes, hipStream_t stream);
 
+// ---- Log probabilities of given tokens (logprobs.hip).
+size_t token_logprobs_workspace_bytes(size_t rows, size_t vocab, size_t alternatives);
+Status token_logprobs(int dtype, const void *logits, size_t rows, size_t vocab, size_t row_stride,
+                      const uint32_t *tokens, float *logprob, uint32_t *rank, float *entropy,
+                      size_t alternatives, uint32_t *top_tokens, float *top_logprobs,
+                      void *workspace, size_t workspace_bytes, hipStream_t stream);
+
 }  // namespace evo::hip

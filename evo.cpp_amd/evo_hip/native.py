@@ -99,6 +99,10 @@ _OPS = {
     "evo_hip_sample_workspace_bytes": (c_size, [c_size, c_size]),
     "evo_hip_sample": (c_int, [c_int, c_void, c_size, c_size, c_size, c_void, c_void, c_void,
                                c_void, c_void, c_void, c_void, c_size, c_void]),
+    "evo_hip_token_logprobs_workspace_bytes": (c_size, [c_size, c_size, c_size]),
+    "evo_hip_token_logprobs": (c_int, [c_int, c_void, c_size, c_size, c_size, c_void, c_void,
+                                       c_void, c_void, c_size, c_void, c_void, c_void, c_size,
+                                       c_void]),
 }
 
 

@@ -450,6 +450,32 @@ EVO_API evo_status evo_hip_sample(evo_hip_dtype dtype, const void *logits, size_
                                   uint32_t *tokens, void *workspace,
                                   size_t workspace_bytes, void *stream);
 
+/* What rows of logits [rows][row_stride] (F32, BF16 or F16; rows and vocab at most 2^20)
+ * say of given tokens. With p = softmax of a row:
+ *   logprob  F32 [rows], ln p of tokens[r] (device uint32 [rows]); NaN where that is no
+ *            token of the vocabulary
+ *   rank     uint32 [rows], how many tokens come before it in the order of evo_sampler_sample
+ *            (logits descending, equal ones by ascending index); UINT32_MAX where
+ *            logprob is NaN
+ *   entropy  F32 [rows], -sum p ln p, in nats
+ *   top_tokens, top_logprobs  uint32 and F32 [rows][alternatives], the first tokens of
+ *            that order and their ln p; alternatives at most 64 and vocab
+ * Each output may be NULL (tokens too, if logprob and rank are; the last two only when
+ * alternatives is 0), but not all. A token whose logit is -infinity has p = 0 and ln p =
+ * -infinity. A row that holds NaN or +infinity, or nothing above -infinity, gets NaN and
+ * UINT32_MAX throughout. Sums are F32 and leave out the largest logit's own 1, so that ln p of
+ * a token that the row is sure of keeps its relative precision.
+ * The workspace (16-byte aligned, no initial contents) is needed above a vocabulary of
+ * 2048. Calls that overlap need one each. */
+EVO_API size_t evo_hip_token_logprobs_workspace_bytes(size_t rows, size_t vocab,
+                                                      size_t alternatives);
+EVO_API evo_status evo_hip_token_logprobs(evo_hip_dtype dtype, const void *logits, size_t rows,
+                                          size_t vocab, size_t row_stride,
+                                          const uint32_t *tokens, float *logprob, uint32_t *rank,
+                                          float *entropy, size_t alternatives,
+                                          uint32_t *top_tokens, float *top_logprobs,
+                                          void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
