@@ -1077,6 +1077,65 @@ evo_status evo_hip_sample(evo_hip_dtype dtype, const void *logits, size_t rows, 
   });
 }
 
+namespace {
+evo::Status adapter_pool(const evo_hip_adapters *pool, size_t rows, evo::hip::AdapterPool *out) {
+  const auto invalid = [](const char *why) {
+    return evo::Status{evo::ErrorCode::kInvalidArgument, std::string("invalid_argument: ") + why};
+  };
+  if (pool == nullptr || pool->struct_size < sizeof(evo_hip_adapters))
+    return invalid("evo_hip_adapters is null or too small");
+  if (pool->adapters == 0 || pool->adapters > evo::hip::kMostAdapters || pool->rank == 0 ||
+      pool->rank > evo::hip::kMostRank || pool->rank % 8 != 0)
+    return invalid("adapters must be 1 to 8192, their rank a multiple of 8 up to 128");
+  constexpr size_t kMost = size_t{1} << 24;
+  if (pool->in_width == 0 || pool->in_width % 8 != 0 || pool->in_width > kMost ||
+      pool->out_width == 0 || pool->out_width > kMost)
+    return invalid("in_width (a multiple of 8) or out_width of the adapters out of range");
+  if (rows == 0 || rows > (size_t{1} << 20))
+    return invalid("rows of the adapters out of range");
+  const size_t down = pool->rank * pool->in_width, up = pool->rank * pool->out_width;
+  const size_t down_stride = pool->down_stride == 0 ? down : pool->down_stride;
+  const size_t up_stride = pool->up_stride == 0 ? up : pool->up_stride;
+  if (pool->down == nullptr || pool->up == nullptr ||
+      (reinterpret_cast<uintptr_t>(pool->down) | reinterpret_cast<uintptr_t>(pool->up)) % 16 != 0)
+    return invalid("the adapters' weights are null or not 16-byte aligned");
+  if (down_stride < down || up_stride < up || (down_stride | up_stride) % 8 != 0 ||
+      (down_stride | up_stride) > (size_t{1} << 40))
+    return invalid("strides of adapters must be multiples of 8 that hold their weights");
+  *out = {static_cast<int>(pool->adapters), static_cast<int>(pool->rank),
+          static_cast<int>(pool->in_width), static_cast<int>(pool->out_width), pool->down, pool->up,
+          down_stride, up_stride, pool->scales, pool->ranks, pool->error};
+  return evo::Status::Ok();
+}
+}  // namespace
+
+size_t evo_hip_adapter_linear_workspace_bytes(const evo_hip_adapters *pool, size_t rows) {
+  try {
+    evo::hip::AdapterPool checked;
+    if (!adapter_pool(pool, rows, &checked).ok())
+      return 0;
+    return evo::hip::adapter_workspace_bytes(checked, rows);
+  } catch (...) {
+    return 0;
+  }
+}
+
+evo_status evo_hip_adapter_linear(const evo_hip_adapters *pool, const int32_t *adapter,
+                                  const uint16_t *x_hi, const uint16_t *x_lo, size_t x_stride,
+                                  size_t rows, const float *residual, float *out,
+                                  size_t out_stride, void *workspace, size_t workspace_bytes,
+                                  void *stream) {
+  return protect([&]() -> evo_status {
+    evo::hip::AdapterPool checked;
+    const auto status = adapter_pool(pool, rows, &checked);
+    if (!status.ok())
+      return publish(status);
+    return publish(evo::hip::adapter_linear(checked, adapter, x_hi, x_lo, x_stride, rows,
+                                            residual, out, out_stride, workspace, workspace_bytes,
+                                            static_cast<hipStream_t>(stream)));
+  });
+}
+
 size_t evo_hip_token_logprobs_workspace_bytes(size_t rows, size_t vocab, size_t alternatives) {
   return evo::hip::token_logprobs_workspace_bytes(rows, vocab, alternatives);
 }

@@ -269,6 +269,23 @@ Status sample_tokens(int dtype, const void *logits, size_t rows, size_t vocab, s
                      const float *min_p, const float *uniform, uint32_t *tokens, void *workspace,
                      size_t workspace_bytes, hipStream_t stream);
 
+// ---- Low-rank adapters of many requests (adapters.hip).
+struct AdapterPool {
+  int adapters, rank, in_width, out_width;
+  const uint16_t *down, *up;  // BF16 [adapters][rank][in_width], [adapters][out_width][rank]
+  size_t down_stride, up_stride;  // elements from one adapter to the next
+  const float *scales;    // null: 1
+  const int32_t *ranks;   // null: rank
+  int32_t *error;
+};
+constexpr int kBadAdapter = 1;
+constexpr int kMostAdapters = 8192, kMostRank = 128;
+size_t adapter_workspace_bytes(const AdapterPool &pool, size_t rows);
+Status adapter_linear(const AdapterPool &pool, const int32_t *adapter, const uint16_t *x_hi,
+                      const uint16_t *x_lo, size_t x_stride, size_t rows, const float *residual,
+                      float *out, size_t out_stride, void *workspace, size_t workspace_bytes,
+                      hipStream_t stream);
+
 // ---- Log probabilities of given tokens (logprobs.hip).
 size_t token_logprobs_workspace_bytes(size_t rows, size_t vocab, size_t alternatives);
 Status token_logprobs(int dtype, const void *logits, size_t rows, size_t vocab, size_t row_stride,

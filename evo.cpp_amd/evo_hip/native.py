@@ -22,6 +22,7 @@ DTYPE_BF16_TAPS = 0x200  # OR-ed into the Hyena dtype: inner taps are BF16 value
 FP8_MFMA_K32, FP8_MFMA_K128, FP8_EXACT = 0, 1, 2
 
 PAGED_BAD_SEQUENCE, PAGED_BAD_PAGE = 1, 2  # bits of PagedBatch.error
+BAD_ADAPTER = 1  # bit of Adapters.error
 
 
 class PagedCacheStruct(ctypes.Structure):
@@ -38,11 +39,19 @@ class PagedBatchStruct(ctypes.Structure):
                 ("shared_length", c_size), ("shared_table", c_void), ("error", c_void)]
 
 
+class AdaptersStruct(ctypes.Structure):
+    _fields_ = [("struct_size", c_size), ("adapters", c_size), ("rank", c_size),
+                ("in_width", c_size), ("out_width", c_size), ("down", c_void), ("up", c_void),
+                ("down_stride", c_size), ("up_stride", c_size), ("scales", c_void),
+                ("ranks", c_void), ("error", c_void)]
+
+
 # PagedCache(dtype=.., ...): the struct with its struct_size; fields not given are 0
 # or NULL. (A decode step makes them for each call: an __init__ of their own would
 # take as long as the rest.)
 PagedCache = partial(PagedCacheStruct, ctypes.sizeof(PagedCacheStruct))
 PagedBatch = partial(PagedBatchStruct, ctypes.sizeof(PagedBatchStruct))
+Adapters = partial(AdaptersStruct, ctypes.sizeof(AdaptersStruct))
 
 _paged = [ctypes.POINTER(PagedCacheStruct), ctypes.POINTER(PagedBatchStruct)]
 
@@ -99,6 +108,10 @@ _OPS = {
     "evo_hip_sample_workspace_bytes": (c_size, [c_size, c_size]),
     "evo_hip_sample": (c_int, [c_int, c_void, c_size, c_size, c_size, c_void, c_void, c_void,
                                c_void, c_void, c_void, c_void, c_size, c_void]),
+    "evo_hip_adapter_linear_workspace_bytes": (c_size, [ctypes.POINTER(AdaptersStruct), c_size]),
+    "evo_hip_adapter_linear": (c_int, [ctypes.POINTER(AdaptersStruct), c_void, c_void, c_void,
+                                       c_size, c_size, c_void, c_void, c_size, c_void, c_size,
+                                       c_void]),
     "evo_hip_token_logprobs_workspace_bytes": (c_size, [c_size, c_size, c_size]),
     "evo_hip_token_logprobs": (c_int, [c_int, c_void, c_size, c_size, c_size, c_void, c_void,
                                        c_void, c_void, c_size, c_void, c_void, c_void, c_size,

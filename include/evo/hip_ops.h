@@ -450,6 +450,55 @@ EVO_API evo_status evo_hip_sample(evo_hip_dtype dtype, const void *logits, size_
                                   uint32_t *tokens, void *workspace,
                                   size_t workspace_bytes, void *stream);
 
+/* Low-rank adapters, each a pair of BF16 matrices: down [rank][in_width] and up
+ * [out_width][rank], `adapters` (at most 8192) of them behind each other.
+ *   rank     rows of down and columns of up as they are stored, a multiple of 8 up to
+ *            128; ranks (device int32 [adapters], or NULL: all `rank`) says how many of
+ *            them each adapter has, 0 to rank. What lies behind those is not used.
+ *   in_width a multiple of 8; both widths at most 2^24.
+ *   down, up 16-byte aligned; down_stride, up_stride: elements from one adapter to the
+ *            next, multiples of 8 (0: dense).
+ *   scales   F32 [adapters], or NULL: 1.
+ *   error    optional device word; EVO_HIP_BAD_ADAPTER is OR-ed into it, never cleared. */
+typedef struct evo_hip_adapters {
+  size_t struct_size;
+  size_t adapters;
+  size_t rank;
+  size_t in_width;
+  size_t out_width;
+  const uint16_t *down;
+  const uint16_t *up;
+  size_t down_stride;
+  size_t up_stride;
+  const float *scales;
+  const int32_t *ranks;
+  int32_t *error;
+} evo_hip_adapters;
+#define EVO_HIP_BAD_ADAPTER 1
+
+/* out[t] = residual[t] + scale_a * up_a . (down_a . x[t]) with a = adapter[t], the adapter of
+ * row t of a batch, beside a product that all rows share (residual: what evo_hip_linear
+ * wrote, its bias included, or NULL: zero).
+ *   adapter  device int32 [rows], read when the call runs; -1: none, the row is its
+ *            residual. An index or a rank outside the pool counts as none:
+ *            EVO_HIP_BAD_ADAPTER. Rows may share adapters in any order; each adapter is read
+ *            once for up to 64 of its rows.
+ *   x        split BF16 planes [rows][x_stride] as evo_hip_linear takes them (x_lo NULL:
+ *            one plane), 16-byte aligned, x_stride a multiple of 8; rows at most 2^20.
+ *   residual, out  F32 [rows][out_stride], 4-byte aligned; out may be residual. Columns
+ *            behind out_width are left as they are, so the columns of one projection may
+ *            have adapters of their own. 16-byte aligned rows of whole 16 bytes run faster.
+ * Sums are F32; the inner values keep all of their 24 bits. An infinity or NaN in x or an
+ * adapter reaches only the rows that use it. Repeated calls give the same bits.
+ * The workspace (16-byte aligned, no initial contents) holds the rows' order and the inner
+ * values; calls that overlap need one each. */
+EVO_API size_t evo_hip_adapter_linear_workspace_bytes(const evo_hip_adapters *pool, size_t rows);
+EVO_API evo_status evo_hip_adapter_linear(const evo_hip_adapters *pool, const int32_t *adapter,
+                                          const uint16_t *x_hi, const uint16_t *x_lo,
+                                          size_t x_stride, size_t rows, const float *residual,
+                                          float *out, size_t out_stride, void *workspace,
+                                          size_t workspace_bytes, void *stream);
+
 /* What rows of logits [rows][row_stride] (F32, BF16 or F16; rows and vocab at most 2^20)
  * say of given tokens. With p = softmax of a row:
  *   logprob  F32 [rows], ln p of tokens[r] (device uint32 [rows]); NaN where that is no

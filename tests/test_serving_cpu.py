@@ -80,3 +80,52 @@ def test_logprobs_workspace_refused():
 def test_logprobs_launch_beyond_32_bit_threads_refused():
     with pytest.raises(N.OpError, match="grid too large"):
         logprobs(rows=1 << 20, vocab=1 << 20, stride=1 << 20, top=0, workspace=A, size=1 << 62)
+
+
+def adapters(pool=None, adapter=A, x_hi=B, x_lo=C, x_stride=64, rows=5, residual=None, out=A,
+             out_stride=40, workspace=B, size=1 << 40):
+    fields = dict(adapters=3, rank=16, in_width=64, out_width=40, down=A, up=B)
+    struct = N.Adapters(**fields)
+    for name, value in (pool or {}).items():
+        setattr(struct, name, value)
+    N.call("evo_hip_adapter_linear", ctypes.byref(struct), adapter, x_hi, x_lo, x_stride, rows,
+           residual, out, out_stride, workspace, size, None)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(struct_size=8), dict(adapters=0), dict(adapters=8193), dict(rank=0), dict(rank=12),
+    dict(rank=136), dict(in_width=0), dict(in_width=60), dict(in_width=1 << 25), dict(out_width=0),
+    dict(out_width=1 << 25), dict(down=None), dict(up=None), dict(down=A + 8), dict(up=A + 2),
+    dict(down_stride=16 * 64 - 8), dict(down_stride=16 * 64 + 4), dict(up_stride=16),
+    dict(up_stride=1 << 41)])
+def test_adapter_pool_refused(bad):
+    with pytest.raises(N.OpError, match="invalid_argument"):
+        adapters(pool=bad)
+    fields = dict(adapters=3, rank=16, in_width=64, out_width=40, down=A, up=B)
+    struct = N.Adapters(**fields)
+    assert N.call("evo_hip_adapter_linear_workspace_bytes", ctypes.byref(struct), 5) > 0
+    for name, value in bad.items():
+        setattr(struct, name, value)
+    assert N.call("evo_hip_adapter_linear_workspace_bytes", ctypes.byref(struct), 5) == 0
+
+
+@pytest.mark.parametrize("bad", [
+    dict(adapter=None), dict(adapter=A + 2), dict(x_hi=None), dict(x_hi=B + 8), dict(x_lo=C + 2),
+    dict(x_stride=56), dict(x_stride=68), dict(rows=0), dict(rows=(1 << 20) + 1), dict(out=None),
+    dict(out=A + 2), dict(residual=A + 1), dict(out_stride=39), dict(workspace=None),
+    dict(workspace=B + 8), dict(size=100)])
+def test_adapter_call_refused(bad):
+    with pytest.raises(N.OpError, match="invalid_argument"):
+        adapters(**bad)
+
+
+def test_adapter_launch_beyond_32_bit_threads_refused():
+    with pytest.raises(N.OpError, match="grid too large"):
+        adapters(pool=dict(adapters=8192, out_width=1 << 24), rows=1 << 20, out_stride=1 << 24,
+                 size=1 << 62)
+
+
+def test_null_pool_refused():
+    with pytest.raises(N.OpError, match="null"):
+        N.call("evo_hip_adapter_linear", None, A, B, C, 64, 5, None, A, 40, B, 1 << 40, None)
+    assert N.call("evo_hip_adapter_linear_workspace_bytes", None, 5) == 0
