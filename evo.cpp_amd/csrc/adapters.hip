@@ -17,14 +17,13 @@
 #include "ops.hpp"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace evo::hip {
 
 namespace {
 
 constexpr int kTileRows = 64, kGroupThreads = 1024;
-constexpr size_t kDirectRows = 16;  // rows up to this are not sorted
+constexpr int kFewRows = 16;  // up to these are not sorted
 
 struct Tile {
   int adapter, first, count;  // rows order[first ..]; adapter -1: rows without one
@@ -42,7 +41,9 @@ struct AdapterArgs {
   int tiles;    // at most
   int parts;    // of the width, in down_kernel
   int chunk;    // output columns of a block, in up_kernel
-  int direct;   // a tile is a row
+  int sorted;   // by group_kernel; else a tile is a row
+  int halves;   // 32s of rows in a tile at most
+  int wide;     // tiles of more than 16 rows go through LDS in up_kernel
   int32_t *bin;    // [rows], the adapter of each as it was read; the pool's size: none
   int32_t *order;  // [rows], sorted by it
   Tile *tile;      // [tiles], count 0 behind the last
@@ -67,62 +68,64 @@ __device__ inline int checked_adapter(const AdapterArgs &a, int row) {
 
 // ------------------------------------------------------------ rows by adapter
 // One block sorts the rows by counting: bin a holds the rows of adapter a, the last one
-// those without.
+// those without. A thread's first kKept rows are requested at once and kept.
+constexpr int kKept = 8;
 __global__ __launch_bounds__(kGroupThreads) void group_kernel(const AdapterArgs a) {
   extern __shared__ int32_t bins[];
   __shared__ int32_t rows_before[kGroupThreads / 64], tiles_before[kGroupThreads / 64];
+  const int threads = static_cast<int>(blockDim.x), waves = threads / 64;
   const int count = a.pool.adapters + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int i = threadIdx.x; i < count; i += kGroupThreads)
+  int kept[kKept];
+#pragma unroll
+  for (int j = 0; j < kKept; ++j) {
+    const int row = threadIdx.x + j * threads;
+    kept[j] = row < a.rows ? checked_adapter(a, row) : -1;
+  }
+  for (int i = threadIdx.x; i < count; i += threads)
     bins[i] = 0;
   __syncthreads();
-  // A wave's place in a bin: one addition where all of its rows share one, as in prompts.
-  const auto add = [&](int row, bool place) {
-    const bool mine = row < a.rows;
-    int bin = -1;
-    if (mine && place)
-      bin = a.bin[row];  // (which this thread wrote: both passes see one adapter)
-    else if (mine)
-      a.bin[row] = bin = checked_adapter(a, row);
+  // The place of a wave's rows (bin -1: none) in their bins: one addition where all of
+  // them share one, as in prompts.
+  const auto add = [&](int bin) {
     const int first = __builtin_amdgcn_readfirstlane(bin);
     const uint64_t same = __ballot(bin == first);
-    if (__ballot(mine) == same && first >= 0) {
+    if (first >= 0 && same == __ballot(bin >= 0)) {
       int at = 0;
       if (lane == 0)
         at = atomicAdd(&bins[first], static_cast<int>(__popcll(same)));
-      at = __builtin_amdgcn_readfirstlane(at);
-      if (place && mine)
-        a.order[at + lane] = row;
-    } else if (mine) {
-      const int at = atomicAdd(&bins[bin], 1);
-      if (place)
-        a.order[at] = row;
+      return __builtin_amdgcn_readfirstlane(at) + lane;
     }
+    return bin < 0 ? 0 : atomicAdd(&bins[bin], 1);
   };
-  for (int row = threadIdx.x; row < (a.rows + 63) / 64 * 64; row += kGroupThreads)
-    add(row, false);
+#pragma unroll
+  for (int j = 0; j < kKept; ++j)
+    if (j * threads < a.rows)
+      add(kept[j]);
+  // (Rows beyond those are read once too: both passes see one adapter.)
+  for (int first = kKept * threads; first < a.rows; first += threads) {
+    const int row = first + threadIdx.x;
+    const int bin = row < a.rows ? checked_adapter(a, row) : -1;
+    if (row < a.rows)
+      a.bin[row] = bin;
+    add(bin);
+  }
   __syncthreads();
 
   // Each thread's bins, and what lies before them.
-  const int each = (count + kGroupThreads - 1) / kGroupThreads, from = threadIdx.x * each;
+  const int each = (count + threads - 1) / threads, from = threadIdx.x * each;
   int rows = 0, tiles = 0;
   for (int i = from; i < min(from + each, count); ++i) {
     rows += bins[i];
     tiles += (bins[i] + kTileRows - 1) / kTileRows;
   }
-  int rows_through = rows, tiles_through = tiles;
-#pragma unroll
-  for (int offset = 1; offset < 64; offset <<= 1) {
-    const int r = __shfl_up(rows_through, offset, 64), t = __shfl_up(tiles_through, offset, 64);
-    rows_through += lane >= offset ? r : 0;
-    tiles_through += lane >= offset ? t : 0;
-  }
+  const int rows_through = wave_scan<Sum>(rows), tiles_through = wave_scan<Sum>(tiles);
   if (lane == 63) {
     rows_before[wave] = rows_through;
     tiles_before[wave] = tiles_through;
   }
   __syncthreads();
   int at = rows_through - rows, tile = tiles_through - tiles, all = 0;
-  for (int w = 0; w < kGroupThreads / 64; ++w) {
+  for (int w = 0; w < waves; ++w) {
     at += w < wave ? rows_before[w] : 0;
     tile += w < wave ? tiles_before[w] : 0;
     all += tiles_before[w];
@@ -134,22 +137,44 @@ __global__ __launch_bounds__(kGroupThreads) void group_kernel(const AdapterArgs 
       a.tile[tile++] = {i < a.pool.adapters ? i : -1, at + j, min(n - j, kTileRows)};
     at += n;
   }
-  for (int i = all + threadIdx.x; i < a.tiles; i += kGroupThreads)
+  for (int i = all + threadIdx.x; i < a.tiles; i += threads)
     a.tile[i] = {-1, 0, 0};
   __syncthreads();
-  for (int row = threadIdx.x; row < (a.rows + 63) / 64 * 64; row += kGroupThreads)
-    add(row, true);
+#pragma unroll
+  for (int j = 0; j < kKept; ++j)
+    if (j * threads < a.rows) {
+      const int place = add(kept[j]);
+      if (kept[j] >= 0)
+        a.order[place] = static_cast<int32_t>(threadIdx.x + j * threads);
+    }
+  for (int first = kKept * threads; first < a.rows; first += threads) {
+    const int row = first + threadIdx.x;
+    const int bin = row < a.rows ? a.bin[row] : -1;
+    const int place = add(bin);
+    if (row < a.rows)
+      a.order[place] = row;
+  }
 }
 
+// A block's tile: its rows in list[0 .. count).
+struct TileRows {
+  Tile tile;
+  int list[kTileRows];
+};
 // Few rows are not sorted: each is a tile.
-__device__ inline Tile tile_at(const AdapterArgs &a, int index) {
-  if (!a.direct)
-    return a.tile[index];
-  const int adapter = checked_adapter(a, index);
-  return {adapter < a.pool.adapters ? adapter : -1, index, 1};
-}
-__device__ inline int row_at(const AdapterArgs &a, int place) {
-  return a.direct ? place : a.order[place];
+__device__ inline void find_tile(const AdapterArgs &a, int index, TileRows &s) {
+  if (a.sorted) {
+    const Tile tile = a.tile[index];
+    if (static_cast<int>(threadIdx.x) < tile.count)
+      s.list[threadIdx.x] = a.order[tile.first + threadIdx.x];
+    if (threadIdx.x == 0)
+      s.tile = tile;
+  } else if (threadIdx.x == 0) {
+    const int adapter = checked_adapter(a, index);
+    s.tile = {adapter < a.pool.adapters ? adapter : -1, index, 1};
+    s.list[0] = index;
+  }
+  __syncthreads();
 }
 
 // --------------------------------------------------------------- inner values
@@ -157,27 +182,38 @@ __device__ inline bf16x8 load8(const uint16_t *from) {
   return *reinterpret_cast<const bf16x8 *>(from);
 }
 
-// D (16 ranks) x X^T (16 rows) of every fourth 32-step of a part, for kCols 16s of rows and
-// kRanks 16s of ranks. Lane l: row l % 16, ranks 4 (l / 16) + i. kAhead steps' operands are
-// requested at once.
+// D (16 ranks) x X^T (16 rows) of a part of the width, for the kCols 16s of rows from `set`
+// on and kRanks 16s of ranks. Each wave takes every eighth 32-step, kAhead of them
+// requested at once; their sums meet in LDS.
+// Loaded as the products take them, 16 neighbouring lanes would read 16 rows, which costs
+// the load unit a cycle each (64 to 85 a load measured, 4096 rows 34 us). Four neighbouring
+// lanes read 64 bytes of one row instead, and the wave turns them in LDS: lane l holds piece
+// (l % 4) ^ (l / 8 % 4) of row l / 4 (so turned, neither side meets bank conflicts), and
+// takes row l % 16, piece l / 16. Its sums are row l % 16, ranks 4 (l / 16) + i.
+constexpr int kDownWaves = 8;
 template <int kRanks, int kCols, bool kLow>
-__device__ inline void down_tile(const AdapterArgs &a, const Tile &tile, int part,
-                                 f32x4 (*sums)[kRanks * 4][64]) {
+__device__ inline void down_tile(const AdapterArgs &a, const TileRows &rows, int set, int part,
+                                 f32x4 *shared) {
+  const Tile &tile = rows.tile;
   constexpr int kLoads = kRanks + (kLow ? 2 : 1) * kCols;
-  constexpr int kAhead = kLoads <= 3 ? 8 : kLoads <= 6 ? 4 : kLoads <= 12 ? 2 : 1;
-  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  constexpr int kAhead = kLoads <= 6 ? 2 : 1;
+  const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rank = rank_of(a.pool, tile.adapter), width = a.pool.in_width;
   const uint16_t *down = a.pool.down + tile.adapter * a.pool.down_stride;
+  // Row r of a load's 16 is at LDS place 4 r + (piece ^ r / 2 % 4).
+  const int owner = lane >> 2, piece = (lane & 3) ^ (lane >> 3 & 3);
+  const int taken = 4 * (lane & 15) + ((lane >> 4) ^ (lane >> 1 & 3));
+  f32x4 *const turn = shared + wave * kLoads * 64;
   // (Ranks that the adapter does not have take its first row; their sums are dropped.)
   const uint16_t *weight[kRanks];
 #pragma unroll
   for (int r = 0; r < kRanks; ++r)
-    weight[r] = down + static_cast<size_t>(16 * r + col < rank ? 16 * r + col : 0) * width + 8 * g;
+    weight[r] = down + static_cast<size_t>(16 * r + owner < rank ? 16 * r + owner : 0) * width;
   size_t from[kCols];
 #pragma unroll
   for (int c = 0; c < kCols; ++c)
-    from[c] = row_at(a, tile.first + min(16 * c + col, tile.count - 1)) * a.x_stride + 8 * g;
+    from[c] = rows.list[min(16 * (set + c) + owner, tile.count - 1)] * a.x_stride;
   f32x4 sum[kRanks][kCols];
 #pragma unroll
   for (int r = 0; r < kRanks; ++r)
@@ -185,109 +221,95 @@ __device__ inline void down_tile(const AdapterArgs &a, const Tile &tile, int par
     for (int c = 0; c < kCols; ++c)
       sum[r][c] = f32x4{0.0F, 0.0F, 0.0F, 0.0F};
 
-  struct Step {
-    bf16x8 weight[kRanks], hi[kCols], lo[kCols];
-  };
-  const auto load = [&](int k, Step &x) {
+  const int steps = (width + 31) / 32, each = (steps + a.parts - 1) / a.parts;
+  const int last = min(steps, (part + 1) * each);
+  for (int step = part * each + wave; step < last; step += kDownWaves * kAhead) {
+    bf16x8 x[kAhead][kLoads];  // weights, hi and lo planes
 #pragma unroll
-    for (int r = 0; r < kRanks; ++r)
-      x.weight[r] = load8(weight[r] + k);
+    for (int u = 0; u < kAhead; ++u) {
+      const int at = 32 * min(step + kDownWaves * u, steps - 1) + 8 * piece;
+      const int k = at < width ? at : 0;
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) {
-      x.hi[c] = load8(a.hi + from[c] + k);
-      if constexpr (kLow)
-        x.lo[c] = load8(a.lo + from[c] + k);
-    }
-  };
-  const auto add = [&](const Step &x) {
-#pragma unroll
-    for (int r = 0; r < kRanks; ++r)
+      for (int r = 0; r < kRanks; ++r)
+        x[u][r] = load8(weight[r] + k);
 #pragma unroll
       for (int c = 0; c < kCols; ++c) {
-        sum[r][c] =
-            __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.weight[r], x.hi[c], sum[r][c], 0, 0, 0);
+        x[u][kRanks + c] = load8(a.hi + from[c] + k);
         if constexpr (kLow)
-          sum[r][c] =
-              __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.weight[r], x.lo[c], sum[r][c], 0, 0, 0);
+          x[u][kRanks + kCols + c] = load8(a.lo + from[c] + k);
       }
-  };
-  const int whole = width / 32, each = (whole + a.parts - 1) / a.parts;
-  const int last = min(whole, (part + 1) * each);
-  int step = part * each + wave;
-  for (; step + 4 * (kAhead - 1) < last; step += 4 * kAhead) {
-    Step x[kAhead];
+    }
+    asm volatile("" ::: "memory");  // every load before the first product
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      load(32 * (step + 4 * u), x[u]);
+    for (int u = 0; u < kAhead; ++u) {
+      const int at = step + kDownWaves * u;
+      if (at >= last)
+        break;
+      // Behind the width: zeros in both operands, as zero times infinity is none.
+      const bool there = 32 * at + 8 * piece < width;
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      add(x[u]);
-  }
-  for (; step < last; step += 4) {
-    Step x;
-    load(32 * step, x);
-    add(x);
-  }
-  if (width % 32 != 0 && part == a.parts - 1 && wave == 0) {
-    // The last step ends inside: zeros in both operands, as zero times infinity is none.
-    Step x{};
-    if (32 * whole + 8 * g < width)
-      load(32 * whole, x);
-    add(x);
-  }
-  // The four waves' sums, always in the same order.
+      for (int j = 0; j < kLoads; ++j)
+        turn[64 * j + lane] = there ? __builtin_bit_cast(f32x4, x[u][j]) : f32x4{};
+      wave_sync();
+      bf16x8 v[kLoads];
 #pragma unroll
-  for (int half = 2; half > 0; half /= 2) {
-    if (wave >= half && wave < 2 * half) {
+      for (int j = 0; j < kLoads; ++j)
+        v[j] = __builtin_bit_cast(bf16x8, turn[64 * j + taken]);
 #pragma unroll
       for (int r = 0; r < kRanks; ++r)
 #pragma unroll
-        for (int c = 0; c < kCols; ++c)
-          sums[wave - half][r * kCols + c][lane] = sum[r][c];
+        for (int c = 0; c < kCols; ++c) {
+          sum[r][c] =
+              __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[r], v[kRanks + c], sum[r][c], 0, 0, 0);
+          if constexpr (kLow)
+            sum[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[r], v[kRanks + kCols + c],
+                                                                sum[r][c], 0, 0, 0);
+        }
+      wave_sync();
     }
-    __syncthreads();
-    if (wave < half) {
-#pragma unroll
-      for (int r = 0; r < kRanks; ++r)
-#pragma unroll
-        for (int c = 0; c < kCols; ++c)
-          sum[r][c] += sums[wave][r * kCols + c][lane];
-    }
-    __syncthreads();
   }
-  if (wave != 0)
-    return;
+  __syncthreads();
+  f32x4 *const sums = shared;
+  constexpr int kSums = kRanks * kCols * 64;  // of a wave
 #pragma unroll
-  for (int c = 0; c < kCols; ++c) {
-    if (16 * c + col >= tile.count)
+  for (int r = 0; r < kRanks; ++r)
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+      sums[wave * kSums + (r * kCols + c) * 64 + lane] = sum[r][c];
+  __syncthreads();
+#pragma unroll 1
+  for (int i = threadIdx.x; i < kSums; i += 64 * kDownWaves) {
+    f32x4 v = sums[i];
+#pragma unroll
+    for (int w = 1; w < kDownWaves; ++w)
+      v += sums[w * kSums + i];
+    const int t = 16 * (set + i / 64 % kCols) + i % 16;
+    const int first = 16 * (i / 64 / kCols) + 4 * (i % 64 / 16);
+    if (t >= tile.count || first >= a.pool.rank)
       continue;
-    const int row = row_at(a, tile.first + 16 * c + col);
-    float *inner = a.inner + (static_cast<size_t>(part) * a.rows + row) * a.pool.rank;
 #pragma unroll
-    for (int r = 0; r < kRanks; ++r) {
-      const int first = 16 * r + 4 * g;
-      if (first >= a.pool.rank)
-        continue;
-      f32x4 v = sum[r][c];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[i] = first + i < rank ? v[i] : 0.0F;
-      *reinterpret_cast<f32x4 *>(inner + first) = v;
-    }
+    for (int e = 0; e < 4; ++e)
+      v[e] = first + e < rank ? v[e] : 0.0F;
+    const size_t row = static_cast<size_t>(part) * a.rows + rows.list[t];
+    *reinterpret_cast<f32x4 *>(a.inner + row * a.pool.rank + first) = v;
   }
 }
 
+// A block takes up to 32 rows of a tile and a part of the width.
 template <int kRanks, bool kLow>
-__global__ __launch_bounds__(256) void down_kernel(const AdapterArgs a) {
-  __shared__ f32x4 sums[2][kRanks * 4][64];
-  const Tile tile = tile_at(a, blockIdx.x / a.parts);
-  if (tile.count == 0 || tile.adapter < 0)
-    return;
+__global__ __launch_bounds__(64 * kDownWaves) void down_kernel(const AdapterArgs a) {
+  extern __shared__ f32x4 down_shared[];
+  __shared__ TileRows rows;
+  const unsigned block = blockIdx.x / a.parts;
   const int part = static_cast<int>(blockIdx.x % a.parts);
-  if (tile.count <= 16)
-    down_tile<kRanks, 1, kLow>(a, tile, part, sums);
+  find_tile(a, static_cast<int>(block / a.halves), rows);
+  const int set = 2 * static_cast<int>(block % a.halves);
+  if (rows.tile.adapter < 0 || 16 * set >= rows.tile.count)
+    return;
+  if (rows.tile.count - 16 * set <= 16)
+    down_tile<kRanks, 1, kLow>(a, rows, set, part, down_shared);
   else
-    down_tile<kRanks, 4, kLow>(a, tile, part, sums);
+    down_tile<kRanks, 2, kLow>(a, rows, set, part, down_shared);
 }
 
 // ------------------------------------------------------------------- outputs
@@ -321,17 +343,18 @@ __device__ inline void planes_of(const float (&v)[8], bf16x8 (&planes)[3]) {
 
 // Rows without an adapter: their residual, or zero.
 template <bool kVector, bool kResidual>
-__device__ inline void copy_rows(const AdapterArgs &a, const Tile &tile, int begin, int last) {
+__device__ inline void copy_rows(const AdapterArgs &a, const TileRows &rows, int begin,
+                                 int last) {
   constexpr int kEach = kVector ? 4 : 1, kAhead = 8;
   typedef float vector __attribute__((ext_vector_type(kEach)));
-  const int across = (last - begin) / kEach, all = tile.count * across;
+  const int across = (last - begin) / kEach, all = rows.tile.count * across;
   for (int first = threadIdx.x; first < all; first += 256 * kAhead) {
     size_t at[kAhead];
     vector v[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int i = min(first + 256 * u, all - 1);
-      at[u] = row_at(a, tile.first + i / across) * a.out_stride + begin + i % across * kEach;
+      at[u] = rows.list[i / across] * a.out_stride + begin + i % across * kEach;
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
@@ -414,14 +437,15 @@ __device__ inline f32x4 up_product(const bf16x8 (&weight)[kSteps], const Inner<k
 // 16 rows a wave, from registers to registers, of every `stride`th 16 columns; kAhead
 // columns' operands are requested at once, by every lane from inside the tensors.
 template <int kSteps, bool kVector, bool kResidual>
-__device__ inline void up_rows(const AdapterArgs &a, const Tile &tile, int set, int n0, int stride,
-                               int last) {
+__device__ inline void up_rows(const AdapterArgs &a, const TileRows &rows, int set, int n0,
+                               int stride, int last) {
+  const Tile &tile = rows.tile;
   constexpr int kAhead = 4;
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int width = a.pool.out_width, rank = rank_of(a.pool, tile.adapter);
   const uint16_t *up = a.pool.up + tile.adapter * a.pool.up_stride;
   const bool mine = 16 * set + col < tile.count;
-  const int row = row_at(a, tile.first + min(16 * set + col, tile.count - 1));
+  const int row = rows.list[min(16 * set + col, tile.count - 1)];
   const size_t at = row * a.out_stride;
   const Inner<kSteps> inner(a, tile.adapter, rank, row);
   const RankMask<kSteps> mask(rank);
@@ -494,14 +518,15 @@ template <int kSteps> struct WideShared {
   __attribute__((aligned(16))) float product[kTileRows][kWide + 4];
 };
 template <int kSteps, bool kResidual>
-__device__ inline void up_wide(const AdapterArgs &a, const Tile &tile, int begin, int last,
+__device__ inline void up_wide(const AdapterArgs &a, const TileRows &list, int begin, int last,
                                WideShared<kSteps> &shared) {
+  const Tile &tile = list.tile;
   constexpr int kPieces = kWide * 4 * kSteps / 256;  // 16 bytes of weights a thread
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int width = a.pool.out_width, rank = rank_of(a.pool, tile.adapter);
   const uint16_t *up = a.pool.up + tile.adapter * a.pool.up_stride;
-  const int row = row_at(a, tile.first + min(16 * wave + col, tile.count - 1));
+  const int row = list.list[min(16 * wave + col, tile.count - 1)];
   const Inner<kSteps> inner(a, tile.adapter, rank, row);
   const RankMask<kSteps> mask(rank);
   const int rows = min(16, tile.count - 16 * wave);  // (0 and below: none)
@@ -566,52 +591,91 @@ __device__ inline void up_wide(const AdapterArgs &a, const Tile &tile, int begin
 
 template <int kSteps, bool kVector, bool kResidual>
 __global__ __launch_bounds__(256) void up_kernel(const AdapterArgs a) {
-  __shared__ std::conditional_t<kVector, WideShared<kSteps>, char> shared;
+  extern __shared__ f32x4 up_shared[];  // WideShared, if any tile goes through it
+  __shared__ TileRows rows;
   const int chunks = (a.pool.out_width + a.chunk - 1) / a.chunk;
-  const Tile tile = tile_at(a, blockIdx.x / chunks);
+  find_tile(a, static_cast<int>(blockIdx.x / chunks), rows);
+  const Tile tile = rows.tile;
   if (tile.count == 0)
     return;
   const int begin = static_cast<int>(blockIdx.x % chunks) * a.chunk;
   const int last = min(a.pool.out_width, begin + a.chunk);
   if (tile.adapter < 0) {
     if (a.residual != a.out)
-      copy_rows<kVector, kResidual>(a, tile, begin, last);
+      copy_rows<kVector, kResidual>(a, rows, begin, last);
     return;
   }
   if constexpr (kVector) {
-    if (tile.count > 16) {
-      up_wide<kSteps, kResidual>(a, tile, begin, last, shared);
+    if (tile.count > 16 && a.wide) {
+      up_wide<kSteps, kResidual>(a, rows, begin, last,
+                                 *reinterpret_cast<WideShared<kSteps> *>(up_shared));
       return;
     }
   }
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int sets = tile.count <= 16 ? 1 : tile.count <= 32 ? 2 : 4;
   if (16 * (wave % sets) < tile.count)
-    up_rows<kSteps, kVector, kResidual>(a, tile, wave % sets, begin + 16 * (wave / sets),
+    up_rows<kSteps, kVector, kResidual>(a, rows, wave % sets, begin + 16 * (wave / sets),
                                         64 / sets, last);
 }
 
 // ---------------------------------------------------------------------- host
 // Tiles at most: each bin's last tile may be short.
 size_t most_tiles(const AdapterPool &pool, size_t rows) {
-  if (rows <= kDirectRows)
+  if (rows <= kFewRows)
     return rows;
   return std::min(rows, rows / kTileRows + std::min<size_t>(rows, pool.adapters + size_t{1}));
 }
-// Parts of the width, so that a few tiles fill the card; eight 32-steps a wave at least.
+// Parts of the width: about four steps a wave, all blocks on the card at once (two a CU).
 size_t parts_of(const AdapterPool &pool, size_t rows) {
   const size_t steps = (static_cast<size_t>(pool.in_width) + 31) / 32;
-  return std::max<size_t>(1, std::min<size_t>({16, 768 / most_tiles(pool, rows), steps / 32}));
+  const size_t blocks = most_tiles(pool, rows) * (rows <= 32 ? 1 : 2);
+  return std::max<size_t>(1, std::min<size_t>({16, 512 / blocks, ceil_div(steps, 4 * kDownWaves)}));
+}
+// Whether tiles are expected to have more than 16 rows: most_tiles is about twice what
+// rows of a few adapters fill.
+bool wide_tiles(const AdapterPool &pool, size_t rows) {
+  return rows > 8 * most_tiles(pool, rows);
+}
+// Output columns of a block.
+size_t chunk_of(const AdapterPool &pool, size_t rows, bool wide) {
+  const size_t width = static_cast<size_t>(pool.out_width), tiles = most_tiles(pool, rows);
+  const size_t unit = wide ? kWide : 64, blocks = wide ? (pool.rank <= 64 ? 768 : 512) : 2048;
+  const size_t chunks = std::max<size_t>(1, std::min<size_t>(ceil_div(width, unit), blocks / tiles));
+  return ceil_div(ceil_div(width, chunks), unit) * unit;
 }
 size_t aligned(size_t bytes) { return (bytes + 15) / 16 * 16; }
 
-template <int kRanks> void (*down_of(bool low))(AdapterArgs) {
-  return low ? down_kernel<kRanks, true> : down_kernel<kRanks, false>;
+template <int kRanks> Status launch_down(const AdapterArgs &a, hipStream_t stream) {
+  const auto kernel = a.lo != nullptr ? down_kernel<kRanks, true> : down_kernel<kRanks, false>;
+  const int cols = a.rows <= 16 ? 1 : 2;  // 16s of rows in a block
+  const int loads = kRanks + cols * (a.lo != nullptr ? 2 : 1);
+  const size_t lds = kDownWaves * std::max(loads, kRanks * cols) * 64 * sizeof(f32x4);
+  if (lds > 64 * 1024)
+    EVO_TRY(hip_status(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize,
+                                           static_cast<int>(lds)),
+                       "adapter down_kernel LDS opt-in"));
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.tiles) * a.parts * a.halves),
+                     dim3(64 * kDownWaves), static_cast<unsigned>(lds), stream, a);
+  return launch_status("adapter down_kernel");
 }
-template <int kSteps> void (*up_of(bool vector, bool residual))(AdapterArgs) {
-  if (vector)
-    return residual ? up_kernel<kSteps, true, true> : up_kernel<kSteps, true, false>;
-  return residual ? up_kernel<kSteps, false, true> : up_kernel<kSteps, false, false>;
+template <int kSteps>
+Status launch_up(const AdapterArgs &a, bool vector, size_t chunks, hipStream_t stream) {
+  const bool residual = a.residual != nullptr;
+  const auto kernel = vector ? (residual ? up_kernel<kSteps, true, true>
+                                         : up_kernel<kSteps, true, false>)
+                             : (residual ? up_kernel<kSteps, false, true>
+                                         : up_kernel<kSteps, false, false>);
+  const size_t lds = vector && a.wide ? sizeof(WideShared<kSteps>) : 0;
+  if (lds > 64 * 1024)
+    EVO_TRY(hip_status(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize,
+                                           static_cast<int>(lds)),
+                       "adapter up_kernel LDS opt-in"));
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.tiles * chunks)), dim3(256),
+                     static_cast<unsigned>(lds), stream, a);
+  return launch_status("adapter up_kernel");
 }
 
 Status invalid(const char *why) { return {ErrorCode::kInvalidArgument, why}; }
@@ -641,13 +705,11 @@ Status adapter_linear(const AdapterPool &pool, const int32_t *adapter, const uin
       workspace_bytes < adapter_workspace_bytes(pool, rows))
     return invalid("adapter_linear: workspace too small or not aligned");
   const size_t tiles = most_tiles(pool, rows), parts = parts_of(pool, rows);
-  // About four blocks a CU, in whole rounds of a block's four waves.
-  const size_t width = static_cast<size_t>(pool.out_width);
-  const size_t chunk =
-      std::min<size_t>(2048, std::max<size_t>(1, width * tiles / 1024 / 64) * 64);
-  const size_t chunks = (width + chunk - 1) / chunk;
+  const bool wide = wide_tiles(pool, rows);
+  const size_t width = static_cast<size_t>(pool.out_width), chunk = chunk_of(pool, rows, wide);
+  const size_t chunks = ceil_div(width, chunk);
   constexpr size_t kMostBlocks = ((size_t{1} << 32) - 1) / 256;
-  if (tiles * parts > kMostBlocks || tiles * chunks > kMostBlocks)
+  if (tiles * parts * 4 > kMostBlocks || tiles * chunks > kMostBlocks)
     return invalid("adapter_linear: grid too large");
   char *const base = static_cast<char *>(workspace);
   const size_t list = aligned(rows * sizeof(int32_t));
@@ -657,24 +719,22 @@ Status adapter_linear(const AdapterPool &pool, const int32_t *adapter, const uin
       out_stride % 4 == 0 && width % 4 == 0;
   const AdapterArgs args{pool, adapter, x_hi, x_lo, x_stride, static_cast<int>(rows), residual,
                          out, out_stride, static_cast<int>(tiles), static_cast<int>(parts),
-                         static_cast<int>(chunk), rows <= kDirectRows ? 1 : 0,
+                         static_cast<int>(chunk), rows <= kFewRows ? 0 : 1, rows <= 32 ? 1 : 2,
+                         wide ? 1 : 0,
                          reinterpret_cast<int32_t *>(base),
                          reinterpret_cast<int32_t *>(base + list), reinterpret_cast<Tile *>(after),
                          reinterpret_cast<float *>(after + aligned(tiles * sizeof(Tile)))};
-  if (!args.direct)
-    hipLaunchKernelGGL(group_kernel, dim3(1), dim3(kGroupThreads),
+  if (args.sorted)
+    hipLaunchKernelGGL(group_kernel, dim3(1), dim3(rows <= 1024 ? 256 : kGroupThreads),
                        static_cast<unsigned>((pool.adapters + 1) * sizeof(int32_t)), stream,
                        args);
-  const auto down = pool.rank <= 16   ? down_of<1>(x_lo != nullptr)
-                    : pool.rank <= 32 ? down_of<2>(x_lo != nullptr)
-                    : pool.rank <= 64 ? down_of<4>(x_lo != nullptr)
-                                      : down_of<8>(x_lo != nullptr);
-  hipLaunchKernelGGL(down, dim3(static_cast<unsigned>(tiles * parts)), dim3(256), 0, stream, args);
-  const auto up = pool.rank <= 32   ? up_of<1>(vector, residual != nullptr)
-                  : pool.rank <= 64 ? up_of<2>(vector, residual != nullptr)
-                                    : up_of<4>(vector, residual != nullptr);
-  hipLaunchKernelGGL(up, dim3(static_cast<unsigned>(tiles * chunks)), dim3(256), 0, stream, args);
-  return launch_status("adapter_linear kernels");
+  EVO_TRY(pool.rank <= 16   ? launch_down<1>(args, stream)
+          : pool.rank <= 32 ? launch_down<2>(args, stream)
+          : pool.rank <= 64 ? launch_down<4>(args, stream)
+                            : launch_down<8>(args, stream));
+  return pool.rank <= 32   ? launch_up<1>(args, vector, chunks, stream)
+         : pool.rank <= 64 ? launch_up<2>(args, vector, chunks, stream)
+                           : launch_up<4>(args, vector, chunks, stream);
 }
 
 }  // namespace evo::hip
