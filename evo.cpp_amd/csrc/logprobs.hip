@@ -63,132 +63,143 @@ __device__ inline uint32_t order_of(uint64_t place) { return static_cast<uint32_
 __device__ inline uint32_t index_of(uint64_t place) { return ~static_cast<uint32_t>(place); }
 
 // kPer logits a lane: 16 bytes at a time where rows start on them (kVec), one by one
-// otherwise.
+// otherwise. Every lane loads from inside its row: a run that would pass its end is moved
+// back to it, and what came twice or lies behind it is -infinity.
 template <typename S, bool kVec, int kPer> struct Logits {
   static constexpr int kEach = kVec ? 16 / static_cast<int>(sizeof(S)) : 1;
   float x[kPer];
 
-  static __device__ int index(int first, int i) {
-    const int lane = threadIdx.x & 63;
-    return first + (i / kEach * 64 + lane) * kEach + i % kEach;
+  // Where run i / kEach of a lane begins in a row, and where it is loaded from.
+  static __device__ int begin(int first, int i) {
+    return first + (i / kEach * 64 + static_cast<int>(threadIdx.x & 63)) * kEach;
   }
-  // Logits first .. of a row; -infinity behind its end.
+  static __device__ int from(int first, int i, int vocab) {
+    return min(begin(first, i), vocab - kEach);
+  }
+  // Logits first .. of a row (vocab >= kEach).
   __device__ void load(const S *row, int first, int vocab) {
-    if (first + kPer * 64 <= vocab) {
+    typedef S vector __attribute__((ext_vector_type(kEach)));
+    typedef vector unaligned __attribute__((aligned(sizeof(S))));
+    unaligned v[kPer / kEach];
 #pragma unroll
-      for (int i = 0; i < kPer; i += kEach)
-        read(row + index(first, i), i);
-      return;
-    }
+    for (int i = 0; i < kPer; i += kEach)
+      v[i / kEach] = *reinterpret_cast<const unaligned *>(row + from(first, i, vocab));
 #pragma unroll
-    for (int i = 0; i < kPer; i += kEach) {
-      const int at = index(first, i);
-      if (at + kEach <= vocab) {
-        read(row + at, i);
-        continue;
-      }
+    for (int i = 0; i < kPer; ++i)
+      x[i] = static_cast<float>(v[i / kEach][i % kEach]);
+    if (first + kPer * 64 > vocab) {
 #pragma unroll
-      for (int e = 0; e < kEach; ++e)
-        x[i + e] = at + e < vocab ? static_cast<float>(row[at + e]) : -INFINITY;
+      for (int i = 0; i < kPer; ++i)
+        x[i] = valid(first, i, vocab) ? x[i] : -INFINITY;
     }
   }
-  __device__ void read(const S *from, int i) {
-    typedef S vector __attribute__((ext_vector_type(kEach)));
-    const vector v = *reinterpret_cast<const vector *>(from);
-#pragma unroll
-    for (int e = 0; e < kEach; ++e)
-      x[i + e] = static_cast<float>(v[e]);
+  static __device__ bool valid(int first, int i, int vocab) {
+    return i % kEach >= begin(first, i) - from(first, i, vocab);
   }
 };
 
+// (fmaxf would quiet each operand first.)
+__device__ inline float largest(float x, float y, float z) {
+  float most;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(most) : "v"(x), "v"(y), "v"(z));
+  return most;
+}
 __device__ inline float larger(float x, float y) { return __builtin_fmaxf(x, y); }
-
-constexpr float kLog2e = 1.44269504088896341F, kLog2eLow = 1.92596299e-8F;
-// exp(d) for d <= 0. Its argument's rounding is off by up to |d| * 2^-24; kExact adds
-// what the rounding lost.
-template <bool kExact> __device__ inline float weight(float d) {
-  const float scaled = d * kLog2e;
-  const float w = __builtin_amdgcn_exp2f(scaled);
-  if constexpr (!kExact)
-    return w;
-  const float lost = fmaf(d, kLog2eLow, fmaf(d, kLog2e, -scaled));
-  // (-infinity leaves no number.)
-  return w == 0.0F ? 0.0F : fmaf(w * lost, 0.693147180559945F, w);
+template <int kCount> __device__ inline float largest_of(const float *x) {
+  if constexpr (kCount == 1)
+    return x[0];
+  else if constexpr (kCount == 2)
+    return largest(x[0], x[1], x[1]);
+  else
+    return largest(largest_of<kCount - 2>(x), x[kCount - 2], x[kCount - 1]);
 }
 
-// The sums of a segment. chunk: registers looked over at once for one that holds the
-// largest.
+constexpr float kLog2e = 1.44269504088896341F, kLog2eLow = 1.92596299e-8F;
+constexpr float kLn2 = 0.693147180559945F;
+// exp(d) for d <= 0 with its argument's rounding, up to |d| * 2^-24, added again.
+__device__ inline float exact_weight(float d) {
+  const float scaled = d * kLog2e;
+  const float w = __builtin_amdgcn_exp2f(scaled);
+  const float lost = fmaf(d, kLog2eLow, fmaf(d, kLog2e, -scaled));
+  // (-infinity leaves no number.)
+  return w == 0.0F ? 0.0F : fmaf(w * lost, kLn2, w);
+}
+
+// The sums of a segment, given the largest of each kChunk registers. A chunk without the
+// largest of all in any lane takes the short way: with base * log2(e) = high + low, a
+// weight is exp2(x log2(e) - high), and 2^-low comes in at the end.
+constexpr int kChunk = 8;
 template <bool kExact, int kPer>
-__device__ inline void sums(const float (&x)[kPer], float top, float &sum, float &spread,
-                            uint32_t &equal) {
-  constexpr int kChunk = 8;
-  const float base = top == -INFINITY ? 0.0F : top;
-  sum = spread = 0.0F;
-  equal = 0;
+__device__ inline void sums(const float (&x)[kPer], const float (&most)[kPer / kChunk],
+                            Segment &s) {
+  const float base = s.top == -INFINITY ? 0.0F : s.top;
+  const float high = base * kLog2e;
+  const float low = fmaf(base, kLog2eLow, fmaf(base, kLog2e, -high));
+  float sum = 0.0F, spread = 0.0F, short_sum = 0.0F, short_spread = 0.0F;
+  uint32_t equal = 0;
 #pragma unroll
   for (int i = 0; i < kPer; i += kChunk) {
-    float most = x[i];
-#pragma unroll
-    for (int e = 1; e < kChunk; ++e)
-      most = larger(most, x[i + e]);
-    if (__any(most == base)) {
+    if (kExact || __any(most[i / kChunk] == base)) {
 #pragma unroll
       for (int e = 0; e < kChunk; ++e) {
         const bool first = x[i + e] == base;
-        const float d = x[i + e] - base, w = first ? 0.0F : weight<kExact>(d);
+        const float d = x[i + e] - base;
+        const float w =
+            first ? 0.0F : kExact ? exact_weight(d) : __builtin_amdgcn_exp2f(d * kLog2e);
         equal += first ? 1U : 0U;
         sum += w;
-        spread = fmaf(w, larger(d, -200.0F), spread);
+        spread = fmaf(w, larger(d, -200.0F), spread);  // (a weight of 0 has d = -infinity)
       }
     } else {
 #pragma unroll
       for (int e = 0; e < kChunk; ++e) {
-        const float d = x[i + e] - base, w = weight<kExact>(d);
-        sum += w;
-        spread = fmaf(w, larger(d, -200.0F), spread);  // (a weight of 0 has d = -infinity)
+        const float scaled = fmaf(x[i + e], kLog2e, -high), w = __builtin_amdgcn_exp2f(scaled);
+        short_sum += w;
+        short_spread = fmaf(w, larger(scaled, -300.0F), short_spread);
       }
     }
   }
-  sum = wave_reduce(sum, Sum());
-  spread = wave_reduce(spread, Sum());
-  equal = wave_reduce(equal, Sum());
+  if constexpr (!kExact) {
+    const float lift = __builtin_amdgcn_exp2f(-low);
+    sum = fmaf(short_sum, lift, sum);
+    spread = fmaf((short_spread - low * short_sum) * lift, kLn2, spread);
+  }
+  s.sum = wave_reduce(sum, Sum());
+  s.spread = wave_reduce(spread, Sum());
+  s.equal = wave_reduce(equal, Sum());
 }
 
 // Largest logit and sums; every lane has them. Sums of a small total come from far
-// logits, whose arguments round worst: they are formed again, exactly.
+// logits, whose arguments round worst: they are formed again, exactly. So are those of
+// logits whose multiple by log2(e) might overflow.
 template <int kPer>
-__device__ inline Segment segment_of(const float (&x)[kPer]) {
+__device__ inline Segment segment_of(const float (&x)[kPer], const float (&most)[kPer / kChunk]) {
   Segment s{};
-  s.top = x[0];
-#pragma unroll
-  for (int i = 1; i < kPer; ++i)
-    s.top = larger(s.top, x[i]);
-  s.top = wave_reduce(s.top, Most());
-  sums<false>(x, s.top, s.sum, s.spread, s.equal);
-  if (s.sum < 0.0625F && s.sum > 0.0F)
-    sums<true>(x, s.top, s.sum, s.spread, s.equal);
+  s.top = wave_reduce(largest_of<kPer / kChunk>(most), Most());
+  if (!(fabsf(s.top) > 0x1p120F))
+    sums<false>(x, most, s);
+  if (!(s.sum >= 0.0625F))
+    sums<true>(x, most, s);
   return s;
 }
 
 // Tokens of the segment in front of `token`, whose logit is `given`.
 template <typename L, int kPer>
-__device__ inline uint32_t count_before(const float (&x)[kPer], int first, float given,
-                                        int token) {
+__device__ inline uint32_t count_before(const float (&x)[kPer], const float (&most)[kPer / kChunk],
+                                        int first, int vocab, float given, int token) {
   // Those behind it in the row come before it only by a larger logit.
   const float above = value_of_order(ordered(given) + 1);
   uint32_t count = 0;
 #pragma unroll
-  for (int i = 0; i < kPer; i += L::kEach) {
-    const int at = L::index(first, i);
-    if (L::kEach > 1 && !__any(at <= token && token < at + L::kEach)) {
-      const float least = at < token ? given : above;
+  for (int i = 0; i < kPer; i += kChunk) {
+    if (!__any(most[i / kChunk] >= given))
+      continue;
+#pragma unroll
+    for (int j = i; j < i + kChunk; j += L::kEach) {
+      const int from = L::from(first, j, vocab);
 #pragma unroll
       for (int e = 0; e < L::kEach; ++e)
-        count += __popcll(__ballot(x[i + e] >= least));
-    } else {
-#pragma unroll
-      for (int e = 0; e < L::kEach; ++e)
-        count += __popcll(__ballot(x[i + e] >= (at + e < token ? given : above)));
+        count += __popcll(__ballot(x[j + e] >= (from + e < token ? given : above)));
     }
   }
   return count;
@@ -281,9 +292,13 @@ __global__ __launch_bounds__(256) void row_kernel(const LogprobArgs a) {
   l.load(logits, 0, a.vocab);
   const bool given = token < static_cast<uint32_t>(a.vocab);
   const float logit = given ? static_cast<float>(logits[token]) : 0.0F;
-  Segment s = segment_of(l.x);
+  float chunks[kPer / kChunk];
+#pragma unroll
+  for (int i = 0; i < kPer; i += kChunk)
+    chunks[i / kChunk] = largest_of<kChunk>(&l.x[i]);
+  Segment s = segment_of(l.x, chunks);
   if (given && a.rank != nullptr)
-    s.before = count_before<L>(l.x, 0, logit, static_cast<int>(token));
+    s.before = count_before<L>(l.x, chunks, 0, a.vocab, logit, static_cast<int>(token));
   const Row r(s);
   if (lane == 0)
     write_row(a, row, r, s.before, given, logit);
@@ -296,7 +311,7 @@ __global__ __launch_bounds__(256) void row_kernel(const LogprobArgs a) {
   uint32_t order[kPer], most = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    order[i] = L::index(0, i) < a.vocab ? ordered(l.x[i]) : 0;
+    order[i] = L::valid(0, i, a.vocab) ? ordered(l.x[i]) : 0;
     most = max(most, order[i]);
   }
   uint32_t border = 0;
@@ -319,7 +334,7 @@ __global__ __launch_bounds__(256) void row_kernel(const LogprobArgs a) {
       continue;
     if (in >> lane & 1)
       list[n + __popcll(in & ((uint64_t{1} << lane) - 1))] =
-          place(order[i], static_cast<uint32_t>(L::index(0, i)));
+          place(order[i], static_cast<uint32_t>(L::from(0, i, a.vocab) + i % L::kEach));
     n += __popcll(in);
   }
   n = keep_best(list, n, n <= 64 ? 64 : k);
@@ -343,61 +358,70 @@ __global__ __launch_bounds__(256) void segment_kernel(const LogprobArgs a) {
   const bool given = token < static_cast<uint32_t>(a.vocab);
   const float logit = given ? static_cast<float>(logits[token]) : 0.0F;
 
-  if (a.alternatives > 0) {
-    // The largest of 64 neighbours: of kEach in each of 64 / kEach lanes.
-    constexpr int kLanes = kGroup / L::kEach, kRegisters = kSegment / 64 / L::kEach;
-    constexpr int kPerRegister = 64 / kLanes;  // groups
-    float mine = -INFINITY;
+  // The largest of each run, of 8 registers and of 64 neighbours: kEach registers in each
+  // of 64 / kEach lanes.
+  constexpr int kPer = kSegment / 64, kLanes = kGroup / L::kEach, kRuns = kPer / L::kEach;
+  float chunks[kPer / kChunk], mine = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < kRegisters; ++j) {
-      float most = l.x[j * L::kEach];
+  for (int i = 0; i < kPer; i += kChunk) {
+    float runs[kChunk / L::kEach];
 #pragma unroll
-      for (int e = 1; e < L::kEach; ++e)
-        most = larger(most, l.x[j * L::kEach + e]);
-      if constexpr (kLanes == 64) {
-        most = wave_reduce(most, Most());
-      } else {
-        most = larger(most, dpp<0xb1, 0xf>(most, most));   // quad_perm 1 0 3 2
-        most = larger(most, dpp<0x4e, 0xf>(most, most));   // quad_perm 2 3 0 1
-        most = larger(most, dpp<0x141, 0xf>(most, most));  // row_half_mirror
-        if constexpr (kLanes == 16)
-          most = larger(most, dpp<0x140, 0xf>(most, most));  // row_mirror
+    for (int j = 0; j < kChunk / L::kEach; ++j)
+      runs[j] = largest_of<L::kEach>(&l.x[i + j * L::kEach]);
+    chunks[i / kChunk] = largest_of<kChunk / L::kEach>(runs);
+    if (a.alternatives > 0) {
+#pragma unroll
+      for (int j = 0; j < kChunk / L::kEach; ++j) {
+        float most = runs[j];
+        if constexpr (kLanes == 64) {
+          most = wave_reduce(most, Most());
+        } else {
+          most = larger(most, dpp<0xb1, 0xf>(most, most));   // quad_perm 1 0 3 2
+          most = larger(most, dpp<0x4e, 0xf>(most, most));   // quad_perm 2 3 0 1
+          most = larger(most, dpp<0x141, 0xf>(most, most));  // row_half_mirror
+          if constexpr (kLanes == 16)
+            most = larger(most, dpp<0x140, 0xf>(most, most));  // row_mirror
+        }
+        mine = lane % kLanes == i / L::kEach + j ? most : mine;
       }
-      mine = lane % kLanes == j ? most : mine;
     }
-    if (lane % kLanes < kRegisters)
-      a.groups[(static_cast<size_t>(row) * a.segments + segment) * kGroups +
-               lane % kLanes * kPerRegister + lane / kLanes] = mine;
   }
-  Segment s = segment_of(l.x);
-  if (given)
-    s.before = count_before<L>(l.x, first, logit, static_cast<int>(token));
+  if (a.alternatives > 0 && lane % kLanes < kRuns)
+    a.groups[(static_cast<size_t>(row) * a.segments + segment) * kGroups +
+             lane % kLanes * (64 / kLanes) + lane / kLanes] = mine;
+  Segment s = segment_of(l.x, chunks);
+  if (given && s.top >= logit)
+    s.before = count_before<L>(l.x, chunks, first, a.vocab, logit, static_cast<int>(token));
   if (lane == 0)
     a.stats[at] = s;
 }
 
 // A row's segments joined, and its first tokens.
 template <typename S> __global__ __launch_bounds__(256) void join_kernel(const LogprobArgs a) {
-  __shared__ uint64_t list[kMostTop * kGroup];
+  __shared__ __attribute__((aligned(16))) uint64_t list[kMostTop * kGroup];
   __shared__ uint32_t chosen[kMostTop];
-  __shared__ uint32_t scratch[4];
-  __shared__ float floats[4];
   __shared__ int count;
   __shared__ uint32_t least;
   static_assert(kMostTop * kGroups <= kMostTop * kGroup, "groups of the best segments fit the list");
-  const int row = blockIdx.x;
+  const int row = blockIdx.x, lane = threadIdx.x & 63;
   const Segment *stats = a.stats + static_cast<size_t>(row) * a.segments;
   const S *logits = static_cast<const S *>(a.logits) + row * a.row_stride;
   const uint32_t token = a.tokens != nullptr ? a.tokens[row] : kNoToken;
   const bool given = token < static_cast<uint32_t>(a.vocab);
   const float logit = given ? static_cast<float>(logits[token]) : 0.0F;
+  const int k = a.alternatives;
 
+  // Every wave joins the sums by itself.
   Segment whole{};
   whole.top = -INFINITY;
-  for (int i = threadIdx.x; i < a.segments; i += 256)
-    whole.top = larger(whole.top, stats[i].top);
-  whole.top = block_reduce<256>(whole.top, floats, Most());
-  for (int i = threadIdx.x; i < a.segments; i += 256) {
+  for (int i = lane; i < a.segments; i += 64) {
+    const float top = stats[i].top;
+    whole.top = larger(whole.top, top);
+    if (k > 0 && threadIdx.x < 64)
+      list[i] = place(ordered(top), static_cast<uint32_t>(i));
+  }
+  whole.top = wave_reduce(whole.top, Most());
+  for (int i = lane; i < a.segments; i += 64) {
     const Segment s = stats[i];
     whole.before += s.before;
     if (s.top == whole.top) {
@@ -412,66 +436,64 @@ template <typename S> __global__ __launch_bounds__(256) void join_kernel(const L
       whole.spread += shrink * fmaf(away, sum, s.spread);
     }
   }
-  whole.sum = block_reduce<256>(whole.sum, floats, Sum());
-  whole.spread = block_reduce<256>(whole.spread, floats, Sum());
-  whole.equal = block_reduce<256>(whole.equal, scratch, Sum());
-  whole.before = block_reduce<256>(whole.before, scratch, Sum());
+  whole.sum = wave_reduce(whole.sum, Sum());
+  whole.spread = wave_reduce(whole.spread, Sum());
+  whole.equal = wave_reduce(whole.equal, Sum());
+  whole.before = wave_reduce(whole.before, Sum());
   const Row r(whole);
   if (threadIdx.x == 0)
     write_row(a, row, r, whole.before, given, logit);
-  const int k = a.alternatives;
   if (k == 0)
     return;
 
-  // The wave's k best of the list: their indexes to `chosen`, the order of the last
-  // one to `least` (0: there are fewer). The list is empty then.
-  const auto choose = [&](int n) {
+  // Each round takes the k best of the list (all, if there are no more) in order: of the
+  // segments, their groups, and those groups' logits.
+  int n = a.segments;
+#pragma unroll 1
+  for (int round = 0;; ++round) {
     __syncthreads();
-    if (threadIdx.x < 64) {
-      const int kept = keep_best(list, n < 0 ? count : n, k);
-      const int lane = threadIdx.x;
-      const uint32_t order = lane < kept ? order_of(list[lane]) : 0xffffffffU;
-      if (lane < kept)
-        chosen[lane] = index_of(list[lane]);
-      const uint32_t last = ~wave_reduce(~order, Most());
-      if (lane == 0) {
-        least = kept < k ? 0 : last;
-        count = 0;
-      }
+    if (n > 256) {
+      // (Few rows: many equal logits, or a very large vocabulary.)
+      if (threadIdx.x < 64)
+        keep_best(list, n, k);
+      n = k;
+      __syncthreads();
+    }
+    const int kept = min(n, k);
+    const int own = threadIdx.x;
+    if (own < n) {
+      const uint64_t mine = list[own];
+      int rank = 0;
+      for (int i = 0; i < n; ++i)
+        rank += list[i] > mine ? 1 : 0;
+      if (rank < kept && round == 2)
+        write_top(a, row, r, rank, mine);
+      if (rank < kept)
+        chosen[rank] = index_of(mine);
+      if (rank == kept - 1)
+        least = order_of(mine);
+    }
+    if (round == 2)
+      return;
+    if (threadIdx.x == 0)
+      count = 0;
+    __syncthreads();
+    // What lies below the k-th of these is below k tokens.
+    const uint32_t border = kept < k ? 0 : least;
+    const int each = round == 0 ? kGroups : kGroup;
+    for (int i = threadIdx.x; i < kept * each; i += 256) {
+      const uint32_t index = chosen[i / each] * each + i % each;
+      uint32_t order = 0;
+      if (round == 0 && index * kGroup < static_cast<uint32_t>(a.vocab))
+        order = ordered(a.groups[static_cast<size_t>(row) * a.segments * kGroups + index]);
+      else if (round == 1 && index < static_cast<uint32_t>(a.vocab))
+        order = ordered(static_cast<float>(logits[index]));
+      if (order != 0 && order >= border)
+        list[atomicAdd(&count, 1)] = place(order, index);
     }
     __syncthreads();
-  };
-  const auto add = [&](uint64_t place) { list[atomicAdd(&count, 1)] = place; };
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.segments; i += 256)
-    list[i] = place(ordered(stats[i].top), static_cast<uint32_t>(i));
-  choose(a.segments);
-  const int segments = min(k, a.segments);
-  const uint32_t border = least;
-  for (int i = threadIdx.x; i < segments * kGroups; i += 256) {
-    const uint32_t group = chosen[i / kGroups] * kGroups + i % kGroups;
-    if (group * kGroup >= static_cast<uint32_t>(a.vocab))
-      continue;
-    const uint32_t order =
-        ordered(a.groups[static_cast<size_t>(row) * a.segments * kGroups + group]);
-    if (order >= border)
-      add(place(order, group));
+    n = count;
   }
-  __syncthreads();
-  const int groups = min(k, count);
-  choose(-1);
-  const uint32_t group_border = least;
-  for (int i = threadIdx.x; i < groups * kGroup; i += 256) {
-    const uint32_t index = chosen[i / kGroup] * kGroup + i % kGroup;
-    if (index >= static_cast<uint32_t>(a.vocab))
-      continue;
-    const uint32_t order = ordered(static_cast<float>(logits[index]));
-    if (order >= group_border)
-      add(place(order, index));
-  }
-  __syncthreads();
-  if (threadIdx.x < 64)
-    write_best(a, row, r, list, keep_best(list, count, k));
 }
 
 template <typename S, bool kVec, int kPer>
@@ -546,7 +568,8 @@ Status token_logprobs(int dtype, const void *logits, size_t rows, size_t vocab, 
                          static_cast<int>(segments), row_stride, tokens, logprob, rank, entropy,
                          static_cast<int>(alternatives), top_tokens, top_logprobs, stats,
                          need > 0 ? reinterpret_cast<float *>(stats + rows * segments) : nullptr};
-  const bool vector = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && row_stride * size % 16 == 0;
+  const bool vector = reinterpret_cast<uintptr_t>(logits) % 16 == 0 &&
+                      row_stride * size % 16 == 0 && vocab * size >= 16;
   if (dtype == kElementF32)
     launch_type<float>(args, vector, stream);
   else if (dtype == kElementBF16)
