@@ -62,11 +62,11 @@ __device__ inline uint64_t place(uint32_t order, uint32_t index) {
 __device__ inline uint32_t order_of(uint64_t place) { return static_cast<uint32_t>(place >> 32); }
 __device__ inline uint32_t index_of(uint64_t place) { return ~static_cast<uint32_t>(place); }
 
-// kPer logits a lane: 16 bytes at a time where rows start on them (kVec), one by one
-// otherwise. Every lane loads from inside its row: a run that would pass its end is moved
-// back to it, and what came twice or lies behind it is -infinity.
-template <typename S, bool kVec, int kPer> struct Logits {
-  static constexpr int kEach = kVec ? 16 / static_cast<int>(sizeof(S)) : 1;
+// kPer logits a lane, in runs of kEach: 16 bytes, wherever a row starts (the loads need no
+// alignment), or one. Every lane loads from inside its row: a run that would pass its end
+// is moved back to it, and what came twice or lies behind it is -infinity.
+template <typename S, int kRun, int kPer> struct Logits {
+  static constexpr int kEach = kRun;
   float x[kPer];
 
   // Where run i / kEach of a lane begins in a row, and where it is loaded from.
@@ -76,14 +76,17 @@ template <typename S, bool kVec, int kPer> struct Logits {
   static __device__ int from(int first, int i, int vocab) {
     return min(begin(first, i), vocab - kEach);
   }
-  // Logits first .. of a row (vocab >= kEach).
-  __device__ void load(const S *row, int first, int vocab) {
+  // Logits first .. of a row (vocab >= kEach), and the given token's among all of them,
+  // whose load follows the token's own and would wait alone behind theirs.
+  __device__ float load(const S *row, int first, int vocab, uint32_t token) {
     typedef S vector __attribute__((ext_vector_type(kEach)));
     typedef vector unaligned __attribute__((aligned(sizeof(S))));
     unaligned v[kPer / kEach];
 #pragma unroll
     for (int i = 0; i < kPer; i += kEach)
       v[i / kEach] = *reinterpret_cast<const unaligned *>(row + from(first, i, vocab));
+    const S given = row[token < static_cast<uint32_t>(vocab) ? token : 0];
+    asm volatile("" ::: "memory");  // every load before the first use
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
       x[i] = static_cast<float>(v[i / kEach][i % kEach]);
@@ -92,6 +95,7 @@ template <typename S, bool kVec, int kPer> struct Logits {
       for (int i = 0; i < kPer; ++i)
         x[i] = valid(first, i, vocab) ? x[i] : -INFINITY;
     }
+    return static_cast<float>(given);
   }
   static __device__ bool valid(int first, int i, int vocab) {
     return i % kEach >= begin(first, i) - from(first, i, vocab);
@@ -105,6 +109,10 @@ __device__ inline float largest(float x, float y, float z) {
   return most;
 }
 __device__ inline float larger(float x, float y) { return __builtin_fmaxf(x, y); }
+template <int kCtrl> __device__ inline float largest_with(float x) {
+  const float other = dpp<kCtrl, 0xf>(x, x);
+  return largest(x, other, other);
+}
 template <int kCount> __device__ inline float largest_of(const float *x) {
   if constexpr (kCount == 1)
     return x[0];
@@ -129,7 +137,7 @@ __device__ inline float exact_weight(float d) {
 // largest of all in any lane takes the short way: with base * log2(e) = high + low, a
 // weight is exp2(x log2(e) - high), and 2^-low comes in at the end.
 constexpr int kChunk = 8;
-template <bool kExact, int kPer>
+template <int kPer>
 __device__ inline void sums(const float (&x)[kPer], const float (&most)[kPer / kChunk],
                             Segment &s) {
   const float base = s.top == -INFINITY ? 0.0F : s.top;
@@ -139,13 +147,12 @@ __device__ inline void sums(const float (&x)[kPer], const float (&most)[kPer / k
   uint32_t equal = 0;
 #pragma unroll
   for (int i = 0; i < kPer; i += kChunk) {
-    if (kExact || __any(most[i / kChunk] == base)) {
+    if (__any(most[i / kChunk] == base)) {
 #pragma unroll
       for (int e = 0; e < kChunk; ++e) {
         const bool first = x[i + e] == base;
         const float d = x[i + e] - base;
-        const float w =
-            first ? 0.0F : kExact ? exact_weight(d) : __builtin_amdgcn_exp2f(d * kLog2e);
+        const float w = first ? 0.0F : __builtin_amdgcn_exp2f(d * kLog2e);
         equal += first ? 1U : 0U;
         sum += w;
         spread = fmaf(w, larger(d, -200.0F), spread);  // (a weight of 0 has d = -infinity)
@@ -159,27 +166,58 @@ __device__ inline void sums(const float (&x)[kPer], const float (&most)[kPer / k
       }
     }
   }
-  if constexpr (!kExact) {
-    const float lift = __builtin_amdgcn_exp2f(-low);
-    sum = fmaf(short_sum, lift, sum);
-    spread = fmaf((short_spread - low * short_sum) * lift, kLn2, spread);
-  }
-  s.sum = wave_reduce(sum, Sum());
-  s.spread = wave_reduce(spread, Sum());
+  const float lift = __builtin_amdgcn_exp2f(-low);
+  s.sum = wave_reduce(fmaf(short_sum, lift, sum), Sum());
+  s.spread = wave_reduce(fmaf((short_spread - low * short_sum) * lift, kLn2, spread), Sum());
   s.equal = wave_reduce(equal, Sum());
 }
+// The same with exact weights, of kPer logits a lane at a time.
+struct ExactSums {
+  float base, sum = 0.0F, spread = 0.0F;
+  uint32_t equal = 0;
+  __device__ explicit ExactSums(float top) : base(top == -INFINITY ? 0.0F : top) {}
+  template <int kPer> __device__ void add(const float (&x)[kPer]) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const float d = x[i] - base, w = x[i] == base ? 0.0F : exact_weight(d);
+      equal += x[i] == base ? 1U : 0U;
+      sum += w;
+      spread = fmaf(w, larger(d, -200.0F), spread);
+    }
+  }
+  __device__ void finish(Segment &s) const {
+    s.sum = wave_reduce(sum, Sum());
+    s.spread = wave_reduce(spread, Sum());
+    s.equal = wave_reduce(equal, Sum());
+  }
+};
 
-// Largest logit and sums; every lane has them. Sums of a small total come from far
-// logits, whose arguments round worst: they are formed again, exactly. So are those of
-// logits whose multiple by log2(e) might overflow.
-template <int kPer>
-__device__ inline Segment segment_of(const float (&x)[kPer], const float (&most)[kPer / kChunk]) {
+// Largest logit and sums of a segment, which x holds; every lane has them. Sums of a small
+// total come from far logits, whose arguments round worst: they are formed again, exactly,
+// from logits that are read again (kept for that, they would cost every wave registers).
+// So are those of logits whose multiple by log2(e) might overflow.
+template <typename S, int kPer>
+__device__ inline Segment segment_of(const S *row, int first, int vocab, const float (&x)[kPer],
+                                     const float (&most)[kPer / kChunk]) {
   Segment s{};
   s.top = wave_reduce(largest_of<kPer / kChunk>(most), Most());
   if (!(fabsf(s.top) > 0x1p120F))
-    sums<false>(x, most, s);
-  if (!(s.sum >= 0.0625F))
-    sums<true>(x, most, s);
+    sums(x, most, s);
+  if (!(s.sum >= 0.0625F)) {
+    ExactSums exact(s.top);
+#pragma unroll 1
+    for (int i = first + static_cast<int>(threadIdx.x & 63); i < first + 64 * kPer; i += 64 * 8) {
+      float again[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        again[j] = static_cast<float>(row[min(i + 64 * j, vocab - 1)]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        again[j] = i + 64 * j < vocab ? again[j] : -INFINITY;
+      exact.add(again);
+    }
+    exact.finish(s);
+  }
   return s;
 }
 
@@ -197,9 +235,16 @@ __device__ inline uint32_t count_before(const float (&x)[kPer], const float (&mo
 #pragma unroll
     for (int j = i; j < i + kChunk; j += L::kEach) {
       const int from = L::from(first, j, vocab);
+      if (L::kEach > 1 && __any(from <= token && token < from + L::kEach)) {
 #pragma unroll
-      for (int e = 0; e < L::kEach; ++e)
-        count += __popcll(__ballot(x[j + e] >= (from + e < token ? given : above)));
+        for (int e = 0; e < L::kEach; ++e)
+          count += __popcll(__ballot(x[j + e] >= (from + e < token ? given : above)));
+      } else {
+        const float least = from < token ? given : above;
+#pragma unroll
+        for (int e = 0; e < L::kEach; ++e)
+          count += __popcll(__ballot(x[j + e] >= least));
+      }
     }
   }
   return count;
@@ -278,9 +323,9 @@ __device__ inline void write_best(const LogprobArgs &a, int row, const Row &r,
 }
 
 // ------------------------------------------------- one wave takes a row
-template <typename S, bool kVec, int kPer>
+template <typename S, int kRun, int kPer>
 __global__ __launch_bounds__(256) void row_kernel(const LogprobArgs a) {
-  typedef Logits<S, kVec, kPer> L;
+  typedef Logits<S, kRun, kPer> L;
   extern __shared__ uint64_t lists[];  // [4][64 * kPer], where alternatives are asked for
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int row = blockIdx.x * 4 + wave;
@@ -289,14 +334,17 @@ __global__ __launch_bounds__(256) void row_kernel(const LogprobArgs a) {
   const S *logits = static_cast<const S *>(a.logits) + row * a.row_stride;
   const uint32_t token = a.tokens != nullptr ? a.tokens[row] : kNoToken;
   L l;
-  l.load(logits, 0, a.vocab);
+  const float logit = l.load(logits, 0, a.vocab, token);
   const bool given = token < static_cast<uint32_t>(a.vocab);
-  const float logit = given ? static_cast<float>(logits[token]) : 0.0F;
   float chunks[kPer / kChunk];
 #pragma unroll
   for (int i = 0; i < kPer; i += kChunk)
     chunks[i / kChunk] = largest_of<kChunk>(&l.x[i]);
-  Segment s = segment_of(l.x, chunks);
+  Segment s{};
+  s.top = wave_reduce(largest_of<kPer / kChunk>(chunks), Most());
+  ExactSums exact(s.top);
+  exact.add(l.x);
+  exact.finish(s);
   if (given && a.rank != nullptr)
     s.before = count_before<L>(l.x, chunks, 0, a.vocab, logit, static_cast<int>(token));
   const Row r(s);
@@ -342,9 +390,8 @@ __global__ __launch_bounds__(256) void row_kernel(const LogprobArgs a) {
 }
 
 // ------------------------------------------------- rows of several segments
-template <typename S, bool kVec>
-__global__ __launch_bounds__(256) void segment_kernel(const LogprobArgs a) {
-  typedef Logits<S, kVec, kSegment / 64> L;
+template <typename S> __global__ __launch_bounds__(256) void segment_kernel(const LogprobArgs a) {
+  typedef Logits<S, 16 / static_cast<int>(sizeof(S)), kSegment / 64> L;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const unsigned at = blockIdx.x * 4 + wave;
   const int row = static_cast<int>(at / a.segments), segment = static_cast<int>(at % a.segments);
@@ -354,9 +401,8 @@ __global__ __launch_bounds__(256) void segment_kernel(const LogprobArgs a) {
   const uint32_t token = a.tokens != nullptr && a.rank != nullptr ? a.tokens[row] : kNoToken;
   const int first = segment * kSegment;
   L l;
-  l.load(logits, first, a.vocab);
+  const float logit = l.load(logits, first, a.vocab, token);
   const bool given = token < static_cast<uint32_t>(a.vocab);
-  const float logit = given ? static_cast<float>(logits[token]) : 0.0F;
 
   // The largest of each run, of 8 registers and of 64 neighbours: kEach registers in each
   // of 64 / kEach lanes.
@@ -372,16 +418,11 @@ __global__ __launch_bounds__(256) void segment_kernel(const LogprobArgs a) {
     if (a.alternatives > 0) {
 #pragma unroll
       for (int j = 0; j < kChunk / L::kEach; ++j) {
-        float most = runs[j];
-        if constexpr (kLanes == 64) {
-          most = wave_reduce(most, Most());
-        } else {
-          most = larger(most, dpp<0xb1, 0xf>(most, most));   // quad_perm 1 0 3 2
-          most = larger(most, dpp<0x4e, 0xf>(most, most));   // quad_perm 2 3 0 1
-          most = larger(most, dpp<0x141, 0xf>(most, most));  // row_half_mirror
-          if constexpr (kLanes == 16)
-            most = larger(most, dpp<0x140, 0xf>(most, most));  // row_mirror
-        }
+        float most = largest_with<0xb1>(runs[j]);  // quad_perm 1 0 3 2
+        most = largest_with<0x4e>(most);           // quad_perm 2 3 0 1
+        most = largest_with<0x141>(most);          // row_half_mirror
+        if constexpr (kLanes == 16)
+          most = largest_with<0x140>(most);  // row_mirror
         mine = lane % kLanes == i / L::kEach + j ? most : mine;
       }
     }
@@ -389,7 +430,7 @@ __global__ __launch_bounds__(256) void segment_kernel(const LogprobArgs a) {
   if (a.alternatives > 0 && lane % kLanes < kRuns)
     a.groups[(static_cast<size_t>(row) * a.segments + segment) * kGroups +
              lane % kLanes * (64 / kLanes) + lane / kLanes] = mine;
-  Segment s = segment_of(l.x, chunks);
+  Segment s = segment_of(logits, first, a.vocab, l.x, chunks);
   if (given && s.top >= logit)
     s.before = count_before<L>(l.x, chunks, first, a.vocab, logit, static_cast<int>(token));
   if (lane == 0)
@@ -496,32 +537,26 @@ template <typename S> __global__ __launch_bounds__(256) void join_kernel(const L
   }
 }
 
-template <typename S, bool kVec, int kPer>
+template <typename S, int kRun, int kPer>
 void launch_rows(const LogprobArgs &a, hipStream_t stream) {
   const size_t lists = a.alternatives > 0 ? 4 * 64 * kPer * sizeof(uint64_t) : 0;
-  hipLaunchKernelGGL((row_kernel<S, kVec, kPer>), dim3(ceil_div(a.rows, 4)), dim3(256),
+  hipLaunchKernelGGL((row_kernel<S, kRun, kPer>), dim3(ceil_div(a.rows, 4)), dim3(256),
                      static_cast<unsigned>(lists), stream, a);
 }
 
-template <typename S, bool kVec> void launch(const LogprobArgs &a, hipStream_t stream) {
+template <typename S> void launch(const LogprobArgs &a, hipStream_t stream) {
+  constexpr int kRun = 16 / static_cast<int>(sizeof(S));
+  if (a.vocab < kRun)
+    return launch_rows<S, 1, 8>(a, stream);
   if (a.vocab <= 512)
-    return launch_rows<S, kVec, 8>(a, stream);
+    return launch_rows<S, kRun, 8>(a, stream);
   if (a.vocab <= 1024)
-    return launch_rows<S, kVec, 16>(a, stream);
+    return launch_rows<S, kRun, 16>(a, stream);
   if (a.vocab <= kSegment)
-    return launch_rows<S, kVec, 32>(a, stream);
+    return launch_rows<S, kRun, 32>(a, stream);
   const size_t waves = static_cast<size_t>(a.rows) * a.segments;
-  hipLaunchKernelGGL((segment_kernel<S, kVec>), dim3(ceil_div(waves, 4)), dim3(256), 0, stream,
-                     a);
+  hipLaunchKernelGGL(segment_kernel<S>, dim3(ceil_div(waves, 4)), dim3(256), 0, stream, a);
   hipLaunchKernelGGL(join_kernel<S>, dim3(a.rows), dim3(256), 0, stream, a);
-}
-
-template <typename S>
-void launch_type(const LogprobArgs &a, bool vector, hipStream_t stream) {
-  if (vector)
-    launch<S, true>(a, stream);
-  else
-    launch<S, false>(a, stream);
 }
 
 constexpr size_t kMostRows = size_t{1} << 20;
@@ -568,14 +603,12 @@ Status token_logprobs(int dtype, const void *logits, size_t rows, size_t vocab, 
                          static_cast<int>(segments), row_stride, tokens, logprob, rank, entropy,
                          static_cast<int>(alternatives), top_tokens, top_logprobs, stats,
                          need > 0 ? reinterpret_cast<float *>(stats + rows * segments) : nullptr};
-  const bool vector = reinterpret_cast<uintptr_t>(logits) % 16 == 0 &&
-                      row_stride * size % 16 == 0 && vocab * size >= 16;
   if (dtype == kElementF32)
-    launch_type<float>(args, vector, stream);
+    launch<float>(args, stream);
   else if (dtype == kElementBF16)
-    launch_type<__bf16>(args, vector, stream);
+    launch<__bf16>(args, stream);
   else
-    launch_type<_Float16>(args, vector, stream);
+    launch<_Float16>(args, stream);
   return launch_status("token_logprobs kernels");
 }
 
