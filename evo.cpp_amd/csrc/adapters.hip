@@ -23,7 +23,8 @@ namespace evo::hip {
 namespace {
 
 constexpr int kTileRows = 64, kGroupThreads = 1024;
-constexpr int kFewRows = 16;  // up to these are not sorted
+constexpr int kSingleRows = 16;  // up to these, each row is a tile of its own
+constexpr int kFewRows = 512;    // up to these are sorted by each block of down_kernel
 
 struct Tile {
   int adapter, first, count;  // rows order[first ..]; adapter -1: rows without one
@@ -41,11 +42,11 @@ struct AdapterArgs {
   int tiles;    // at most
   int parts;    // of the width, in down_kernel
   int chunk;    // output columns of a block, in up_kernel
-  int sorted;   // by group_kernel; else a tile is a row
+  int sorted;   // by group_kernel
   int halves;   // 32s of rows in a tile at most
   int wide;     // tiles of more than 16 rows go through LDS in up_kernel
   int32_t *bin;    // [rows], the adapter of each as it was read; the pool's size: none
-  int32_t *order;  // [rows], sorted by it
+  int32_t *order;  // rows sorted by it; kTileRows for each tile, where down_kernel sorts
   Tile *tile;      // [tiles], count 0 behind the last
   float *inner;    // [parts][rows][rank]
 };
@@ -161,19 +162,76 @@ struct TileRows {
   Tile tile;
   int list[kTileRows];
 };
-// Few rows are not sorted: each is a tile.
 __device__ inline void find_tile(const AdapterArgs &a, int index, TileRows &s) {
-  if (a.sorted) {
-    const Tile tile = a.tile[index];
-    if (static_cast<int>(threadIdx.x) < tile.count)
-      s.list[threadIdx.x] = a.order[tile.first + threadIdx.x];
-    if (threadIdx.x == 0)
-      s.tile = tile;
-  } else if (threadIdx.x == 0) {
-    const int adapter = checked_adapter(a, index);
-    s.tile = {adapter < a.pool.adapters ? adapter : -1, index, 1};
-    s.list[0] = index;
+  const Tile tile = a.tile[index];
+  if (static_cast<int>(threadIdx.x) < tile.count)
+    s.list[threadIdx.x] = a.order[tile.first + threadIdx.x];
+  if (threadIdx.x == 0)
+    s.tile = tile;
+  __syncthreads();
+}
+
+// Up to 512 rows are sorted by each block of down_kernel for itself, which costs it 1 to 2
+// us, a launch for it 4 to 5: a wave votes on each bit of its rows' adapters, so that a row
+// finds all others of its adapter, and its place among them, in a few words. Rows in front
+// of which the number of those is a multiple of 64 begin a tile, in row order.
+constexpr int kDownWaves = 8;
+struct Votes {
+  // 64 rows a word: bit b of their adapters, and which begin a tile.
+  uint64_t bit[14][kDownWaves], leader[kDownWaves];
+};
+static_assert(kMostAdapters < 1 << 14, "adapters and none in 14 bits");
+__device__ inline void sort_tile(const AdapterArgs &a, int index, Votes &votes, TileRows &s) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int words = (a.rows + 63) / 64, bits = 32 - __builtin_clz(a.pool.adapters);
+  const int row = threadIdx.x;
+  const uint64_t below = (uint64_t{1} << lane) - 1;
+  const int own = row < a.rows ? checked_adapter(a, row) : -1;
+  if (wave < words) {
+#pragma unroll 1
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t vote = __ballot(own >> b & 1);
+      if (lane == 0)
+        votes.bit[b][wave] = vote;
+    }
   }
+  if (threadIdx.x == 0)
+    s.tile = {-1, 0, 0};
+  __syncthreads();
+  int before = 0, all = 0;
+  if (wave < words) {
+#pragma unroll 1
+    for (int w = 0; w < words; ++w) {
+      uint64_t same = 64 * w + 64 <= a.rows ? ~uint64_t{0} : (uint64_t{1} << (a.rows & 63)) - 1;
+#pragma unroll 1
+      for (int b = 0; b < bits; ++b) {
+        const uint64_t vote = votes.bit[b][w];
+        same &= (own >> b & 1) != 0 ? vote : ~vote;
+      }
+      all += __popcll(same);
+      before += __popcll(w < wave ? same : w == wave ? same & below : 0);
+    }
+    const uint64_t leads = __ballot(own >= 0 && before % kTileRows == 0);
+    if (lane == 0)
+      votes.leader[wave] = leads;
+  }
+  __syncthreads();
+  if (own >= 0 && before % kTileRows == 0) {
+    int place = __popcll(votes.leader[wave] & below);
+    for (int w = 0; w < wave; ++w)
+      place += __popcll(votes.leader[w]);
+    if (place == index)
+      s.tile = {own, before, min(all - before, kTileRows)};
+  }
+  __syncthreads();
+  const Tile tile = s.tile;
+  const int place = before - tile.first;
+  if (own >= 0 && own == tile.adapter && place >= 0 && place < tile.count)
+    s.list[place] = row;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    s.tile = {tile.adapter < a.pool.adapters ? tile.adapter : -1, index * kTileRows, tile.count};
   __syncthreads();
 }
 
@@ -190,7 +248,6 @@ __device__ inline bf16x8 load8(const uint16_t *from) {
 // lanes read 64 bytes of one row instead, and the wave turns them in LDS: lane l holds piece
 // (l % 4) ^ (l / 8 % 4) of row l / 4 (so turned, neither side meets bank conflicts), and
 // takes row l % 16, piece l / 16. Its sums are row l % 16, ranks 4 (l / 16) + i.
-constexpr int kDownWaves = 8;
 template <int kRanks, int kCols, bool kLow>
 __device__ inline void down_tile(const AdapterArgs &a, const TileRows &rows, int set, int part,
                                  f32x4 *shared) {
@@ -300,10 +357,31 @@ template <int kRanks, bool kLow>
 __global__ __launch_bounds__(64 * kDownWaves) void down_kernel(const AdapterArgs a) {
   extern __shared__ f32x4 down_shared[];
   __shared__ TileRows rows;
+  __shared__ Votes votes;
   const unsigned block = blockIdx.x / a.parts;
   const int part = static_cast<int>(blockIdx.x % a.parts);
-  find_tile(a, static_cast<int>(block / a.halves), rows);
+  const int index = static_cast<int>(block / a.halves);
   const int set = 2 * static_cast<int>(block % a.halves);
+  if (a.sorted) {
+    find_tile(a, index, rows);
+  } else {
+    if (a.rows <= kSingleRows) {
+      if (threadIdx.x == 0) {
+        const int adapter = checked_adapter(a, index);
+        rows.tile = {adapter < a.pool.adapters ? adapter : -1, index * kTileRows, 1};
+        rows.list[0] = index;
+      }
+      __syncthreads();
+    } else {
+      sort_tile(a, index, votes, rows);
+    }
+    if (part == 0 && set == 0) {  // for up_kernel
+      if (static_cast<int>(threadIdx.x) < rows.tile.count)
+        a.order[rows.tile.first + threadIdx.x] = rows.list[threadIdx.x];
+      if (threadIdx.x == 0)
+        a.tile[index] = rows.tile;
+    }
+  }
   if (rows.tile.adapter < 0 || 16 * set >= rows.tile.count)
     return;
   if (rows.tile.count - 16 * set <= 16)
@@ -491,19 +569,16 @@ __device__ inline void up_rows(const AdapterArgs &a, const TileRows &rows, int s
           out[i] = v[i];
     }
   };
-  for (; n0 + (kAhead - 1) * stride < last; n0 += kAhead * stride) {
+  for (; n0 < last; n0 += kAhead * stride) {
     Columns x[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
-      load(n0 + u * stride, x[u]);
+      if (n0 + u * stride < last)
+        load(n0 + u * stride, x[u]);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
-      finish(n0 + u * stride, x[u]);
-  }
-  for (; n0 < last; n0 += stride) {
-    Columns x;
-    load(n0, x);
-    finish(n0, x);
+      if (n0 + u * stride < last)
+        finish(n0 + u * stride, x[u]);
   }
 }
 
@@ -527,8 +602,6 @@ __device__ inline void up_wide(const AdapterArgs &a, const TileRows &list, int b
   const int width = a.pool.out_width, rank = rank_of(a.pool, tile.adapter);
   const uint16_t *up = a.pool.up + tile.adapter * a.pool.up_stride;
   const int row = list.list[min(16 * wave + col, tile.count - 1)];
-  const Inner<kSteps> inner(a, tile.adapter, rank, row);
-  const RankMask<kSteps> mask(rank);
   const int rows = min(16, tile.count - 16 * wave);  // (0 and below: none)
   // Two rows of 32 lanes at a time.
   size_t at[8];
@@ -547,6 +620,8 @@ __device__ inline void up_wide(const AdapterArgs &a, const TileRows &list, int b
     }
   };
   request(begin);
+  const Inner<kSteps> inner(a, tile.adapter, rank, row);
+  const RankMask<kSteps> mask(rank);
   for (int n0 = begin; n0 < last; n0 += kWide) {
     __syncthreads();  // the last weights have been read
 #pragma unroll
@@ -622,7 +697,7 @@ __global__ __launch_bounds__(256) void up_kernel(const AdapterArgs a) {
 // ---------------------------------------------------------------------- host
 // Tiles at most: each bin's last tile may be short.
 size_t most_tiles(const AdapterPool &pool, size_t rows) {
-  if (rows <= kFewRows)
+  if (rows <= kSingleRows)
     return rows;
   return std::min(rows, rows / kTileRows + std::min<size_t>(rows, pool.adapters + size_t{1}));
 }
@@ -643,6 +718,9 @@ size_t chunk_of(const AdapterPool &pool, size_t rows, bool wide) {
   const size_t unit = wide ? kWide : 64, blocks = wide ? (pool.rank <= 64 ? 768 : 512) : 2048;
   const size_t chunks = std::max<size_t>(1, std::min<size_t>(ceil_div(width, unit), blocks / tiles));
   return ceil_div(ceil_div(width, chunks), unit) * unit;
+}
+size_t order_of(const AdapterPool &pool, size_t rows) {
+  return rows <= kFewRows ? most_tiles(pool, rows) * kTileRows : rows;
 }
 size_t aligned(size_t bytes) { return (bytes + 15) / 16 * 16; }
 
@@ -683,7 +761,8 @@ Status invalid(const char *why) { return {ErrorCode::kInvalidArgument, why}; }
 }  // namespace
 
 size_t adapter_workspace_bytes(const AdapterPool &pool, size_t rows) {
-  return 2 * aligned(rows * sizeof(int32_t)) + aligned(most_tiles(pool, rows) * sizeof(Tile)) +
+  return aligned(rows * sizeof(int32_t)) + aligned(order_of(pool, rows) * sizeof(int32_t)) +
+         aligned(most_tiles(pool, rows) * sizeof(Tile)) +
          parts_of(pool, rows) * rows * pool.rank * sizeof(float);
 }
 
@@ -713,7 +792,7 @@ Status adapter_linear(const AdapterPool &pool, const int32_t *adapter, const uin
     return invalid("adapter_linear: grid too large");
   char *const base = static_cast<char *>(workspace);
   const size_t list = aligned(rows * sizeof(int32_t));
-  char *const after = base + 2 * list;
+  char *const after = base + list + aligned(order_of(pool, rows) * sizeof(int32_t));
   const bool vector =
       (reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(residual)) % 16 == 0 &&
       out_stride % 4 == 0 && width % 4 == 0;
