@@ -658,7 +658,8 @@ __device__ inline void up_wide(const AdapterArgs &a, const TileRows &list, int b
       const int t = 2 * i + (lane >> 5);
       const f32x4 v = *reinterpret_cast<const f32x4 *>(&shared.product[16 * wave + t][quad]);
       if (t < rows && n < last)
-        *reinterpret_cast<f32x4 *>(a.out + at[i] + n) = base[i] + v;
+        __builtin_nontemporal_store(base[i] + v,
+                                    reinterpret_cast<f32x4 *>(a.out + at[i] + n));
     }
     wave_sync();
   }
@@ -715,7 +716,7 @@ bool wide_tiles(const AdapterPool &pool, size_t rows) {
 // Output columns of a block.
 size_t chunk_of(const AdapterPool &pool, size_t rows, bool wide) {
   const size_t width = static_cast<size_t>(pool.out_width), tiles = most_tiles(pool, rows);
-  const size_t unit = wide ? kWide : 64, blocks = wide ? (pool.rank <= 64 ? 768 : 512) : 2048;
+  const size_t unit = wide ? kWide : 64, blocks = wide ? 512 : 2048;
   const size_t chunks = std::max<size_t>(1, std::min<size_t>(ceil_div(width, unit), blocks / tiles));
   return ceil_div(ceil_div(width, chunks), unit) * unit;
 }
