@@ -28,6 +28,7 @@ constexpr int kFewRows = 512;    // up to these are sorted by each block of down
 
 struct Tile {
   int adapter, first, count;  // rows order[first ..]; adapter -1: rows without one
+  int parts;                  // that its inner values come in
 };
 
 struct AdapterArgs {
@@ -40,13 +41,14 @@ struct AdapterArgs {
   float *out;
   size_t out_stride;
   int tiles;    // at most
-  int parts;    // of the width, in down_kernel
+  int parts;    // of the width at most, in down_kernel
   int chunk;    // output columns of a block, in up_kernel
   int sorted;   // by group_kernel
   int halves;   // 32s of rows in a tile at most
   int wide;     // tiles of more than 16 rows go through LDS in up_kernel
   int32_t *bin;    // [rows], the adapter of each as it was read; the pool's size: none
   int32_t *order;  // rows sorted by it; kTileRows for each tile, where down_kernel sorts
+  int places;      // in order
   Tile *tile;      // [tiles], count 0 behind the last
   float *inner;    // [parts][rows][rank]
 };
@@ -135,11 +137,11 @@ __global__ __launch_bounds__(kGroupThreads) void group_kernel(const AdapterArgs 
     const int n = bins[i];
     bins[i] = at;
     for (int j = 0; j < n; j += kTileRows)
-      a.tile[tile++] = {i < a.pool.adapters ? i : -1, at + j, min(n - j, kTileRows)};
+      a.tile[tile++] = {i < a.pool.adapters ? i : -1, at + j, min(n - j, kTileRows), a.parts};
     at += n;
   }
   for (int i = all + threadIdx.x; i < a.tiles; i += threads)
-    a.tile[i] = {-1, 0, 0};
+    a.tile[i] = {-1, 0, 0, 0};
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < kKept; ++j)
@@ -150,9 +152,9 @@ __global__ __launch_bounds__(kGroupThreads) void group_kernel(const AdapterArgs 
     }
   for (int first = kKept * threads; first < a.rows; first += threads) {
     const int row = first + threadIdx.x;
-    const int bin = row < a.rows ? a.bin[row] : -1;
+    const int bin = row < a.rows ? max(0, min(a.bin[row], count - 1)) : -1;
     const int place = add(bin);
-    if (row < a.rows)
+    if (row < a.rows && place < a.rows)
       a.order[place] = row;
   }
 }
@@ -162,10 +164,16 @@ struct TileRows {
   Tile tile;
   int list[kTileRows];
 };
+// Tile `index` of the list. What stands there is bounded before it is followed: a workspace
+// that someone else writes meanwhile costs the call its values and no more.
 __device__ inline void find_tile(const AdapterArgs &a, int index, TileRows &s) {
-  const Tile tile = a.tile[index];
+  Tile tile = a.tile[index];
+  if (tile.adapter < -1 || tile.adapter >= a.pool.adapters || tile.count < 0 ||
+      tile.count > kTileRows || tile.first < 0 || tile.first > a.places - tile.count ||
+      tile.parts < 0 || tile.parts > a.parts)
+    tile = {-1, 0, 0, 0};
   if (static_cast<int>(threadIdx.x) < tile.count)
-    s.list[threadIdx.x] = a.order[tile.first + threadIdx.x];
+    s.list[threadIdx.x] = max(0, min(a.order[tile.first + threadIdx.x], a.rows - 1));
   if (threadIdx.x == 0)
     s.tile = tile;
   __syncthreads();
@@ -174,14 +182,27 @@ __device__ inline void find_tile(const AdapterArgs &a, int index, TileRows &s) {
 // Up to 512 rows are sorted by each block of down_kernel for itself, which costs it 1 to 2
 // us, a launch for it 4 to 5: a wave votes on each bit of its rows' adapters, so that a row
 // finds all others of its adapter, and its place among them, in a few words. Rows in front
-// of which the number of those is a multiple of 64 begin a tile, in row order.
+// of which the number of those is a multiple of 64 begin a tile, in row order. The number
+// of tiles says into how many parts the blocks divide the width.
 constexpr int kDownWaves = 8;
 struct Votes {
   // 64 rows a word: bit b of their adapters, and which begin a tile.
   uint64_t bit[14][kDownWaves], leader[kDownWaves];
 };
 static_assert(kMostAdapters < 1 << 14, "adapters and none in 14 bits");
-__device__ inline void sort_tile(const AdapterArgs &a, int index, Votes &votes, TileRows &s) {
+// What a block of down_kernel takes: a tile (its rows in TileRows), up to 32 of its rows
+// from 16 set, and a part of the width.
+struct DownWork {
+  int tiles, index, set, part;
+};
+__device__ inline int parts_for(const AdapterArgs &a, int tiles) {
+  return max(1, min(a.parts, static_cast<int>(gridDim.x) / max(1, tiles * a.halves)));
+}
+__device__ inline DownWork down_work(const AdapterArgs &a, int tiles, int parts) {
+  const int unit = static_cast<int>(blockIdx.x) / parts;
+  return {tiles, unit / a.halves, unit % a.halves * 2, static_cast<int>(blockIdx.x) % parts};
+}
+__device__ inline DownWork sort_tile(const AdapterArgs &a, Votes &votes, TileRows &s) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int words = (a.rows + 63) / 64, bits = 32 - __builtin_clz(a.pool.adapters);
@@ -197,7 +218,7 @@ __device__ inline void sort_tile(const AdapterArgs &a, int index, Votes &votes, 
     }
   }
   if (threadIdx.x == 0)
-    s.tile = {-1, 0, 0};
+    s.tile = {-1, 0, 0, 0};
   __syncthreads();
   int before = 0, all = 0;
   if (wave < words) {
@@ -217,22 +238,45 @@ __device__ inline void sort_tile(const AdapterArgs &a, int index, Votes &votes, 
       votes.leader[wave] = leads;
   }
   __syncthreads();
-  if (own >= 0 && before % kTileRows == 0) {
-    int place = __popcll(votes.leader[wave] & below);
-    for (int w = 0; w < wave; ++w)
-      place += __popcll(votes.leader[w]);
-    if (place == index)
-      s.tile = {own, before, min(all - before, kTileRows)};
+  int ahead = 0, tiles = 0;  // tiles of the rows before this wave's, and all
+  for (int w = 0; w < words; ++w) {
+    const int here = __popcll(votes.leader[w]);
+    ahead += w < wave ? here : 0;
+    tiles += here;
   }
+  const int parts = parts_for(a, tiles);
+  const DownWork work = down_work(a, tiles, parts);
+  if (own >= 0 && before % kTileRows == 0 &&
+      ahead + __popcll(votes.leader[wave] & below) == work.index)
+    s.tile = {own, before, min(all - before, kTileRows), parts};
   __syncthreads();
   const Tile tile = s.tile;
   const int place = before - tile.first;
   if (own >= 0 && own == tile.adapter && place >= 0 && place < tile.count)
     s.list[place] = row;
   __syncthreads();
-  if (threadIdx.x == 0)
-    s.tile = {tile.adapter < a.pool.adapters ? tile.adapter : -1, index * kTileRows, tile.count};
+  if (threadIdx.x == 0) {
+    s.tile.first = work.index * kTileRows;
+    if (tile.adapter == a.pool.adapters)
+      s.tile.adapter = -1;
+  }
   __syncthreads();
+  return work;
+}
+// Up to 16 rows: each is a tile.
+__device__ inline DownWork single_tile(const AdapterArgs &a, TileRows &s) {
+  const int parts = parts_for(a, a.rows);
+  const DownWork work = down_work(a, a.rows, parts);
+  if (threadIdx.x == 0) {
+    s.tile = {-1, 0, 0, 0};
+    if (work.index < a.rows) {
+      const int adapter = checked_adapter(a, work.index);
+      s.tile = {adapter < a.pool.adapters ? adapter : -1, work.index * kTileRows, 1, parts};
+      s.list[0] = work.index;
+    }
+  }
+  __syncthreads();
+  return work;
 }
 
 // --------------------------------------------------------------- inner values
@@ -278,7 +322,7 @@ __device__ inline void down_tile(const AdapterArgs &a, const TileRows &rows, int
     for (int c = 0; c < kCols; ++c)
       sum[r][c] = f32x4{0.0F, 0.0F, 0.0F, 0.0F};
 
-  const int steps = (width + 31) / 32, each = (steps + a.parts - 1) / a.parts;
+  const int steps = (width + 31) / 32, each = (steps + tile.parts - 1) / tile.parts;
   const int last = min(steps, (part + 1) * each);
   for (int step = part * each + wave; step < last; step += kDownWaves * kAhead) {
     bf16x8 x[kAhead][kLoads];  // weights, hi and lo planes
@@ -358,30 +402,24 @@ __global__ __launch_bounds__(64 * kDownWaves) void down_kernel(const AdapterArgs
   extern __shared__ f32x4 down_shared[];
   __shared__ TileRows rows;
   __shared__ Votes votes;
-  const unsigned block = blockIdx.x / a.parts;
-  const int part = static_cast<int>(blockIdx.x % a.parts);
-  const int index = static_cast<int>(block / a.halves);
-  const int set = 2 * static_cast<int>(block % a.halves);
+  DownWork work;
   if (a.sorted) {
-    find_tile(a, index, rows);
+    work = down_work(a, a.tiles, a.parts);
+    find_tile(a, work.index, rows);
   } else {
-    if (a.rows <= kSingleRows) {
-      if (threadIdx.x == 0) {
-        const int adapter = checked_adapter(a, index);
-        rows.tile = {adapter < a.pool.adapters ? adapter : -1, index * kTileRows, 1};
-        rows.list[0] = index;
-      }
-      __syncthreads();
-    } else {
-      sort_tile(a, index, votes, rows);
-    }
-    if (part == 0 && set == 0) {  // for up_kernel
+    work = a.rows <= kSingleRows ? single_tile(a, rows) : sort_tile(a, votes, rows);
+    // For up_kernel: this tile, and that there are none behind the last.
+    if (rows.tile.count > 0 && work.part == 0 && work.set == 0) {
       if (static_cast<int>(threadIdx.x) < rows.tile.count)
         a.order[rows.tile.first + threadIdx.x] = rows.list[threadIdx.x];
       if (threadIdx.x == 0)
-        a.tile[index] = rows.tile;
+        a.tile[work.index] = rows.tile;
     }
+    if (blockIdx.x == 0)
+      for (int i = work.tiles + static_cast<int>(threadIdx.x); i < a.tiles; i += blockDim.x)
+        a.tile[i] = {-1, 0, 0, 0};
   }
+  const int set = work.set, part = work.part;
   if (rows.tile.adapter < 0 || 16 * set >= rows.tile.count)
     return;
   if (rows.tile.count - 16 * set <= 16)
@@ -451,9 +489,9 @@ __device__ inline void copy_rows(const AdapterArgs &a, const TileRows &rows, int
 // holds row l % 16, ranks 8 (l / 16) .. of each 32-step. Zero behind the adapter's rank.
 template <int kSteps> struct Inner {
   bf16x8 plane[kSteps][3];
-  __device__ Inner(const AdapterArgs &a, int adapter, int rank, int row) {
+  __device__ Inner(const AdapterArgs &a, const Tile &tile, int rank, int row) {
     const int g = (threadIdx.x & 63) >> 4;
-    const float scale = a.pool.scales == nullptr ? 1.0F : a.pool.scales[adapter];
+    const float scale = a.pool.scales == nullptr ? 1.0F : a.pool.scales[tile.adapter];
     const size_t part_size = static_cast<size_t>(a.rows) * a.pool.rank;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
@@ -462,7 +500,7 @@ template <int kSteps> struct Inner {
           a.inner + static_cast<size_t>(row) * a.pool.rank + (k < rank ? k : 0);
       f32x4 low{0.0F, 0.0F, 0.0F, 0.0F}, high = low;
 #pragma unroll 4
-      for (int part = 0; part < a.parts; ++part) {
+      for (int part = 0; part < tile.parts; ++part) {
         low += *reinterpret_cast<const f32x4 *>(source + part * part_size);
         high += *reinterpret_cast<const f32x4 *>(source + part * part_size + 4);
       }
@@ -525,7 +563,7 @@ __device__ inline void up_rows(const AdapterArgs &a, const TileRows &rows, int s
   const bool mine = 16 * set + col < tile.count;
   const int row = rows.list[min(16 * set + col, tile.count - 1)];
   const size_t at = row * a.out_stride;
-  const Inner<kSteps> inner(a, tile.adapter, rank, row);
+  const Inner<kSteps> inner(a, tile, rank, row);
   const RankMask<kSteps> mask(rank);
   int from[kSteps];
 #pragma unroll
@@ -620,7 +658,7 @@ __device__ inline void up_wide(const AdapterArgs &a, const TileRows &list, int b
     }
   };
   request(begin);
-  const Inner<kSteps> inner(a, tile.adapter, rank, row);
+  const Inner<kSteps> inner(a, tile, rank, row);
   const RankMask<kSteps> mask(rank);
   for (int n0 = begin; n0 < last; n0 += kWide) {
     __syncthreads();  // the last weights have been read
@@ -702,11 +740,19 @@ size_t most_tiles(const AdapterPool &pool, size_t rows) {
     return rows;
   return std::min(rows, rows / kTileRows + std::min<size_t>(rows, pool.adapters + size_t{1}));
 }
-// Parts of the width: about four steps a wave, all blocks on the card at once (two a CU).
+// Blocks of down_kernel: all on the card at once (two a CU).
+size_t down_blocks(const AdapterPool &pool, size_t rows, size_t parts) {
+  const size_t units = most_tiles(pool, rows) * (rows <= 32 ? 1 : 2);
+  return rows <= kFewRows ? std::max<size_t>(units, 512) : units * parts;
+}
+// Parts of the width at most: about four steps a wave. With more rows, of which the sort's
+// launch makes an unknown number of tiles, as many as fit the card if that is its most.
 size_t parts_of(const AdapterPool &pool, size_t rows) {
   const size_t steps = (static_cast<size_t>(pool.in_width) + 31) / 32;
-  const size_t blocks = most_tiles(pool, rows) * (rows <= 32 ? 1 : 2);
-  return std::max<size_t>(1, std::min<size_t>({16, 512 / blocks, ceil_div(steps, 4 * kDownWaves)}));
+  const size_t parts = std::min<size_t>(16, ceil_div(steps, 4 * kDownWaves));
+  if (rows <= kFewRows)
+    return parts;
+  return std::max<size_t>(1, std::min(parts, 512 / (2 * most_tiles(pool, rows))));
 }
 // Whether tiles are expected to have more than 16 rows: most_tiles is about twice what
 // rows of a few adapters fill.
@@ -725,7 +771,8 @@ size_t order_of(const AdapterPool &pool, size_t rows) {
 }
 size_t aligned(size_t bytes) { return (bytes + 15) / 16 * 16; }
 
-template <int kRanks> Status launch_down(const AdapterArgs &a, hipStream_t stream) {
+template <int kRanks>
+Status launch_down(const AdapterArgs &a, size_t blocks, hipStream_t stream) {
   const auto kernel = a.lo != nullptr ? down_kernel<kRanks, true> : down_kernel<kRanks, false>;
   const int cols = a.rows <= 16 ? 1 : 2;  // 16s of rows in a block
   const int loads = kRanks + cols * (a.lo != nullptr ? 2 : 1);
@@ -735,7 +782,7 @@ template <int kRanks> Status launch_down(const AdapterArgs &a, hipStream_t strea
                                            hipFuncAttributeMaxDynamicSharedMemorySize,
                                            static_cast<int>(lds)),
                        "adapter down_kernel LDS opt-in"));
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.tiles) * a.parts * a.halves),
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)),
                      dim3(64 * kDownWaves), static_cast<unsigned>(lds), stream, a);
   return launch_status("adapter down_kernel");
 }
@@ -789,7 +836,8 @@ Status adapter_linear(const AdapterPool &pool, const int32_t *adapter, const uin
   const size_t width = static_cast<size_t>(pool.out_width), chunk = chunk_of(pool, rows, wide);
   const size_t chunks = ceil_div(width, chunk);
   constexpr size_t kMostBlocks = ((size_t{1} << 32) - 1) / 256;
-  if (tiles * parts * 4 > kMostBlocks || tiles * chunks > kMostBlocks)
+  const size_t blocks = down_blocks(pool, rows, parts);
+  if (blocks * 2 > kMostBlocks || tiles * chunks > kMostBlocks)
     return invalid("adapter_linear: grid too large");
   char *const base = static_cast<char *>(workspace);
   const size_t list = aligned(rows * sizeof(int32_t));
@@ -800,18 +848,18 @@ Status adapter_linear(const AdapterPool &pool, const int32_t *adapter, const uin
   const AdapterArgs args{pool, adapter, x_hi, x_lo, x_stride, static_cast<int>(rows), residual,
                          out, out_stride, static_cast<int>(tiles), static_cast<int>(parts),
                          static_cast<int>(chunk), rows <= kFewRows ? 0 : 1, rows <= 32 ? 1 : 2,
-                         wide ? 1 : 0,
-                         reinterpret_cast<int32_t *>(base),
-                         reinterpret_cast<int32_t *>(base + list), reinterpret_cast<Tile *>(after),
+                         wide ? 1 : 0, reinterpret_cast<int32_t *>(base),
+                         reinterpret_cast<int32_t *>(base + list),
+                         static_cast<int>(order_of(pool, rows)), reinterpret_cast<Tile *>(after),
                          reinterpret_cast<float *>(after + aligned(tiles * sizeof(Tile)))};
   if (args.sorted)
     hipLaunchKernelGGL(group_kernel, dim3(1), dim3(rows <= 1024 ? 256 : kGroupThreads),
                        static_cast<unsigned>((pool.adapters + 1) * sizeof(int32_t)), stream,
                        args);
-  EVO_TRY(pool.rank <= 16   ? launch_down<1>(args, stream)
-          : pool.rank <= 32 ? launch_down<2>(args, stream)
-          : pool.rank <= 64 ? launch_down<4>(args, stream)
-                            : launch_down<8>(args, stream));
+  EVO_TRY(pool.rank <= 16   ? launch_down<1>(args, blocks, stream)
+          : pool.rank <= 32 ? launch_down<2>(args, blocks, stream)
+          : pool.rank <= 64 ? launch_down<4>(args, blocks, stream)
+                            : launch_down<8>(args, blocks, stream));
   return pool.rank <= 32   ? launch_up<1>(args, vector, chunks, stream)
          : pool.rank <= 64 ? launch_up<2>(args, vector, chunks, stream)
                            : launch_up<4>(args, vector, chunks, stream);

@@ -437,9 +437,56 @@ template <typename S> __global__ __launch_bounds__(256) void segment_kernel(cons
     a.stats[at] = s;
 }
 
+// The k best and at most 256 of n places, n up to 4096, to `best`; returns how many. Each
+// wave has k places in its lanes' largest, if they are that many, so the highest of the
+// waves' k-th ones bounds the k-th from below. All threads of the block call it.
+__device__ inline int filter(uint64_t *list, int n, int k, uint64_t *best, int *count) {
+  __shared__ uint32_t borders[4];
+  const int lane = threadIdx.x & 63;
+  uint32_t most = 0;
+  for (int i = threadIdx.x; i < n; i += 256)
+    most = max(most, order_of(list[i]));
+  uint32_t border = 0;
+#pragma unroll 1
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t tried = border | 1U << bit;
+    const int have = __popcll(__ballot(most >= tried));
+    if (have >= k)
+      border = tried;
+    if (have == k)
+      break;
+  }
+  if (lane == 0)
+    borders[threadIdx.x >> 6] = border;
+  if (threadIdx.x == 0)
+    *count = 0;
+  __syncthreads();
+  border = max(max(borders[0], borders[1]), max(borders[2], borders[3]));
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const uint64_t own = list[i];
+    if (order_of(own) >= border) {
+      const int at = atomicAdd(count, 1);
+      if (at < 256)
+        best[at] = own;
+    }
+  }
+  __syncthreads();
+  if (*count <= 256)
+    return *count;
+  // (Many equal logits.)
+  if (threadIdx.x < 64) {
+    const int kept = keep_best(list, n, k);
+    if (lane < kept)
+      best[lane] = list[lane];
+  }
+  __syncthreads();
+  return min(n, k);
+}
+
 // A row's segments joined, and its first tokens.
 template <typename S> __global__ __launch_bounds__(256) void join_kernel(const LogprobArgs a) {
   __shared__ __attribute__((aligned(16))) uint64_t list[kMostTop * kGroup];
+  __shared__ __attribute__((aligned(16))) uint64_t fewer[256];
   __shared__ uint32_t chosen[kMostTop];
   __shared__ int count;
   __shared__ uint32_t least;
@@ -493,20 +540,18 @@ template <typename S> __global__ __launch_bounds__(256) void join_kernel(const L
 #pragma unroll 1
   for (int round = 0;; ++round) {
     __syncthreads();
-    if (n > 256) {
-      // (Few rows: many equal logits, or a very large vocabulary.)
-      if (threadIdx.x < 64)
-        keep_best(list, n, k);
-      n = k;
-      __syncthreads();
+    const uint64_t *from = list;
+    if (n > 128) {
+      from = fewer;
+      n = filter(list, n, k, fewer, &count);
     }
     const int kept = min(n, k);
-    const int own = threadIdx.x;
-    if (own < n) {
-      const uint64_t mine = list[own];
+    if (static_cast<int>(threadIdx.x) < n) {
+      const uint64_t mine = from[threadIdx.x];
       int rank = 0;
+#pragma unroll 4
       for (int i = 0; i < n; ++i)
-        rank += list[i] > mine ? 1 : 0;
+        rank += from[i] > mine ? 1 : 0;
       if (rank < kept && round == 2)
         write_top(a, row, r, rank, mine);
       if (rank < kept)

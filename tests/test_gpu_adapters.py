@@ -199,6 +199,22 @@ def test_bad_ranks_count_as_none(bad):
     check(pool, of_rows, high, low, base, out)
 
 
+@pytest.mark.parametrize("fill", [0, 1, 127, 255])
+@pytest.mark.parametrize("rows,adapters,used", [(341, 55, 1), (12, 8192, 3), (40, 300, 2),
+                                                (700, 64, 2), (512, 512, 9)])
+def test_workspace_without_initial_contents(rows, adapters, used, fill):
+    """Fewer tiles than there might be: whatever the workspace held, nothing of it is read."""
+    pool = Pool(adapters, 8, 64, 70, seed=rows)
+    ids = [i % used for i in range(rows)]
+    high, low = pool.planes(rows)
+    base, out = pool.normal(rows, 70), torch.empty(rows, 70, device=DEVICE)
+    need = N.call("evo_hip_adapter_linear_workspace_bytes", pool.struct(), rows)
+    workspace = torch.full((need,), fill, dtype=torch.uint8, device=DEVICE)
+    of_rows = pool.ints(ids)
+    adapt(pool, of_rows, high, low, base, out, workspace=workspace)
+    check(pool, of_rows, high, low, base, out)
+
+
 def test_largest_pool():
     """8192 adapters, each on its own row and some on two, beside rows without."""
     pool = Pool(8192, 8, 32, 16)
