@@ -745,11 +745,13 @@ size_t down_blocks(const AdapterPool &pool, size_t rows, size_t parts) {
   const size_t units = most_tiles(pool, rows) * (rows <= 32 ? 1 : 2);
   return rows <= kFewRows ? std::max<size_t>(units, 512) : units * parts;
 }
-// Parts of the width at most: about four steps a wave. With more rows, of which the sort's
-// launch makes an unknown number of tiles, as many as fit the card if that is its most.
+// Parts of the width at most: about four steps a wave, but no more than eight, as the second
+// product adds them up (width 11264, us with 16, 8 and 4: 143 rows of rank 80 25.1, 23.6 and
+// 26.9, 341 rows of rank 96 36.3, 32.7 and 36.7). With more rows, of which the sort's launch
+// makes an unknown number of tiles, as many as fit the card if that is its most.
 size_t parts_of(const AdapterPool &pool, size_t rows) {
   const size_t steps = (static_cast<size_t>(pool.in_width) + 31) / 32;
-  const size_t parts = std::min<size_t>(16, ceil_div(steps, 4 * kDownWaves));
+  const size_t parts = std::min<size_t>(8, ceil_div(steps, 4 * kDownWaves));
   if (rows <= kFewRows)
     return parts;
   return std::max<size_t>(1, std::min(parts, 512 / (2 * most_tiles(pool, rows))));
@@ -763,7 +765,8 @@ bool wide_tiles(const AdapterPool &pool, size_t rows) {
 size_t chunk_of(const AdapterPool &pool, size_t rows, bool wide) {
   const size_t width = static_cast<size_t>(pool.out_width), tiles = most_tiles(pool, rows);
   const size_t unit = wide ? kWide : 64, blocks = wide ? 512 : 2048;
-  const size_t chunks = std::max<size_t>(1, std::min<size_t>(ceil_div(width, unit), blocks / tiles));
+  const size_t chunks =
+      std::max<size_t>(1, std::min<size_t>(ceil_div(width, unit), blocks / tiles));
   return ceil_div(ceil_div(width, chunks), unit) * unit;
 }
 size_t order_of(const AdapterPool &pool, size_t rows) {

@@ -235,10 +235,13 @@ __device__ inline uint32_t count_before(const float (&x)[kPer], const float (&mo
 #pragma unroll
     for (int j = i; j < i + kChunk; j += L::kEach) {
       const int from = L::from(first, j, vocab);
-      if (L::kEach > 1 && __any(from <= token && token < from + L::kEach)) {
+      // (What stands in for a logit that came twice, -infinity, comes before no token.)
+      if (__any((from <= token && token < from + L::kEach) || from != L::begin(first, j))) {
 #pragma unroll
-        for (int e = 0; e < L::kEach; ++e)
-          count += __popcll(__ballot(x[j + e] >= (from + e < token ? given : above)));
+        for (int e = 0; e < L::kEach; ++e) {
+          const bool ahead = from + e < token && L::valid(first, j + e, vocab);
+          count += __popcll(__ballot(x[j + e] >= (ahead ? given : above)));
+        }
       } else {
         const float least = from < token ? given : above;
 #pragma unroll
@@ -323,6 +326,45 @@ __device__ inline void write_best(const LogprobArgs &a, int row, const Row &r,
 }
 
 // ------------------------------------------------- one wave takes a row
+// The first tokens of a row that a wave holds; list: 64 * kPer places.
+template <typename L, int kPer>
+__device__ inline void first_tokens(const LogprobArgs &a, int row, const Row &r,
+                                    const float (&x)[kPer], uint64_t *list) {
+  const int lane = threadIdx.x & 63, k = a.alternatives;
+  // The k-th largest of the lanes' largest (0: fewer lanes have one) bounds the k-th
+  // token from below.
+  uint32_t order[kPer], most = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    order[i] = L::valid(0, i, a.vocab) ? ordered(x[i]) : 0;
+    most = max(most, order[i]);
+  }
+  uint32_t border = 0;
+#pragma unroll 1
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t tried = border | 1U << bit;
+    const int count = __popcll(__ballot(most >= tried));
+    if (count >= k)
+      border = tried;
+    if (count == k)
+      break;
+  }
+  border = max(border, 1U);
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint64_t in = __ballot(order[i] >= border);
+    if (in == 0)
+      continue;
+    if (in >> lane & 1)
+      list[n + __popcll(in & ((uint64_t{1} << lane) - 1))] =
+          place(order[i], static_cast<uint32_t>(L::from(0, i, a.vocab) + i % L::kEach));
+    n += __popcll(in);
+  }
+  n = keep_best(list, n, n <= 64 ? 64 : k);
+  write_best(a, row, r, list, n);
+}
+
 template <typename S, int kRun, int kPer>
 __global__ __launch_bounds__(256) void row_kernel(const LogprobArgs a) {
   typedef Logits<S, kRun, kPer> L;
@@ -350,43 +392,8 @@ __global__ __launch_bounds__(256) void row_kernel(const LogprobArgs a) {
   const Row r(s);
   if (lane == 0)
     write_row(a, row, r, s.before, given, logit);
-  const int k = a.alternatives;
-  if (k == 0)
-    return;
-
-  // The k-th largest of the lanes' largest (0: fewer lanes have one) bounds the k-th
-  // token from below.
-  uint32_t order[kPer], most = 0;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    order[i] = L::valid(0, i, a.vocab) ? ordered(l.x[i]) : 0;
-    most = max(most, order[i]);
-  }
-  uint32_t border = 0;
-#pragma unroll 1
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t tried = border | 1U << bit;
-    const int count = __popcll(__ballot(most >= tried));
-    if (count >= k)
-      border = tried;
-    if (count == k)
-      break;
-  }
-  border = max(border, 1U);
-  uint64_t *list = lists + wave * (64 * kPer);
-  int n = 0;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const uint64_t in = __ballot(order[i] >= border);
-    if (in == 0)
-      continue;
-    if (in >> lane & 1)
-      list[n + __popcll(in & ((uint64_t{1} << lane) - 1))] =
-          place(order[i], static_cast<uint32_t>(L::from(0, i, a.vocab) + i % L::kEach));
-    n += __popcll(in);
-  }
-  n = keep_best(list, n, n <= 64 ? 64 : k);
-  write_best(a, row, r, list, n);
+  if (a.alternatives > 0)
+    first_tokens<L>(a, row, r, l.x, lists + wave * (64 * kPer));
 }
 
 // ------------------------------------------------- rows of several segments
@@ -490,7 +497,7 @@ template <typename S> __global__ __launch_bounds__(256) void join_kernel(const L
   __shared__ uint32_t chosen[kMostTop];
   __shared__ int count;
   __shared__ uint32_t least;
-  static_assert(kMostTop * kGroups <= kMostTop * kGroup, "groups of the best segments fit the list");
+  static_assert(kGroups <= kGroup, "groups of the best segments fit the list");
   const int row = blockIdx.x, lane = threadIdx.x & 63;
   const Segment *stats = a.stats + static_cast<size_t>(row) * a.segments;
   const S *logits = static_cast<const S *>(a.logits) + row * a.row_stride;

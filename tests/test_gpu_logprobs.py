@@ -129,6 +129,36 @@ def test_rows(rows, vocab):
     check(logits, tokens, 4)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("vocab", [8, 9, 64, 100, 257, 511, 512])
+def test_many_rows_of_a_small_vocabulary(vocab, kind):
+    """Ragged vocabularies and row counts, rows of equal logits, masked and invalid ones
+    among ordinary ones."""
+    rows = 1027
+    logits, tokens = inputs(rows, vocab, kind, seed=vocab, stride=vocab + 3, offset=1)
+    logits[5] = 0.0
+    logits[6, ::2] = 1.5
+    logits[700:705] = -2.0
+    logits[9, 3:] = -math.inf
+    logits[11] = torch.arange(vocab, device=DEVICE) / 64
+    logits[1026] = logits[1026].round()
+    for top in sorted({0, 1, 4, 8}):
+        check(logits, tokens, min(top, vocab))
+    bad = [2, 3, 64, 801]
+    logits[2, 1], logits[3, vocab - 1], logits[64], logits[801, 0] = (math.nan, math.inf,
+                                                                      -math.inf, -math.nan)
+    tokens[7], tokens[8] = -1, vocab
+    out = logprobs(logits, tokens, 8)
+    good = torch.ones(rows, dtype=torch.bool, device=DEVICE)
+    good[bad] = False
+    for name in ("logprob", "entropy", "top_logprobs"):
+        assert out[name][bad].isnan().all()
+    assert (out["rank"][bad] == NONE).all() and (out["top_tokens"][bad] == NONE).all()
+    assert out["logprob"][7:9].isnan().all() and (out["rank"][7:9] == NONE).all()
+    good[7:9] = False
+    check(logits[good], tokens[good], 8, {name: x[good] for name, x in out.items()})
+
+
 @pytest.mark.parametrize("vocab", [64, 512, 1500, 2048, 5000, 70000])
 def test_ties(vocab):
     """Equal logits come in the order of their index: rows of one value, of two, of few."""
@@ -164,6 +194,18 @@ def test_masked_logits(vocab):
     tokens[1] = 0
     out = check(logits, tokens, 12)
     assert out["entropy"][1] == 0 and out["logprob"][1] == -math.inf
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [9, 61, 509, 1021, 2047, 2053, 4100, 30001])
+def test_rank_of_masked_tokens(vocab, kind):
+    """Among tokens of -infinity the rank counts those in front, at a row's end too."""
+    logits, tokens = inputs(12, vocab, kind, seed=vocab)
+    for r in range(12):
+        logits[r, vocab - 1 - r % 8:] = -math.inf
+        logits[r, r % 3] = -math.inf
+        tokens[r] = vocab - 1 - r // 4
+    check(logits, tokens, 0)
 
 
 @pytest.mark.parametrize("vocab", [200, 512, 2048, 7000])
