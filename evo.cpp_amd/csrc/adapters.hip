@@ -17,6 +17,7 @@
 #include "ops.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace evo::hip {
 
@@ -457,31 +458,66 @@ __device__ inline void planes_of(const float (&v)[8], bf16x8 (&planes)[3]) {
     __builtin_memcpy(&planes[p], word[p], 16);
 }
 
+// Output widths: of whole quads, not, and below one.
+enum Width : int { kWhole, kRagged, kNarrow };
+// Four columns of an output row, 16 bytes that may start anywhere a float may.
+typedef f32x4 quad __attribute__((aligned(4)));
+// Columns n .. n + 3 of a residual row of at least 4, whatever n: loaded from inside the row.
+// `ends`: some lane's columns may pass its end, where a quad does not end.
+__device__ inline f32x4 load_quad(const float *row, int n, int width, bool ends) {
+  f32x4 v = *reinterpret_cast<const quad *>(row + min(n, width - 4));
+  if (ends && n < width && n + 4 > width) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = row[min(n + i, width - 1)];
+  }
+  return v;
+}
+template <bool kStream>
+__device__ inline void store_quad(float *row, int n, int width, bool ends, const f32x4 &v) {
+  if (n + 4 <= width) {
+    if constexpr (kStream)
+      __builtin_nontemporal_store(v, reinterpret_cast<quad *>(row + n));
+    else
+      *reinterpret_cast<quad *>(row + n) = v;
+  } else if (ends) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < width)
+        row[n + i] = v[i];
+  }
+}
+
 // Rows without an adapter: their residual, or zero.
-template <bool kVector, bool kResidual>
+template <bool kResidual>
 __device__ inline void copy_rows(const AdapterArgs &a, const TileRows &rows, int begin,
                                  int last) {
-  constexpr int kEach = kVector ? 4 : 1, kAhead = 8;
-  typedef float vector __attribute__((ext_vector_type(kEach)));
-  const int across = (last - begin) / kEach, all = rows.tile.count * across;
+  constexpr int kAhead = 8;
+  const int across = (last - begin) / 4, all = rows.tile.count * across;
   for (int first = threadIdx.x; first < all; first += 256 * kAhead) {
     size_t at[kAhead];
-    vector v[kAhead];
+    f32x4 v[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int i = min(first + 256 * u, all - 1);
-      at[u] = rows.list[i / across] * a.out_stride + begin + i % across * kEach;
+      at[u] = rows.list[i / across] * a.out_stride + begin + i % across * 4;
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      v[u] = 0.0F;
+      v[u] = f32x4{0.0F, 0.0F, 0.0F, 0.0F};
       if constexpr (kResidual)
-        v[u] = *reinterpret_cast<const vector *>(a.residual + at[u]);
+        v[u] = *reinterpret_cast<const quad *>(a.residual + at[u]);
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
       if (first + 256 * u < all)
-        *reinterpret_cast<vector *>(a.out + at[u]) = v[u];
+        *reinterpret_cast<quad *>(a.out + at[u]) = v[u];
+  }
+  // What no quad holds.
+  const int rest = (last - begin) % 4;
+  for (int i = threadIdx.x; i < rows.tile.count * rest; i += 256) {
+    const size_t at = rows.list[i / rest] * a.out_stride + last - rest + i % rest;
+    a.out[at] = kResidual ? a.residual[at] : 0.0F;
   }
 }
 
@@ -552,7 +588,7 @@ __device__ inline f32x4 up_product(const bf16x8 (&weight)[kSteps], const Inner<k
 
 // 16 rows a wave, from registers to registers, of every `stride`th 16 columns; kAhead
 // columns' operands are requested at once, by every lane from inside the tensors.
-template <int kSteps, bool kVector, bool kResidual>
+template <int kSteps, int kWidth, bool kResidual>
 __device__ inline void up_rows(const AdapterArgs &a, const TileRows &rows, int set, int n0,
                                int stride, int last) {
   const Tile &tile = rows.tile;
@@ -581,8 +617,8 @@ __device__ inline void up_rows(const AdapterArgs &a, const TileRows &rows, int s
       x.weight[s] = load8(up + column * a.pool.rank + from[s]);
     if constexpr (!kResidual) {
       x.base = f32x4{0.0F, 0.0F, 0.0F, 0.0F};
-    } else if constexpr (kVector) {
-      x.base = *reinterpret_cast<const f32x4 *>(a.residual + at + min(n + 4 * g, width - 4));
+    } else if constexpr (kWidth != kNarrow) {
+      x.base = load_quad(a.residual + at, n + 4 * g, width, kWidth == kRagged && n + 16 > width);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -596,15 +632,13 @@ __device__ inline void up_rows(const AdapterArgs &a, const TileRows &rows, int s
     const f32x4 v = up_product<kSteps>(x.weight, inner) + x.base;
     if (!mine)
       return;
-    float *out = a.out + at + n + 4 * g;
-    if constexpr (kVector) {
-      if (n + 4 * g < last)
-        *reinterpret_cast<f32x4 *>(out) = v;
+    if constexpr (kWidth != kNarrow) {
+      store_quad<false>(a.out + at, n + 4 * g, width, kWidth == kRagged, v);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (n + 4 * g + i < last)
-          out[i] = v[i];
+          a.out[at + n + 4 * g + i] = v[i];
     }
   };
   for (; n0 < last; n0 += kAhead * stride) {
@@ -630,7 +664,7 @@ template <int kSteps> struct WideShared {
   __attribute__((aligned(16))) uint16_t weight[kWide][32 * kSteps + 8];
   __attribute__((aligned(16))) float product[kTileRows][kWide + 4];
 };
-template <int kSteps, bool kResidual>
+template <int kSteps, int kWidth, bool kResidual>
 __device__ inline void up_wide(const AdapterArgs &a, const TileRows &list, int begin, int last,
                                WideShared<kSteps> &shared) {
   const Tile &tile = list.tile;
@@ -675,7 +709,7 @@ __device__ inline void up_wide(const AdapterArgs &a, const TileRows &list, int b
     for (int i = 0; i < 8; ++i) {
       base[i] = f32x4{0.0F, 0.0F, 0.0F, 0.0F};
       if constexpr (kResidual)
-        base[i] = *reinterpret_cast<const f32x4 *>(a.residual + at[i] + min(n, width - 4));
+        base[i] = load_quad(a.residual + at[i], n, width, kWidth == kRagged && n0 + kWide > width);
     }
     request(n0 + kWide);
     if (rows > 0) {
@@ -695,15 +729,14 @@ __device__ inline void up_wide(const AdapterArgs &a, const TileRows &list, int b
     for (int i = 0; i < 8; ++i) {
       const int t = 2 * i + (lane >> 5);
       const f32x4 v = *reinterpret_cast<const f32x4 *>(&shared.product[16 * wave + t][quad]);
-      if (t < rows && n < last)
-        __builtin_nontemporal_store(base[i] + v,
-                                    reinterpret_cast<f32x4 *>(a.out + at[i] + n));
+      if (t < rows)
+        store_quad<true>(a.out + at[i], n, width, kWidth == kRagged, base[i] + v);
     }
     wave_sync();
   }
 }
 
-template <int kSteps, bool kVector, bool kResidual>
+template <int kSteps, int kWidth, bool kResidual>
 __global__ __launch_bounds__(256) void up_kernel(const AdapterArgs a) {
   extern __shared__ f32x4 up_shared[];  // WideShared, if any tile goes through it
   __shared__ TileRows rows;
@@ -716,12 +749,12 @@ __global__ __launch_bounds__(256) void up_kernel(const AdapterArgs a) {
   const int last = min(a.pool.out_width, begin + a.chunk);
   if (tile.adapter < 0) {
     if (a.residual != a.out)
-      copy_rows<kVector, kResidual>(a, rows, begin, last);
+      copy_rows<kResidual>(a, rows, begin, last);
     return;
   }
-  if constexpr (kVector) {
+  if constexpr (kWidth != kNarrow) {
     if (tile.count > 16 && a.wide) {
-      up_wide<kSteps, kResidual>(a, rows, begin, last,
+      up_wide<kSteps, kWidth, kResidual>(a, rows, begin, last,
                                  *reinterpret_cast<WideShared<kSteps> *>(up_shared));
       return;
     }
@@ -729,7 +762,7 @@ __global__ __launch_bounds__(256) void up_kernel(const AdapterArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int sets = tile.count <= 16 ? 1 : tile.count <= 32 ? 2 : 4;
   if (16 * (wave % sets) < tile.count)
-    up_rows<kSteps, kVector, kResidual>(a, rows, wave % sets, begin + 16 * (wave / sets),
+    up_rows<kSteps, kWidth, kResidual>(a, rows, wave % sets, begin + 16 * (wave / sets),
                                         64 / sets, last);
 }
 
@@ -790,13 +823,17 @@ Status launch_down(const AdapterArgs &a, size_t blocks, hipStream_t stream) {
   return launch_status("adapter down_kernel");
 }
 template <int kSteps>
-Status launch_up(const AdapterArgs &a, bool vector, size_t chunks, hipStream_t stream) {
-  const bool residual = a.residual != nullptr;
-  const auto kernel = vector ? (residual ? up_kernel<kSteps, true, true>
-                                         : up_kernel<kSteps, true, false>)
-                             : (residual ? up_kernel<kSteps, false, true>
-                                         : up_kernel<kSteps, false, false>);
-  const size_t lds = vector && a.wide ? sizeof(WideShared<kSteps>) : 0;
+Status launch_up(const AdapterArgs &a, size_t chunks, hipStream_t stream) {
+  const auto choose = [&](auto width) {
+    constexpr int kWidth = decltype(width)::value;
+    return a.residual != nullptr ? up_kernel<kSteps, kWidth, true>
+                                 : up_kernel<kSteps, kWidth, false>;
+  };
+  const bool quads = a.pool.out_width >= 4;
+  const auto kernel = !quads                      ? choose(std::integral_constant<int, kNarrow>{})
+                      : a.pool.out_width % 4 == 0 ? choose(std::integral_constant<int, kWhole>{})
+                                                  : choose(std::integral_constant<int, kRagged>{});
+  const size_t lds = quads && a.wide ? sizeof(WideShared<kSteps>) : 0;
   if (lds > 64 * 1024)
     EVO_TRY(hip_status(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                            hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -845,9 +882,6 @@ Status adapter_linear(const AdapterPool &pool, const int32_t *adapter, const uin
   char *const base = static_cast<char *>(workspace);
   const size_t list = aligned(rows * sizeof(int32_t));
   char *const after = base + list + aligned(order_of(pool, rows) * sizeof(int32_t));
-  const bool vector =
-      (reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(residual)) % 16 == 0 &&
-      out_stride % 4 == 0 && width % 4 == 0;
   const AdapterArgs args{pool, adapter, x_hi, x_lo, x_stride, static_cast<int>(rows), residual,
                          out, out_stride, static_cast<int>(tiles), static_cast<int>(parts),
                          static_cast<int>(chunk), rows <= kFewRows ? 0 : 1, rows <= 32 ? 1 : 2,
@@ -863,9 +897,9 @@ Status adapter_linear(const AdapterPool &pool, const int32_t *adapter, const uin
           : pool.rank <= 32 ? launch_down<2>(args, blocks, stream)
           : pool.rank <= 64 ? launch_down<4>(args, blocks, stream)
                             : launch_down<8>(args, blocks, stream));
-  return pool.rank <= 32   ? launch_up<1>(args, vector, chunks, stream)
-         : pool.rank <= 64 ? launch_up<2>(args, vector, chunks, stream)
-                           : launch_up<4>(args, vector, chunks, stream);
+  return pool.rank <= 32   ? launch_up<1>(args, chunks, stream)
+         : pool.rank <= 64 ? launch_up<2>(args, chunks, stream)
+                           : launch_up<4>(args, chunks, stream);
 }
 
 }  // namespace evo::hip

@@ -487,7 +487,7 @@ typedef struct evo_hip_adapters {
  *            one plane), 16-byte aligned, x_stride a multiple of 8; rows at most 2^20.
  *   residual, out  F32 [rows][out_stride], 4-byte aligned; out may be residual. Columns
  *            behind out_width are left as they are, so the columns of one projection may
- *            have adapters of their own. 16-byte aligned rows of whole 16 bytes run faster.
+ *            have adapters of their own. Whole 16 bytes of columns run faster.
  * Sums are F32; the inner values keep all of their 24 bits. An infinity or NaN in x or an
  * adapter reaches only the rows that use it. Repeated calls give the same bits.
  * The workspace (16-byte aligned, no initial contents) holds the rows' order and the inner
