@@ -185,25 +185,41 @@ __device__ inline void find_tile(const AdapterArgs &a, int index, TileRows &s) {
 // finds all others of its adapter, and its place among them, in a few words. Rows in front
 // of which the number of those is a multiple of 64 begin a tile, in row order. The number
 // of tiles says into how many parts the blocks divide the width.
-constexpr int kDownWaves = 8;
+constexpr int kDownWaves = 8, kCus = 256;
 struct Votes {
   // 64 rows a word: bit b of their adapters, and which begin a tile.
   uint64_t bit[14][kDownWaves], leader[kDownWaves];
 };
 static_assert(kMostAdapters < 1 << 14, "adapters and none in 14 bits");
 // What a block of down_kernel takes: a tile (its rows in TileRows), up to 32 of its rows
-// from 16 set, and a part of the width.
+// from 16 set, up to 16 group_ranks of its ranks and a part of the width.
 struct DownWork {
-  int tiles, index, set, part;
+  int tiles, parts, group_ranks, index, set, group, part;
 };
-__device__ inline int parts_for(const AdapterArgs &a, int tiles) {
-  return max(1, min(a.parts, static_cast<int>(gridDim.x) / max(1, tiles * a.halves)));
+// How the blocks share `tiles` tiles: as many parts of the width as there are blocks for.
+// Where that leaves half the card, 32 ranks a block rather than 64: each reads x, but half
+// as many weights one after the other (512 rows of 6 adapters of rank 64 25.1 us for 26.3,
+// 182 rows of 2 of rank 88 18.6 for 21.5; 460 rows of 16 of rank 40 and width 11264, which
+// fill the card, 35.0 for 31.7).
+__device__ inline DownWork down_work(const AdapterArgs &a, int tiles, int kernel_ranks) {
+  int ranks = kernel_ranks, groups = 1, parts = a.parts;
+  if (!a.sorted) {
+    const int all = (a.pool.rank + 15) / 16, units = max(1, tiles) * a.halves;
+    const auto divide = [&](int of_block) {
+      ranks = of_block;
+      groups = (all + ranks - 1) / ranks;
+      parts = max(1, min(a.parts, static_cast<int>(gridDim.x) / (units * groups)));
+    };
+    divide(min(kernel_ranks, 2));
+    if (kernel_ranks > 2 && units * groups * parts > kCus)
+      divide(kernel_ranks);
+  }
+  const int unit = static_cast<int>(blockIdx.x) / parts, half = unit / groups;
+  return {tiles, parts, ranks, half / a.halves, half % a.halves * 2, unit % groups,
+          static_cast<int>(blockIdx.x) % parts};
 }
-__device__ inline DownWork down_work(const AdapterArgs &a, int tiles, int parts) {
-  const int unit = static_cast<int>(blockIdx.x) / parts;
-  return {tiles, unit / a.halves, unit % a.halves * 2, static_cast<int>(blockIdx.x) % parts};
-}
-__device__ inline DownWork sort_tile(const AdapterArgs &a, Votes &votes, TileRows &s) {
+__device__ inline DownWork sort_tile(const AdapterArgs &a, int kernel_ranks, Votes &votes,
+                                     TileRows &s) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int words = (a.rows + 63) / 64, bits = 32 - __builtin_clz(a.pool.adapters);
@@ -245,11 +261,10 @@ __device__ inline DownWork sort_tile(const AdapterArgs &a, Votes &votes, TileRow
     ahead += w < wave ? here : 0;
     tiles += here;
   }
-  const int parts = parts_for(a, tiles);
-  const DownWork work = down_work(a, tiles, parts);
+  const DownWork work = down_work(a, tiles, kernel_ranks);
   if (own >= 0 && before % kTileRows == 0 &&
       ahead + __popcll(votes.leader[wave] & below) == work.index)
-    s.tile = {own, before, min(all - before, kTileRows), parts};
+    s.tile = {own, before, min(all - before, kTileRows), work.parts};
   __syncthreads();
   const Tile tile = s.tile;
   const int place = before - tile.first;
@@ -265,14 +280,14 @@ __device__ inline DownWork sort_tile(const AdapterArgs &a, Votes &votes, TileRow
   return work;
 }
 // Up to 16 rows: each is a tile.
-__device__ inline DownWork single_tile(const AdapterArgs &a, TileRows &s) {
-  const int parts = parts_for(a, a.rows);
-  const DownWork work = down_work(a, a.rows, parts);
+__device__ inline DownWork single_tile(const AdapterArgs &a, int kernel_ranks, TileRows &s) {
+  const DownWork work = down_work(a, a.rows, kernel_ranks);
   if (threadIdx.x == 0) {
     s.tile = {-1, 0, 0, 0};
     if (work.index < a.rows) {
       const int adapter = checked_adapter(a, work.index);
-      s.tile = {adapter < a.pool.adapters ? adapter : -1, work.index * kTileRows, 1, parts};
+      s.tile = {adapter < a.pool.adapters ? adapter : -1, work.index * kTileRows, 1,
+                work.parts};
       s.list[0] = work.index;
     }
   }
@@ -294,7 +309,7 @@ __device__ inline bf16x8 load8(const uint16_t *from) {
 // (l % 4) ^ (l / 8 % 4) of row l / 4 (so turned, neither side meets bank conflicts), and
 // takes row l % 16, piece l / 16. Its sums are row l % 16, ranks 4 (l / 16) + i.
 template <int kRanks, int kCols, bool kLow>
-__device__ inline void down_tile(const AdapterArgs &a, const TileRows &rows, int set, int part,
+__device__ inline void down_tile(const AdapterArgs &a, const TileRows &rows, const DownWork &work,
                                  f32x4 *shared) {
   const Tile &tile = rows.tile;
   constexpr int kLoads = kRanks + (kLow ? 2 : 1) * kCols;
@@ -303,6 +318,9 @@ __device__ inline void down_tile(const AdapterArgs &a, const TileRows &rows, int
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rank = rank_of(a.pool, tile.adapter), width = a.pool.in_width;
   const uint16_t *down = a.pool.down + tile.adapter * a.pool.down_stride;
+  const int set = work.set, part = work.part, base = 16 * kRanks * work.group;
+  if (base >= rank)
+    return;
   // Row r of a load's 16 is at LDS place 4 r + (piece ^ r / 2 % 4).
   const int owner = lane >> 2, piece = (lane & 3) ^ (lane >> 3 & 3);
   const int taken = 4 * (lane & 15) + ((lane >> 4) ^ (lane >> 1 & 3));
@@ -311,7 +329,7 @@ __device__ inline void down_tile(const AdapterArgs &a, const TileRows &rows, int
   const uint16_t *weight[kRanks];
 #pragma unroll
   for (int r = 0; r < kRanks; ++r)
-    weight[r] = down + static_cast<size_t>(16 * r + owner < rank ? 16 * r + owner : 0) * width;
+    weight[r] = down + static_cast<size_t>(base + 16 * r + owner < rank ? base + 16 * r + owner : 0) * width;
   size_t from[kCols];
 #pragma unroll
   for (int c = 0; c < kCols; ++c)
@@ -386,7 +404,7 @@ __device__ inline void down_tile(const AdapterArgs &a, const TileRows &rows, int
     for (int w = 1; w < kDownWaves; ++w)
       v += sums[w * kSums + i];
     const int t = 16 * (set + i / 64 % kCols) + i % 16;
-    const int first = 16 * (i / 64 / kCols) + 4 * (i % 64 / 16);
+    const int first = base + 16 * (i / 64 / kCols) + 4 * (i % 64 / 16);
     if (t >= tile.count || first >= a.pool.rank)
       continue;
 #pragma unroll
@@ -405,12 +423,13 @@ __global__ __launch_bounds__(64 * kDownWaves) void down_kernel(const AdapterArgs
   __shared__ Votes votes;
   DownWork work;
   if (a.sorted) {
-    work = down_work(a, a.tiles, a.parts);
+    work = down_work(a, a.tiles, kRanks);
     find_tile(a, work.index, rows);
   } else {
-    work = a.rows <= kSingleRows ? single_tile(a, rows) : sort_tile(a, votes, rows);
+    work = a.rows <= kSingleRows ? single_tile(a, kRanks, rows)
+                                 : sort_tile(a, kRanks, votes, rows);
     // For up_kernel: this tile, and that there are none behind the last.
-    if (rows.tile.count > 0 && work.part == 0 && work.set == 0) {
+    if (rows.tile.count > 0 && work.part == 0 && work.set == 0 && work.group == 0) {
       if (static_cast<int>(threadIdx.x) < rows.tile.count)
         a.order[rows.tile.first + threadIdx.x] = rows.list[threadIdx.x];
       if (threadIdx.x == 0)
@@ -420,13 +439,19 @@ __global__ __launch_bounds__(64 * kDownWaves) void down_kernel(const AdapterArgs
       for (int i = work.tiles + static_cast<int>(threadIdx.x); i < a.tiles; i += blockDim.x)
         a.tile[i] = {-1, 0, 0, 0};
   }
-  const int set = work.set, part = work.part;
-  if (rows.tile.adapter < 0 || 16 * set >= rows.tile.count)
+  const int left = rows.tile.count - 16 * work.set;
+  if (rows.tile.adapter < 0 || left <= 0)
     return;
-  if (rows.tile.count - 16 * set <= 16)
-    down_tile<kRanks, 1, kLow>(a, rows, set, part, down_shared);
+  const auto take = [&](auto ranks) {
+    if (left <= 16)
+      down_tile<decltype(ranks)::value, 1, kLow>(a, rows, work, down_shared);
+    else
+      down_tile<decltype(ranks)::value, 2, kLow>(a, rows, work, down_shared);
+  };
+  if (kRanks == 4 && work.group_ranks == 2)
+    take(std::integral_constant<int, 2>());
   else
-    down_tile<kRanks, 2, kLow>(a, rows, set, part, down_shared);
+    take(std::integral_constant<int, kRanks>());
 }
 
 // ------------------------------------------------------------------- outputs
@@ -752,18 +777,18 @@ __global__ __launch_bounds__(256) void up_kernel(const AdapterArgs a) {
       copy_rows<kResidual>(a, rows, begin, last);
     return;
   }
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if constexpr (kWidth != kNarrow) {
     if (tile.count > 16 && a.wide) {
-      up_wide<kSteps, kWidth, kResidual>(a, rows, begin, last,
-                                 *reinterpret_cast<WideShared<kSteps> *>(up_shared));
+      up_wide<kSteps, kWidth, kResidual>(
+          a, rows, begin, last, *reinterpret_cast<WideShared<kSteps> *>(up_shared));
       return;
     }
   }
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int sets = tile.count <= 16 ? 1 : tile.count <= 32 ? 2 : 4;
   if (16 * (wave % sets) < tile.count)
     up_rows<kSteps, kWidth, kResidual>(a, rows, wave % sets, begin + 16 * (wave / sets),
-                                        64 / sets, last);
+                                       64 / sets, last);
 }
 
 // ---------------------------------------------------------------------- host
@@ -773,9 +798,14 @@ size_t most_tiles(const AdapterPool &pool, size_t rows) {
     return rows;
   return std::min(rows, rows / kTileRows + std::min<size_t>(rows, pool.adapters + size_t{1}));
 }
+// 16s of ranks in a block of down_kernel at most.
+int ranks_of(const AdapterPool &pool, size_t rows) {
+  return pool.rank <= 16 ? 1 : pool.rank <= 32 ? 2 : pool.rank <= 64 || rows <= kFewRows ? 4 : 8;
+}
 // Blocks of down_kernel: all on the card at once (two a CU).
 size_t down_blocks(const AdapterPool &pool, size_t rows, size_t parts) {
-  const size_t units = most_tiles(pool, rows) * (rows <= 32 ? 1 : 2);
+  const size_t units = most_tiles(pool, rows) * (rows <= 32 ? 1 : 2) *
+                       ceil_div(pool.rank, 16 * ranks_of(pool, rows));
   return rows <= kFewRows ? std::max<size_t>(units, 512) : units * parts;
 }
 // Parts of the width at most: about four steps a wave, but no more than eight, as the second
@@ -893,10 +923,11 @@ Status adapter_linear(const AdapterPool &pool, const int32_t *adapter, const uin
     hipLaunchKernelGGL(group_kernel, dim3(1), dim3(rows <= 1024 ? 256 : kGroupThreads),
                        static_cast<unsigned>((pool.adapters + 1) * sizeof(int32_t)), stream,
                        args);
-  EVO_TRY(pool.rank <= 16   ? launch_down<1>(args, blocks, stream)
-          : pool.rank <= 32 ? launch_down<2>(args, blocks, stream)
-          : pool.rank <= 64 ? launch_down<4>(args, blocks, stream)
-                            : launch_down<8>(args, blocks, stream));
+  const int ranks = ranks_of(pool, rows);
+  EVO_TRY(ranks == 1   ? launch_down<1>(args, blocks, stream)
+          : ranks == 2 ? launch_down<2>(args, blocks, stream)
+          : ranks == 4 ? launch_down<4>(args, blocks, stream)
+                       : launch_down<8>(args, blocks, stream));
   return pool.rank <= 32   ? launch_up<1>(args, chunks, stream)
          : pool.rank <= 64 ? launch_up<2>(args, chunks, stream)
                            : launch_up<4>(args, chunks, stream);
