@@ -503,21 +503,24 @@ template <typename S> __global__ __launch_bounds__(256) void join_kernel(const L
   const S *logits = static_cast<const S *>(a.logits) + row * a.row_stride;
   const uint32_t token = a.tokens != nullptr ? a.tokens[row] : kNoToken;
   const bool given = token < static_cast<uint32_t>(a.vocab);
-  const float logit = given ? static_cast<float>(logits[token]) : 0.0F;
   const int k = a.alternatives;
 
   // Every wave joins the sums by itself.
-  Segment whole{};
-  whole.top = -INFINITY;
+  Segment whole{}, own{};
+  whole.top = own.top = -INFINITY;
+  if (lane < a.segments)
+    own = stats[lane];
   for (int i = lane; i < a.segments; i += 64) {
-    const float top = stats[i].top;
+    const float top = i < 64 ? own.top : stats[i].top;
     whole.top = larger(whole.top, top);
     if (k > 0 && threadIdx.x < 64)
       list[i] = place(ordered(top), static_cast<uint32_t>(i));
   }
+  // (After the first statistics, which would wait for the token.)
+  const float logit = given ? static_cast<float>(logits[token]) : 0.0F;
   whole.top = wave_reduce(whole.top, Most());
   for (int i = lane; i < a.segments; i += 64) {
-    const Segment s = stats[i];
+    const Segment s = i < 64 ? own : stats[i];
     whole.before += s.before;
     if (s.top == whole.top) {
       whole.equal += s.equal;
@@ -556,7 +559,7 @@ template <typename S> __global__ __launch_bounds__(256) void join_kernel(const L
     if (static_cast<int>(threadIdx.x) < n) {
       const uint64_t mine = from[threadIdx.x];
       int rank = 0;
-#pragma unroll 4
+#pragma unroll 16
       for (int i = 0; i < n; ++i)
         rank += from[i] > mine ? 1 : 0;
       if (rank < kept && round == 2)
