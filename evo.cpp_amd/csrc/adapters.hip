@@ -2,16 +2,25 @@
 // Low-rank adapters of many requests beside a shared product:
 //   out[t] = residual[t] + s_a U_a (D_a x[t]),  a the adapter of row t (or none).
 //
-// Rows are sorted by adapter on the device (group_kernel), so that an adapter is read
-// once for up to 64 of its rows wherever they lie. down_kernel forms the inner values
-// D_a x of such a tile for a part of the width, up_kernel adds the parts up, scales them
-// and forms a chunk of the output columns. Both take their operands from memory to
-// registers: a 16 x 16 x 32 matrix instruction wants 16 bytes of a row from each lane.
+// Rows are sorted by adapter on the device, so that an adapter is read once for up to 64
+// of its rows wherever they lie: by group_kernel, or up to 512 rows by each block of
+// down_kernel for itself. down_kernel forms the inner values D_a x of such a tile for a part
+// of the width, up_kernel adds the parts up, scales them and forms a chunk of the output
+// columns. Two launches, as the second product needs all of the width.
 // x comes as the planes hi (+ lo) of a split-BF16 activation, whose products with BF16
 // weights are exact in F32. The inner values are F32, and stay so in the second product:
-// each is cut into three BF16 planes, 8 bits each, which hold all of its 24.
+// each is cut into three BF16 planes, 8 bits each, which hold all of its 24 (one plane
+// would round them to 2^-9, and the update with them; the two more cost matrix
+// instructions, which are not what bounds it).
 // A row's values come from its own column of each product: an infinity or NaN of one row
 // or adapter reaches no other row.
+//
+// What bounds it. Many rows: bytes, nearly all of them the residual and the outputs. 4096
+// prompt rows on 8 adapters of rank 64, width 4096 -> 12288 (481 MB): sort 7.6 us, first
+// product 23.6 (67 MB of x, 2.8 TB/s), second 81 (403 MB and weights, 5.0 TB/s, a copy's
+// rate). Few rows: the chain of launch, sort and loads that wait for each other. One row of
+// rank 16: 4.7 + 4.5 us; 96 rows of 40 adapters: 7.8 + 10.3 (30 MB, 5.9 us of a copy);
+// 512 rows of 6 adapters of rank 64, width 4096 -> 11264: 9.9 + 15.9 (62 MB, 12.2).
 #include "common.hpp"
 #include "lanes.hpp"
 #include "ops.hpp"
@@ -72,7 +81,9 @@ __device__ inline int checked_adapter(const AdapterArgs &a, int row) {
 
 // ------------------------------------------------------------ rows by adapter
 // One block sorts the rows by counting: bin a holds the rows of adapter a, the last one
-// those without. A thread's first kKept rows are requested at once and kept.
+// those without. A thread's first kKept rows are requested at once and kept. 4096 rows
+// take 7.6 us, most of it the launch, one load and the additions to bins in LDS; more
+// blocks would have to count together, which takes a launch more.
 constexpr int kKept = 8;
 __global__ __launch_bounds__(kGroupThreads) void group_kernel(const AdapterArgs a) {
   extern __shared__ int32_t bins[];
@@ -302,7 +313,7 @@ __device__ inline bf16x8 load8(const uint16_t *from) {
 
 // D (16 ranks) x X^T (16 rows) of a part of the width, for the kCols 16s of rows from `set`
 // on and kRanks 16s of ranks. Each wave takes every eighth 32-step, kAhead of them
-// requested at once; their sums meet in LDS.
+// requested at once (with more, no faster); their sums meet in LDS.
 // Loaded as the products take them, 16 neighbouring lanes would read 16 rows, which costs
 // the load unit a cycle each (64 to 85 a load measured, 4096 rows 34 us). Four neighbouring
 // lanes read 64 bytes of one row instead, and the wave turns them in LDS: lane l holds piece
@@ -329,7 +340,8 @@ __device__ inline void down_tile(const AdapterArgs &a, const TileRows &rows, con
   const uint16_t *weight[kRanks];
 #pragma unroll
   for (int r = 0; r < kRanks; ++r)
-    weight[r] = down + static_cast<size_t>(base + 16 * r + owner < rank ? base + 16 * r + owner : 0) * width;
+    weight[r] = down + static_cast<size_t>(base + 16 * r + owner < rank ? base + 16 * r + owner
+                                                                        : 0) * width;
   size_t from[kCols];
 #pragma unroll
   for (int c = 0; c < kCols; ++c)
@@ -679,7 +691,10 @@ __device__ inline void up_rows(const AdapterArgs &a, const TileRows &rows, int s
   }
 }
 
-// Tiles of more than 16 rows: a block takes 128 columns at a time, a wave 16 rows of them.
+// Tiles of more than 16 rows: a block takes 128 columns at a time, a wave 16 rows of them
+// (4096 prompt rows 141 us against 178 from registers in rows of 64 bytes, where 16
+// neighbouring lanes write 16 rows; 127 -> 116 with stores that pass the cache by, as the
+// outputs are not read here again).
 // The columns' weights pass through LDS for the four waves, the next ones on their way
 // meanwhile; so do a wave's products, which it adds to the residual in whole runs of 512
 // bytes of a row.
@@ -809,8 +824,10 @@ size_t down_blocks(const AdapterPool &pool, size_t rows, size_t parts) {
   return rows <= kFewRows ? std::max<size_t>(units, 512) : units * parts;
 }
 // Parts of the width at most: about four steps a wave, but no more than eight, as the second
-// product adds them up (width 11264, us with 16, 8 and 4: 143 rows of rank 80 25.1, 23.6 and
-// 26.9, 341 rows of rank 96 36.3, 32.7 and 36.7). With more rows, of which the sort's launch
+// product adds them up (width 11264, us with 8, 6 and 4: 220 rows of rank 40 17.8, 21.0 and
+// 22.3, 109 rows of rank 24 15.1, 16.6 and 18.2; with 16 in a former state 36.3 for 32.7, 341
+// rows of rank 96; half the steps a wave gain 1 us with 301 rows of width 1920 and lose 4
+// with 94 rows of rank 96). With more rows, of which the sort's launch
 // makes an unknown number of tiles, as many as fit the card if that is its most.
 size_t parts_of(const AdapterPool &pool, size_t rows) {
   const size_t steps = (static_cast<size_t>(pool.in_width) + 31) / 32;
@@ -820,11 +837,13 @@ size_t parts_of(const AdapterPool &pool, size_t rows) {
   return std::max<size_t>(1, std::min(parts, 512 / (2 * most_tiles(pool, rows))));
 }
 // Whether tiles are expected to have more than 16 rows: most_tiles is about twice what
-// rows of a few adapters fill.
+// rows of a few adapters fill. (Tiles of 16 rows and fewer are formed from registers: their
+// lanes write whole 64 bytes of few rows.)
 bool wide_tiles(const AdapterPool &pool, size_t rows) {
   return rows > 8 * most_tiles(pool, rows);
 }
-// Output columns of a block.
+// Output columns of a block: as many blocks as the card holds at once (two a CU with
+// their LDS, eight without), as each forms its tile's inner values again.
 size_t chunk_of(const AdapterPool &pool, size_t rows, bool wide) {
   const size_t width = static_cast<size_t>(pool.out_width), tiles = most_tiles(pool, rows);
   const size_t unit = wide ? kWide : 64, blocks = wide ? 512 : 2048;
