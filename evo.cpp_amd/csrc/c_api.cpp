@@ -1102,6 +1102,9 @@ evo::Status adapter_pool(const evo_hip_adapters *pool, size_t rows, evo::hip::Ad
   if (down_stride < down || up_stride < up || (down_stride | up_stride) % 8 != 0 ||
       (down_stride | up_stride) > (size_t{1} << 40))
     return invalid("strides of adapters must be multiples of 8 that hold their weights");
+  if ((reinterpret_cast<uintptr_t>(pool->scales) | reinterpret_cast<uintptr_t>(pool->ranks) |
+       reinterpret_cast<uintptr_t>(pool->error)) % 4 != 0)
+    return invalid("scales, ranks or error of the adapters are not 4-byte aligned");
   *out = {static_cast<int>(pool->adapters), static_cast<int>(pool->rank),
           static_cast<int>(pool->in_width), static_cast<int>(pool->out_width), pool->down, pool->up,
           down_stride, up_stride, pool->scales, pool->ranks, pool->error};

@@ -646,9 +646,13 @@ Status token_logprobs(int dtype, const void *logits, size_t rows, size_t vocab, 
     return {ErrorCode::kInvalidArgument, "token_logprobs: logits are F32, BF16 or F16"};
   const size_t size = dtype == kElementF32 ? 4 : 2;
   if (logits == nullptr || rows == 0 || rows > kMostRows || vocab == 0 || vocab > kMostRows ||
-      row_stride < vocab || reinterpret_cast<uintptr_t>(logits) % size != 0)
+      row_stride < vocab || row_stride > (size_t{1} << 40) ||
+      reinterpret_cast<uintptr_t>(logits) % size != 0)
     return {ErrorCode::kInvalidArgument,
-            "token_logprobs: rows or vocab out of range, or row_stride below vocab"};
+            "token_logprobs: rows, vocab or row_stride out of range, or misaligned logits"};
+  const auto at = [](const void *tensor) { return reinterpret_cast<uintptr_t>(tensor); };
+  if ((at(tokens) | at(logprob) | at(rank) | at(entropy) | at(top_tokens) | at(top_logprobs)) % 4)
+    return {ErrorCode::kInvalidArgument, "token_logprobs: tokens or outputs not 4-byte aligned"};
   if (tokens == nullptr && (logprob != nullptr || rank != nullptr))
     return {ErrorCode::kInvalidArgument, "token_logprobs: logprob and rank need tokens"};
   if (alternatives > kMostTop || alternatives > vocab ||

@@ -499,8 +499,8 @@ EVO_API evo_status evo_hip_adapter_linear(const evo_hip_adapters *pool, const in
                                           float *out, size_t out_stride, void *workspace,
                                           size_t workspace_bytes, void *stream);
 
-/* What rows of logits [rows][row_stride] (F32, BF16 or F16; rows and vocab at most 2^20)
- * say of given tokens. With p = softmax of a row:
+/* What rows of logits [rows][row_stride] (F32, BF16 or F16; rows and vocab at most 2^20,
+ * row_stride at most 2^40) say of given tokens. With p = softmax of a row:
  *   logprob  F32 [rows], ln p of tokens[r] (device uint32 [rows]); NaN where that is no
  *            token of the vocabulary
  *   rank     uint32 [rows], how many tokens come before it in the order of evo_sampler_sample

@@ -129,3 +129,17 @@ def test_null_pool_refused():
     with pytest.raises(N.OpError, match="null"):
         N.call("evo_hip_adapter_linear", None, A, B, C, 64, 5, None, A, 40, B, 1 << 40, None)
     assert N.call("evo_hip_adapter_linear_workspace_bytes", None, 5) == 0
+
+
+@pytest.mark.parametrize("bad", [
+    dict(stride=(1 << 40) + 1), dict(tokens=B + 2), dict(logprob=C + 1), dict(rank=C + 2),
+    dict(entropy=C + 3), dict(top_tokens=C + 2), dict(top_logprobs=C + 2)])
+def test_logprobs_strides_and_alignment_refused(bad):
+    with pytest.raises(N.OpError, match="token_logprobs"):
+        logprobs(**bad)
+
+
+@pytest.mark.parametrize("name", ["scales", "ranks", "error"])
+def test_misaligned_adapter_arrays_refused(name):
+    with pytest.raises(N.OpError, match="4-byte aligned"):
+        adapters(pool={name: A + 2})
