@@ -923,11 +923,9 @@ Status adapter_linear(const AdapterPool &pool, const int32_t *adapter, const uin
   const size_t tiles = most_tiles(pool, rows), parts = parts_of(pool, rows);
   const bool wide = wide_tiles(pool, rows);
   const size_t width = static_cast<size_t>(pool.out_width), chunk = chunk_of(pool, rows, wide);
+  // (2^20 rows are 24577 tiles at most, so both grids are far from 2^32 threads.)
   const size_t chunks = ceil_div(width, chunk);
-  constexpr size_t kMostBlocks = ((size_t{1} << 32) - 1) / 256;
   const size_t blocks = down_blocks(pool, rows, parts);
-  if (blocks * 2 > kMostBlocks || tiles * chunks > kMostBlocks)
-    return invalid("adapter_linear: grid too large");
   char *const base = static_cast<char *>(workspace);
   const size_t list = aligned(rows * sizeof(int32_t));
   char *const after = base + list + aligned(order_of(pool, rows) * sizeof(int32_t));

@@ -119,12 +119,6 @@ def test_adapter_call_refused(bad):
         adapters(**bad)
 
 
-def test_adapter_launch_beyond_32_bit_threads_refused():
-    with pytest.raises(N.OpError, match="grid too large"):
-        adapters(pool=dict(adapters=8192, out_width=1 << 24), rows=1 << 20, out_stride=1 << 24,
-                 size=1 << 62)
-
-
 def test_null_pool_refused():
     with pytest.raises(N.OpError, match="null"):
         N.call("evo_hip_adapter_linear", None, A, B, C, 64, 5, None, A, 40, B, 1 << 40, None)
