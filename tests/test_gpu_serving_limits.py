@@ -157,3 +157,18 @@ def test_captured_launches(rows, rank):
             eager = adapt(pool, of_rows[i], high, low, base, torch.empty_like(base))
             check(pool, of_rows[i], high, low, base, outs[i])
             assert torch.equal(eager, outs[i])
+
+
+@pytest.mark.parametrize("top", [33, 47, 63, 64])
+@pytest.mark.parametrize("levels", [0.02, 0.25, 1.0, 40.0])
+@pytest.mark.parametrize("vocab", [64, 65, 300, 512, 900, 2000, 4097, 9000, 70001])
+def test_long_lists_of_alternatives(vocab, levels, top):
+    """About as many alternatives as a wave has lanes, of logits with none, few and many equals
+    at the list's end."""
+    gen = torch.Generator(device=DEVICE).manual_seed(vocab + top)
+    logits = torch.randn(6, vocab, generator=gen, device=DEVICE) * 2.5
+    logits = ((logits / levels).round() * levels).to(torch.bfloat16)
+    logits[4, vocab // 3:] = -math.inf
+    logits[5, 10:] = -math.inf
+    tokens = torch.randint(0, vocab, (6,), generator=gen, device=DEVICE).to(torch.int32)
+    check_logprobs(logits, tokens, top)
