@@ -35,6 +35,7 @@ namespace {
 constexpr int kTileRows = 64, kGroupThreads = 1024;
 constexpr int kSingleRows = 16;  // up to these, each row is a tile of its own
 constexpr int kFewRows = 512;    // up to these are sorted by each block of down_kernel
+constexpr int kManyRows = 2048;  // from these on work is divided by the tiles expected
 
 struct Tile {
   int adapter, first, count;  // rows order[first ..]; adapter -1: rows without one
@@ -54,7 +55,7 @@ struct AdapterArgs {
   int parts;    // of the width at most, in down_kernel
   int chunk;    // output columns of a block, in up_kernel
   int sorted;   // by group_kernel
-  int halves;   // 32s of rows in a tile at most
+  int halves;   // blocks of down_kernel that share a tile's rows, 32 at a time
   int wide;     // tiles of more than 16 rows go through LDS in up_kernel
   int32_t *bin;    // [rows], the adapter of each as it was read; the pool's size: none
   int32_t *order;  // rows sorted by it; kTileRows for each tile, where down_kernel sorts
@@ -321,7 +322,7 @@ __device__ inline bf16x8 load8(const uint16_t *from) {
 // takes row l % 16, piece l / 16. Its sums are row l % 16, ranks 4 (l / 16) + i.
 template <int kRanks, int kCols, bool kLow>
 __device__ inline void down_tile(const AdapterArgs &a, const TileRows &rows, const DownWork &work,
-                                 f32x4 *shared) {
+                                 int set, f32x4 *shared) {
   const Tile &tile = rows.tile;
   constexpr int kLoads = kRanks + (kLow ? 2 : 1) * kCols;
   constexpr int kAhead = kLoads <= 6 ? 2 : 1;
@@ -329,7 +330,7 @@ __device__ inline void down_tile(const AdapterArgs &a, const TileRows &rows, con
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rank = rank_of(a.pool, tile.adapter), width = a.pool.in_width;
   const uint16_t *down = a.pool.down + tile.adapter * a.pool.down_stride;
-  const int set = work.set, part = work.part, base = 16 * kRanks * work.group;
+  const int part = work.part, base = 16 * kRanks * work.group;
   if (base >= rank)
     return;
   // Row r of a load's 16 is at LDS place 4 r + (piece ^ r / 2 % 4).
@@ -427,7 +428,7 @@ __device__ inline void down_tile(const AdapterArgs &a, const TileRows &rows, con
   }
 }
 
-// A block takes up to 32 rows of a tile and a part of the width.
+// A block takes up to 32 rows of a tile at a time and a part of the width.
 template <int kRanks, bool kLow>
 __global__ __launch_bounds__(64 * kDownWaves) void down_kernel(const AdapterArgs a) {
   extern __shared__ f32x4 down_shared[];
@@ -451,19 +452,22 @@ __global__ __launch_bounds__(64 * kDownWaves) void down_kernel(const AdapterArgs
       for (int i = work.tiles + static_cast<int>(threadIdx.x); i < a.tiles; i += blockDim.x)
         a.tile[i] = {-1, 0, 0, 0};
   }
-  const int left = rows.tile.count - 16 * work.set;
-  if (rows.tile.adapter < 0 || left <= 0)
+  if (rows.tile.adapter < 0)
     return;
-  const auto take = [&](auto ranks) {
-    if (left <= 16)
-      down_tile<decltype(ranks)::value, 1, kLow>(a, rows, work, down_shared);
+  const auto take = [&](auto ranks, int set) {
+    if (rows.tile.count - 16 * set <= 16)
+      down_tile<decltype(ranks)::value, 1, kLow>(a, rows, work, set, down_shared);
     else
-      down_tile<decltype(ranks)::value, 2, kLow>(a, rows, work, down_shared);
+      down_tile<decltype(ranks)::value, 2, kLow>(a, rows, work, set, down_shared);
   };
-  if (kRanks == 4 && work.group_ranks == 2)
-    take(std::integral_constant<int, 2>());
-  else
-    take(std::integral_constant<int, kRanks>());
+#pragma unroll 1
+  for (int set = work.set; 16 * set < rows.tile.count; set += 2 * a.halves) {
+    if (kRanks == 4 && work.group_ranks == 2)
+      take(std::integral_constant<int, 2>(), set);
+    else
+      take(std::integral_constant<int, kRanks>(), set);
+    __syncthreads();
+  }
 }
 
 // ------------------------------------------------------------------- outputs
@@ -813,28 +817,13 @@ size_t most_tiles(const AdapterPool &pool, size_t rows) {
     return rows;
   return std::min(rows, rows / kTileRows + std::min<size_t>(rows, pool.adapters + size_t{1}));
 }
-// 16s of ranks in a block of down_kernel at most.
-int ranks_of(const AdapterPool &pool, size_t rows) {
-  return pool.rank <= 16 ? 1 : pool.rank <= 32 ? 2 : pool.rank <= 64 || rows <= kFewRows ? 4 : 8;
-}
-// Blocks of down_kernel: all on the card at once (two a CU).
-size_t down_blocks(const AdapterPool &pool, size_t rows, size_t parts) {
-  const size_t units = most_tiles(pool, rows) * (rows <= 32 ? 1 : 2) *
-                       ceil_div(pool.rank, 16 * ranks_of(pool, rows));
-  return rows <= kFewRows ? std::max<size_t>(units, 512) : units * parts;
-}
-// Parts of the width at most: about four steps a wave, but no more than eight, as the second
-// product adds them up (width 11264, us with 8, 6 and 4: 220 rows of rank 40 17.8, 21.0 and
-// 22.3, 109 rows of rank 24 15.1, 16.6 and 18.2; with 16 in a former state 36.3 for 32.7, 341
-// rows of rank 96; half the steps a wave gain 1 us with 301 rows of width 1920 and lose 4
-// with 94 rows of rank 96). With more rows, of which the sort's launch
-// makes an unknown number of tiles, as many as fit the card if that is its most.
-size_t parts_of(const AdapterPool &pool, size_t rows) {
-  const size_t steps = (static_cast<size_t>(pool.in_width) + 31) / 32;
-  const size_t parts = std::min<size_t>(8, ceil_div(steps, 4 * kDownWaves));
-  if (rows <= kFewRows)
-    return parts;
-  return std::max<size_t>(1, std::min(parts, 512 / (2 * most_tiles(pool, rows))));
+// 32s of ranks in the second product.
+int steps_of(const AdapterPool &pool) { return pool.rank <= 32 ? 1 : pool.rank <= 64 ? 2 : 4; }
+// From kManyRows on their own tiles outweigh those that adapters add, so the tiles that there
+// usually are (the adapters' last ones half as many) say how full the card is.
+size_t usual_tiles(const AdapterPool &pool, size_t rows) {
+  return std::min(most_tiles(pool, rows),
+                  rows / kTileRows + std::min<size_t>(rows, pool.adapters + size_t{1}) / 2 + 1);
 }
 // Whether tiles are expected to have more than 16 rows: most_tiles is about twice what
 // rows of a few adapters fill. (Tiles of 16 rows and fewer are formed from registers: their
@@ -842,13 +831,65 @@ size_t parts_of(const AdapterPool &pool, size_t rows) {
 bool wide_tiles(const AdapterPool &pool, size_t rows) {
   return rows > 8 * most_tiles(pool, rows);
 }
-// Output columns of a block: as many blocks as the card holds at once (two a CU with
-// their LDS, eight without), as each forms its tile's inner values again.
+// Blocks for a tile's rows: two where many tiles have more than 32, or there are few rows.
+// (8192 rows of 8000 adapters 157 us, now 134; 1000 rows of 1000 131 and 113.)
+size_t halves_of(const AdapterPool &pool, size_t rows) {
+  return rows <= 32 || (rows > kFewRows && !wide_tiles(pool, rows)) ? 1 : 2;
+}
+// 16s of ranks in a block of down_kernel at most.
+int ranks_of(const AdapterPool &pool, size_t rows) {
+  return pool.rank <= 16 ? 1 : pool.rank <= 32 ? 2 : pool.rank <= 64 || rows <= kFewRows ? 4 : 8;
+}
+// Blocks of down_kernel: all on the card at once (two a CU).
+size_t down_blocks(const AdapterPool &pool, size_t rows, size_t parts) {
+  const size_t units = most_tiles(pool, rows) * halves_of(pool, rows) *
+                       ceil_div(pool.rank, 16 * ranks_of(pool, rows));
+  return rows <= kFewRows ? std::max<size_t>(units, 512) : units * parts;
+}
+// Parts of the width at most: about four steps a wave, but no more than eight, as the second
+// product adds them up (width 11264, us with 8, 6 and 4: 220 rows of rank 40 17.8, 21.0 and
+// 22.3, 109 rows of rank 24 15.1, 16.6 and 18.2; half the steps a wave gain 1 us with 301
+// rows of width 1920 and lose 4 with 94 rows of rank 96). The kernel takes fewer, by the
+// tiles that it finds. Behind the sort's launch they are chosen here: as many as fit the
+// card if the tiles are its most; for many rows so that the busiest CU has least to do, its
+// blocks' steps and about 8 more for each, and for a part what the second product does with it.
+size_t parts_of(const AdapterPool &pool, size_t rows) {
+  const size_t steps = (static_cast<size_t>(pool.in_width) + 31) / 32;
+  const size_t parts = std::min<size_t>(8, ceil_div(steps, 4 * kDownWaves));
+  if (rows <= kFewRows)
+    return parts;
+  const size_t halves = halves_of(pool, rows);
+  if (rows < kManyRows)
+    return std::max<size_t>(1, std::min(parts, 512 / (halves * most_tiles(pool, rows))));
+  const size_t units = usual_tiles(pool, rows) * halves;
+  size_t best = 1, least = ~size_t{0};
+  for (size_t p = 1; p <= parts; ++p) {
+    const size_t cost =
+        ceil_div(units * p, kCus) * (ceil_div(steps, p) + 8) + 4 * p * steps_of(pool);
+    if (cost < least)
+      best = p, least = cost;
+  }
+  return best;
+}
+// Output columns of a block: as many blocks as the card holds at once (two a CU with their
+// LDS, eight without), as each forms its tile's inner values again. With many rows that would
+// leave some CUs one block and others two, so there the busiest CU has least to do, in
+// quarters of 128 columns, of which inner values cost a block two for each 32 ranks (with the
+// parts above, width 4096, rank 16: 16384 rows 207 us for 261, 8192 rows 96 for 107, 4096 rows
+// of 256 adapters 67 for 83).
 size_t chunk_of(const AdapterPool &pool, size_t rows, bool wide) {
-  const size_t width = static_cast<size_t>(pool.out_width), tiles = most_tiles(pool, rows);
-  const size_t unit = wide ? kWide : 64, blocks = wide ? 512 : 2048;
-  const size_t chunks =
-      std::max<size_t>(1, std::min<size_t>(ceil_div(width, unit), blocks / tiles));
+  const size_t width = static_cast<size_t>(pool.out_width), unit = wide ? kWide : 64;
+  const size_t units = ceil_div(width, unit), fit = (wide ? 512 : 2048) / most_tiles(pool, rows);
+  size_t chunks = std::max<size_t>(1, std::min(units, fit));
+  if (wide && rows >= kManyRows) {
+    size_t least = ~size_t{0};
+    for (size_t c = 1; c <= std::min<size_t>(units, 16); ++c) {
+      const size_t cost = ceil_div(usual_tiles(pool, rows) * c, kCus) *
+                          (4 * ceil_div(units, c) + 2 * steps_of(pool));
+      if (cost < least)
+        chunks = c, least = cost;
+    }
+  }
   return ceil_div(ceil_div(width, chunks), unit) * unit;
 }
 size_t order_of(const AdapterPool &pool, size_t rows) {
@@ -931,8 +972,9 @@ Status adapter_linear(const AdapterPool &pool, const int32_t *adapter, const uin
   char *const after = base + list + aligned(order_of(pool, rows) * sizeof(int32_t));
   const AdapterArgs args{pool, adapter, x_hi, x_lo, x_stride, static_cast<int>(rows), residual,
                          out, out_stride, static_cast<int>(tiles), static_cast<int>(parts),
-                         static_cast<int>(chunk), rows <= kFewRows ? 0 : 1, rows <= 32 ? 1 : 2,
-                         wide ? 1 : 0, reinterpret_cast<int32_t *>(base),
+                         static_cast<int>(chunk), rows <= kFewRows ? 0 : 1,
+                         static_cast<int>(halves_of(pool, rows)), wide ? 1 : 0,
+                         reinterpret_cast<int32_t *>(base),
                          reinterpret_cast<int32_t *>(base + list),
                          static_cast<int>(order_of(pool, rows)), reinterpret_cast<Tile *>(after),
                          reinterpret_cast<float *>(after + aligned(tiles * sizeof(Tile)))};

@@ -172,3 +172,18 @@ def test_long_lists_of_alternatives(vocab, levels, top):
     logits[5, 10:] = -math.inf
     tokens = torch.randint(0, vocab, (6,), generator=gen, device=DEVICE).to(torch.int32)
     check_logprobs(logits, tokens, top)
+
+
+@pytest.mark.parametrize("rows,adapters,used", [(700, 200, 2), (700, 200, 20), (2047, 3, 3),
+                                                (2048, 3, 3), (2048, 300, 2), (5000, 40, 40),
+                                                (17000, 6, 6)])
+@pytest.mark.parametrize("rank,width,out", [(16, 2056, 1030), (72, 1032, 516)])
+def test_divisions_of_many_rows(rows, adapters, used, rank, width, out):
+    """Full tiles where short ones are expected, and each way to divide widths and columns."""
+    pool = Pool(adapters, rank, width, out, seed=rows)
+    of_rows = torch.randint(-1, used, (rows,), generator=pool.gen, device=DEVICE).to(torch.int32)
+    high, low = pool.planes(rows)
+    base = pool.normal(rows, out)
+    result = adapt(pool, of_rows, high, low, base, torch.empty_like(base))
+    assert pool.error.item() == 0
+    check(pool, of_rows, high, low, base, result)
