@@ -810,6 +810,125 @@ __global__ __launch_bounds__(256) void up_kernel(const AdapterArgs a) {
                                        64 / sets, last);
 }
 
+// ------------------------------------------------------------- little work
+// Both products of a row in one launch, which waits for nothing but the row's adapter: each
+// block forms all inner values of its row again, and some columns. A wave takes 8 ranks and
+// 512 of the width, whole runs of 1 KB; kLanes neighbouring lanes share a column, 8 ranks
+// each. The products are too small for tiles, so these are multiplications of F32.
+// One row of rank 16, width 4096 -> 12288, takes 6.6 us, two launches 8.9; 96 rows of 40
+// adapters 14.1 and 18.7. Bound by L2, from which every block reads its adapter.
+constexpr int kBothThreads = 1024, kSliceWidth = 512;
+constexpr size_t kBothWeights = size_t{1} << 17;  // values of an adapter's down at most
+constexpr int kBothUnits = static_cast<int>(kBothWeights / (8 * kSliceWidth)) + kMostRank / 8;
+template <int kLanes> __device__ inline float lanes_sum(float v) {
+  if constexpr (kLanes > 1)
+    v += dpp<0xb1, 0xf>(v, v);  // quad_perm 1 0 3 2
+  if constexpr (kLanes > 2)
+    v += dpp<0x4e, 0xf>(v, v);  // quad_perm 2 3 0 1
+  if constexpr (kLanes > 4)
+    v += dpp<0x141, 0xf>(v, v);  // row_half_mirror
+  if constexpr (kLanes > 8)
+    v += dpp<0x140, 0xf>(v, v);  // row_mirror
+  return v;
+}
+template <int kLanes, bool kLow, bool kResidual>
+__global__ __launch_bounds__(kBothThreads) void both_kernel(const AdapterArgs a) {
+  __shared__ __attribute__((aligned(16))) float partial[kBothUnits][8], inner[kMostRank];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int out_width = a.pool.out_width, width = a.pool.in_width;
+  const int chunks = (out_width + a.chunk - 1) / a.chunk;
+  const int row = static_cast<int>(blockIdx.x / chunks);
+  const int begin = static_cast<int>(blockIdx.x % chunks) * a.chunk;
+  const int last = min(out_width, begin + a.chunk);
+  const size_t at = row * a.out_stride;
+  const int adapter = checked_adapter(a, row);
+  if (adapter == a.pool.adapters) {
+    if (a.residual != a.out)
+      for (int n = begin + threadIdx.x; n < last; n += kBothThreads)
+        a.out[at + n] = kResidual ? a.residual[at + n] : 0.0F;
+    return;
+  }
+  const int rank = rank_of(a.pool, adapter);
+  const uint16_t *down = a.pool.down + adapter * a.pool.down_stride;
+  const uint16_t *up = a.pool.up + adapter * a.pool.up_stride;
+
+  // The first columns' operands are on their way with the inner values'.
+  constexpr int kColumns = kBothThreads / kLanes;
+  const int k = 8 * (threadIdx.x % kLanes);
+  int n0 = begin, n = begin + static_cast<int>(threadIdx.x) / kLanes;
+  bf16x8 weight;
+  float base = 0.0F;
+  const auto request = [&]() {
+    const size_t column = min(n, out_width - 1);
+    weight = load8(up + column * a.pool.rank + (k < a.pool.rank ? k : 0));
+    if constexpr (kResidual)
+      base = a.residual[at + column];
+  };
+  request();
+
+  const int groups = (rank + 7) / 8, units = groups * ((width + kSliceWidth - 1) / kSliceWidth);
+  for (int unit = wave; unit < units; unit += kBothThreads / 64) {
+    const int from = unit / groups * kSliceWidth + 8 * lane, first = unit % groups * 8;
+    const int where = from < width ? from : 0;
+    bf16x8 w[8], low{};
+    const bf16x8 high = load8(a.hi + row * a.x_stride + where);
+    if constexpr (kLow)
+      low = load8(a.lo + row * a.x_stride + where);
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      w[r] = load8(down + static_cast<size_t>(min(first + r, rank - 1)) * width + where);
+    asm volatile("" ::: "memory");
+    float sum[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      sum[r] = 0.0F;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float value = static_cast<float>(w[r][e]);
+        sum[r] = fmaf(value, static_cast<float>(high[e]), sum[r]);
+        if constexpr (kLow)
+          sum[r] = fmaf(value, static_cast<float>(low[e]), sum[r]);
+      }
+      sum[r] = wave_reduce(from < width ? sum[r] : 0.0F, Sum());
+    }
+    if (lane == 0) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        partial[unit][r] = sum[r];
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < kMostRank) {
+    const int r = threadIdx.x;
+    float v = 0.0F;
+    if (r < rank) {
+      for (int unit = r / 8; unit < units; unit += groups)
+        v += partial[unit][r % 8];
+      v *= a.pool.scales == nullptr ? 1.0F : a.pool.scales[adapter];
+    }
+    inner[r] = v;
+  }
+  __syncthreads();
+  float values[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    values[e] = inner[k + e];
+  for (;;) {
+    float v = 0.0F;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)  // (Behind the rank the weights may be anything.)
+      v = k + e < rank ? fmaf(static_cast<float>(weight[e]), values[e], v) : v;
+    v = lanes_sum<kLanes>(v);
+    if (k == 0 && n < last)
+      a.out[at + n] = base + v;
+    n0 += kColumns;
+    n += kColumns;
+    if (n0 >= last)
+      break;
+    request();
+  }
+}
+
 // ---------------------------------------------------------------------- host
 // Tiles at most: each bin's last tile may be short.
 size_t most_tiles(const AdapterPool &pool, size_t rows) {
@@ -897,6 +1016,31 @@ size_t order_of(const AdapterPool &pool, size_t rows) {
 }
 size_t aligned(size_t bytes) { return (bytes + 15) / 16 * 16; }
 
+// Whether both_kernel takes the call: where an adapter is read in 3 us, and all rows' work takes
+// no longer than a launch (us of both_kernel and of tiles, 4 adapters, width 4096 -> 12288: 128
+// rows of rank 16 11.6 and 14.8, 192 rows 17.7 and 15.3; 64 rows of rank 32 13.4 and 15.0, 96
+// rows 19.1 and 15.3; of one row, rank 16 of width 11264 11.6 and 10.9).
+bool both_at_once(const AdapterPool &pool, size_t rows) {
+  const size_t rank = static_cast<size_t>(pool.rank), width = static_cast<size_t>(pool.in_width);
+  return rows <= kFewRows && rank * width <= kBothWeights &&
+         rows * rank * (width + pool.out_width) <= size_t{1} << 25;
+}
+template <int kLanes> Status launch_both(AdapterArgs a, hipStream_t stream) {
+  const size_t width = static_cast<size_t>(a.pool.out_width);
+  // (Twice as many blocks than CUs take 1 to 3 us more.)
+  const size_t chunks = std::max<size_t>(1, kCus / a.rows);
+  a.chunk = static_cast<int>(ceil_div(ceil_div(width, chunks), 16) * 16);
+  const size_t blocks = a.rows * ceil_div(width, a.chunk);
+  const auto choose = [&](auto low) {
+    constexpr bool kLow = decltype(low)::value;
+    return a.residual != nullptr ? both_kernel<kLanes, kLow, true>
+                                 : both_kernel<kLanes, kLow, false>;
+  };
+  const auto kernel = a.lo != nullptr ? choose(std::true_type()) : choose(std::false_type());
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kBothThreads), 0, stream,
+                     a);
+  return launch_status("adapter both_kernel");
+}
 template <int kRanks>
 Status launch_down(const AdapterArgs &a, size_t blocks, hipStream_t stream) {
   const auto kernel = a.lo != nullptr ? down_kernel<kRanks, true> : down_kernel<kRanks, false>;
@@ -978,6 +1122,12 @@ Status adapter_linear(const AdapterPool &pool, const int32_t *adapter, const uin
                          reinterpret_cast<int32_t *>(base + list),
                          static_cast<int>(order_of(pool, rows)), reinterpret_cast<Tile *>(after),
                          reinterpret_cast<float *>(after + aligned(tiles * sizeof(Tile)))};
+  if (both_at_once(pool, rows))
+    return pool.rank <= 8    ? launch_both<1>(args, stream)
+           : pool.rank <= 16 ? launch_both<2>(args, stream)
+           : pool.rank <= 32 ? launch_both<4>(args, stream)
+           : pool.rank <= 64 ? launch_both<8>(args, stream)
+                             : launch_both<16>(args, stream);
   if (args.sorted)
     hipLaunchKernelGGL(group_kernel, dim3(1), dim3(rows <= 1024 ? 256 : kGroupThreads),
                        static_cast<unsigned>((pool.adapters + 1) * sizeof(int32_t)), stream,
