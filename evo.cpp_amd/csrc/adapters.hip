@@ -814,12 +814,16 @@ __global__ __launch_bounds__(256) void up_kernel(const AdapterArgs a) {
 // Both products of a row in one launch, which waits for nothing but the row's adapter: each
 // block forms all inner values of its row again, and some columns. A wave takes 8 ranks and
 // 512 of the width, whole runs of 1 KB; kLanes neighbouring lanes share a column, 8 ranks
-// each. The products are too small for tiles, so these are multiplications of F32.
-// One row of rank 16, width 4096 -> 12288, takes 6.6 us, two launches 8.9; 96 rows of 40
-// adapters 14.1 and 18.7. Bound by L2, from which every block reads its adapter.
+// each. One row of rank 16, width 4096 -> 12288, takes 6.6 us, two launches 8.9; 96 rows of 40
+// adapters 14.1 and 18.7. Bound by L2, from which every block reads its adapter, and up to
+// rank 32 by as many instructions; above, matrix instructions form the inner values, which cost
+// 1 us more to begin with (rank 8 6.5 and 7.8 us; rank 128, width 1920, 13.3 and 11.4).
 constexpr int kBothThreads = 1024, kSliceWidth = 512;
-constexpr size_t kBothWeights = size_t{1} << 17;  // values of an adapter's down at most
-constexpr int kBothUnits = static_cast<int>(kBothWeights / (8 * kSliceWidth)) + kMostRank / 8;
+// Values of an adapter's down that this pays for at most.
+constexpr size_t both_weights(int rank) { return rank <= 32 ? 1 << 17 : (1 << 18) - 1; }
+constexpr int kBothSums = static_cast<int>(both_weights(32) / (8 * kSliceWidth)) + 32 / 8;
+static_assert(kBothSums >= kBothThreads / 64 && kMostRank / 8 <= kBothThreads / 64,
+              "all partial sums have a place, each 8 ranks a wave");
 template <int kLanes> __device__ inline float lanes_sum(float v) {
   if constexpr (kLanes > 1)
     v += dpp<0xb1, 0xf>(v, v);  // quad_perm 1 0 3 2
@@ -833,7 +837,7 @@ template <int kLanes> __device__ inline float lanes_sum(float v) {
 }
 template <int kLanes, bool kLow, bool kResidual>
 __global__ __launch_bounds__(kBothThreads) void both_kernel(const AdapterArgs a) {
-  __shared__ __attribute__((aligned(16))) float partial[kBothUnits][8], inner[kMostRank];
+  __shared__ __attribute__((aligned(16))) float partial[kBothSums][8], inner[kMostRank];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int out_width = a.pool.out_width, width = a.pool.in_width;
   const int chunks = (out_width + a.chunk - 1) / a.chunk;
@@ -866,35 +870,83 @@ __global__ __launch_bounds__(kBothThreads) void both_kernel(const AdapterArgs a)
   };
   request();
 
-  const int groups = (rank + 7) / 8, units = groups * ((width + kSliceWidth - 1) / kSliceWidth);
-  for (int unit = wave; unit < units; unit += kBothThreads / 64) {
-    const int from = unit / groups * kSliceWidth + 8 * lane, first = unit % groups * 8;
-    const int where = from < width ? from : 0;
-    bf16x8 w[8], low{};
-    const bf16x8 high = load8(a.hi + row * a.x_stride + where);
-    if constexpr (kLow)
-      low = load8(a.lo + row * a.x_stride + where);
-#pragma unroll
-    for (int r = 0; r < 8; ++r)
-      w[r] = load8(down + static_cast<size_t>(min(first + r, rank - 1)) * width + where);
-    asm volatile("" ::: "memory");
-    float sum[8];
-#pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      sum[r] = 0.0F;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float value = static_cast<float>(w[r][e]);
-        sum[r] = fmaf(value, static_cast<float>(high[e]), sum[r]);
-        if constexpr (kLow)
-          sum[r] = fmaf(value, static_cast<float>(low[e]), sum[r]);
-      }
-      sum[r] = wave_reduce(from < width ? sum[r] : 0.0F, Sum());
-    }
-    if (lane == 0) {
+  constexpr int kWaves = kBothThreads / 64;
+  const int groups = (rank + 7) / 8;
+  int sums;  // of a group
+  if constexpr (kLanes <= 4) {
+    sums = (width + kSliceWidth - 1) / kSliceWidth;
+    for (int unit = wave; unit < groups * sums; unit += kWaves) {
+      const int from = unit / groups * kSliceWidth + 8 * lane, first = unit % groups * 8;
+      const int where = from < width ? from : 0;
+      bf16x8 w[8], low{};
+      const bf16x8 high = load8(a.hi + row * a.x_stride + where);
+      if constexpr (kLow)
+        low = load8(a.lo + row * a.x_stride + where);
 #pragma unroll
       for (int r = 0; r < 8; ++r)
-        partial[unit][r] = sum[r];
+        w[r] = load8(down + static_cast<size_t>(min(first + r, rank - 1)) * width + where);
+      asm volatile("" ::: "memory");
+      float sum[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        sum[r] = 0.0F;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float value = static_cast<float>(w[r][e]);
+          sum[r] = fmaf(value, static_cast<float>(high[e]), sum[r]);
+          if constexpr (kLow)
+            sum[r] = fmaf(value, static_cast<float>(low[e]), sum[r]);
+        }
+        sum[r] = wave_reduce(from < width ? sum[r] : 0.0F, Sum());
+      }
+      if (lane == 0) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          partial[unit][r] = sum[r];
+      }
+    }
+  } else {
+    // The same runs as both operands of a matrix product: what element i of its diagonal
+    // sums up are lanes i, i + 16, .. of both. A wave takes every `sums`th slice.
+    sums = max(1, kWaves / max(1, groups));
+    if (wave < groups * sums) {
+      const int first = wave % groups * 8;
+      f32x4 sum[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        sum[r] = f32x4{0.0F, 0.0F, 0.0F, 0.0F};
+      for (int slice = wave / groups * kSliceWidth; slice < width; slice += sums * kSliceWidth) {
+        const int from = slice + 8 * lane, where = from < width ? from : 0;
+        bf16x8 w[8], low{}, high = load8(a.hi + row * a.x_stride + where);
+        if constexpr (kLow)
+          low = load8(a.lo + row * a.x_stride + where);
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          w[r] = load8(down + static_cast<size_t>(min(first + r, rank - 1)) * width + where);
+        asm volatile("" ::: "memory");
+        if (slice + kSliceWidth > width && from >= width) {
+          high = low = bf16x8{};
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            w[r] = bf16x8{};
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          sum[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[r], high, sum[r], 0, 0, 0);
+          if constexpr (kLow)
+            sum[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[r], low, sum[r], 0, 0, 0);
+        }
+      }
+      const bool diagonal = lane >> 4 == (lane & 15) >> 2;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const float even = (lane & 2) != 0 ? sum[r][2] : sum[r][0];
+        const float odd = (lane & 2) != 0 ? sum[r][3] : sum[r][1];
+        const float own = (lane & 1) != 0 ? odd : even;
+        const float all = wave_reduce(diagonal ? own : 0.0F, Sum());
+        if (lane == 0)
+          partial[wave][r] = all;
+      }
     }
   }
   __syncthreads();
@@ -902,8 +954,8 @@ __global__ __launch_bounds__(kBothThreads) void both_kernel(const AdapterArgs a)
     const int r = threadIdx.x;
     float v = 0.0F;
     if (r < rank) {
-      for (int unit = r / 8; unit < units; unit += groups)
-        v += partial[unit][r % 8];
+      for (int i = 0; i < sums; ++i)
+        v += partial[i * groups + r / 8][r % 8];
       v *= a.pool.scales == nullptr ? 1.0F : a.pool.scales[adapter];
     }
     inner[r] = v;
@@ -1017,12 +1069,13 @@ size_t order_of(const AdapterPool &pool, size_t rows) {
 size_t aligned(size_t bytes) { return (bytes + 15) / 16 * 16; }
 
 // Whether both_kernel takes the call: where an adapter is read in 3 us, and all rows' work takes
-// no longer than a launch (us of both_kernel and of tiles, 4 adapters, width 4096 -> 12288: 128
-// rows of rank 16 11.6 and 14.8, 192 rows 17.7 and 15.3; 64 rows of rank 32 13.4 and 15.0, 96
-// rows 19.1 and 15.3; of one row, rank 16 of width 11264 11.6 and 10.9).
+// no longer than a launch. us of both_kernel and of tiles: width 4096 -> 12288, 128 rows of
+// rank 16 11.6 and 14.8, 192 rows 17.7 and 15.3; 64 rows of rank 32 13.4 and 15.0, 96 rows
+// 19.1 and 15.3; 16 rows of rank 48 13.0 and 17.5; one row of rank 64 12.4 and 11.3, of rank 32
+// and width 11264 13.9 and 11.2; width 1920 -> 5760, 32 rows of rank 128 18.6 and 20.3.
 bool both_at_once(const AdapterPool &pool, size_t rows) {
   const size_t rank = static_cast<size_t>(pool.rank), width = static_cast<size_t>(pool.in_width);
-  return rows <= kFewRows && rank * width <= kBothWeights &&
+  return rows <= kFewRows && rank * width <= both_weights(pool.rank) &&
          rows * rank * (width + pool.out_width) <= size_t{1} << 25;
 }
 template <int kLanes> Status launch_both(AdapterArgs a, hipStream_t stream) {

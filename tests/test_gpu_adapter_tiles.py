@@ -11,7 +11,7 @@ from adapter_util import Pool, adapt, check
 from paged_util import DEVICE
 
 pytestmark = pytest.mark.gpu
-SHAPES = [(16, 8200, 130), (24, 5464, 97), (72, 2056, 260), (128, 1032, 66)]
+SHAPES = [(16, 8200, 130), (24, 5464, 97), (72, 3648, 260), (128, 2048, 66)]
 
 
 def picks(rows, adapters, seed=0, runs=False):
@@ -108,7 +108,7 @@ def test_workspace_without_initial_contents(rows, adapters, used, fill):
 @pytest.mark.parametrize("rows", [7, 150])
 def test_order_in_place_and_captured(rows):
     """The same bits again, in another order of the rows, in place, and from a graph."""
-    pool = Pool(4, 72, 2056, 300)
+    pool = Pool(4, 72, 3648, 300)
     of_rows, high, low, base, out = run(pool, picks(rows, 4))
     turn = torch.randperm(rows, generator=torch.Generator().manual_seed(1)).to(DEVICE)
     turned = adapt(pool, of_rows[turn].contiguous(), high[turn].contiguous(),
@@ -134,11 +134,14 @@ def test_order_in_place_and_captured(rows):
         assert torch.equal(eager, result)
 
 
-@pytest.mark.parametrize("rank,width", [(16, 8192), (16, 8200), (128, 1024), (128, 1032), (8, 8),
-                                        (8, 512), (8, 520), (120, 1088)])
+@pytest.mark.parametrize("rank,width", [(16, 8192), (16, 8200), (32, 4096), (32, 4104), (8, 8),
+                                        (8, 512), (8, 520), (40, 6552), (40, 6560), (64, 4088),
+                                        (64, 4096), (48, 1920), (72, 520), (120, 1088), (128, 8),
+                                        (128, 2040), (128, 2048)])
 @pytest.mark.parametrize("rows", [1, 3, 40])
 def test_border_of_weights(rank, width, rows):
-    """2^17 weights and just more or fewer; slices of the width that end in each place."""
+    """2^17 and 2^18 weights and just more or fewer; slices of the width that end in each
+    place."""
     pool = Pool(3, rank, width, 77)
     run(pool, picks(rows, 3, rows))
 
@@ -163,3 +166,22 @@ def test_column_groups(rank):
         adapt(pool, pool.ints(ids), high, low, part, part)
         check(pool, pool.ints(ids), high, low, base, part)
         assert (whole[:, :3] == 55.0).all() and (whole[:, 3 + out:] == 55.0).all()
+
+
+@pytest.mark.parametrize("rank,width", [(16, 4096), (72, 2056)])
+def test_one_launch_keeps_infinities_and_ranks_apart(rank, width):
+    """Rows of one launch: an infinity in x, NaN in an adapter, ranks of their own, rows without."""
+    pool = Pool(5, rank, width, 70, ranks=[rank, 0, 3, rank - 1, rank // 2 + 1], gap=16)
+    ids = [0, 1, 2, 3, 4, -1, 0, 3, 2, -1, 4, 4]
+    of_rows, high, low, base, out = run(pool, ids)
+    high[0, width - 1] = math.inf
+    high[3, 0] = math.nan
+    high[5, 7] = math.inf
+    high[1, 7] = math.nan
+    pool.up[4, 69, 0] = math.inf
+    spoilt = adapt(pool, of_rows, high, low, base, torch.empty_like(out))
+    same = torch.tensor([i not in (0, 3) and a != 4 for i, a in enumerate(ids)], device=DEVICE)
+    assert torch.equal(out[same], spoilt[same])
+    assert not torch.isfinite(spoilt[0]).any() and spoilt[3].isnan().all()
+    assert torch.equal(out[of_rows == 4][:, :69], spoilt[of_rows == 4][:, :69])
+    assert not torch.isfinite(spoilt[of_rows == 4][:, 69]).any()
