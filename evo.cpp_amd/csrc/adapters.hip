@@ -33,7 +33,7 @@ namespace evo::hip {
 namespace {
 
 constexpr int kTileRows = 64, kGroupThreads = 1024;
-constexpr int kSingleRows = 16;  // up to these, each row is a tile of its own
+constexpr int kSingleRows = 4;   // up to these, each row is a tile of its own
 constexpr int kFewRows = 512;    // up to these are sorted by each block of down_kernel
 constexpr int kManyRows = 2048;  // from these on work is divided by the tiles expected
 
@@ -291,7 +291,9 @@ __device__ inline DownWork sort_tile(const AdapterArgs &a, int kernel_ranks, Vot
   __syncthreads();
   return work;
 }
-// Up to 16 rows: each is a tile.
+// Up to 4 rows: each is a tile. (Rank 64, width 4096 -> 12288, us sorted and not: 4 rows of 4
+// adapters 13.6 and 12.8, 8 rows of 2 13.3 and 16.9, 16 rows of 2 13.8 and 18.8, of 16 20.3
+// and 19.3.)
 __device__ inline DownWork single_tile(const AdapterArgs &a, int kernel_ranks, TileRows &s) {
   const DownWork work = down_work(a, a.rows, kernel_ranks);
   if (threadIdx.x == 0) {
