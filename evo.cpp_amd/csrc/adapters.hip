@@ -198,6 +198,7 @@ __device__ inline void find_tile(const AdapterArgs &a, int index, TileRows &s) {
 // of which the number of those is a multiple of 64 begin a tile, in row order. The number
 // of tiles says into how many parts the blocks divide the width.
 constexpr int kDownWaves = 8, kCus = 256;
+constexpr int kUsualWidth = 32 * 4 * kDownWaves;  // of a part: four steps a wave
 struct Votes {
   // 64 rows a word: bit b of their adapters, and which begin a tile.
   uint64_t bit[14][kDownWaves], leader[kDownWaves];
@@ -208,8 +209,10 @@ static_assert(kMostAdapters < 1 << 14, "adapters and none in 14 bits");
 struct DownWork {
   int tiles, parts, group_ranks, index, set, group, part;
 };
-// How the blocks share `tiles` tiles: as many parts of the width as there are blocks for.
-// Where that leaves half the card, 32 ranks a block rather than 64: each reads x, but half
+// How the blocks share `tiles` tiles: parts of the width, about four steps a wave, or two
+// where that leaves half the card (301 rows of 9 adapters of width 1920 16.4 us for 17.5, but
+// 300 rows of 40 21.3 for 19.9).
+// And where parts leave half the card, 32 ranks a block rather than 64: each reads x, but half
 // as many weights one after the other (512 rows of 6 adapters of rank 64 25.1 us for 26.3,
 // 182 rows of 2 of rank 88 18.6 for 21.5; 460 rows of 16 of rank 40 and width 11264, which
 // fill the card, 35.0 for 31.7).
@@ -220,7 +223,9 @@ __device__ inline DownWork down_work(const AdapterArgs &a, int tiles, int kernel
     const auto divide = [&](int of_block) {
       ranks = of_block;
       groups = (all + ranks - 1) / ranks;
-      parts = max(1, min(a.parts, static_cast<int>(gridDim.x) / (units * groups)));
+      const int usual = min(a.parts, (a.pool.in_width + kUsualWidth - 1) / kUsualWidth);
+      parts = max(usual, min(a.parts, kCus / (units * groups)));
+      parts = max(1, min(parts, static_cast<int>(gridDim.x) / (units * groups)));
     };
     divide(min(kernel_ranks, 2));
     if (kernel_ranks > 2 && units * groups * parts > kCus)
@@ -1019,18 +1024,18 @@ size_t down_blocks(const AdapterPool &pool, size_t rows, size_t parts) {
                        ceil_div(pool.rank, 16 * ranks_of(pool, rows));
   return rows <= kFewRows ? std::max<size_t>(units, 512) : units * parts;
 }
-// Parts of the width at most: about four steps a wave, but no more than eight, as the second
+// Parts of the width at most: about four steps a wave (two up to rank 32, whose parts are
+// cheap to add up: 94 rows of rank 96 lose 4 us), but no more than eight, as the second
 // product adds them up (width 11264, us with 8, 6 and 4: 220 rows of rank 40 17.8, 21.0 and
-// 22.3, 109 rows of rank 24 15.1, 16.6 and 18.2; half the steps a wave gain 1 us with 301
-// rows of width 1920 and lose 4 with 94 rows of rank 96). The kernel takes fewer, by the
-// tiles that it finds. Behind the sort's launch they are chosen here: as many as fit the
+// 22.3, 109 rows of rank 24 15.1, 16.6 and 18.2). The kernel takes fewer, by the tiles that it
+// finds. Behind the sort's launch they are chosen here: as many as fit the
 // card if the tiles are its most; for many rows so that the busiest CU has least to do, its
 // blocks' steps and about 8 more for each, and for a part what the second product does with it.
 size_t parts_of(const AdapterPool &pool, size_t rows) {
   const size_t steps = (static_cast<size_t>(pool.in_width) + 31) / 32;
   const size_t parts = std::min<size_t>(8, ceil_div(steps, 4 * kDownWaves));
   if (rows <= kFewRows)
-    return parts;
+    return pool.rank <= 32 ? std::min<size_t>(8, ceil_div(steps, 2 * kDownWaves)) : parts;
   const size_t halves = halves_of(pool, rows);
   if (rows < kManyRows)
     return std::max<size_t>(1, std::min(parts, 512 / (halves * most_tiles(pool, rows))));
