@@ -3,8 +3,8 @@
 //   out[t] = residual[t] + s_a U_a (D_a x[t]),  a the adapter of row t (or none).
 //
 // Rows are sorted by adapter on the device, so that an adapter is read once for up to 64
-// of its rows wherever they lie: by group_kernel, or up to 512 rows by each block of
-// down_kernel for itself. down_kernel forms the inner values D_a x of such a tile for a part
+// of its rows wherever they lie: by group_kernel, or where they are few enough by each block
+// of down_kernel for itself. down_kernel forms the inner values D_a x of such a tile for a part
 // of the width, up_kernel adds the parts up, scales them and forms a chunk of the output
 // columns. Two launches, as the second product needs all of the width.
 // x comes as the planes hi (+ lo) of a split-BF16 activation, whose products with BF16
@@ -34,7 +34,9 @@ namespace {
 
 constexpr int kTileRows = 64, kGroupThreads = 1024;
 constexpr int kSingleRows = 4;   // up to these, each row is a tile of its own
-constexpr int kFewRows = 512;    // up to these are sorted by each block of down_kernel
+constexpr int kFewRows = 512;    // up to these the tiles found say how work is divided
+constexpr int kSelfRows = 4096;  // up to these blocks of down_kernel may sort for themselves
+constexpr int kMostSorts = 640;  // blocks that do at most
 constexpr int kManyRows = 2048;  // from these on work is divided by the tiles expected
 
 struct Tile {
@@ -192,18 +194,17 @@ __device__ inline void find_tile(const AdapterArgs &a, int index, TileRows &s) {
   __syncthreads();
 }
 
-// Up to 512 rows are sorted by each block of down_kernel for itself, which costs it 1 to 2
-// us, a launch for it 4 to 5: a wave votes on each bit of its rows' adapters, so that a row
-// finds all others of its adapter, and its place among them, in a few words. Rows in front
-// of which the number of those is a multiple of 64 begin a tile, in row order. The number
-// of tiles says into how many parts the blocks divide the width.
+// Rows are sorted by each block of down_kernel for itself where that takes it less than a
+// launch, 5 to 8 us: it counts the adapters' rows, so the tiles of each, finds the adapter
+// of its own tile, and in row order that adapter's rows. The number of tiles says into how
+// many parts the blocks divide the width.
 constexpr int kDownWaves = 8, kCus = 256;
 constexpr int kUsualWidth = 32 * 4 * kDownWaves;  // of a part: four steps a wave
-struct Votes {
-  // 64 rows a word: bit b of their adapters, and which begin a tile.
-  uint64_t bit[14][kDownWaves], leader[kDownWaves];
+constexpr int kOwnRows = kSelfRows / (64 * kDownWaves);
+struct Counts {
+  int tiles[kDownWaves], words[kSelfRows / 64];
 };
-static_assert(kMostAdapters < 1 << 14, "adapters and none in 14 bits");
+static_assert(kSelfRows / 64 <= 64, "a wave adds up the words' counts");
 // What a block of down_kernel takes: a tile (its rows in TileRows), up to 32 of its rows
 // from 16 set, up to 16 group_ranks of its ranks and a part of the width.
 struct DownWork {
@@ -218,7 +219,7 @@ struct DownWork {
 // fill the card, 35.0 for 31.7).
 __device__ inline DownWork down_work(const AdapterArgs &a, int tiles, int kernel_ranks) {
   int ranks = kernel_ranks, groups = 1, parts = a.parts;
-  if (!a.sorted) {
+  if (a.rows <= kFewRows) {
     const int all = (a.pool.rank + 15) / 16, units = max(1, tiles) * a.halves;
     const auto divide = [&](int of_block) {
       ranks = of_block;
@@ -235,59 +236,84 @@ __device__ inline DownWork down_work(const AdapterArgs &a, int tiles, int kernel
   return {tiles, parts, ranks, half / a.halves, half % a.halves * 2, unit % groups,
           static_cast<int>(blockIdx.x) % parts};
 }
-__device__ inline DownWork sort_tile(const AdapterArgs &a, int kernel_ranks, Votes &votes,
-                                     TileRows &s) {
+__device__ inline DownWork sort_tile(const AdapterArgs &a, int kernel_ranks, Counts &counts,
+                                     int32_t *bins, TileRows &s) {
+  constexpr int kThreads = 64 * kDownWaves;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int words = (a.rows + 63) / 64, bits = 32 - __builtin_clz(a.pool.adapters);
-  const int row = threadIdx.x;
-  const uint64_t below = (uint64_t{1} << lane) - 1;
-  const int own = row < a.rows ? checked_adapter(a, row) : -1;
-  if (wave < words) {
-#pragma unroll 1
-    for (int b = 0; b < bits; ++b) {
-      const uint64_t vote = __ballot(own >> b & 1);
-      if (lane == 0)
-        votes.bit[b][wave] = vote;
-    }
+  const int count = a.pool.adapters + 1;
+  int own[kOwnRows];
+#pragma unroll
+  for (int j = 0; j < kOwnRows; ++j) {
+    const int row = threadIdx.x + j * kThreads;
+    own[j] = row < a.rows ? checked_adapter(a, row) : -1;
   }
+  for (int i = threadIdx.x; i < count; i += kThreads)
+    bins[i] = 0;
   if (threadIdx.x == 0)
     s.tile = {-1, 0, 0, 0};
   __syncthreads();
-  int before = 0, all = 0;
-  if (wave < words) {
-#pragma unroll 1
-    for (int w = 0; w < words; ++w) {
-      uint64_t same = 64 * w + 64 <= a.rows ? ~uint64_t{0} : (uint64_t{1} << (a.rows & 63)) - 1;
-#pragma unroll 1
-      for (int b = 0; b < bits; ++b) {
-        const uint64_t vote = votes.bit[b][w];
-        same &= (own >> b & 1) != 0 ? vote : ~vote;
-      }
-      all += __popcll(same);
-      before += __popcll(w < wave ? same : w == wave ? same & below : 0);
+#pragma unroll
+  for (int j = 0; j < kOwnRows; ++j) {
+    if (j * kThreads >= a.rows)
+      break;
+    // One addition where all of a wave's rows share an adapter, as in prompts.
+    const int first = __builtin_amdgcn_readfirstlane(own[j]);
+    const uint64_t same = __ballot(own[j] == first);
+    if (first >= 0 && same == __ballot(own[j] >= 0)) {
+      if (lane == 0)
+        atomicAdd(&bins[first], static_cast<int>(__popcll(same)));
+    } else if (own[j] >= 0) {
+      atomicAdd(&bins[own[j]], 1);
     }
-    const uint64_t leads = __ballot(own >= 0 && before % kTileRows == 0);
-    if (lane == 0)
-      votes.leader[wave] = leads;
   }
   __syncthreads();
-  int ahead = 0, tiles = 0;  // tiles of the rows before this wave's, and all
-  for (int w = 0; w < words; ++w) {
-    const int here = __popcll(votes.leader[w]);
-    ahead += w < wave ? here : 0;
-    tiles += here;
+  const int each = (count + kThreads - 1) / kThreads, from = threadIdx.x * each;
+  int mine = 0;
+  for (int i = from; i < min(from + each, count); ++i)
+    mine += (bins[i] + kTileRows - 1) / kTileRows;
+  const int through = wave_scan<Sum>(mine);
+  if (lane == 63)
+    counts.tiles[wave] = through;
+  __syncthreads();
+  int at = through - mine, tiles = 0;  // tiles of the bins before this thread's, and all
+#pragma unroll
+  for (int w = 0; w < kDownWaves; ++w) {
+    at += w < wave ? counts.tiles[w] : 0;
+    tiles += counts.tiles[w];
   }
   const DownWork work = down_work(a, tiles, kernel_ranks);
-  if (own >= 0 && before % kTileRows == 0 &&
-      ahead + __popcll(votes.leader[wave] & below) == work.index)
-    s.tile = {own, before, min(all - before, kTileRows), work.parts};
+  if (at <= work.index && work.index < at + mine) {
+    int bin = from, first = (work.index - at) * kTileRows;
+    for (; first >= bins[bin]; ++bin)
+      first -= (bins[bin] + kTileRows - 1) / kTileRows * kTileRows;
+    s.tile = {bin, first, min(bins[bin] - first, kTileRows), work.parts};
+  }
   __syncthreads();
   const Tile tile = s.tile;
-  const int place = before - tile.first;
-  if (own >= 0 && own == tile.adapter && place >= 0 && place < tile.count)
-    s.list[place] = row;
+  if (tile.count == 0)
+    return work;
+  uint64_t same[kOwnRows];
+#pragma unroll
+  for (int j = 0; j < kOwnRows; ++j) {
+    if (j * kThreads >= a.rows)
+      break;
+    same[j] = __ballot(own[j] == tile.adapter);
+    if (lane == 0)
+      counts.words[wave + j * kDownWaves] = __popcll(same[j]);
+  }
   __syncthreads();
+  const int here = 64 * lane < a.rows ? counts.words[lane] : 0;
+  const int before = wave_scan<Sum>(here) - here;
+#pragma unroll
+  for (int j = 0; j < kOwnRows; ++j) {
+    if (j * kThreads >= a.rows)
+      break;
+    const int place = __builtin_amdgcn_readlane(before, wave + j * kDownWaves) - tile.first +
+                      __popcll(same[j] & ((uint64_t{1} << lane) - 1));
+    if (own[j] == tile.adapter && place >= 0 && place < tile.count)
+      s.list[place] = threadIdx.x + j * kThreads;
+  }
   if (threadIdx.x == 0) {
     s.tile.first = work.index * kTileRows;
     if (tile.adapter == a.pool.adapters)
@@ -440,14 +466,15 @@ template <int kRanks, bool kLow>
 __global__ __launch_bounds__(64 * kDownWaves) void down_kernel(const AdapterArgs a) {
   extern __shared__ f32x4 down_shared[];
   __shared__ TileRows rows;
-  __shared__ Votes votes;
+  __shared__ Counts counts;
   DownWork work;
   if (a.sorted) {
     work = down_work(a, a.tiles, kRanks);
     find_tile(a, work.index, rows);
   } else {
     work = a.rows <= kSingleRows ? single_tile(a, kRanks, rows)
-                                 : sort_tile(a, kRanks, votes, rows);
+                                 : sort_tile(a, kRanks, counts,
+                                             reinterpret_cast<int32_t *>(down_shared), rows);
     // For up_kernel: this tile, and that there are none behind the last.
     if (rows.tile.count > 0 && work.part == 0 && work.set == 0 && work.group == 0) {
       if (static_cast<int>(threadIdx.x) < rows.tile.count)
@@ -1049,6 +1076,13 @@ size_t parts_of(const AdapterPool &pool, size_t rows) {
   }
   return best;
 }
+// Whether group_kernel sorts: many rows, or many blocks that would each sort them (us with and
+// without its launch: 4096 prompt rows on 8 adapters, 438 blocks, 113.1 and 110.2, 513 rows of
+// 4 19.1 and 16.9; 4000 rows of 2000 adapters, 2062 blocks, 193 and 218).
+bool sorted_first(const AdapterPool &pool, size_t rows) {
+  return rows > kSelfRows ||
+         (rows > kFewRows && down_blocks(pool, rows, parts_of(pool, rows)) > kMostSorts);
+}
 // Output columns of a block: as many blocks as the card holds at once (two a CU with their
 // LDS, eight without), as each forms its tile's inner values again. With many rows that would
 // leave some CUs one block and others two, so there the busiest CU has least to do, in
@@ -1071,7 +1105,7 @@ size_t chunk_of(const AdapterPool &pool, size_t rows, bool wide) {
   return ceil_div(ceil_div(width, chunks), unit) * unit;
 }
 size_t order_of(const AdapterPool &pool, size_t rows) {
-  return rows <= kFewRows ? most_tiles(pool, rows) * kTileRows : rows;
+  return !sorted_first(pool, rows) ? most_tiles(pool, rows) * kTileRows : rows;
 }
 size_t aligned(size_t bytes) { return (bytes + 15) / 16 * 16; }
 
@@ -1106,7 +1140,9 @@ Status launch_down(const AdapterArgs &a, size_t blocks, hipStream_t stream) {
   const auto kernel = a.lo != nullptr ? down_kernel<kRanks, true> : down_kernel<kRanks, false>;
   const int cols = a.rows <= 16 ? 1 : 2;  // 16s of rows in a block
   const int loads = kRanks + cols * (a.lo != nullptr ? 2 : 1);
-  const size_t lds = kDownWaves * std::max(loads, kRanks * cols) * 64 * sizeof(f32x4);
+  const size_t bins = a.sorted ? 0 : (a.pool.adapters + 1) * sizeof(int32_t);
+  const size_t lds =
+      std::max(bins, kDownWaves * std::max(loads, kRanks * cols) * 64 * sizeof(f32x4));
   if (lds > 64 * 1024)
     EVO_TRY(hip_status(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                            hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -1176,7 +1212,7 @@ Status adapter_linear(const AdapterPool &pool, const int32_t *adapter, const uin
   char *const after = base + list + aligned(order_of(pool, rows) * sizeof(int32_t));
   const AdapterArgs args{pool, adapter, x_hi, x_lo, x_stride, static_cast<int>(rows), residual,
                          out, out_stride, static_cast<int>(tiles), static_cast<int>(parts),
-                         static_cast<int>(chunk), rows <= kFewRows ? 0 : 1,
+                         static_cast<int>(chunk), sorted_first(pool, rows) ? 1 : 0,
                          static_cast<int>(halves_of(pool, rows)), wide ? 1 : 0,
                          reinterpret_cast<int32_t *>(base),
                          reinterpret_cast<int32_t *>(base + list),

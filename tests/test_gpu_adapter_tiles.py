@@ -185,3 +185,21 @@ def test_one_launch_keeps_infinities_and_ranks_apart(rank, width):
     assert not torch.isfinite(spoilt[0]).any() and spoilt[3].isnan().all()
     assert torch.equal(out[of_rows == 4][:, :69], spoilt[of_rows == 4][:, :69])
     assert not torch.isfinite(spoilt[of_rows == 4][:, 69]).any()
+
+
+@pytest.mark.parametrize("fill", [0, 127, 255])
+@pytest.mark.parametrize("rows,adapters,used", [(513, 3, 3), (700, 100, 1), (1600, 60, 60),
+                                                (4000, 300, 2), (4095, 5, 5), (4096, 2, 2),
+                                                (4097, 2, 2), (4096, 2000, 900)])
+def test_rows_sorted_by_blocks_or_first(rows, adapters, used, fill):
+    """Around the borders between both; words of 64 rows, and tiles that begin inside them."""
+    pool = Pool(adapters, 16, 136, 70, seed=rows)
+    of_rows = torch.randint(-1, used, (rows,), generator=pool.gen, device=DEVICE).to(torch.int32)
+    of_rows[rows // 4: rows // 2] = used - 1
+    high, low = pool.planes(rows)
+    base, out = pool.normal(rows, 70), torch.empty(rows, 70, device=DEVICE)
+    need = N.call("evo_hip_adapter_linear_workspace_bytes", pool.struct(), rows)
+    workspace = torch.full((need,), fill, dtype=torch.uint8, device=DEVICE)
+    adapt(pool, of_rows, high, low, base, out, workspace=workspace)
+    check(pool, of_rows, high, low, base, out)
+    assert pool.error.item() == 0
