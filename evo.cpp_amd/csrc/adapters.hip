@@ -6,7 +6,8 @@
 // of its rows wherever they lie: by group_kernel, or where they are few enough by each block
 // of down_kernel for itself. down_kernel forms the inner values D_a x of such a tile for a part
 // of the width, up_kernel adds the parts up, scales them and forms a chunk of the output
-// columns. Two launches, as the second product needs all of the width.
+// columns. Two launches, as the second product needs all of the width; both_kernel takes calls
+// of little work in one.
 // x comes as the planes hi (+ lo) of a split-BF16 activation, whose products with BF16
 // weights are exact in F32. The inner values are F32, and stay so in the second product:
 // each is cut into three BF16 planes, 8 bits each, which hold all of its 24 (one plane
@@ -16,11 +17,11 @@
 // or adapter reaches no other row.
 //
 // What bounds it. Many rows: bytes, nearly all of them the residual and the outputs. 4096
-// prompt rows on 8 adapters of rank 64, width 4096 -> 12288 (481 MB): sort 7.6 us, first
-// product 23.6 (67 MB of x, 2.8 TB/s), second 81 (403 MB and weights, 5.0 TB/s, a copy's
-// rate). Few rows: the chain of launch, sort and loads that wait for each other. One row of
-// rank 16: 4.7 + 4.5 us; 96 rows of 40 adapters: 7.8 + 10.3 (30 MB, 5.9 us of a copy);
-// 512 rows of 6 adapters of rank 64, width 4096 -> 11264: 9.9 + 15.9 (62 MB, 12.2).
+// prompt rows on 8 adapters of rank 64, width 4096 -> 12288 (481 MB): first product 29 us, 5
+// of them the sort (67 MB of x), second 78 (403 MB and weights, 5.2 TB/s, a copy's rate). Few
+// rows: the chain of launch, sort and loads that wait for each other. 512 rows of 6 adapters
+// of rank 64, width 4096 -> 11264: 7.8 + 16.5 us (62 MB, 12.2 us of a copy); in one launch one
+// row of rank 16 6.2 us, 96 rows of 40 adapters 13.4 (30 MB, 5.9).
 #include "common.hpp"
 #include "lanes.hpp"
 #include "ops.hpp"
