@@ -481,8 +481,7 @@ typedef struct evo_hip_adapters {
  * wrote, its bias included, or NULL: zero).
  *   adapter  device int32 [rows], read when the call runs; -1: none, the row is its
  *            residual. An index or a rank outside the pool counts as none:
- *            EVO_HIP_BAD_ADAPTER. Rows may share adapters in any order; each adapter is read
- *            once for up to 64 of its rows.
+ *            EVO_HIP_BAD_ADAPTER. Rows may share adapters in any order.
  *   x        split BF16 planes [rows][x_stride] as evo_hip_linear takes them (x_lo NULL:
  *            one plane), 16-byte aligned, x_stride a multiple of 8; rows at most 2^20.
  *   residual, out  F32 [rows][out_stride], 4-byte aligned; out may be residual. Columns
