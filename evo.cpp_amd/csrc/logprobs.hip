@@ -295,6 +295,34 @@ __device__ inline void write_top(const LogprobArgs &a, int row, const Row &r, in
   a.top_logprobs[at] = r.logprob(value_of_order(order_of(place)));
 }
 
+// A value that k of the wave's lanes reach, and with one less few more (0: fewer lanes have
+// any): a few from the top down, more by the bits of it (8192 x 512, us with 1, 4 and 10
+// alternatives: 10.0, 11.1 and 12.6, by bits 11.0, 11.5 and 12.0).
+__device__ inline uint32_t reached_by(uint32_t mine, int k) {
+  uint32_t border = 0;
+  if (k <= 8) {
+#pragma unroll 1
+    for (int count = 0; count < k;) {
+      border = wave_reduce(mine, Most());
+      if (border == 0)
+        break;
+      const bool first = mine == border;
+      count += __popcll(__ballot(first));
+      mine = first ? 0 : mine;
+    }
+    return border;
+  }
+#pragma unroll 1
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t tried = border | 1U << bit;
+    const int count = __popcll(__ballot(mine >= tried));
+    if (count >= k)
+      border = tried;
+    if (count == k)
+      break;
+  }
+  return border;
+}
 // The k largest of n different places in LDS, moved to the list's beginning in any
 // order; returns how many (n, if there are no more). One wave calls it.
 __device__ inline int keep_best(uint64_t *list, int n, int k) {
@@ -356,17 +384,7 @@ __device__ inline void first_tokens(const LogprobArgs &a, int row, const Row &r,
     order[i] = L::valid(0, i, a.vocab) ? ordered(x[i]) : 0;
     most = max(most, order[i]);
   }
-  uint32_t border = 0;
-#pragma unroll 1
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t tried = border | 1U << bit;
-    const int count = __popcll(__ballot(most >= tried));
-    if (count >= k)
-      border = tried;
-    if (count == k)
-      break;
-  }
-  border = max(border, 1U);
+  uint32_t border = max(reached_by(most, k), 1U);
   int n = 0;
 #pragma unroll 1
   for (bool closer = false;; closer = true) {
@@ -506,16 +524,7 @@ __device__ inline int filter(uint64_t *list, int n, int k, uint64_t *best, int *
     most = max(most, order_of(list[i]));
   const bool all = n >= 256;
   const int wanted = all ? (k + 3) / 4 : k;
-  uint32_t border = 0;
-#pragma unroll 1
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t tried = border | 1U << bit;
-    const int have = __popcll(__ballot(most >= tried));
-    if (have >= wanted)
-      border = tried;
-    if (have == wanted)
-      break;
-  }
+  uint32_t border = reached_by(most, wanted);
   if (lane == 0)
     borders[threadIdx.x >> 6] = border;
   if (threadIdx.x == 0)
