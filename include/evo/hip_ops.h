@@ -483,7 +483,8 @@ typedef struct evo_hip_adapters {
  *            residual. An index or a rank outside the pool counts as none:
  *            EVO_HIP_BAD_ADAPTER. Rows may share adapters in any order.
  *   x        split BF16 planes [rows][x_stride] as evo_hip_linear takes them (x_lo NULL:
- *            one plane), 16-byte aligned, x_stride a multiple of 8; rows at most 2^20.
+ *            one plane), 16-byte aligned, x_stride a multiple of 8; rows at most 2^20,
+ *            both strides at most 2^40.
  *   residual, out  F32 [rows][out_stride], 4-byte aligned; out may be residual. Columns
  *            behind out_width are left as they are, so the columns of one projection may
  *            have adapters of their own. Whole 16 bytes of columns run faster.
@@ -512,7 +513,8 @@ EVO_API evo_status evo_hip_adapter_linear(const evo_hip_adapters *pool, const in
  * alternatives is 0), but not all. A token whose logit is -infinity has p = 0 and ln p =
  * -infinity. A row that holds NaN or +infinity, or nothing above -infinity, gets NaN and
  * UINT32_MAX throughout. Sums are F32 and leave out the largest logit's own 1, so that ln p of
- * a token that the row is sure of keeps its relative precision.
+ * a token that the row is sure of keeps its relative precision, down to 2^-126, below which
+ * a weight counts as none.
  * The workspace (16-byte aligned, no initial contents) is needed above a vocabulary of
  * 2048. Calls that overlap need one each. */
 EVO_API size_t evo_hip_token_logprobs_workspace_bytes(size_t rows, size_t vocab,
