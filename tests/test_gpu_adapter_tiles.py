@@ -203,3 +203,21 @@ def test_rows_sorted_by_blocks_or_first(rows, adapters, used, fill):
     adapt(pool, of_rows, high, low, base, out, workspace=workspace)
     check(pool, of_rows, high, low, base, out)
     assert pool.error.item() == 0
+
+
+@pytest.mark.parametrize("fill", [0, 127, 255])
+@pytest.mark.parametrize("rows,adapters,used", [(200, 8, 1), (400, 20, 3), (513, 20, 20),
+                                                (1600, 20, 1), (2047, 100, 7)])
+@pytest.mark.parametrize("rank,width,out", [(16, 8200, 1030), (72, 4104, 516), (128, 4104, 3),
+                                            (24, 8200, 129)])
+def test_columns_by_the_tiles_found(rows, adapters, used, rank, width, out, fill):
+    """Batches that use few adapters of a pool: the second product's chunks get narrower."""
+    pool = Pool(adapters, rank, width, out, seed=rows)
+    of_rows = torch.randint(-1, used, (rows,), generator=pool.gen, device=DEVICE).to(torch.int32)
+    high, low = pool.planes(rows, 1)
+    base, result = pool.normal(rows, out), torch.empty(rows, out, device=DEVICE)
+    need = N.call("evo_hip_adapter_linear_workspace_bytes", pool.struct(), rows)
+    workspace = torch.full((need,), fill, dtype=torch.uint8, device=DEVICE)
+    adapt(pool, of_rows, high, low, base, result, workspace=workspace)
+    check(pool, of_rows, high, low, base, result)
+    assert pool.error.item() == 0
