@@ -516,8 +516,11 @@ template <typename S> __global__ __launch_bounds__(256) void segment_kernel(cons
 // threads of the block call it. Where every lane has places, each wave finds the border that
 // k / 4 of its lanes' largest reach, and the lowest of the four has k above it; with fewer
 // places, the highest of those that k of a wave's reach (0: no wave has so many) does.
-__device__ inline int filter(uint64_t *list, int n, int k, uint64_t *best, int *count) {
+// The counter is its own: waves that are late may still read it when others, behind no
+// barrier, begin the next list.
+__device__ inline int filter(uint64_t *list, int n, int k, uint64_t *best) {
   __shared__ uint32_t borders[4];
+  __shared__ int found;
   const int lane = threadIdx.x & 63;
   uint32_t most = 0;
   for (int i = threadIdx.x; i < n; i += 256)
@@ -528,21 +531,21 @@ __device__ inline int filter(uint64_t *list, int n, int k, uint64_t *best, int *
   if (lane == 0)
     borders[threadIdx.x >> 6] = border;
   if (threadIdx.x == 0)
-    *count = 0;
+    found = 0;
   __syncthreads();
   border = all ? min(min(borders[0], borders[1]), min(borders[2], borders[3]))
                : max(max(borders[0], borders[1]), max(borders[2], borders[3]));
   for (int i = threadIdx.x; i < n; i += 256) {
     const uint64_t own = list[i];
     if (order_of(own) >= border) {
-      const int at = atomicAdd(count, 1);
+      const int at = atomicAdd(&found, 1);
       if (at < 256)
         best[at] = own;
     }
   }
   __syncthreads();
-  if (*count <= 256)
-    return *count;
+  if (found <= 256)
+    return found;
   // (Many equal logits.)
   if (threadIdx.x < 64) {
     const int kept = keep_best(list, n, k);
@@ -608,7 +611,9 @@ template <typename S> __global__ __launch_bounds__(256) void join_kernel(const L
     return;
 
   // Each round takes the k best of the list (all, if there are no more) in order: of the
-  // segments, their groups, and those groups' logits.
+  // segments, their groups, and those groups' logits. What waves share is written a barrier
+  // after its last reads: fewer, chosen, least, count and what filter shares behind the one
+  // that begins a round, the list behind the one in its middle.
   int n = a.segments;
 #pragma unroll 1
   for (int round = 0;; ++round) {
@@ -616,7 +621,7 @@ template <typename S> __global__ __launch_bounds__(256) void join_kernel(const L
     const uint64_t *from = list;
     if (n > 128) {  // (Ranks take n steps, the threshold about 32: 184 x 17449 41 -> 16 us.)
       from = fewer;
-      n = filter(list, n, k, fewer, &count);
+      n = filter(list, n, k, fewer);
     }
     const int kept = min(n, k);
     if (static_cast<int>(threadIdx.x) < n) {
