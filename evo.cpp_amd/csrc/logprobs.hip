@@ -291,8 +291,18 @@ __device__ inline void write_row(const LogprobArgs &a, int row, const Row &r, ui
 __device__ inline void write_top(const LogprobArgs &a, int row, const Row &r, int rank,
                                  uint64_t place) {
   const size_t at = static_cast<size_t>(row) * a.alternatives + rank;
-  a.top_tokens[at] = r.valid ? index_of(place) : kNoToken;
+  a.top_tokens[at] = index_of(place);
   a.top_logprobs[at] = r.logprob(value_of_order(order_of(place)));
+}
+// The alternatives of a row without them. (Its NaN are in no order that a search could follow:
+// one may stand for a maximum or not, and the order of some is 0, that of no token.)
+__device__ inline void write_no_top(const LogprobArgs &a, int row) {
+  const int lane = threadIdx.x & 63;
+  if (lane < a.alternatives) {
+    const size_t at = static_cast<size_t>(row) * a.alternatives + lane;
+    a.top_tokens[at] = kNoToken;
+    a.top_logprobs[at] = __builtin_nanf("");
+  }
 }
 
 // A value that k of the wave's lanes reach, and with one less few more (0: fewer lanes have
@@ -460,8 +470,10 @@ __global__ __launch_bounds__(256) void row_kernel(const LogprobArgs a) {
   const Row r(s);
   if (lane == 0)
     write_row(a, row, r, s.before, given, logit);
-  if (a.alternatives > 0)
+  if (a.alternatives > 0 && r.valid)
     first_tokens<L>(a, row, r, l.x, lists + wave * (64 * kPer));
+  else
+    write_no_top(a, row);
 }
 
 // ------------------------------------------------- rows of several segments
@@ -609,6 +621,11 @@ template <typename S> __global__ __launch_bounds__(256) void join_kernel(const L
     write_row(a, row, r, whole.before, given, logit);
   if (k == 0)
     return;
+  if (!r.valid) {  // (All waves find the same.)
+    if (threadIdx.x < 64)
+      write_no_top(a, row);
+    return;
+  }
 
   // Each round takes the k best of the list (all, if there are no more) in order: of the
   // segments, their groups, and those groups' logits. What waves share is written a barrier
