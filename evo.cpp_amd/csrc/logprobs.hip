@@ -143,15 +143,17 @@ __device__ inline float exact_weight(float d) {
 }
 
 // The sums of a segment, given the largest of each kChunk registers. A chunk without the
-// largest of all in any lane takes the short way: with base * log2(e) = high + low, a
-// weight is exp2(x log2(e) - high), and 2^-low comes in at the end.
+// largest of all in any lane takes the short way: with base * kLog2e = high + low, a
+// weight is exp2(x kLog2e - high), and 2^-low comes in at the end. (What log2(e) has beyond
+// kLog2e is left out of both products, so an exponent lacks |x - base| 2^-25.6, less than its
+// rounding to F32 may take; in low alone it would be a factor of 2^(base 2^-25.6).)
 constexpr int kChunk = 8;
 template <int kPer>
 __device__ inline void sums(const float (&x)[kPer], const float (&most)[kPer / kChunk],
                             Segment &s) {
   const float base = s.top == -INFINITY ? 0.0F : s.top;
   const float high = base * kLog2e;
-  const float low = fmaf(base, kLog2eLow, fmaf(base, kLog2e, -high));
+  const float low = fmaf(base, kLog2e, -high);
   float sum = 0.0F, spread = 0.0F, short_sum = 0.0F, short_spread = 0.0F;
   uint32_t equal = 0;
 #pragma unroll

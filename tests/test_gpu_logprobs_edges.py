@@ -72,3 +72,20 @@ def test_nan_where_maxima_begin(vocab, top, bits):
     check_invalid(out, [2])
     good = [0, 1, 3]
     check(logits[good], tokens[good], top, {name: x[good] for name, x in out.items()})
+
+
+@pytest.mark.parametrize("vocab", [300, 512, 2000, 6000, 131072])
+@pytest.mark.parametrize("offset", [30.0, -30.0, 200.0, -1000.0, 1000.0, 1e5, -1e6, 3e7])
+def test_rows_far_from_zero(vocab, offset):
+    """Softmax does not see what is added to all logits: weights are as exact there, within
+    the bound of rows about zero."""
+    logits, tokens = inputs(6, vocab, "f32", seed=vocab)
+    logits += offset
+    check(logits, tokens, 4)
+
+
+@pytest.mark.parametrize("offset", [128.0, -4096.0])
+def test_16_bit_rows_far_from_zero(offset):
+    logits, tokens = inputs(6, 5000, "f32", std=20.0)
+    for kind in (torch.bfloat16, torch.float16):
+        check((logits + offset).to(kind), tokens, 4)
