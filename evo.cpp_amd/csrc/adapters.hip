@@ -1220,10 +1220,30 @@ Status invalid(const char *why) { return {ErrorCode::kInvalidArgument, why}; }
 
 }  // namespace
 
-size_t adapter_workspace_bytes(const AdapterPool &pool, size_t rows) {
+// What a call uses: the rows' bins, their order, the tiles, how many there are, inner values.
+size_t adapter_workspace_used(const AdapterPool &pool, size_t rows) {
   return aligned(rows * sizeof(int32_t)) + aligned(order_of(pool, rows) * sizeof(int32_t)) +
          aligned(most_tiles(pool, rows) * sizeof(Tile)) + 16 +
          parts_of(pool, rows) * rows * pool.rank * sizeof(float);
+}
+// That falls where more rows take fewer parts or another sort; this bounds it for `rows` and
+// all fewer. Its terms, for r <= rows: tiles grow with r but from 4 rows on to 5; the order
+// holds r, or 64 for each tile up to kSelfRows. Parts times r is at most `few` r up to
+// kFewRows and `many` r above; and never more than r + 2048 (steps + 8): below kManyRows as
+// parts are steps / 16 + 1 at most, from there on as the model of parts_of takes p > 1 only if
+// units / 256 * 8 (p - 1) < steps + 8, and units exceed r / 64 - 1.
+size_t adapter_workspace_bytes(const AdapterPool &pool, size_t rows) {
+  const auto tiles = [&](size_t r) {
+    return std::max(most_tiles(pool, r), std::min<size_t>(r, kSingleRows));
+  };
+  const size_t order = std::max(rows, tiles(std::min<size_t>(rows, kSelfRows)) * kTileRows);
+  const size_t steps = (static_cast<size_t>(pool.in_width) + 31) / 32;
+  const size_t few = std::min<size_t>(8, ceil_div(steps, 2 * kDownWaves));
+  const size_t many = std::min<size_t>(8, ceil_div(steps, 4 * kDownWaves));
+  const size_t inner = std::min(std::max(few * std::min<size_t>(rows, kFewRows), many * rows),
+                                rows + 2048 * (steps + 8));
+  return aligned(rows * sizeof(int32_t)) + aligned(order * sizeof(int32_t)) +
+         aligned(tiles(rows) * sizeof(Tile)) + 16 + inner * pool.rank * sizeof(float);
 }
 
 Status adapter_linear(const AdapterPool &pool, const int32_t *adapter, const uint16_t *x_hi,
@@ -1241,7 +1261,7 @@ Status adapter_linear(const AdapterPool &pool, const int32_t *adapter, const uin
       out_stride < static_cast<size_t>(pool.out_width) || out_stride > (size_t{1} << 40))
     return invalid("adapter_linear: out_stride below out_width, or misaligned outputs");
   if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||
-      workspace_bytes < adapter_workspace_bytes(pool, rows))
+      workspace_bytes < adapter_workspace_used(pool, rows))
     return invalid("adapter_linear: workspace too small or not aligned");
   const size_t tiles = most_tiles(pool, rows), parts = parts_of(pool, rows);
   const bool wide = wide_tiles(pool, rows);

@@ -280,7 +280,8 @@ struct AdapterPool {
 };
 constexpr int kBadAdapter = 1;
 constexpr int kMostAdapters = 8192, kMostRank = 128;
-size_t adapter_workspace_bytes(const AdapterPool &pool, size_t rows);
+size_t adapter_workspace_bytes(const AdapterPool &pool, size_t rows);  // for fewer rows too
+size_t adapter_workspace_used(const AdapterPool &pool, size_t rows);
 Status adapter_linear(const AdapterPool &pool, const int32_t *adapter, const uint16_t *x_hi,
                       const uint16_t *x_lo, size_t x_stride, size_t rows, const float *residual,
                       float *out, size_t out_stride, void *workspace, size_t workspace_bytes,

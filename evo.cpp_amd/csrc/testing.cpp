@@ -128,3 +128,14 @@ EVO_TEST_API int evo_test_paged_sequence(const int *sizes, const int32_t *token_
 EVO_TEST_API int evo_test_paged_page(const int32_t *table, int index, int pages) {
   return evo::hip::checked_page(table, index, pages);
 }
+
+// What a call of the adapters uses of its workspace.
+EVO_TEST_API size_t evo_test_adapter_workspace(int adapters, int rank, int in_width,
+                                               int out_width, size_t rows) {
+  evo::hip::AdapterPool pool{};
+  pool.adapters = adapters;
+  pool.rank = rank;
+  pool.in_width = in_width;
+  pool.out_width = out_width;
+  return evo::hip::adapter_workspace_used(pool, rows);
+}

@@ -491,7 +491,8 @@ typedef struct evo_hip_adapters {
  * Sums are F32; the inner values keep all of their 24 bits. An infinity or NaN in x or an
  * adapter reaches only the rows that use it. Repeated calls give the same bits.
  * The workspace (16-byte aligned, no initial contents) holds the rows' order and the inner
- * values; calls that overlap need one each. */
+ * values; calls that overlap need one each. One of the size for some rows serves calls of
+ * fewer rows on the same pool too. */
 EVO_API size_t evo_hip_adapter_linear_workspace_bytes(const evo_hip_adapters *pool, size_t rows);
 EVO_API evo_status evo_hip_adapter_linear(const evo_hip_adapters *pool, const int32_t *adapter,
                                           const uint16_t *x_hi, const uint16_t *x_lo,
