@@ -703,11 +703,14 @@ template <typename S> void launch(const LogprobArgs &a, hipStream_t stream) {
 
 constexpr size_t kMostRows = size_t{1} << 20;
 size_t segments_of(size_t vocab) { return (vocab + kSegment - 1) / kSegment; }
+// Waves of segment_kernel that its launch takes, four a block: it counts threads in 32 bits.
+constexpr size_t kMostSegments = ((size_t{1} << 32) - 1) / 256 * 4;
 
 }  // namespace
 
 size_t token_logprobs_workspace_bytes(size_t rows, size_t vocab, size_t alternatives) {
-  if (rows > kMostRows || vocab > kMostRows || vocab <= kSegment)
+  if (rows > kMostRows || vocab > kMostRows || vocab <= kSegment ||
+      rows * segments_of(vocab) > kMostSegments)
     return 0;
   return rows * segments_of(vocab) *
          (sizeof(Segment) + (alternatives > 0 ? kGroups * sizeof(float) : 0));
@@ -736,14 +739,13 @@ Status token_logprobs(int dtype, const void *logits, size_t rows, size_t vocab, 
             "token_logprobs: at most 64 alternatives, no more than vocab, with their outputs"};
   if (logprob == nullptr && rank == nullptr && entropy == nullptr && alternatives == 0)
     return {ErrorCode::kInvalidArgument, "token_logprobs: no output"};
+  const size_t segments = segments_of(vocab);
+  if (rows * segments > kMostSegments)
+    return {ErrorCode::kInvalidArgument, "token_logprobs: grid too large"};
   const size_t need = token_logprobs_workspace_bytes(rows, vocab, alternatives);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need ||
                    reinterpret_cast<uintptr_t>(workspace) % 16 != 0))
     return {ErrorCode::kInvalidArgument, "token_logprobs: workspace too small or not aligned"};
-  const size_t segments = segments_of(vocab);
-  // (A launch counts its threads in 32 bits.)
-  if (ceil_div(rows * segments, 4) > ((size_t{1} << 32) - 1) / 256)
-    return {ErrorCode::kInvalidArgument, "token_logprobs: grid too large"};
   Segment *const stats = static_cast<Segment *>(workspace);
   const LogprobArgs args{logits, static_cast<int>(rows), static_cast<int>(vocab),
                          static_cast<int>(segments), row_stride, tokens, logprob, rank, entropy,

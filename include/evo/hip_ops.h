@@ -501,7 +501,8 @@ EVO_API evo_status evo_hip_adapter_linear(const evo_hip_adapters *pool, const in
                                           size_t workspace_bytes, void *stream);
 
 /* What rows of logits [rows][row_stride] (F32, BF16 or F16; rows and vocab at most 2^20,
- * row_stride at most 2^40) say of given tokens. With p = softmax of a row:
+ * rows * ceil(vocab / 2048) at most 2^26 - 4, row_stride at most 2^40) say of given tokens.
+ * With p = softmax of a row:
  *   logprob  F32 [rows], ln p of tokens[r] (device uint32 [rows]); NaN where that is no
  *            token of the vocabulary
  *   rank     uint32 [rows], how many tokens come before it in the order of evo_sampler_sample
@@ -517,7 +518,8 @@ EVO_API evo_status evo_hip_adapter_linear(const evo_hip_adapters *pool, const in
  * a token that the row is sure of keeps its relative precision, down to 2^-126, below which
  * a weight counts as none.
  * The workspace (16-byte aligned, no initial contents) is needed above a vocabulary of
- * 2048. Calls that overlap need one each. */
+ * 2048; its size is 0 below, and for rows and vocabularies that are refused. Calls that
+ * overlap need one each. */
 EVO_API size_t evo_hip_token_logprobs_workspace_bytes(size_t rows, size_t vocab,
                                                       size_t alternatives);
 EVO_API evo_status evo_hip_token_logprobs(evo_hip_dtype dtype, const void *logits, size_t rows,
