@@ -126,14 +126,15 @@ __device__ inline HeadSize head_size(const float (&u)[8], const float (&v)[8],
     return {1.0F, 1.0F / (norm.inside ? sqrtf(mean + norm.eps) : sqrtf(mean) + norm.eps)};
   }
   // Squares beyond the range, infinities, NaN and zeros. The largest element is
-  // brought near one; eps is at most 1, so it does not overflow.
+  // brought near one; eps is at most 1, so it does not overflow. (Zeros are lifted too, as
+  // 1 / eps may overflow where eps 2^120 is no small number.)
   float most = 0.0F;
 #pragma unroll
   for (int e = 0; e < 8; ++e)
     most = fmaxf(most, fmaxf(fabsf(u[e]), fabsf(v[e])));
   most = over_head<kLanes>(most, [](float x, float y) { return fmaxf(x, y); });
-  const bool plain = most == 0.0F || !(most < INFINITY);
-  const float lift = plain ? 1.0F : ldexpf(1.0F, max(-126, min(-ilogbf(most), 120)));
+  const int power = most == 0.0F ? 120 : max(-126, min(-ilogbf(most), 120));
+  const float lift = !(most < INFINITY) ? 1.0F : ldexpf(1.0F, power);
   const float rms = sqrtf(squares(lift) * kMean);
   const float size = norm.inside ? hypotf(rms, sqrtf(norm.eps) * lift) : rms + norm.eps * lift;
   return {lift, 1.0F / size};
