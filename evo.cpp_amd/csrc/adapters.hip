@@ -1080,7 +1080,8 @@ size_t halves_of(const AdapterPool &pool, size_t rows) {
 int ranks_of(const AdapterPool &pool, size_t rows) {
   return pool.rank <= 16 ? 1 : pool.rank <= 32 ? 2 : pool.rank <= 64 || rows <= kFewRows ? 4 : 8;
 }
-// Blocks of down_kernel: all on the card at once (two a CU).
+// Blocks of down_kernel. Two fit a CU, but where a block takes 128 ranks (above rank 64, with
+// more than kFewRows rows), 128 KB of LDS and 160 registers, one.
 size_t down_blocks(const AdapterPool &pool, size_t rows, size_t parts) {
   const size_t units = most_tiles(pool, rows) * halves_of(pool, rows) *
                        ceil_div(pool.rank, 16 * ranks_of(pool, rows));
@@ -1090,9 +1091,12 @@ size_t down_blocks(const AdapterPool &pool, size_t rows, size_t parts) {
 // cheap to add up: 94 rows of rank 96 lose 4 us), but no more than eight, as the second
 // product adds them up (width 11264, us with 8, 6 and 4: 220 rows of rank 40 17.8, 21.0 and
 // 22.3, 109 rows of rank 24 15.1, 16.6 and 18.2). The kernel takes fewer, by the tiles that it
-// finds. Behind the sort's launch they are chosen here: as many as fit the
-// card if the tiles are its most; for many rows so that the busiest CU has least to do, its
+// finds. Above kFewRows they are chosen here: as many as make 512 blocks if the tiles
+// are its most; for many rows so that the busiest CU has least to do, its
 // blocks' steps and about 8 more for each, and for a part what the second product does with it.
+// (512 blocks of 128 ranks may take two rounds. us with 512 and 256 of them, 12 adapters of
+// rank 128, width 11264: 513 rows 35.0 and 39.5, 700 rows 36.4 and 42.5, 1000 rows 56.2 and
+// 48.3, 1500 rows 84.7 and 72.4; 2047 rows of 4, width 4096, 72.6 and 75.0; others within 1 %.)
 size_t parts_of(const AdapterPool &pool, size_t rows) {
   const size_t steps = (static_cast<size_t>(pool.in_width) + 31) / 32;
   const size_t parts = std::min<size_t>(8, ceil_div(steps, 4 * kDownWaves));
@@ -1118,8 +1122,11 @@ bool sorted_first(const AdapterPool &pool, size_t rows) {
   return rows > kSelfRows ||
          (rows > kFewRows && down_blocks(pool, rows, parts_of(pool, rows)) > kMostSorts);
 }
-// Output columns of a block: as many blocks as the card holds at once (two a CU with their
-// LDS, eight without), as each forms its tile's inner values again. With many rows that would
+// Output columns of a block: few blocks, as each forms its tile's inner values again: 512 with
+// LDS, 2048 without. (Two with LDS fit a CU at once, up to rank 64 mostly three. us with 512
+// and 768 blocks: 513 rows of 4 adapters of rank 16 20.3 and 19.9, 512 of 6 of rank 64 23.9 and
+// 23.5, but 2047 of 4 of rank 64 59.5 and 61.7, and of 7, width 11264 -> 4096, 57.2 and 54.4,
+// 1000 of them 27.2 and 29.0.) With many rows 512 would
 // leave some CUs one block and others two, so there the busiest CU has least to do, in
 // quarters of 128 columns, of which inner values cost a block two for each 32 ranks (with the
 // parts above, width 4096, rank 16: 16384 rows 207 us for 261, 8192 rows 96 for 107, 4096 rows
