@@ -12,7 +12,8 @@
 // weights are exact in F32. The inner values are F32, and stay so in the second product:
 // each is cut into three BF16 planes, 8 bits each, which hold all of its 24 (one plane
 // would round them to 2^-9, and the update with them; the two more cost matrix
-// instructions, which are not what bounds it).
+// instructions, which are not what bounds it). An infinity in U meets the planes that are zero
+// too, and gives NaN; both_kernel, which has no planes, gives the infinity.
 // A row's values come from its own column of each product: an infinity or NaN of one row
 // or adapter reaches no other row.
 //

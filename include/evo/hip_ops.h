@@ -489,7 +489,8 @@ typedef struct evo_hip_adapters {
  *            behind out_width are left as they are, so the columns of one projection may
  *            have adapters of their own. Whole 16 bytes of columns run faster.
  * Sums are F32; the inner values keep all of their 24 bits. An infinity or NaN in x or an
- * adapter reaches only the rows that use it. Repeated calls give the same bits.
+ * adapter reaches only the rows that use it; an infinity in up makes its column of those
+ * infinite or NaN, which of both the call's sizes decide. Repeated calls give the same bits.
  * The workspace (16-byte aligned, no initial contents) holds the rows' order and the inner
  * values; calls that overlap need one each. One of the size for some rows serves calls of
  * fewer rows on the same pool too. */
