@@ -1097,7 +1097,7 @@ size_t down_blocks(const AdapterPool &pool, size_t rows, size_t parts) {
 // blocks' steps and about 8 more for each, and for a part what the second product does with it.
 // (512 blocks of 128 ranks may take two rounds. us with 512 and 256 of them, 12 adapters of
 // rank 128, width 11264: 513 rows 35.0 and 39.5, 700 rows 36.4 and 42.5, 1000 rows 56.2 and
-// 48.3, 1500 rows 84.7 and 72.4; 2047 rows of 4, width 4096, 72.6 and 75.0; others within 1 %.)
+// 48.3, 1500 rows 84.7 and 72.4; 2047 rows of 4, width 4096, 72.6 and 75.0. Rank 72 is alike.)
 size_t parts_of(const AdapterPool &pool, size_t rows) {
   const size_t steps = (static_cast<size_t>(pool.in_width) + 31) / 32;
   const size_t parts = std::min<size_t>(8, ceil_div(steps, 4 * kDownWaves));
